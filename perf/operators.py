@@ -505,7 +505,7 @@ def _verify_plain(case, s):
     rest = rest.clamp(min=0.0)
     rest = torch.where(rest.sum(-1, keepdim=True) > 0, rest, w)
     upto = torch.cumsum(rest, dim=-1)
-    aim = s["u"].double()[row].view(-1, 1) * upto[:, -1:]
+    aim = s["u"].double()[last].view(-1, 1) * upto[:, -1:]          # a number that no draft was held against
     drawn = torch.searchsorted(upto, aim, right=True).view(-1)
     most = torch.where(rest > 0, torch.arange(V, device="cuda"), -1).amax(-1)
     drawn = torch.minimum(drawn, most)
