@@ -339,7 +339,7 @@ def _tables_plain(case, s):
     upto_takes, upto_tokens = torch.cumsum(takes, 0), torch.cumsum(fresh, 0)
     ok = valid & ((takes == 0) | (upto_takes <= count)) & ((fresh == 0) | (upto_tokens <= s["room"]))
     gives = torch.where(ok, (have - want).clamp(min=0), torch.zeros_like(have))
-    took = torch.where(ok, upto_takes, torch.zeros_like(takes)).amax()
+    took = torch.where(ok & (takes > 0), upto_takes, torch.zeros_like(takes)).amax()
     first = upto_takes - takes
     # Pages that go back to the ring, in request order.
     col = torch.arange(n, device="cuda").view(1, n)
