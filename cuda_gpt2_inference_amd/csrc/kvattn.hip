@@ -39,6 +39,7 @@
 #include <tuple>
 #include <type_traits>
 
+#include "kv4.hpp"
 #include "kvattn.h"
 #include "lanes.hpp"
 
@@ -2859,6 +2860,47 @@ __attribute__((visibility("hidden"))) void set_last_hip_error(int e) { t_last_hi
 __attribute__((visibility("hidden"))) int merge_poll_limit() { return g_merge_polls.load(std::memory_order_relaxed); }
 }  // namespace kvattn_internal
 
+namespace {
+
+using kvattn_internal::is_4bit;
+
+// The checks of an 8-bit call: a 4-bit one needs the same of its pointers and sizes.
+int check_common4(const void* qkv, const void* kv, const float* kv_scale, int B, int NH, int hs, int maxT) {
+    return check_common(qkv, kv, kv_scale, B, NH, hs, maxT, KVATTN_KV_INT8);
+}
+
+int cache_write4(void* kv, float* kv_scale, const void* qkv, int B, int NH, int hs, int maxT, const int* d_cur_len,
+                 int lens_per_seq, int kv_dtype, const CacheMap& cm, void* stream) {
+    KV_TRY(check_common4(qkv, kv, kv_scale, B, NH, hs, maxT));
+    KV_TRY(resolve_len(d_cur_len));
+    return kvattn_internal::append4(kv, kv_scale, qkv, B, NH, maxT, d_cur_len, lens_per_seq ? 1 : 0, cm.table,
+                                    cm.max_pages, cm.page_rows, cm.num_pages, kv_dtype, stream);
+}
+
+// decode_impl for a 4-bit cache: the last-block merge is the one strategy there is.
+int decode4(void* out, const void* qkv, const void* kv, const float* kv_scale, int B, int NH, int hs, int maxT,
+            const int* d_cur_len, int lens_per_seq, int len_hint, void* workspace, size_t workspace_bytes, int S,
+            int strategy, int kv_dtype, void* stream, bool append, const CacheMap& cm) {
+    KV_TRY(check_common4(qkv, kv, kv_scale, B, NH, hs, maxT));
+    if (!out) return KVATTN_ERR_NULL_POINTER;
+    if (!aligned16(out)) return KVATTN_ERR_MISALIGNED;
+    if (len_hint < -1 || len_hint > maxT - 1) return KVATTN_ERR_LENGTH;
+    if (strategy != KVATTN_AUTO && strategy != KVATTN_SPLIT_LASTBLOCK) return KVATTN_ERR_STRATEGY;
+    KV_TRY(resolve_len(d_cur_len));
+    const kvattn_internal::Attend4 c{out, qkv, kv, kv_scale, cm.table, nullptr, d_cur_len, cm.max_pages, cm.page_rows,
+                                     cm.num_pages, B, NH, maxT, B, 1, lens_per_seq ? 1 : 0, len_hint, S, kv_dtype,
+                                     workspace, workspace_bytes, stream};
+    if (append) {
+        KV_TRY(kvattn_internal::attend4(c, false));   // nothing is appended by a call that is refused
+        KV_TRY(kvattn_internal::append4(const_cast<void*>(kv), const_cast<float*>(kv_scale), qkv, B, NH, maxT, d_cur_len,
+                                        lens_per_seq ? 1 : 0, cm.table, cm.max_pages, cm.page_rows, cm.num_pages,
+                                        kv_dtype, stream));
+    }
+    return kvattn_internal::attend4(c, true);
+}
+
+}  // namespace
+
 // ======================================================================================
 // C ABI
 // ======================================================================================
@@ -2871,7 +2913,7 @@ const char* kvattn_strerror(int status) {
         case KVATTN_ERR_MISALIGNED: return "a buffer is not 16-byte aligned";
         case KVATTN_ERR_HEAD_DIM: return "head size must be 64";
         case KVATTN_ERR_SHAPE: return "B, NH or maxT out of range";
-        case KVATTN_ERR_DTYPE: return "unknown kv dtype or missing kv_scale for an 8-bit cache";
+        case KVATTN_ERR_DTYPE: return "unknown or unsupported kv dtype, or missing kv_scale for an 8-bit or 4-bit cache";
         case KVATTN_ERR_STRATEGY: return "unknown strategy";
         case KVATTN_ERR_WORKSPACE: return "workspace missing or too small";
         case KVATTN_ERR_SPLIT: return "segment count or segment length out of range";
@@ -2912,6 +2954,9 @@ int kvattn_set_cur_len_async(int* d_cur_len, int cur_len, void* stream) {
 
 int kvattn_cache_write(void* kv_cache, float* kv_scale, const void* qkv, int B, int NH, int hs, int maxT,
                        const int* d_cur_len, int lens_per_seq, int kv_dtype, void* stream_v) {
+    if (is_4bit(kv_dtype))
+        return cache_write4(kv_cache, kv_scale, qkv, B, NH, hs, maxT, d_cur_len, lens_per_seq, kv_dtype, CacheMap{},
+                            stream_v);
     KV_TRY(check_common(qkv, kv_cache, kv_scale, B, NH, hs, maxT, kv_dtype));
     KV_TRY(resolve_len(d_cur_len));
     return launch_cache_write(kv_cache, kv_scale, qkv, B, NH, maxT, d_cur_len, lens_per_seq, kv_dtype, CacheMap{},
@@ -2928,10 +2973,13 @@ int kvattn_paged_cache_write(void* pages, float* page_scales, const int* block_t
                              const int* d_cur_len, int lens_per_seq, int kv_dtype, void* stream) {
     int maxT = 0;
     KV_TRY(check_paged(block_table, max_pages, page_rows, num_pages, NH, maxT));
+    const CacheMap cm{block_table, max_pages, page_rows, num_pages};
+    if (is_4bit(kv_dtype))
+        return cache_write4(pages, page_scales, qkv, B, NH, hs, maxT, d_cur_len, lens_per_seq, kv_dtype, cm, stream);
     KV_TRY(check_common(qkv, pages, page_scales, B, NH, hs, maxT, kv_dtype));
     KV_TRY(resolve_len(d_cur_len));
-    return launch_cache_write(pages, page_scales, qkv, B, NH, maxT, d_cur_len, lens_per_seq, kv_dtype,
-                              CacheMap{block_table, max_pages, page_rows, num_pages}, (hipStream_t)stream);
+    return launch_cache_write(pages, page_scales, qkv, B, NH, maxT, d_cur_len, lens_per_seq, kv_dtype, cm,
+                              (hipStream_t)stream);
 }
 
 int kvattn_paged_decode(void* out, const void* qkv, void* pages, float* page_scales, const int* block_table,
@@ -2941,8 +2989,28 @@ int kvattn_paged_decode(void* out, const void* qkv, void* pages, float* page_sca
     int maxT = 0;
     KV_TRY(check_paged(block_table, max_pages, page_rows, num_pages, NH, maxT));
     const CacheMap cm{block_table, max_pages, page_rows, num_pages};
+    if (is_4bit(kv_dtype))
+        return decode4(out, qkv, pages, page_scales, B, NH, hs, maxT, d_cur_len, lens_per_seq, len_hint, workspace,
+                       workspace_bytes, S, strategy, kv_dtype, stream, append != 0, cm);
     return decode_impl(out, qkv, pages, page_scales, B, NH, hs, maxT, d_cur_len, lens_per_seq, len_hint, workspace,
                        workspace_bytes, S, strategy, kv_dtype, stream, append != 0, &cm);
+}
+
+int kvattn_paged_decode_tokens(void* out, const void* qkv, const void* pages, const float* page_scales,
+                               const int* block_table, int max_pages, int page_rows, int num_pages,
+                               const int* token_start, const int* lens, int B, int num_tokens, int max_new, int NH,
+                               int hs, void* workspace, size_t workspace_bytes, int S, int kv_dtype, void* stream) {
+    int maxT = 0;
+    KV_TRY(check_paged(block_table, max_pages, page_rows, num_pages, NH, maxT));
+    if (hs == kHeadDim && !is_4bit(kv_dtype)) return KVATTN_ERR_DTYPE;
+    KV_TRY(check_common4(qkv, pages, page_scales, B, NH, hs, maxT));
+    if (num_tokens < 1 || max_new < 1 || (long long)num_tokens * NH > (1ll << 24)) return KVATTN_ERR_SHAPE;
+    if (!out || !token_start || !lens) return KVATTN_ERR_NULL_POINTER;
+    if (!aligned16(out) || ((uintptr_t)token_start & 3u) || ((uintptr_t)lens & 3u)) return KVATTN_ERR_MISALIGNED;
+    const kvattn_internal::Attend4 c{out, qkv, pages, page_scales, block_table, token_start, lens, max_pages, page_rows,
+                                     num_pages, B, NH, maxT, num_tokens, max_new, 1, -1, S, kv_dtype, workspace,
+                                     workspace_bytes, stream};
+    return kvattn_internal::attend4(c, true);
 }
 
 int kvattn_forward_small(void* out, const void* qkv, const void* kv_cache, const float* kv_scale, int B, int NH,
@@ -3077,8 +3145,18 @@ int kvattn_plan(int B, int NH, int hs, int maxT, int len_hint, int S, int strate
                 int* strategy_out, int* segments_out, int* seg_rows_out) {
     if (hs != kHeadDim) return KVATTN_ERR_HEAD_DIM;
     if (B < 1 || NH < 1 || maxT < 1 || maxT > kMaxT || (long long)B * NH > (1ll << 24)) return KVATTN_ERR_SHAPE;
-    if (kv_dtype < KVATTN_KV_F32 || kv_dtype > KVATTN_KV_FP8_E4M3) return KVATTN_ERR_DTYPE;
+    if (kv_dtype < KVATTN_KV_F32 || kv_dtype > KVATTN_KV_FP4_E2M1) return KVATTN_ERR_DTYPE;
     if (!strategy_out || !segments_out || !seg_rows_out) return KVATTN_ERR_NULL_POINTER;
+    if (is_4bit(kv_dtype)) {
+        if (len_hint < -1 || len_hint > maxT - 1) return KVATTN_ERR_LENGTH;
+        if (strategy != KVATTN_AUTO && strategy != KVATTN_SPLIT_LASTBLOCK) return KVATTN_ERR_STRATEGY;
+        kvattn_internal::Plan4 p4{};
+        KV_TRY(kvattn_internal::plan4(B * NH, maxT, len_hint, S, p4));
+        *strategy_out = KVATTN_SPLIT_LASTBLOCK;
+        *segments_out = p4.S;
+        *seg_rows_out = S > 0 ? 0 : p4.seg_tiles * kMinSegRows;
+        return KVATTN_OK;
+    }
     Plan p{};
     KV_TRY(make_plan(B, NH, maxT, len_hint, S, strategy, kv_dtype, p));
     *strategy_out = p.strategy;
@@ -3090,6 +3168,9 @@ int kvattn_plan(int B, int NH, int hs, int maxT, int len_hint, int S, int strate
 int kvattn_decode(void* out, const void* qkv, const void* kv_cache, const float* kv_scale, int B, int NH, int hs,
                   int maxT, const int* d_cur_len, int lens_per_seq, int len_hint, void* workspace,
                   size_t workspace_bytes, int S, int strategy, int kv_dtype, void* stream) {
+    if (is_4bit(kv_dtype))
+        return decode4(out, qkv, kv_cache, kv_scale, B, NH, hs, maxT, d_cur_len, lens_per_seq, len_hint, workspace,
+                       workspace_bytes, S, strategy, kv_dtype, stream, false, CacheMap{});
     return decode_impl(out, qkv, kv_cache, kv_scale, B, NH, hs, maxT, d_cur_len, lens_per_seq, len_hint,
                        workspace, workspace_bytes, S, strategy, kv_dtype, stream, false);
 }
@@ -3104,6 +3185,9 @@ int kvattn_decode_static(void* out, const void* qkv, const void* kv_cache, const
 int kvattn_append_decode(void* out, const void* qkv, void* kv_cache, float* kv_scale, int B, int NH, int hs,
                          int maxT, const int* d_cur_len, int lens_per_seq, int len_hint, void* workspace,
                          size_t workspace_bytes, int S, int strategy, int kv_dtype, void* stream) {
+    if (is_4bit(kv_dtype))
+        return decode4(out, qkv, kv_cache, kv_scale, B, NH, hs, maxT, d_cur_len, lens_per_seq, len_hint, workspace,
+                       workspace_bytes, S, strategy, kv_dtype, stream, true, CacheMap{});
     return decode_impl(out, qkv, kv_cache, kv_scale, B, NH, hs, maxT, d_cur_len, lens_per_seq, len_hint,
                        workspace, workspace_bytes, S, strategy, kv_dtype, stream, true);
 }

@@ -1,0 +1,520 @@
+// pages.hip -- the bookkeeping of a paged KV cache on the GPU, and its rows by slot map (gfx950):
+// block tables, token offsets, slot map and positions from what every request holds, keeps and
+// adds; K and V rows into the pool and out of it for every cache type; the append of one token a
+// sequence into a 4-bit cache.
+#include "kv4.hpp"
+
+#include <limits.h>
+
+#include "lanes.hpp"
+#include "layout.hpp"
+
+namespace {
+
+using kvattn_internal::is_4bit;
+
+constexpr int kHd = 64;
+constexpr int kBlock = 256;
+constexpr int kMaxT = 1 << 23;
+
+int hip_status(hipError_t e) {
+    if (e == hipSuccess) return KVATTN_OK;
+    kvattn_internal::set_last_hip_error((int)e);
+    return KVATTN_ERR_HIP;
+}
+
+// ------------------------------------------------------------------------------------
+// Pages of requests.
+//
+// The pool is a ring of free page ids: taken at its head, given back at its tail, so a call's
+// reads (entries head ..) and writes (entries head + count ..) never meet.  Every workgroup reads
+// all requests and scans them (tokens, pages taken, pages given back: prefix sums in request
+// order), then does its share of the tokens and pages, which need nothing of one another.  What the
+// outputs may share with the inputs (held, kept, the pool's head and count) is written by the
+// workgroup that was the last to have read it all, so one launch does, in place too.  The call is
+// bound by launch and a few memory round trips (24 requests), then by the slot map's writes.
+// ------------------------------------------------------------------------------------
+constexpr int kPoolHead = 0, kPoolCount = 1, kPoolTicket = 2, kPoolRing = 4;
+constexpr int kMaxRequests = 4096;
+constexpr int kRequestInts = 6;            // LDS words of a request
+constexpr int kReserveTokens = 1024;       // token rows a workgroup is launched for, up to
+constexpr int kReserveMostBlocks = 256;    // so many workgroups
+constexpr int kRefused = 1 << 30;          // beside the positions a request keeps
+
+struct ReserveArgs {
+    int* table;
+    int* pool;
+    const int* held;
+    const int* kept;
+    const int* fresh;
+    int* held_out;
+    int* lens;
+    int* token_start;
+    long long* slot_map;
+    int* positions;
+    int* pool_next;
+    int max_pages, R, num_pages, B, max_tokens;
+};
+
+__device__ __forceinline__ int add_sat(int a, int b) {   // a, b >= 0
+    const unsigned s = (unsigned)a + (unsigned)b;
+    return s > (unsigned)INT_MAX ? INT_MAX : (int)s;
+}
+
+// Exclusive prefix of v over the workgroup's threads, and its total.
+__device__ __forceinline__ int block_prefix(int v, int* wave_sums, int& total) {
+    const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+    int in = v;
+#pragma unroll
+    for (int d = 1; d < kWave; d <<= 1) {
+        const int o = __shfl_up(in, d);
+        in = lane >= d ? add_sat(in, o) : in;
+    }
+    __syncthreads();
+    if (lane == kWave - 1) wave_sums[wave] = in;
+    __syncthreads();
+    int before = 0;
+    total = 0;
+#pragma unroll
+    for (int w = 0; w < kBlock / kWave; ++w) {
+        before = w < wave ? add_sat(before, wave_sums[w]) : before;
+        total = add_sat(total, wave_sums[w]);
+    }
+    const int up = __shfl_up(in, 1);
+    return add_sat(before, lane > 0 ? up : 0);
+}
+
+// The last i of 0 .. n-1 with start[i] <= x (start[0] = 0): the owner of item x.
+__device__ __forceinline__ int owner(const int* start, int n, int x) {
+    int lo = 0, hi = n - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (start[mid] <= x) lo = mid;
+        else hi = mid - 1;
+    }
+    return lo;
+}
+
+__global__ __launch_bounds__(kBlock) void reserve_kernel(ReserveArgs a) {
+    extern __shared__ int lds[];
+    __shared__ int wave_sums[kBlock / kWave];
+    __shared__ int shared_took, shared_turn;
+    int* const tok = lds;                 // first token
+    int* const take = tok + a.B;          // first of the pages it takes
+    int* const give = take + a.B;         // first of the pages it gives back
+    int* const have = give + a.B;         // pages it holds
+    int* const want = have + a.B;         // pages it will hold (refused: those it holds)
+    int* const kept = want + a.B;         // positions it keeps, and kRefused
+    const int P = a.num_pages;
+    const int head = (int)((unsigned)a.pool[kPoolHead] % (unsigned)P);
+    const int count = min(max(a.pool[kPoolCount], 0), P);
+    const long long most = (long long)a.max_pages * a.R;
+    const int each = (a.B + kBlock - 1) / kBlock, i0 = min((int)threadIdx.x * each, a.B), i1 = min(i0 + each, a.B);
+
+    // Tokens and pages asked for.  A request whose lengths make no sense asks for nothing.
+    int toks = 0, takes = 0;
+    for (int i = i0; i < i1; ++i) {
+        const int hd = a.held[i], kp = a.kept[i], fr = a.fresh[i];
+        const bool ok = kp >= 0 && kp <= hd && hd <= most && fr >= 0 && (long long)kp + fr <= most;
+        have[i] = ok ? (hd + a.R - 1) / a.R : 0;
+        want[i] = ok ? (kp + fr + a.R - 1) / a.R : 0;
+        kept[i] = ok ? kp : kRefused;
+        tok[i] = ok ? fr : 0;
+        toks = add_sat(toks, tok[i]);
+        takes = add_sat(takes, max(want[i] - have[i], 0));
+    }
+    int all_toks, all_takes, all_gives;
+    int t = block_prefix(toks, wave_sums, all_toks), k = block_prefix(takes, wave_sums, all_takes);
+    // Granted in request order while pages and token rows last: once one that takes pages is refused
+    // for want of pages (or tokens), so is every later one that takes any, so pages taken have no gaps.
+    int gives = 0, took = 0;
+    for (int i = i0; i < i1; ++i) {
+        const int fr = tok[i], tk = max(want[i] - have[i], 0);
+        tok[i] = t;
+        take[i] = k;
+        t = add_sat(t, fr);
+        k = add_sat(k, tk);
+        const bool ok = !(kept[i] & kRefused) && (tk == 0 || k <= count) && (fr == 0 || t <= a.max_tokens);
+        if (!ok) {
+            kept[i] |= kRefused;
+            want[i] = have[i];
+        }
+        if (ok && tk > 0) took = k;
+        gives = add_sat(gives, max(have[i] - want[i], 0));
+    }
+    int gv = block_prefix(gives, wave_sums, all_gives);
+    for (int i = i0; i < i1; ++i) {
+        give[i] = gv;
+        gv = add_sat(gv, max(have[i] - want[i], 0));
+    }
+    if (threadIdx.x == 0) shared_took = 0;
+    __syncthreads();
+    if (took > 0) atomicMax(&shared_took, took);
+    // Everything that another workgroup's outputs may overwrite has been read.
+    wait_vm_stores();
+    __syncthreads();
+    const int all_took = shared_took;
+    if (threadIdx.x == 0) {
+        bool turn = true;
+        if (gridDim.x > 1) {
+            const unsigned seen = __hip_atomic_fetch_add((unsigned*)a.pool + kPoolTicket, 1u, __ATOMIC_RELAXED,
+                                                         __HIP_MEMORY_SCOPE_AGENT);
+            turn = seen == gridDim.x - 1;
+            if (turn)
+                __hip_atomic_store((unsigned*)a.pool + kPoolTicket, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        }
+        shared_turn = turn;
+    }
+    __syncthreads();
+
+    const int me = blockIdx.x * kBlock + threadIdx.x, step = gridDim.x * kBlock;
+    int* const ring = a.pool + kPoolRing;
+    auto ring_at = [&](int i) {           // entry i of the ring from its head on, i <= P
+        const int at = head + i;
+        return at >= P ? at - P : at;
+    };
+    // Tokens.
+    const int n_tok = min(all_toks, a.max_tokens);
+    for (int x = me; x < n_tok; x += step) {
+        const int b = owner(tok, a.B, x);
+        const int kp = kept[b] & ~kRefused, pos = kp + (x - tok[b]), pi = pos / a.R;
+        if (a.positions) a.positions[x] = pos;
+        long long slot = -1;
+        if (!(kept[b] & kRefused)) {
+            const int page = pi < have[b] ? a.table[(size_t)b * a.max_pages + pi] : ring[ring_at(take[b] + pi - have[b])];
+            if (page >= 0 && page < P) slot = (long long)page * a.R + pos % a.R;
+        }
+        a.slot_map[x] = slot;
+    }
+    // Pages taken.
+    for (int x = me; x < all_took; x += step) {
+        const int b = owner(take, a.B, x);
+        a.table[(size_t)b * a.max_pages + have[b] + x - take[b]] = ring[ring_at(x)];
+    }
+    // Pages given back.  (More than the ring has room for means a pool that was not this one's.)
+    const int n_give = min(all_gives, P - count);
+    for (int x = me; x < n_give; x += step) {
+        const int b = owner(give, a.B, x);
+        ring[ring_at(count + x)] = a.table[(size_t)b * a.max_pages + want[b] + x - give[b]];
+    }
+    if (!shared_turn) return;
+    for (int i = threadIdx.x; i < a.B; i += kBlock) {
+        const bool ok = !(kept[i] & kRefused);
+        const int hd = a.held[i], kp = a.kept[i];
+        const int fr = (i + 1 < a.B ? tok[i + 1] : all_toks) - tok[i];
+        a.held_out[i] = ok ? kp + fr : hd;
+        a.lens[i] = ok ? kp + fr : kp;
+        a.token_start[i] = tok[i];
+    }
+    if (threadIdx.x == 0) {
+        a.token_start[a.B] = all_toks;
+        int* const next = a.pool_next ? a.pool_next : a.pool;
+        next[kPoolHead] = ring_at(all_took);
+        next[kPoolCount] = count - all_took + n_give;
+    }
+}
+
+// Every page free, in order.
+__global__ __launch_bounds__(kBlock) void pool_init_kernel(int* pool, int num_pages) {
+    const int i = blockIdx.x * kBlock + threadIdx.x;
+    if (i < kPoolRing) pool[i] = i == kPoolCount ? num_pages : 0;
+    if (i < num_pages) pool[kPoolRing + i] = i;
+}
+
+// ------------------------------------------------------------------------------------
+// Rows.  Eight lanes hold a row, 8 channels each; a wave takes eight neighbouring tokens of one
+// head's K or V, which lie in neighbouring rows of a page (one line of 4-bit rows).  Bound by
+// memory: 128 bytes of bf16 and 36 of codes and scale a row.
+// ------------------------------------------------------------------------------------
+template <int DT> struct Fmt {            // stored bytes of 8 channels
+    static constexpr bool kF32 = DT == KVATTN_KV_F32;
+    static constexpr bool k4 = DT == KVATTN_KV_INT4 || DT == KVATTN_KV_FP4_E2M1;
+    static constexpr bool k8 = DT == KVATTN_KV_INT8 || DT == KVATTN_KV_FP8_E4M3;
+    static constexpr bool kCoded = k4 || k8;
+    static constexpr int kBytes = kF32 ? 32 : (DT == KVATTN_KV_BF16 ? 16 : (k8 ? 8 : 4));
+};
+
+__device__ __forceinline__ void load_bf16x8(const uint16_t* p, float (&x)[8]) {
+    const uint4 v = *reinterpret_cast<const uint4*>(p);
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        x[2 * i] = bf16_lo(w[i]);
+        x[2 * i + 1] = bf16_hi(w[i]);
+    }
+}
+
+// A 4-bit row's scale is its largest magnitude times the float nearest 1/7 or 1/6.
+template <int DT> constexpr float kScaleOfMax4 = DT == KVATTN_KV_INT4 ? 1.0f / 7.0f : 1.0f / 6.0f;
+
+// Eight 4-bit codes of x / scale; no scale (a row of zeros) and NaN give zero.
+template <int DT>
+__device__ __forceinline__ uint32_t codes4(const float (&x)[8], float scale) {
+    uint32_t w = 0;
+    const bool live = scale > 0.0f;
+    float y[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        y[i] = x[i] / scale;
+        y[i] = live && y[i] == y[i] ? y[i] : 0.0f;
+    }
+    if constexpr (DT == KVATTN_KV_FP4_E2M1) {
+        w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, y[0], y[1], 1.0f, 0);   // nearest, ties to even
+        w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, y[2], y[3], 1.0f, 1);
+        w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, y[4], y[5], 1.0f, 2);
+        w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, y[6], y[7], 1.0f, 3);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int c = (int)fminf(fmaxf(rintf(y[i]), -7.0f), 7.0f) + 8;
+            w |= (uint32_t)c << (4 * i);
+        }
+    }
+    return w;
+}
+
+template <int DT>
+__device__ __forceinline__ void values4(uint32_t w, float (&x)[8]) {
+    if constexpr (DT == KVATTN_KV_FP4_E2M1) {
+        const auto a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, 0);
+        const auto b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, 1);
+        const auto c = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, 2);
+        const auto d = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, 3);
+        x[0] = a[0]; x[1] = a[1]; x[2] = b[0]; x[3] = b[1];
+        x[4] = c[0]; x[5] = c[1]; x[6] = d[0]; x[7] = d[1];
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = (float)((int)((w >> (4 * i)) & 15u) - 8);
+    }
+}
+
+// Where a token's rows lie: by slot (page * R + row of the page), or at the position that the
+// append writes (contiguous or paged).
+struct RowsArgs {
+    uint8_t* kv;
+    float* scale;
+    void* act;                 // qkv [n][3][NH][64], or the loaded rows [n][2][NH][64]
+    const long long* slots;
+    const int* cur_len;
+    const int* table;
+    int lens_per_seq, max_pages, R, num_pages, n, NH, maxT;
+    int shift;                 // log2 of R, or -1
+};
+
+// The row (of 64 channels) of token tok's K (part 0) or V in head h; false: none.
+template <bool kSlots>
+__device__ __forceinline__ bool row_of(const RowsArgs& a, int tok, int part, int h, size_t& row) {
+    long long page;
+    int r;
+    if constexpr (kSlots) {
+        const long long slot = a.slots[tok];
+        if (slot < 0) return false;
+        page = a.shift >= 0 ? slot >> a.shift : slot / a.R;
+        if (page >= a.num_pages) return false;
+        r = (int)(slot - page * a.R);
+    } else {
+        const int cl = min(max(a.cur_len[a.lens_per_seq ? tok : 0], 0), a.maxT - 1);
+        if (!a.table) {
+            row = (((size_t)part * a.n + tok) * a.NH + h) * a.maxT + cl;
+            return true;
+        }
+        page = a.table[(size_t)tok * a.max_pages + cl / a.R];
+        if (page < 0 || page >= a.num_pages) return false;
+        r = cl % a.R;
+    }
+    row = (((size_t)page * 2 + part) * a.NH + h) * a.R + r;
+    return true;
+}
+
+template <int DT, bool kSlots>
+__global__ __launch_bounds__(kBlock) void store_rows_kernel(RowsArgs a) {
+    using F = Fmt<DT>;
+    const int lane = threadIdx.x & (kWave - 1), c = lane & 7;
+    const int item = blockIdx.x * (kBlock / kWave) + threadIdx.x / kWave;    // eight tokens, part, head
+    const int heads = 2 * a.NH;
+    const int tok = item / heads * 8 + (lane >> 3), ph = item % heads, part = ph / a.NH, h = ph % a.NH;
+    if (tok >= a.n) return;
+    const size_t src = (((size_t)tok * 3 + 1 + part) * a.NH + h) * kHd + c * 8;
+    size_t row = 0;
+    const bool there = row_of<kSlots>(a, tok, part, h, row);     // the same for the row's eight lanes
+    uint8_t* const dst = a.kv + (row * 8 + c) * F::kBytes;
+    if constexpr (F::kF32) {
+        const uint4* p = reinterpret_cast<const uint4*>((const float*)a.act + src);
+        const uint4 x = p[0], y = p[1];
+        if (!there) return;
+        reinterpret_cast<uint4*>(dst)[0] = x;
+        reinterpret_cast<uint4*>(dst)[1] = y;
+    } else if constexpr (!F::kCoded) {
+        const uint4 x = *reinterpret_cast<const uint4*>((const uint16_t*)a.act + src);
+        if (there) *reinterpret_cast<uint4*>(dst) = x;
+    } else {
+        float x[8], amax = 0.0f;
+        load_bf16x8((const uint16_t*)a.act + src, x);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) amax = fmaxf(amax, fabsf(x[i]));
+        amax = row_max<8>(amax);
+        if constexpr (F::k4) {
+            const float scale = amax * kScaleOfMax4<DT>;
+            if (c == 0 && there) a.scale[row] = scale;
+            const uint32_t w = codes4<DT>(x, scale);
+            if (there) *reinterpret_cast<uint32_t*>(dst) = w;
+        } else {
+            const float scale = amax / kW8Limit<DT>;
+            if (c == 0 && there) a.scale[row] = scale;
+            uint32_t w[2] = {0, 0};
+#pragma unroll
+            for (int i = 0; i < 8; ++i) w[i / 4] |= (uint32_t)w8_code<DT>(x[i], scale) << (8 * (i % 4));
+            if (there) *reinterpret_cast<uint2*>(dst) = make_uint2(w[0], w[1]);
+        }
+    }
+}
+
+template <int DT>
+__global__ __launch_bounds__(kBlock) void load_rows_kernel(RowsArgs a) {
+    using F = Fmt<DT>;
+    const int lane = threadIdx.x & (kWave - 1), c = lane & 7;
+    const int item = blockIdx.x * (kBlock / kWave) + threadIdx.x / kWave;
+    const int heads = 2 * a.NH;
+    const int tok = item / heads * 8 + (lane >> 3), ph = item % heads, part = ph / a.NH, h = ph % a.NH;
+    size_t row;
+    if (tok >= a.n || !row_of<true>(a, tok, part, h, row)) return;
+    const size_t dst = (((size_t)tok * 2 + part) * a.NH + h) * kHd + c * 8;
+    const uint8_t* const src = a.kv + (row * 8 + c) * F::kBytes;
+    if constexpr (F::kF32) {
+        const uint4 x = reinterpret_cast<const uint4*>(src)[0], y = reinterpret_cast<const uint4*>(src)[1];
+        uint4* const p = reinterpret_cast<uint4*>((float*)a.act + dst);
+        p[0] = x;
+        p[1] = y;
+    } else if constexpr (!F::kCoded) {
+        *reinterpret_cast<uint4*>((uint16_t*)a.act + dst) = *reinterpret_cast<const uint4*>(src);
+    } else {
+        float x[8];
+        if constexpr (F::k4) {
+            values4<DT>(*reinterpret_cast<const uint32_t*>(src), x);
+        } else {
+            const uint2 w = *reinterpret_cast<const uint2*>(src);
+            float y[16];
+            decode_codes<DT == KVATTN_KV_FP8_E4M3>(make_uint4(w.x, w.y, 0, 0), y);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] = y[i];
+        }
+        const float scale = a.scale[row];
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            w[i] = f32_to_bf16(x[2 * i] * scale) | (uint32_t)f32_to_bf16(x[2 * i + 1] * scale) << 16;
+        *reinterpret_cast<uint4*>((uint16_t*)a.act + dst) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+}
+
+int launch_rows(const void* fn, RowsArgs a, void* stream) {
+    a.shift = a.R > 0 && (a.R & (a.R - 1)) == 0 ? __builtin_ctz((unsigned)a.R) : -1;
+    const long long items = (long long)((a.n + 7) / 8) * 2 * a.NH;
+    const long long grid = (items + kBlock / kWave - 1) / (kBlock / kWave);
+    void* params[] = {&a};
+    return hip_status(hipLaunchKernel(fn, dim3((unsigned)grid), dim3(kBlock), params, 0, (hipStream_t)stream));
+}
+
+template <template <int> class K>
+const void* by_type(int dt) {
+    switch (dt) {
+        case KVATTN_KV_F32: return K<KVATTN_KV_F32>::fn();
+        case KVATTN_KV_BF16: return K<KVATTN_KV_BF16>::fn();
+        case KVATTN_KV_INT8: return K<KVATTN_KV_INT8>::fn();
+        case KVATTN_KV_FP8_E4M3: return K<KVATTN_KV_FP8_E4M3>::fn();
+        case KVATTN_KV_INT4: return K<KVATTN_KV_INT4>::fn();
+        case KVATTN_KV_FP4_E2M1: return K<KVATTN_KV_FP4_E2M1>::fn();
+        default: return nullptr;
+    }
+}
+template <int DT> struct StoreFn { static const void* fn() { return (const void*)&store_rows_kernel<DT, true>; } };
+template <int DT> struct LoadFn { static const void* fn() { return (const void*)&load_rows_kernel<DT>; } };
+
+// Checks shared by paged_store and paged_load, then the launch.
+int rows_call(const void* fn, void* act, void* pages, float* scales, int page_rows, int num_pages,
+              const long long* slots, int n, int NH, int hs, int dt, void* stream) {
+    if (hs != kHd) return KVATTN_ERR_HEAD_DIM;
+    if (n < 1 || NH < 1 || page_rows < 1 || page_rows > kMaxT || num_pages < 1) return KVATTN_ERR_SHAPE;
+    if ((long long)n * NH > (1ll << 27)) return KVATTN_ERR_SHAPE;
+    if (!fn) return KVATTN_ERR_DTYPE;
+    if (!act || !pages || !slots) return KVATTN_ERR_NULL_POINTER;
+    const bool coded = dt != KVATTN_KV_F32 && dt != KVATTN_KV_BF16;
+    if (coded && !scales) return KVATTN_ERR_DTYPE;
+    if (((uintptr_t)act & 15u) || ((uintptr_t)pages & 15u) || ((uintptr_t)slots & 7u) || ((uintptr_t)scales & 3u))
+        return KVATTN_ERR_MISALIGNED;
+    RowsArgs a{(uint8_t*)pages, scales, act, slots, nullptr, nullptr, 0, 0, page_rows, num_pages, n, NH, 0, -1};
+    return launch_rows(fn, a, stream);
+}
+
+}  // namespace
+
+namespace kvattn_internal {
+int append4(void* kv, float* scale, const void* qkv, int B, int NH, int maxT, const int* cur_len, int lens_per_seq,
+            const int* table, int max_pages, int page_rows, int num_pages, int kv_dtype, void* stream) {
+    const void* fn = kv_dtype == KVATTN_KV_INT4 ? (const void*)&store_rows_kernel<KVATTN_KV_INT4, false>
+                                                : (const void*)&store_rows_kernel<KVATTN_KV_FP4_E2M1, false>;
+    RowsArgs a{(uint8_t*)kv, scale, (void*)qkv, nullptr, cur_len, table, lens_per_seq, max_pages, page_rows, num_pages,
+               B, NH, maxT, -1};
+    return launch_rows(fn, a, stream);
+}
+}  // namespace kvattn_internal
+
+extern "C" {
+
+size_t kvattn_paged_pool_bytes(int num_pages) {
+    if (num_pages < 1 || num_pages > (1 << 28)) return 0;
+    return (size_t)(kPoolRing + num_pages) * sizeof(int);
+}
+
+int kvattn_paged_pool_init(int* pool, int num_pages, void* stream) {
+    if (num_pages < 1 || num_pages > (1 << 28)) return KVATTN_ERR_SHAPE;
+    if (!pool) return KVATTN_ERR_NULL_POINTER;
+    if ((uintptr_t)pool & 3u) return KVATTN_ERR_MISALIGNED;
+    const int most = num_pages > kPoolRing ? num_pages : kPoolRing;
+    void* params[] = {&pool, &num_pages};
+    return hip_status(hipLaunchKernel((const void*)&pool_init_kernel, dim3((most + kBlock - 1) / kBlock), dim3(kBlock),
+                                      params, 0, (hipStream_t)stream));
+}
+
+int kvattn_paged_reserve(int* block_table, int max_pages, int page_rows, int num_pages, int* pool, const int* held,
+                         const int* kept, const int* fresh, int B, int max_tokens, int* held_out, int* lens,
+                         int* token_start, long long* slot_map, int* positions, int* pool_next, void* stream) {
+    if (B < 1 || B > kMaxRequests || max_pages < 1 || page_rows < 1 || num_pages < 1 || num_pages > (1 << 28) ||
+        (long long)max_pages * page_rows > kMaxT || max_tokens < 0)
+        return KVATTN_ERR_SHAPE;
+    if (!block_table || !pool || !held || !kept || !fresh || !held_out || !lens || !token_start ||
+        (!slot_map && max_tokens > 0))
+        return KVATTN_ERR_NULL_POINTER;
+    const void* ints[] = {block_table, pool, held, kept, fresh, held_out, lens, token_start, positions, pool_next};
+    for (const void* p : ints)
+        if ((uintptr_t)p & 3u) return KVATTN_ERR_MISALIGNED;
+    if ((uintptr_t)slot_map & 7u) return KVATTN_ERR_MISALIGNED;
+    ReserveArgs a{block_table, pool, held, kept, fresh, held_out, lens, token_start, slot_map, positions, pool_next,
+                  max_pages, page_rows, num_pages, B, max_tokens};
+    const int lds = kRequestInts * B * (int)sizeof(int);
+    static_assert(kRequestInts * kMaxRequests * sizeof(int) <= 128 * 1024, "LDS of a CU");
+    if (lds > 64 * 1024) {
+        const int st = hip_status(hipFuncSetAttribute((const void*)&reserve_kernel,
+                                                      hipFuncAttributeMaxDynamicSharedMemorySize, lds));
+        if (st != KVATTN_OK) return st;
+    }
+    const long long blocks = ((long long)max_tokens + kReserveTokens - 1) / kReserveTokens;
+    const unsigned grid = (unsigned)(blocks < 1 ? 1 : blocks > kReserveMostBlocks ? kReserveMostBlocks : blocks);
+    void* params[] = {&a};
+    return hip_status(hipLaunchKernel((const void*)&reserve_kernel, dim3(grid), dim3(kBlock), params, (size_t)lds,
+                                      (hipStream_t)stream));
+}
+
+int kvattn_paged_store(void* pages, float* page_scales, int page_rows, int num_pages, const long long* slot_map,
+                       const void* qkv, int num_tokens, int NH, int hs, int kv_dtype, void* stream) {
+    return rows_call(by_type<StoreFn>(kv_dtype), (void*)qkv, pages, page_scales, page_rows, num_pages, slot_map,
+                     num_tokens, NH, hs, kv_dtype, stream);
+}
+
+int kvattn_paged_load(void* kv, const void* pages, const float* page_scales, int page_rows, int num_pages,
+                      const long long* slot_map, int num_tokens, int NH, int hs, int kv_dtype, void* stream) {
+    return rows_call(by_type<LoadFn>(kv_dtype), kv, (void*)pages, (float*)page_scales, page_rows, num_pages, slot_map,
+                     num_tokens, NH, hs, kv_dtype, stream);
+}
+
+}  // extern "C"

@@ -46,7 +46,10 @@ KV_F32 = 0
 KV_BF16 = 1
 KV_INT8 = 2
 KV_FP8_E4M3 = 3
-KV_DTYPES = {"f32": KV_F32, "bf16": KV_BF16, "int8": KV_INT8, "fp8": KV_FP8_E4M3}
+KV_INT4 = 4
+KV_FP4_E2M1 = 5
+KV_DTYPES = {"f32": KV_F32, "bf16": KV_BF16, "int8": KV_INT8, "fp8": KV_FP8_E4M3, "int4": KV_INT4,
+             "fp4": KV_FP4_E2M1}
 
 # kvattn_strategy
 AUTO = 0
@@ -70,6 +73,7 @@ HEAD_DIM = 64
 
 _vp = ctypes.c_void_p
 _i = ctypes.c_int
+_ll = ctypes.c_longlong
 _sz = ctypes.c_size_t
 
 # name -> (restype, argtypes); mirrors include/kvattn.h one to one.
@@ -105,6 +109,15 @@ SIGNATURES = {
     "kvattn_paged_cache_write": (_i, [_vp, _vp, _vp, _i, _i, _i, _vp, _i, _i, _i, _vp, _i, _i, _vp]),
     "kvattn_paged_decode": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _vp, _i, _i, _vp, _sz, _i, _i,
                                  _i, _i, _vp]),
+    "kvattn_paged_decode_tokens": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _i, _i, _vp, _vp, _i, _i, _i, _i, _i, _vp, _sz,
+                                        _i, _i, _vp]),
+    "kvattn_paged_pool_bytes": (_sz, [_i]),
+    "kvattn_paged_pool_init": (_i, [_vp, _i, _vp]),
+    "kvattn_paged_reserve": (_i, [_vp, _i, _i, _i, _vp, _vp, _vp, _vp, _i, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "kvattn_paged_store": (_i, [_vp, _vp, _i, _i, _vp, _vp, _i, _i, _i, _i, _vp]),
+    "kvattn_paged_load": (_i, [_vp, _vp, _vp, _i, _i, _vp, _i, _i, _i, _i, _vp]),
+    "kvattn_verify_workspace_bytes": (_sz, [_i, _i]),
+    "kvattn_verify_drafts": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _ll, _i, _vp, _sz, _vp]),
 }
 
 
@@ -374,8 +387,9 @@ def gemv_qkv_append_workspace_bytes(B: int, NH: int) -> int:
 
 
 class PagedCache:
-    """A paged KV cache: a page pool [num_pages][2][NH][page_rows][hs] (+ row scales for
-    8-bit caches) and a block table [B][max_pages] of page ids (device tensors)."""
+    """A paged KV cache: a page pool [num_pages][2][NH][page_rows][hs] (hs / 2 bytes a row for 4-bit
+    caches; + row scales for 8-bit and 4-bit caches) and a block table [B][max_pages] of page ids
+    (device tensors)."""
 
     def __init__(self, pages, block_table, max_pages, page_rows, num_pages, page_scales=None):
         self.pages, self.block_table, self.page_scales = pages, block_table, page_scales
@@ -408,6 +422,69 @@ def paged_decode(out, qkv, cache: PagedCache, B, NH, hs, *, kv_dtype, cur_len=No
                                      int(workspace_nbytes), int(S), strategy_code(strategy),
                                      kv_dtype_code(kv_dtype), int(bool(append)), _stream(stream)),
            "kvattn_paged_decode")
+
+
+def paged_decode_tokens(out, qkv, cache: PagedCache, token_start, lens, B, num_tokens, NH, hs, *, kv_dtype, max_new,
+                        workspace=None, workspace_nbytes=0, S=0, stream=None) -> None:
+    """Attention of several new tokens of every sequence over a paged 4-bit cache that holds their rows
+    (kvattn_paged_decode_tokens); the workspace is that of num_tokens sequences."""
+    _check(lib().kvattn_paged_decode_tokens(_ptr(out), _ptr(qkv), _ptr(cache.pages), _ptr(cache.page_scales),
+                                            _ptr(cache.block_table), cache.max_pages, cache.page_rows, cache.num_pages,
+                                            _ptr(token_start), _ptr(lens), B, num_tokens, int(max_new), NH, hs,
+                                            _ptr(workspace), int(workspace_nbytes), int(S), kv_dtype_code(kv_dtype),
+                                            _stream(stream)), "kvattn_paged_decode_tokens")
+
+
+def paged_pool(num_pages, device="cuda", stream=None):
+    """A pool of free pages for paged_reserve: int32 [4 + num_pages], every page free."""
+    import torch
+    nbytes = int(lib().kvattn_paged_pool_bytes(int(num_pages)))
+    if nbytes == 0:
+        raise KvAttnError(ERR_SHAPE, "kvattn_paged_pool_bytes")
+    pool = torch.empty(nbytes // 4, dtype=torch.int32, device=device)
+    _check(lib().kvattn_paged_pool_init(_ptr(pool), int(num_pages), _stream(stream)), "kvattn_paged_pool_init")
+    return pool
+
+
+def paged_reserve(cache: PagedCache, pool, held, kept, fresh, B, *, lens, token_start, slot_map, max_tokens,
+                  held_out=None, positions=None, pool_next=None, stream=None) -> None:
+    """Pages, token offsets, slot map and positions of a step from what every request holds, keeps and
+    adds (kvattn_paged_reserve).  held_out None: held is updated in place."""
+    _check(lib().kvattn_paged_reserve(_ptr(cache.block_table), cache.max_pages, cache.page_rows, cache.num_pages,
+                                      _ptr(pool), _ptr(held), _ptr(kept), _ptr(fresh), B, int(max_tokens),
+                                      _ptr(held if held_out is None else held_out), _ptr(lens), _ptr(token_start),
+                                      _ptr(slot_map), _ptr(positions), _ptr(pool_next), _stream(stream)),
+           "kvattn_paged_reserve")
+
+
+def paged_store(cache: PagedCache, qkv, slot_map, num_tokens, NH, hs, *, kv_dtype, stream=None) -> None:
+    """K and V of a batch of tokens into the pool by slot (kvattn_paged_store)."""
+    _check(lib().kvattn_paged_store(_ptr(cache.pages), _ptr(cache.page_scales), cache.page_rows, cache.num_pages,
+                                    _ptr(slot_map), _ptr(qkv), num_tokens, NH, hs, kv_dtype_code(kv_dtype),
+                                    _stream(stream)), "kvattn_paged_store")
+
+
+def paged_load(kv, cache: PagedCache, slot_map, num_tokens, NH, hs, *, kv_dtype, stream=None) -> None:
+    """Rows of the pool by slot into kv [num_tokens][2][NH][hs] (kvattn_paged_load)."""
+    _check(lib().kvattn_paged_load(_ptr(kv), _ptr(cache.pages), _ptr(cache.page_scales), cache.page_rows,
+                                   cache.num_pages, _ptr(slot_map), num_tokens, NH, hs, kv_dtype_code(kv_dtype),
+                                   _stream(stream)), "kvattn_paged_load")
+
+
+def verify_workspace_bytes(B, V) -> int:
+    """Workspace bytes of verify_drafts, to be zeroed once with workspace_init."""
+    return int(lib().kvattn_verify_workspace_bytes(B, V))
+
+
+def verify_drafts(tokens, counts, target_probs, draft_tokens, uniform, token_start, B, num_tokens, V, *,
+                  draft_probs=None, row_stride=None, dtype="f32", workspace=None, workspace_nbytes=0,
+                  stream=None) -> None:
+    """Accepts drafted tokens against the target's probabilities and draws the next one
+    (kvattn_verify_drafts).  draft_probs None: drafts without probabilities."""
+    _check(lib().kvattn_verify_drafts(_ptr(tokens), _ptr(counts), _ptr(target_probs), _ptr(draft_probs),
+                                      _ptr(draft_tokens), _ptr(uniform), _ptr(token_start), B, num_tokens, V,
+                                      V if row_stride is None else int(row_stride), kv_dtype_code(dtype),
+                                      _ptr(workspace), int(workspace_nbytes), _stream(stream)), "kvattn_verify_drafts")
 
 
 class Workspace:

@@ -64,7 +64,15 @@ typedef enum kvattn_dtype {
     KVATTN_KV_F32 = 0,       /* reference ENABLE_FP32 build (Makefile:78-79) */
     KVATTN_KV_BF16 = 1,      /* reference default BF16 build (Makefile:88-89) */
     KVATTN_KV_INT8 = 2,      /* reference USE_KV_W8 + USE_INT8 (Makefile:80-82,100-106) */
-    KVATTN_KV_FP8_E4M3 = 3   /* reference USE_KV_W8 + USE_FP8 (Makefile:83-85,100-106) */
+    KVATTN_KV_FP8_E4M3 = 3,  /* reference USE_KV_W8 + USE_FP8 (Makefile:83-85,100-106) */
+    /* 4-bit caches: 32 bytes a row, channel 2i in the low half of byte i and 2i+1 in the high
+     * half, one float scale a row (1/7 and 1/6 rounded to float); qkv and out are bf16.  No reference counterpart (its cache
+     * types end at 8 bits).  Taken by kvattn_cache_write, kvattn_append, kvattn_decode,
+     * kvattn_append_decode, kvattn_plan and the kvattn_paged_* calls; the others return
+     * KVATTN_ERR_DTYPE. */
+    KVATTN_KV_INT4 = 4,      /* scale = amax * (1/7); the half byte holds round(x / scale) + 8 */
+    KVATTN_KV_FP4_E2M1 = 5   /* scale = amax * (1/6); sign and one of 0 .5 1 1.5 2 3 4 6,
+                                to nearest, ties to the even code */
 } kvattn_dtype;
 
 typedef enum kvattn_strategy {
@@ -372,6 +380,100 @@ int kvattn_paged_decode(void* out, const void* qkv, void* pages, float* page_sca
                         const int* d_cur_len, int lens_per_seq, int len_hint,
                         void* workspace, size_t workspace_bytes,
                         int S, int strategy, int kv_dtype, int append, void* stream);
+
+/* Attention of several new tokens of every sequence over a paged 4-bit cache (kv_dtype INT4 or
+ * FP4_E2M1; other types: KVATTN_ERR_DTYPE), as verifying drafted tokens needs it: the new rows
+ * are in the cache already (kvattn_paged_store), and each token attends the positions up to its
+ * own.  The cache is read once for eight tokens of a sequence.
+ *   token_start [B+1] device: sequence b's tokens are rows token_start[b] .. token_start[b+1]-1 of
+ *               qkv [num_tokens][3][NH][hs] (only Q is read) and out [num_tokens][NH][hs]; their
+ *               number may be 0
+ *   lens        [B] device: positions of sequence b, its new tokens among them; token i of n
+ *               attends the first lens[b] - n + i + 1 of them (none: its output is zero)
+ *   max_new     the most tokens of one sequence; with more, those beyond the next multiple of 8
+ *               are left out
+ * Rows of out behind token_start[B] are left as they were.  Values of token_start and lens are
+ * clamped into [0, num_tokens] and [0, max_pages * page_rows].  Workspace:
+ * kvattn_workspace_bytes(num_tokens, NH, hs, max_pages * page_rows, S); S as in kvattn_decode with
+ * a 4-bit cache.
+ * No reference counterpart (the reference decodes one token at a time). */
+int kvattn_paged_decode_tokens(void* out, const void* qkv, const void* pages, const float* page_scales,
+                               const int* block_table, int max_pages, int page_rows, int num_pages,
+                               const int* token_start, const int* lens, int B, int num_tokens, int max_new,
+                               int NH, int hs, void* workspace, size_t workspace_bytes, int S, int kv_dtype,
+                               void* stream);
+
+/* ---- Pages from request lengths --------------------------------------------------------
+ * The bookkeeping of a paged cache, on the device: no length, table or page count goes through the
+ * host, so a captured step allocates too.  No reference counterpart (the reference has one
+ * contiguous cache).
+ *   pool  int32 [4 + num_pages]: {index of the first free page in the ring, number of free pages, a
+ *         word of the library's, unused}, then the ring of free page ids.
+ *         kvattn_paged_pool_bytes bytes; kvattn_paged_pool_init makes every page free. */
+size_t kvattn_paged_pool_bytes(int num_pages);
+int kvattn_paged_pool_init(int* pool, int num_pages, void* stream);
+
+/* Gives every request the pages of its next step.  Request b holds pages for held[b] positions
+ * (those of block_table row b), keeps the first kept[b] of them (fewer after refused drafts, 0 when
+ * it has ended) and adds fresh[b] tokens:
+ *   pages    ceil((kept + fresh) / page_rows) - ceil(held / page_rows) pages are taken from the
+ *            ring, in request order, and entered behind the ones held; if negative, the last pages
+ *            go back to the ring in the same order (to be taken by later calls).  Entries of
+ *            block_table behind a request's pages are left as they were.
+ *   held_out [B], lens [B]: kept + fresh.  Either may be its input (held, kept).
+ *   token_start [B+1]: sums of fresh; tokens token_start[b] .. token_start[b+1]-1 are request b's
+ *   slot_map [max_tokens]: page * page_rows + row of each token's position, for kvattn_paged_store
+ *   positions [max_tokens] (may be NULL): each token's position
+ *            Entries behind the last token are left as they were.
+ *   pool_next [2] (may be NULL: the pool itself): the pool's first two words after the call.  With
+ *            a buffer of its own the pool's words stay, so the call can be made again.
+ * A request is refused, and keeps its pages and kept[b] positions (held_out = held, lens = kept), when
+ * it needs pages and those up to its own in request order are more than the free ones, or its tokens
+ * end behind max_tokens; its tokens then have slot -1.  So is one whose lengths are not
+ * 0 <= kept <= held, 0 <= fresh, kept + fresh <= max_pages * page_rows; it counts as having no
+ * tokens.  Table entries outside [0, num_pages) give slot -1 and go back to the ring as they are.
+ * B <= 4096.  Calls on one pool must be ordered. */
+int kvattn_paged_reserve(int* block_table, int max_pages, int page_rows, int num_pages, int* pool,
+                         const int* held, const int* kept, const int* fresh, int B, int max_tokens,
+                         int* held_out, int* lens, int* token_start, long long* slot_map, int* positions,
+                         int* pool_next, void* stream);
+
+/* K and V rows of num_tokens tokens, from qkv [num_tokens][3][NH][hs], into the pool at slots
+ * slot_map[t] = page * page_rows + row, for every kv_dtype, as kvattn_paged_cache_write writes a
+ * row.  Slots outside [0, num_pages * page_rows) are skipped; the others must differ from one
+ * another. */
+int kvattn_paged_store(void* pages, float* page_scales, int page_rows, int num_pages, const long long* slot_map,
+                       const void* qkv, int num_tokens, int NH, int hs, int kv_dtype, void* stream);
+
+/* The rows at slot_map[t] out of the pool into kv [num_tokens][2][NH][hs] (K, then V), in the
+ * activation type (float for F32, else bf16): code * scale, rounded once.  Rows of skipped slots are
+ * left as they were.  As prefill attention over earlier positions reads them. */
+int kvattn_paged_load(void* kv, const void* pages, const float* page_scales, int page_rows, int num_pages,
+                      const long long* slot_map, int num_tokens, int NH, int hs, int kv_dtype, void* stream);
+
+/* ---- Verification of drafted tokens ----------------------------------------------------
+ * Row t = token_start[b] + i holds the target's distribution behind token i of sequence b's n
+ * tokens; draft_tokens[t] is the draft that followed it, drawn from draft_probs row t (the last row
+ * has none: its draft_tokens entry and its draft_probs row are not read).  With uniform[t] in [0, 1):
+ *   drafts are accepted in order while uniform[t] * q(x) < p(x);
+ *   at the first that is not, the next token is drawn from max(0, p - q) of its row, or where that
+ *   is zero everywhere from its p; if all are accepted, from the last row's p.  A draw is the
+ *   lowest token whose running sum passes uniform[last row] times the total, in 64 bits.
+ * tokens [num_tokens]: accepted drafts, the drawn token, -1 behind it; counts [B]: accepted plus
+ * drawn.  A row without any mass draws nothing (counts: accepted alone).  A sequence without tokens
+ * has count 0; rows behind token_start[B] are left as they were.
+ *   target_probs, draft_probs  [num_tokens] rows of V probabilities, row_stride elements apart, float
+ *               (dtype KVATTN_KV_F32) or bf16 (KVATTN_KV_BF16); NaN, infinite and negative ones weigh
+ *               nothing in a draw.  draft_probs NULL: drafts without probabilities (q = 1 at the draft)
+ *   draft_tokens  ids outside [0, V) are refused
+ *   workspace   kvattn_verify_workspace_bytes(B, V) bytes, 256-byte aligned, zeroed once
+ *               (kvattn_workspace_init).  Calls sharing a workspace must be ordered.
+ * No reference counterpart (the reference samples one token at a time on the host). */
+size_t kvattn_verify_workspace_bytes(int B, int V);
+int kvattn_verify_drafts(int* tokens, int* counts, const void* target_probs, const void* draft_probs,
+                         const int* draft_tokens, const float* uniform, const int* token_start, int B,
+                         int num_tokens, int V, long long row_stride, int dtype, void* workspace,
+                         size_t workspace_bytes, void* stream);
 
 /* The decode step's fully connected layer, used after the attention for the output
  * projection: for b < B, m < M
