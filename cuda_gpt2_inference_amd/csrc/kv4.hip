@@ -1,21 +1,23 @@
 // kv4.hip -- decode attention over a 4-bit KV cache on MI355X (gfx950), for one or several new
 // tokens of every sequence.
 //
-// A row costs 36 bytes, so at the memory's rate the vector units have about 3.4 instructions for
-// each element; the products go to the matrix cores, which leaves the vector units the codes'
-// conversion (FP4: one instruction for two values) and the softmax.  A wave walks tiles of 64
-// positions with an online softmax:
-//   S^T[key][query]  = K Q^T   v_mfma_f32_16x16x32_bf16, codes exact in bf16, q as it is stored
-//   O^T[chan][query] = V^T P^T the same; P^T's operand is S^T's result where it lies: lane
-//                              16 g + n holds query n at keys 16 t + 4 g + i, and a sum over keys
-//                              may take them in any order as long as V's operand does
-// V comes row-major and is needed channel-major: tiles pass through the wave's own LDS, and
-// ds_read_b64_tr_b4 hands lane 16 g + c channel c of the 16 rows that group g names.
+// A row costs 36 bytes, so at the memory's rate a wave has about 27 cycles for each: the products go
+// to the matrix cores (16x16x32 bf16: codes and q are exact there, sums are float), which leaves the
+// vector units the codes' conversion and the softmax.  A wave walks tiles of 64 positions with an
+// online softmax.
+//   Scores.  The 16 rows of the left operand are 1, 4 or 8 queries, repeated; the columns 16 positions.
+//   Of a result, lane 16 g + n holds rows 4 g .. 4 g + 3 of column n, so it takes from the results of
+//   the tile's four groups of positions those that no other lane takes for the same query: one
+//   position and up to four queries a lane, or two positions and four of eight.  (With queries as columns,
+//   one query's softmax was done 16 times over, and that bound the call.)
+//   Outputs.  O^T[channel][column] = V^T P^T.  A column is one query's weights in bf16, once their
+//   upper half and once the rest (a weight is the sum of the two to 2^-14; one bf16 would round a
+//   sharp head's output by 2^-9 before the output's own rounding).  Weights go from positions in lanes
+//   to the operand's layout through LDS, and V, which is needed channel-major, through
+//   ds_read_b64_tr_b4: lane 16 g + c receives channel c of the 16 rows that group g names.
 //
-// Eight queries share a call to the matrix cores (the drafted tokens of a sequence read the cache
-// once).  Each takes two of the 16 columns: a weight p = hi + lo in two bf16 halves, hi in column n
-// and lo in column n + 8, so weights keep 14 bits or more where one bf16 would round a sharp head's
-// output by 2^-9 before the output's own rounding.  Scores, maxima, sums and outputs are float.
+// The FP8-rate matrix instructions would take FP4 codes as they are, but cut small products against
+// large ones (2^-14 of the sum of magnitudes, measured), which a score cannot afford.
 //
 // Waves of a workgroup take the tiles of a segment in turn and join through LDS; segments of a
 // head join in the workgroup that finishes last (one launch).
@@ -41,13 +43,14 @@ typedef float F32x4 __attribute__((ext_vector_type(4)));
 constexpr int kHd = 64;
 constexpr int kTile = 64;                  // positions of a tile
 constexpr int kRowBytes = 32;
-constexpr int kGroup = 8;                  // queries of a workgroup
 constexpr int kTileBytes = kTile * kRowBytes;
-constexpr int kWaveLds = 2 * kTileBytes + 2 * kTile * 4;   // K, V, their scales
+constexpr int kWaveLds = 2 * kTileBytes;   // K (then the weights), V
 constexpr float kQScale = 0.125f * 1.4426950408889634f;    // 1/sqrt(64) * log2(e)
+constexpr float kSlack = 8.0f;
 constexpr int kMaxT = 1 << 23;
-constexpr int kMaxSegments = 1 << 16;
-constexpr int kMostBlocks = 1 << 16;       // AUTO's segments stay longer beyond that many workgroups
+constexpr int kMaxSegments = 65535;        // the grid's third side
+constexpr int kWaves = 4;                  // waves of a workgroup
+constexpr int kFullGrid = 1024;            // workgroups that the GPU runs at once: four a CU
 
 struct Args {
     const uint8_t* kv;
@@ -66,32 +69,43 @@ struct Args {
     int max_pages, num_pages, lens_per_seq, NH, maxT, groups, S, seg_tiles, num_tokens;
 };
 
-// A tile on its way: 16-byte chunks lane and lane + 64 of K and V, row lane's scales.
+// A tile on its way: 16-byte chunks lane and lane + 64 of K and V, and the scales of the kC positions
+// that the lane's scores are of (key0 and 32 on).
+template <int kC>
 struct Raw {
     uint4 k[2], v[2];
-    float ks, vs;
+    float ks[kC], vs[kC];
+    bool there;            // its page is in the pool
 };
 
-__device__ __forceinline__ Raw load_tile(const Args& a, size_t row0, int last, int lane) {
-    Raw r;
-    const size_t v0 = row0 + a.v_rows;
+constexpr size_t kNoPage = ~(size_t)0;
+
+template <int kC>
+__device__ __forceinline__ Raw<kC> load_tile(const Args& a, size_t row0, int last, int lane, int key0) {
+    Raw<kC> r;
+    const uint8_t* const k = a.kv + row0 * kRowBytes;
+    const uint8_t* const v = k + a.v_rows * kRowBytes;
+    const float* const s = a.sc + row0;
     // Rows past the last attended one are not read: their lanes read that one again, so that what
     // an unwritten row holds never matters and the end of a page or slot is never passed.
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
         const uint32_t at = (uint32_t)min((lane >> 1) + 32 * j, last) * kRowBytes + (lane & 1) * 16;
-        r.k[j] = load16<false>(a.kv + row0 * kRowBytes + at);
-        r.v[j] = load16<false>(a.kv + v0 * kRowBytes + at);
+        r.k[j] = load16<false>(k + at);
+        r.v[j] = load16<false>(v + at);
     }
-    const int row = min(lane, last);
-    r.ks = a.sc[row0 + row];
-    r.vs = a.sc[v0 + row];
+#pragma unroll
+    for (int j = 0; j < kC; ++j) {
+        const uint32_t row = min(key0 + 32 * j, last);
+        r.ks[j] = s[row];
+        r.vs[j] = (s + a.v_rows)[row];
+    }
     return r;
 }
 
-// Eight 4-bit codes as a matrix-core operand.  FP4: the values, in order (pairs 0 1, 2 3, ...).
-// INT4: 24 + code (16 + nibble: the nibble's bits at the top of the mantissa of 16.0), in pairs
-// 0 4, 1 5, 2 6, 3 7, which takes two instructions for two values; the callers take the 24 off.
+// Eight 4-bit codes as a matrix-core operand.  FP4: the values, in order.  INT4: 8 + code, which the
+// callers take off again: a half byte alone in a byte is an E4M3 number 2^-9 times it, and one
+// instruction makes bf16 of two; in the order 0 2 4 6 1 3 5 7.
 template <bool kFp4>
 __device__ __forceinline__ Bf16x8 operand(uint32_t w) {
     U32x4 d;
@@ -101,35 +115,34 @@ __device__ __forceinline__ Bf16x8 operand(uint32_t w) {
         d[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, 1.0f, 2));
         d[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, 1.0f, 3));
     } else {
-        constexpr uint32_t kMask = 0x00780078u, kBase = 0x41804180u;
-        d[0] = ((w << 3) & kMask) | kBase;
-        d[1] = ((w >> 1) & kMask) | kBase;
-        d[2] = ((w >> 5) & kMask) | kBase;
-        d[3] = ((w >> 9) & kMask) | kBase;
+        const uint32_t even = w & 0x0F0F0F0Fu, odd = (w >> 4) & 0x0F0F0F0Fu;
+        d[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(even, 512.0f, false));
+        d[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(even, 512.0f, true));
+        d[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(odd, 512.0f, false));
+        d[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(odd, 512.0f, true));
     }
     return __builtin_bit_cast(Bf16x8, d);
 }
+
+// The place of code r of eight in operand().
+template <bool kFp4>
+__device__ __forceinline__ int place(int r) { return kFp4 ? r : ((r & 1) << 2) + (r >> 1); }
 
 // Eight bf16 values in the order of operand()'s.
 template <bool kFp4>
 __device__ __forceinline__ Bf16x8 in_order(const uint4& w) {
     U32x4 d = {w.x, w.y, w.z, w.w};
     if constexpr (!kFp4) {
-        d[0] = (w.x & 0xffffu) | (w.z << 16);
-        d[1] = (w.x >> 16) | (w.z & 0xffff0000u);
-        d[2] = (w.y & 0xffffu) | (w.w << 16);
-        d[3] = (w.y >> 16) | (w.w & 0xffff0000u);
+        d[0] = (w.x & 0xffffu) | (w.y << 16);
+        d[1] = (w.z & 0xffffu) | (w.w << 16);
+        d[2] = (w.x >> 16) | (w.y & 0xffff0000u);
+        d[3] = (w.z >> 16) | (w.w & 0xffff0000u);
     }
     return __builtin_bit_cast(Bf16x8, d);
 }
 
 __device__ __forceinline__ F32x4 mfma(Bf16x8 a, Bf16x8 b, F32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
-}
-
-// The upper halves of two floats: both cut to bf16.
-__device__ __forceinline__ uint32_t pack_hi(float lo, float hi) {
-    return __builtin_amdgcn_perm(__float_as_uint(hi), __float_as_uint(lo), 0x07060302u);
 }
 
 __device__ __forceinline__ void put(float* p, float v) {
@@ -142,19 +155,21 @@ __device__ __forceinline__ float get(const float* p) {
 // exp2(m - M) with an empty side (m = -inf) weighing nothing.
 __device__ __forceinline__ float weight_of(float m, float M) { return m == -INFINITY ? 0.0f : exp2_fast(m - M); }
 
-template <bool kFp4, int kW>
-__global__ __launch_bounds__(kW * kWave) void attend4_kernel(Args a) {
-    __shared__ __align__(16) uint8_t lds[kW * kWaveLds];
-    __shared__ float red_m[kW][kGroup], red_l[kW][kGroup];
-    __shared__ int is_last;
-    static_assert(kGroup * kHd * 4 <= kWaveLds, "a wave's outputs take its tile's place");
+// The wave's LDS operations run in order, so what its lanes hand one another there needs no barrier;
+// this keeps the compiler from moving one lane's reads over another's writes.
+__device__ __forceinline__ void lds_order() { asm volatile("" ::: "memory"); }
 
-    int x = blockIdx.x;
-    const int s = x % a.S;
-    x /= a.S;
-    const int h = x % a.NH;
-    x /= a.NH;
-    const int grp = x % a.groups, b = x / a.groups;
+// kQ: queries of a workgroup (1, 4 or 8); kW: its waves.
+template <bool kFp4, int kQ, int kW>
+__global__ __launch_bounds__(kW * kWave) __attribute__((amdgpu_waves_per_eu(4))) void attend4_kernel(Args a) {
+    __shared__ __align__(16) uint8_t lds[kW * kWaveLds];
+    __shared__ float red_m[kW][kQ], red_l[kW][kQ];
+    __shared__ int is_last;
+    static_assert(kQ * kHd * 4 <= kWaveLds && kQ * 2 * kTile * 2 <= kTileBytes, "outputs and weights take a tile's place");
+    // A lane scores kC positions of a tile for kS of the queries.
+    constexpr int kC = kQ <= 4 ? 1 : 2, kS = kQ == 1 ? 1 : 4;
+
+    const int b = blockIdx.x, grp = a.groups == 1 ? 0 : blockIdx.y / a.NH, h = blockIdx.y - grp * a.NH, s = blockIdx.z;
     int t0, n, total;
     if (a.start) {
         t0 = min(max(a.start[b], 0), a.num_tokens);
@@ -165,9 +180,9 @@ __global__ __launch_bounds__(kW * kWave) void attend4_kernel(Args a) {
         n = 1;
         total = min(max(a.lens[a.lens_per_seq ? b : 0], 0), a.maxT - 1) + 1;
     }
-    const int q0 = grp * kGroup;
+    const int q0 = grp * kQ;
     if (q0 >= n) return;
-    const int nq = min(kGroup, n - q0);
+    const int nq = min(kQ, n - q0);
     // Query i of the group attends the first seen0 + i rows.
     const int seen0 = total - n + q0 + 1;
     const int rows = max(seen0 + nq - 1, 0);
@@ -179,164 +194,212 @@ __global__ __launch_bounds__(kW * kWave) void attend4_kernel(Args a) {
 
     const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int col = lane & 15, g = lane >> 4;
-    const int qi = min(col & (kGroup - 1), nq - 1);       // columns past the last query repeat it
-    const uint4* qp = reinterpret_cast<const uint4*>(a.qkv + ((size_t)(t0 + q0 + qi) * 3 * a.NH + h) * kHd + 16 * g);
-    const uint4 q_lo = qp[0], q_hi = qp[1];
+    const int key0 = 16 * (g / kC) + col, my_q = 4 * (g % kC);   // the first position and query a lane scores
+    const int mine = (end - first - wave + kW - 1) / kW;    // tiles of this wave: first + wave + k kW
+
+    // The first rows of this wave's tiles, one a lane, 64 tiles ahead; all ones: no such page.
+    size_t starts = 0;
+    auto load_starts = [&](int k0) {
+        const int pos = (first + wave + (k0 + lane) * kW) * kTile;
+        long long id = b;
+        int in_page = pos;
+        if (a.table) {
+            id = -1;
+            if (k0 + lane < mine) {
+                const int page = div_uniform(pos, a.R);
+                in_page = pos - page * a.R;
+                id = a.table[(size_t)b * a.max_pages + page];
+            }
+            if (id >= a.num_pages) id = -1;
+        }
+        starts = id < 0 ? kNoPage : (size_t)(id * a.id_mul + h) * a.R + in_page;
+    };
+    auto start_of = [&](int k) {
+        const int lo = __builtin_amdgcn_readlane((int)starts, k & (kWave - 1));
+        const int hi = __builtin_amdgcn_readlane((int)(starts >> 32), k & (kWave - 1));
+        return ((size_t)(unsigned)hi << 32) | (unsigned)lo;
+    };
+    // The tile on its way.  (Two or three on their way, in registers, were 3 to 15 % slower.)
+    Raw<kC> raw;
+    auto request = [&](int k) {
+        if (k >= mine) return;
+        if ((k & (kWave - 1)) == 0) load_starts(k);
+        const int pos = (first + wave + k * kW) * kTile;
+        const size_t row0 = start_of(k);
+        raw = load_tile<kC>(a, row0 == kNoPage ? 0 : row0, min(kTile, rows - pos) - 1, lane, key0);
+        raw.there = row0 != kNoPage;
+    };
+    request(0);
+
+    // The left operand: row i is query i % kQ (the last one again past it).
+    Bf16x8 qa[2];
+    {
+        const int qi = min(col % kQ, nq - 1);
+        const uint4* qp = reinterpret_cast<const uint4*>(a.qkv + ((size_t)(t0 + q0 + qi) * 3 * a.NH + h) * kHd + 16 * g);
+        qa[0] = in_order<kFp4>(qp[0]);
+        qa[1] = in_order<kFp4>(qp[1]);
+    }
+    // INT4: the operand's codes are 8 too large, so every score starts at -8 times the sum of q.
+    const Bf16x8 minus8 = (Bf16x8)(__bf16)(-8.0f);
+    F32x4 s_init = {0.0f, 0.0f, 0.0f, 0.0f};
+    if constexpr (!kFp4) s_init = mfma(qa[1], minus8, mfma(qa[0], minus8, s_init));
 
     uint8_t* const lk = lds + wave * kWaveLds;
     uint8_t* const lv = lk + kTileBytes;
-    float* const lks = reinterpret_cast<float*>(lk + 2 * kTileBytes);
-    float* const lvs = lks + kTile;
-
-    // Pages of this wave's tiles, one a lane, 64 tiles ahead.
-    int ids = 0;
-    auto load_ids = [&](int k0) {
-        const int tile = first + wave + (k0 + lane) * kW;
-        ids = b;
-        if (a.table) {
-            ids = -1;
-            if (tile < end) ids = a.table[(size_t)b * a.max_pages + tile * kTile / a.R];
-            if (ids >= a.num_pages) ids = -1;
-        }
-    };
-    auto start_tile = [&](int k) {
-        const int tile = first + wave + k * kW;
-        const int id = max(__builtin_amdgcn_readlane(ids, k & (kWave - 1)), 0);
-        const int pos = tile * kTile;
-        const size_t row0 = (size_t)((long long)id * a.id_mul + h) * a.R + (a.table ? pos % a.R : pos);
-        return load_tile(a, row0, min(kTile, rows - pos) - 1, lane);
-    };
-    const int mine = (end - first - wave + kW - 1) / kW;    // tiles of this wave
-    Raw next;
-    if (mine > 0) {
-        load_ids(0);
-        next = start_tile(0);
-    }
-    const Bf16x8 qa = in_order<kFp4>(q_lo), qb = in_order<kFp4>(q_hi);
-    // INT4: every product is 24 q too large.
-    F32x4 s_init = {0.0f, 0.0f, 0.0f, 0.0f};
-    if constexpr (!kFp4) {
-        float sum = 0.0f;
-        const uint32_t w[8] = {q_lo.x, q_lo.y, q_lo.z, q_lo.w, q_hi.x, q_hi.y, q_hi.z, q_hi.w};
+    // Weights [query][upper, rest][place of a position]: with two positions a lane, those are neighbours.
+    uint16_t* const lp = reinterpret_cast<uint16_t*>(lk);
+    F32x4 acc[4] = {};                     // channels 16 c + 4 g + i of column col: query col % kQ
+    float m[kS], l[kS];                    // m: what the exponents are taken off, alike in a query's lanes
 #pragma unroll
-        for (int i = 0; i < 8; ++i) sum += bf16_lo(w[i]) + bf16_hi(w[i]);
-        sum = op_xor32<false>(op_xor16<false>(sum));
-        s_init = -24.0f * sum;
+    for (int i = 0; i < kS; ++i) {
+        m[i] = -INFINITY;
+        l[i] = 0.0f;
     }
-    const Bf16x8 minus24 = (Bf16x8)(__bf16)(-24.0f);
-
-    F32x4 acc[4] = {};                     // channels 16 c + 4 g + i of query col
-    float m = -INFINITY, l = 0.0f;         // l: this lane's keys alone
-    const uint32_t lo_mask = col >= kGroup ? 0xffff0000u : 0u;
-    const int tr_row = 16 * (col >> 2) + 4 * g + (col & 3);
+    // Column col's weights: query col % kQ, part col / kQ (further columns repeat these).
+    const int p_at = ((col & (kQ - 1)) * 2 + ((col / kQ) & 1)) * kTile + 8 * g;
+    // The row that this lane names to the transposing read: place 32 (col / 8) + 8 g + place(col % 8).
+    const int tr_place = 32 * (col >> 3) + 8 * g + place<kFp4>(col & 7);
+    const int tr_row = kC == 1 ? tr_place : (tr_place >> 1) + 32 * (tr_place & 1);
 
     for (int k = 0; k < mine; ++k) {
-        const Raw t = next;
         const int pos = (first + wave + k * kW) * kTile;
-        const bool there = __builtin_amdgcn_readlane(ids, k & (kWave - 1)) >= 0;
-        // The wave's LDS operations run in order, so a tile needs no barrier; the compiler is kept
-        // from moving one lane's reads over another's writes.
-        asm volatile("" ::: "memory");
+        const bool there = raw.there;
+        float ks[kC], vs[kC];
+#pragma unroll
+        for (int j = 0; j < kC; ++j) {
+            ks[j] = raw.ks[j] * kQScale;
+            vs[j] = raw.vs[j];
+        }
+        lds_order();
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-            reinterpret_cast<uint4*>(lk)[lane + 64 * j] = t.k[j];
-            reinterpret_cast<uint4*>(lv)[lane + 64 * j] = t.v[j];
+            reinterpret_cast<uint4*>(lk)[lane + 64 * j] = raw.k[j];
+            reinterpret_cast<uint4*>(lv)[lane + 64 * j] = raw.v[j];
         }
-        lks[lane] = t.ks * kQScale;
-        lvs[lane] = t.vs;
-        asm volatile("" ::: "memory");
-        if (k + 1 < mine) {
-            if (((k + 1) & (kWave - 1)) == 0) load_ids(k + 1);
-            next = start_tile(k + 1);
-        }
+        lds_order();
+        request(k + 1);
 
-        float sc[16];
+        uint2 kw[4];
 #pragma unroll
-        for (int tt = 0; tt < 4; ++tt) {
-            const uint2 kw = *reinterpret_cast<const uint2*>(lk + (16 * tt + col) * kRowBytes + 8 * g);
-            F32x4 d = mfma(operand<kFp4>(kw.x), qa, s_init);
-            d = mfma(operand<kFp4>(kw.y), qb, d);
-            const F32x4 ks = *reinterpret_cast<const F32x4*>(lks + 16 * tt + 4 * g);
+        for (int t = 0; t < 4; ++t) kw[t] = *reinterpret_cast<const uint2*>(lk + (16 * t + col) * kRowBytes + 8 * g);
+        I32x2 vw[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) sc[4 * tt + i] = d[i] * ks[i];
+        for (int c = 0; c < 4; ++c)
+            vw[c] = __builtin_amdgcn_ds_read_tr4_b64_v2i32(
+                (__attribute__((address_space(3))) I32x2*)(lv + tr_row * kRowBytes + 8 * c));
+        lds_order();
+        F32x4 d[4];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+            d[t] = mfma(qa[0], operand<kFp4>(kw[t].x), s_init);
+            d[t] = mfma(qa[1], operand<kFp4>(kw[t].y), d[t]);
+        }
+        // This lane's: group of positions g, or g / 2 and g / 2 + 2.
+        float own[kC][kS];
+#pragma unroll
+        for (int i = 0; i < kS; ++i) {
+            if constexpr (kC == 1) {
+                const float even = (g & 2) ? d[2][i] : d[0][i], odd = (g & 2) ? d[3][i] : d[1][i];
+                own[0][i] = (g & 1) ? odd : even;
+            } else {
+                own[0][i] = (g & 2) ? d[1][i] : d[0][i];
+                own[1][i] = (g & 2) ? d[3][i] : d[2][i];
+            }
         }
         // Rows that a query does not see: its later drafts, what is past the last row, a missing page.
         const bool masked = !there || pos + kTile > seen0;
-        const int seen = there ? seen0 + qi - pos - 4 * g : 0;      // of this lane's keys 16 tt + i
-        if (masked) {
+        const int seen = there ? seen0 - pos - key0 + my_q : -kTile;     // query my_q + i sees position key0 + 32 j: seen + i > 32 j
+        float sc[kC][kS];
+        bool grows = false;
 #pragma unroll
-            for (int e = 0; e < 16; ++e) sc[e] = 16 * (e >> 2) + (e & 3) < seen ? sc[e] : -INFINITY;
-        }
-        float top = sc[0];
+        for (int j = 0; j < kC; ++j)
 #pragma unroll
-        for (int e = 1; e < 16; ++e) top = fmaxf(top, sc[e]);
-        top = op_xor32<true>(op_xor16<true>(top));
-        const float mn = fmaxf(m, top);
-        if (__any(mn != m)) {
-            const float keep = weight_of(m, mn);
-            l *= keep;
+            for (int i = 0; i < kS; ++i) {
+                sc[j][i] = own[j][i] * ks[j];
+                if (masked) sc[j][i] = seen + i > 32 * j ? sc[j][i] : -INFINITY;
+                grows |= sc[j][i] > m[i] + kSlack;
+            }
+        // Exponents are taken off a maximum that may lag behind by kSlack: weights up to 2^kSlack lose
+        // nothing, and after a wave's first tile this is rarely entered.
+        if (__any(grows)) {
+            float f[kS];
+#pragma unroll
+            for (int i = 0; i < kS; ++i) {
+                float top = sc[0][i];
+                if constexpr (kC == 2) top = op_xor32<true>(row_max<16>(fmaxf(top, sc[1][i])));
+                else top = wave_max(top);
+                const float mn = fmaxf(m[i], top);
+                f[i] = weight_of(m[i], mn);
+                m[i] = mn;
+                l[i] *= f[i];
+            }
+            float keep = f[0];
+#pragma unroll
+            for (int q = 0; q < (kQ == 1 ? 0 : kQ); ++q) {
+                const float fq = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(f[q % 4]), 16 * (q / 4)));
+                keep = (col & (kQ - 1)) == q ? fq : keep;
+            }
 #pragma unroll
             for (int c = 0; c < 4; ++c) acc[c] *= keep;
-            m = mn;
         }
-        const float ms = m == -INFINITY ? 0.0f : m;
-        float p[16];
-        {
-            // Not fused with the product that made the score: the largest one's difference is zero.
+#pragma unroll
+        for (int i = 0; i < kS; ++i) {
+            uint32_t hi[kC], lo[kC];
+#pragma unroll
+            for (int j = 0; j < kC; ++j) {
+                // Not fused with the product that made the score: the largest one's difference is exact.
+                float p;
+                {
 #pragma clang fp contract(off)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) p[e] = exp2_fast(sc[e] - ms);
+                    p = exp2_fast(sc[j][i] - (m[i] == -INFINITY ? 0.0f : m[i]));
+                }
+                l[i] += p;
+                p *= vs[j];
+                if (masked) p = seen + i > 32 * j ? p : 0.0f;
+                hi[j] = __float_as_uint(p);
+                lo[j] = __float_as_uint(p - __uint_as_float(hi[j] & 0xffff0000u));
+            }
+            const int at_q = 2 * (my_q + i) * kTile;
+            if constexpr (kC == 1) {
+                lp[at_q + lane] = (uint16_t)(hi[0] >> 16);
+                lp[at_q + kTile + lane] = (uint16_t)(lo[0] >> 16);
+            } else {
+                *reinterpret_cast<uint32_t*>(lp + at_q + 2 * key0) = __builtin_amdgcn_perm(hi[1], hi[0], 0x07060302u);
+                *reinterpret_cast<uint32_t*>(lp + at_q + kTile + 2 * key0) = __builtin_amdgcn_perm(lo[1], lo[0], 0x07060302u);
+            }
         }
-#pragma unroll
-        for (int e = 0; e < 16; ++e) l += p[e];
-#pragma unroll
-        for (int tt = 0; tt < 4; ++tt) {
-            const F32x4 vs = *reinterpret_cast<const F32x4*>(lvs + 16 * tt + 4 * g);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) p[4 * tt + i] *= vs[i];
-        }
-        if (masked) {
-#pragma unroll
-            for (int e = 0; e < 16; ++e) p[e] = 16 * (e >> 2) + (e & 3) < seen ? p[e] : 0.0f;
-        }
-        // hi (columns 0-7) or lo (8-15), both cut: together within 2^-14 of the weight.
-#pragma unroll
-        for (int e = 0; e < 16; ++e) p[e] -= __uint_as_float(__float_as_uint(p[e]) & lo_mask);
-        Bf16x8 pw[2];
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            U32x4 d;
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-                d[j] = kFp4 ? pack_hi(p[8 * u + 2 * j], p[8 * u + 2 * j + 1]) : pack_hi(p[8 * u + j], p[8 * u + 4 + j]);
-            pw[u] = __builtin_bit_cast(Bf16x8, d);
-        }
+        lds_order();
+        const Bf16x8 p0 = __builtin_bit_cast(Bf16x8, *reinterpret_cast<const uint4*>(lp + p_at));
+        const Bf16x8 p1 = __builtin_bit_cast(Bf16x8, *reinterpret_cast<const uint4*>(lp + p_at + 32));
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-            const I32x2 vw = __builtin_amdgcn_ds_read_tr4_b64_v2i32(
-                (__attribute__((address_space(3))) I32x2*)(lv + tr_row * kRowBytes + 8 * c));
             if constexpr (!kFp4) {
-                acc[c] = mfma(minus24, pw[0], acc[c]);
-                acc[c] = mfma(minus24, pw[1], acc[c]);
+                acc[c] = mfma(minus8, p0, acc[c]);
+                acc[c] = mfma(minus8, p1, acc[c]);
             }
-            acc[c] = mfma(operand<kFp4>((uint32_t)vw[0]), pw[0], acc[c]);
-            acc[c] = mfma(operand<kFp4>((uint32_t)vw[1]), pw[1], acc[c]);
+            acc[c] = mfma(operand<kFp4>((uint32_t)vw[c][0]), p0, acc[c]);
+            acc[c] = mfma(operand<kFp4>((uint32_t)vw[c][1]), p1, acc[c]);
         }
     }
 
     // Join the halves of the weights, then the waves.
-    l = op_xor32<false>(op_xor16<false>(l));
-    asm volatile("" ::: "memory");
+    lds_order();
     float* const ro = reinterpret_cast<float*>(lk);
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) acc[c][i] += dpp<kDppRowRor8>(acc[c][i]);
-        if (col < kGroup) *reinterpret_cast<F32x4*>(ro + col * kHd + 16 * c + 4 * g) = acc[c];
+        for (int i = 0; i < 4; ++i)
+            acc[c][i] += kQ == 1 ? dpp<kDppQuadXor1>(acc[c][i])
+                                 : (kQ == 4 ? dpp<kDppRowRor4>(acc[c][i]) : dpp<kDppRowRor8>(acc[c][i]));
+        if (col < kQ) *reinterpret_cast<F32x4*>(ro + col * kHd + 16 * c + 4 * g) = acc[c];
     }
-    if (lane < kGroup) {
-        red_m[wave][lane] = m;
-        red_l[wave][lane] = l;
+#pragma unroll
+    for (int i = 0; i < kS; ++i) {
+        l[i] = kC == 2 ? op_xor32<false>(row_sum<16>(l[i])) : wave_sum(l[i]);
+        if (col == 0 && g < kC) {
+            red_m[wave][my_q + i] = m[i];
+            red_l[wave][my_q + i] = l[i];
+        }
     }
     __syncthreads();
     const size_t tok0 = (size_t)t0 + q0;
@@ -381,14 +444,38 @@ __global__ __launch_bounds__(kW * kWave) void attend4_kernel(Args a) {
         const int qq = e / kHd, ch = e % kHd;
         const size_t head = (tok0 + qq) * a.NH + h, slot0 = head * a.S;
         float M = -INFINITY, L = 0.0f, o = 0.0f;
-        for (int j = 0; j < segs; ++j) M = fmaxf(M, get(a.part_max + slot0 + j));
-        for (int j = 0; j < segs; ++j) {
-            const float f = weight_of(get(a.part_max + slot0 + j), M);
-            L += f * get(a.part_lse + slot0 + j);
-            o += f * get(a.part_out + (slot0 + j) * kHd + ch);
+        // Eight segments' words on their way at once.
+        for (int j0 = 0; j0 < segs; j0 += 8) {
+            float mj[8], lj[8], oj[8], top = M;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const size_t slot = slot0 + min(j0 + j, segs - 1);
+                mj[j] = get(a.part_max + slot);
+                lj[j] = get(a.part_lse + slot);
+                oj[j] = get(a.part_out + slot * kHd + ch);
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j) top = j0 + j < segs ? fmaxf(top, mj[j]) : top;
+            const float f0 = weight_of(M, top);
+            L *= f0;
+            o *= f0;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                if (j0 + j < segs) {
+                    const float f = weight_of(mj[j], top);
+                    L += f * lj[j];
+                    o += f * oj[j];
+                }
+            }
+            M = top;
         }
         a.out[head * kHd + ch] = f32_to_bf16(L == 0.0f ? 0.0f : o / L);
     }
+}
+
+template <int kQ>
+const void* kernel_for(bool fp4) {
+    return fp4 ? (const void*)&attend4_kernel<true, kQ, kWaves> : (const void*)&attend4_kernel<false, kQ, kWaves>;
 }
 
 }  // namespace
@@ -397,7 +484,7 @@ namespace kvattn_internal {
 
 int plan4(int heads, int maxT, int len_hint, int S, Plan4& p) {
     const int tiles = ((len_hint >= 0 ? len_hint + 1 : maxT) + kTile - 1) / kTile;
-    p.waves = 4;
+    p.waves = kWaves;
     if (S > 0) {
         if (S > kMaxSegments) return KVATTN_ERR_SPLIT;
         p.S = S;
@@ -411,20 +498,24 @@ int plan4(int heads, int maxT, int len_hint, int S, Plan4& p) {
         p.S = (most + p.seg_tiles - 1) / p.seg_tiles;
         return p.S > kMaxSegments ? KVATTN_ERR_SPLIT : KVATTN_OK;
     }
-    p.seg_tiles = 16;
-    p.S = (tiles + p.seg_tiles - 1) / p.seg_tiles;
-    const int most = kMostBlocks / heads;
-    if (p.S > most) p.S = most < 1 ? 1 : most;
+    // Enough workgroups to fill the GPU once, each with a tile or more for every wave.
+    p.S = kFullGrid / heads;
+    if (p.S > (tiles + kWaves - 1) / kWaves) p.S = (tiles + kWaves - 1) / kWaves;
+    if (p.S < 1) p.S = 1;
+    p.seg_tiles = (tiles + p.S - 1) / p.S;
     return KVATTN_OK;
 }
 
 int attend4(const Attend4& c, bool launch) {
     Plan4 plan;
-    const int groups = c.start ? (c.max_new + kGroup - 1) / kGroup : 1;
+    // Queries of a workgroup: the fewest that take a sequence's new tokens at once, up to eight.
+    const int most_new = c.start ? c.max_new : 1;
+    const int per = most_new == 1 ? 1 : (most_new <= 4 ? 4 : 8);
+    const int groups = (most_new + per - 1) / per;
     const int st = plan4((int)std::min<long long>((long long)c.B * c.NH * groups, 1 << 30), c.maxT, c.len_hint, c.S, plan);
     if (st != KVATTN_OK) return st;
-    const long long grid = (long long)c.B * groups * c.NH * plan.S;
-    if (grid * plan.waves * kWave > 0xffffffffll) return KVATTN_ERR_SHAPE;
+    const long long rows = (long long)c.NH * groups;
+    if (rows > 65535 || rows * c.B * plan.S * plan.waves * kWave > 0xffffffffll) return KVATTN_ERR_SHAPE;
     Args a{};
     if (plan.S > 1) {
         if (!c.ws) return KVATTN_ERR_WORKSPACE;
@@ -458,9 +549,9 @@ int attend4(const Attend4& c, bool launch) {
     a.seg_tiles = plan.seg_tiles;
     a.num_tokens = c.num_tokens;
     const bool fp4 = c.kv_dtype == KVATTN_KV_FP4_E2M1;
-    const void* fn = fp4 ? (const void*)&attend4_kernel<true, 4> : (const void*)&attend4_kernel<false, 4>;
+    const void* fn = per == 1 ? kernel_for<1>(fp4) : per == 4 ? kernel_for<4>(fp4) : kernel_for<8>(fp4);
     void* params[] = {&a};
-    const hipError_t e = hipLaunchKernel(fn, dim3((unsigned)grid), dim3(plan.waves * kWave), params, 0,
+    const hipError_t e = hipLaunchKernel(fn, dim3(c.B, (unsigned)rows, plan.S), dim3(plan.waves * kWave), params, 0,
                                          (hipStream_t)c.stream);
     if (e != hipSuccess) {
         set_last_hip_error((int)e);
