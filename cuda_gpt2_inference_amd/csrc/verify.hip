@@ -3,12 +3,17 @@
 // max(0, p - q) where a draft was refused, from p where none was, by the inverse of the running sum.
 //
 // Only one row of p and one of q a sequence is read whole (2 x 200 KB at GPT-2's vocabulary): which
-// one follows from a few single values, which every workgroup of a sequence looks up for itself.
-// The row is cut into tiles of 1024 tokens, one a wave; their sums go to the workspace, and the
-// workgroup that finishes last finds the tile that the random number falls into and then the token
-// in it.  One launch, bound by memory for batches and by four dependent round trips for one
-// sequence.  Sums are double: a running float sum over 50,000 tokens would move the border between
-// two tokens by more than most tokens' whole probability.
+// one follows from a few single values, which every wave looks up for itself.  The row is cut into
+// tiles of 1024 tokens; a wave sums one at a time, then one wave finds the tile that the random number
+// falls into and the token in it.  Sums are double: a running float sum over 50,000 tokens would move
+// the border between two tokens by more than most tokens' whole probability.
+//
+// Bound by a chain of dependent memory round trips (offsets, drafts, their probabilities, the row, the
+// sums, the tile).  Workgroups of a sequence run on one XCD, so that the values that each of them looks
+// up, and the tile that is read again, come from its L2.  One workgroup of 16 waves a sequence, whose
+// sums stay in LDS, saves the join's round trips but draws the row through one CU: 19 us against 8 for
+// one sequence, 32 against 13 for 64.  Workgroups of 4 / 8 / 16 waves: one sequence 6.7 / 7.1 / 7.6 us, 64
+// of them 12.1 / 11.5 / 10.7, 300 22.6 / 21.4 / 23.6.
 #include <hip/hip_runtime.h>
 
 #include "kvattn.h"
@@ -20,12 +25,12 @@ void set_last_hip_error(int e);   // kvattn.hip: read back by kvattn_last_hip_er
 
 namespace {
 
-constexpr int kBlock = 256;
+constexpr int kBlock = 512;
 constexpr int kWaves = kBlock / kWave;
-constexpr int kTile = 1024;               // tokens of a wave's tile: 16 a lane
+constexpr int kTile = 16 * kWave;         // tokens of a wave's tile: 16 a lane
 constexpr int kMaxVocab = 1 << 24;
 constexpr int kMaxSequences = 1 << 16;
-constexpr int kFillBlocks = 1024;         // workgroups that keep the memory busy
+constexpr int kFillBlocks = 256;          // workgroups that keep the memory busy, one a CU
 
 struct VerifyArgs {
     int* tokens;
@@ -47,40 +52,80 @@ __device__ __forceinline__ float prob(const void* p, size_t i) {
     else return bf16_to_f32(reinterpret_cast<const uint16_t*>(p)[i]);
 }
 
-// Four neighbouring probabilities from token v on; zero past the vocabulary.
-template <bool kF32, bool kVec>
-__device__ __forceinline__ void probs4(const void* p, size_t row0, int v, int V, float (&x)[4]) {
-    if (kVec && v + 3 < V) {
-        if constexpr (kF32) {
-            const float4 w = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(p) + row0 + v);
-            x[0] = w.x; x[1] = w.y; x[2] = w.z; x[3] = w.w;
-        } else {
-            const uint2 w = *reinterpret_cast<const uint2*>(reinterpret_cast<const uint16_t*>(p) + row0 + v);
-            x[0] = bf16_lo(w.x); x[1] = bf16_hi(w.x); x[2] = bf16_lo(w.y); x[3] = bf16_hi(w.y);
-        }
+// Four neighbouring probabilities from token v on.
+template <bool kF32>
+__device__ __forceinline__ void probs4(const void* p, size_t row0, int v, float* x) {
+    if constexpr (kF32) {
+        const float4 w = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(p) + row0 + v);
+        x[0] = w.x; x[1] = w.y; x[2] = w.z; x[3] = w.w;
+    } else {
+        const uint2 w = *reinterpret_cast<const uint2*>(reinterpret_cast<const uint16_t*>(p) + row0 + v);
+        x[0] = bf16_lo(w.x); x[1] = bf16_hi(w.x); x[2] = bf16_lo(w.y); x[3] = bf16_hi(w.y);
+    }
+}
+
+// A lane's 16 probabilities of a tile: kNear: 16 neighbours, else four runs of four, each run next to
+// the neighbouring lanes'.  Zero past the vocabulary.  The branch is the wave's, so that all of the
+// tile's loads are on their way at once.
+template <bool kNear>
+__device__ __forceinline__ int token_at(int tile, int j, int lane) {
+    return tile * kTile + (kNear ? lane * 16 + j * 4 : (j * kWave + lane) * 4);
+}
+template <bool kF32, bool kVec, bool kNear>
+__device__ __forceinline__ void tile_probs(const void* p, size_t row0, int tile, int V, int lane, float (&x)[16]) {
+    if (kVec && tile * kTile + kTile <= V) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) probs4<kF32>(p, row0, token_at<kNear>(tile, j, lane), x + 4 * j);
         return;
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) x[i] = v + i < V ? prob<kF32>(p, row0 + v + i) : 0.0f;
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int v = token_at<kNear>(tile, j, lane) + i;
+            const float w = prob<kF32>(p, row0 + min(v, V - 1));
+            x[4 * j + i] = v < V ? w : 0.0f;
+        }
 }
 
 // What a token weighs: a finite positive number, or nothing.
 __device__ __forceinline__ double mass(double w) { return w > 0.0 && w < INFINITY ? w : 0.0; }
 
+// Sums across lanes through DPP, as the float ones: a shuffle's trip through LDS in each of the six
+// steps of four sums added up to a microsecond.
+template <int kCtrl, int kRows = 0xF>
+__device__ __forceinline__ double dpp64(double x) {      // lanes without a source, or outside kRows, get zero
+    const unsigned long long u = __builtin_bit_cast(unsigned long long, x);
+    const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)u, kCtrl, kRows, 0xF, true);
+    const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)(u >> 32), kCtrl, kRows, 0xF, true);
+    return __builtin_bit_cast(double, (unsigned long long)hi << 32 | lo);
+}
+template <bool k32>
+__device__ __forceinline__ double add_across(double x) { // x + x of lane ^ 16 or ^ 32
+    const unsigned long long u = __builtin_bit_cast(unsigned long long, x);
+    const uint32_t lo = (uint32_t)u, hi = (uint32_t)(u >> 32);
+    const auto l = k32 ? __builtin_amdgcn_permlane32_swap(lo, lo, false, false) : __builtin_amdgcn_permlane16_swap(lo, lo, false, false);
+    const auto h = k32 ? __builtin_amdgcn_permlane32_swap(hi, hi, false, false) : __builtin_amdgcn_permlane16_swap(hi, hi, false, false);
+    return __builtin_bit_cast(double, (unsigned long long)h[0] << 32 | l[0]) +
+           __builtin_bit_cast(double, (unsigned long long)h[1] << 32 | l[1]);
+}
 __device__ __forceinline__ double wave_sum64(double x) {
-#pragma unroll
-    for (int d = 1; d < kWave; d <<= 1) x += __shfl_xor(x, d);
-    return x;
+    x += dpp64<kDppQuadXor1>(x);
+    x += dpp64<kDppQuadXor2>(x);
+    x += dpp64<kDppHalfMirror>(x);
+    x += dpp64<kDppRowMirror>(x);
+    return add_across<true>(add_across<false>(x));
 }
 
-// Inclusive prefix over the wave's lanes.
+// Inclusive prefix over the wave's lanes: rows of 16 by shifts, then the last lane of the row before into
+// rows 1 and 3, and lane 31 into the upper two.
 __device__ __forceinline__ double wave_prefix64(double x) {
-    const int lane = threadIdx.x & (kWave - 1);
-#pragma unroll
-    for (int d = 1; d < kWave; d <<= 1) {
-        const double o = __shfl_up(x, d);
-        x += lane >= d ? o : 0.0;
-    }
+    x += dpp64<0x111>(x);                  // row_shr:1, 2, 4, 8
+    x += dpp64<0x112>(x);
+    x += dpp64<0x114>(x);
+    x += dpp64<0x118>(x);
+    x += dpp64<0x142, 0xA>(x);             // row_bcast:15
+    x += dpp64<0x143, 0xC>(x);             // row_bcast:31
     return x;
 }
 
@@ -94,7 +139,8 @@ __device__ __forceinline__ double get64(const double* p) {
 template <bool kF32, bool kVec>
 __global__ __launch_bounds__(kBlock) void verify_kernel(VerifyArgs a) {
     __shared__ int is_last;
-    const int b = blockIdx.x / a.blocks, blk = blockIdx.x - b * a.blocks;
+    const int slot = xcd_slot(blockIdx.x, a.blocks), b = slot / a.blocks, blk = slot - b * a.blocks;
+    if (b >= a.B) return;
     const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
     const int t0 = min(max(a.start[b], 0), a.num_tokens);
     const int n = min(max(a.start[b + 1], t0), a.num_tokens) - t0;
@@ -102,6 +148,7 @@ __global__ __launch_bounds__(kBlock) void verify_kernel(VerifyArgs a) {
         if (blk == 0 && threadIdx.x == 0) a.count[b] = 0;
         return;
     }
+    const float u_last = a.u[t0 + n - 1];  // a number that no draft is held against
     // The first row whose draft is not accepted (the last row has none): 64 rows at a time, a lane
     // each.  The comparison is exact: products of two floats fit a double.
     int row = n - 1;
@@ -128,34 +175,18 @@ __global__ __launch_bounds__(kBlock) void verify_kernel(VerifyArgs a) {
     const bool less_q = refused && a.q;
     const size_t row0 = (size_t)(t0 + row) * a.row;
 
-    // Four tokens' weights: with the draft's distribution taken off, or without.
-    auto weights = [&](int v, bool rest, double (&w)[4]) {
-        float p[4], q[4];
-        probs4<kF32, kVec>(a.p, row0, v, a.V, p);
-        if (rest && less_q) probs4<kF32, kVec>(a.q, row0, v, a.V, q);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            w[i] = (double)p[i];
-            if (rest && less_q) w[i] -= (double)q[i];
-            else if (rest && v + i == draft) w[i] = 0.0;      // a draft without probabilities had it all
-            w[i] = mass(w[i]);
-        }
-    };
-
     for (int tile = blk * kWaves + wave; tile < a.tiles; tile += a.blocks * kWaves) {
+        float p[16], q[16];
+        tile_probs<kF32, kVec, false>(a.p, row0, tile, a.V, lane, p);
+        if (less_q) tile_probs<kF32, kVec, false>(a.q, row0, tile, a.V, lane, q);
         double rest = 0.0, all = 0.0;
 #pragma unroll
-        for (int j = 0; j < kTile / (4 * kWave); ++j) {
-            const int v = tile * kTile + (j * kWave + lane) * 4;
-            float p[4], q[4];
-            probs4<kF32, kVec>(a.p, row0, v, a.V, p);
-            if (less_q) probs4<kF32, kVec>(a.q, row0, v, a.V, q);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                all += mass((double)p[i]);
-                if (less_q) rest += mass((double)p[i] - (double)q[i]);
-                else if (v + i != draft) rest += mass((double)p[i]);
-            }
+        for (int e = 0; e < 16; ++e) {
+            const double w = (double)p[e];
+            all += mass(w);
+            // A draft without probabilities had it all, and leaves its own token nothing.
+            if (less_q) rest += mass(w - (double)q[e]);
+            else rest += token_at<false>(tile, e / 4, lane) + e % 4 == draft ? 0.0 : mass(w);
         }
         rest = wave_sum64(rest);
         all = wave_sum64(all);
@@ -165,34 +196,41 @@ __global__ __launch_bounds__(kBlock) void verify_kernel(VerifyArgs a) {
             put64(s + 1, all);
         }
     }
-    if (a.blocks > 1) {
-        wait_vm_stores();
-        __syncthreads();
-        if (threadIdx.x == 0) {
-            const unsigned before = __hip_atomic_fetch_add(a.counters + b, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            is_last = before == (unsigned)(a.blocks - 1);
-            if (is_last) __hip_atomic_store(a.counters + b, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        }
-        __syncthreads();
-        if (!is_last) return;
-    } else {
-        wait_vm_stores();
-        __syncthreads();
+    wait_vm_stores();
+    __syncthreads();
+    if (threadIdx.x == 0 && a.blocks == 1) is_last = 1;
+    if (threadIdx.x == 0 && a.blocks > 1) {
+        const unsigned before = __hip_atomic_fetch_add(a.counters + b, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        is_last = before == (unsigned)(a.blocks - 1);
+        if (is_last) __hip_atomic_store(a.counters + b, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
+    __syncthreads();
+    if (!is_last) return;
     if (wave != 0) return;
 
     // Totals, and which weights count: where a refused draft leaves nothing (p = q), p's own.
     const double* const s = a.sums + (size_t)b * a.tiles * 2;
-    double rest = 0.0, all = 0.0;
-    for (int t = lane; t < a.tiles; t += kWave) {
-        rest += get64(s + 2 * t);
-        all += get64(s + 2 * t + 1);
+    auto sums_at = [&](int t, double& r, double& l) {
+        const int at = min(t, a.tiles - 1);
+        r = get64(s + 2 * at);
+        l = get64(s + 2 * at + 1);
+        if (t >= a.tiles) r = l = 0.0;
+    };
+    double rest0, all0, rest, all;         // of tile lane, kept; of every 64th from there
+    sums_at(lane, rest0, all0);
+    rest = rest0;
+    all = all0;
+    for (int t = lane + kWave; t < a.tiles; t += kWave) {
+        double r, l;
+        sums_at(t, r, l);
+        rest += r;
+        all += l;
     }
     rest = wave_sum64(rest);
     all = wave_sum64(all);
     const bool use_rest = rest > 0.0;
     const double total = use_rest ? rest : all;
-    const double aim = (double)a.u[t0 + n - 1] * total;   // a number that no draft was held against
+    const double aim = (double)u_last * total;
     int drawn = -1;
     if (total > 0.0) {
         // The first tile whose running sum passes the aim (rounding may leave none: the last that weighs
@@ -200,8 +238,9 @@ __global__ __launch_bounds__(kBlock) void verify_kernel(VerifyArgs a) {
         int tile = -1;
         double base = 0.0, before = 0.0;
         for (int t1 = 0; t1 < a.tiles; t1 += kWave) {
-            const int t = t1 + lane;
-            const double w = t < a.tiles ? get64(s + 2 * t + (use_rest ? 0 : 1)) : 0.0;
+            double r = rest0, l = all0;
+            if (t1 > 0) sums_at(t1 + lane, r, l);
+            const double w = use_rest ? r : l;
             const double upto = before + wave_prefix64(w);
             const unsigned long long pass = __ballot(w > 0.0 && upto > aim), some = __ballot(w > 0.0);
             if (some) {
@@ -212,30 +251,31 @@ __global__ __launch_bounds__(kBlock) void verify_kernel(VerifyArgs a) {
             if (pass) break;
             before = __shfl(upto, kWave - 1);
         }
-        for (int j = 0; j < kTile / (4 * kWave); ++j) {
-            const int v = tile * kTile + (j * kWave + lane) * 4;
-            double w[4];
-            weights(v, use_rest, w);
-            const double mine = (w[0] + w[1]) + (w[2] + w[3]);
-            const double upto = base + wave_prefix64(mine);
-            double run = upto - mine;
-            int hit = -1, last = -1;
+        float p[16], q[16];
+        tile_probs<kF32, kVec, true>(a.p, row0, tile, a.V, lane, p);
+        if (use_rest && less_q) tile_probs<kF32, kVec, true>(a.q, row0, tile, a.V, lane, q);
+        double w[16], mine = 0.0;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                run += w[i];
-                if (w[i] > 0.0) {
-                    last = v + i;
-                    if (hit < 0 && run > aim) hit = v + i;
-                }
-            }
-            const unsigned long long pass = __ballot(hit >= 0), some = __ballot(last >= 0);
-            if (pass) {
-                drawn = __shfl(hit, __ffsll((long long)pass) - 1);
-                break;
-            }
-            if (some) drawn = __shfl(last, 63 - __clzll((long long)some));
-            base = __shfl(upto, kWave - 1);
+        for (int e = 0; e < 16; ++e) {
+            w[e] = (double)p[e];
+            if (use_rest && less_q) w[e] -= (double)q[e];
+            w[e] = mass(w[e]);
+            if (use_rest && tile * kTile + lane * 16 + e == draft && !less_q) w[e] = 0.0;
+            mine += w[e];
         }
+        double run = base + (wave_prefix64(mine) - mine);
+        int hit = -1, last = -1;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            run += w[e];
+            if (w[e] > 0.0) {
+                last = tile * kTile + lane * 16 + e;
+                if (hit < 0 && run > aim) hit = last;
+            }
+        }
+        const unsigned long long pass = __ballot(hit >= 0), some = __ballot(last >= 0);
+        if (pass) drawn = __shfl(hit, __ffsll((long long)pass) - 1);
+        else if (some) drawn = __shfl(last, 63 - __clzll((long long)some));
     }
     for (int i = lane; i < n; i += kWave) a.tokens[t0 + i] = i < row ? a.drafts[t0 + i] : (i == row ? drawn : -1);
     if (lane == 0) a.count[b] = row + (drawn >= 0 ? 1 : 0);
@@ -289,8 +329,9 @@ int kvattn_verify_drafts(int* tokens, int* counts, const void* target_probs, con
     const void* fn = dtype == KVATTN_KV_F32
                          ? (vec ? (const void*)&verify_kernel<true, true> : (const void*)&verify_kernel<true, false>)
                          : (vec ? (const void*)&verify_kernel<false, true> : (const void*)&verify_kernel<false, false>);
+    const long long grid = 8ll * ((B + 7) / 8) * a.blocks;      // whole rounds of the eight XCDs
     void* params[] = {&a};
-    const hipError_t e = hipLaunchKernel(fn, dim3((unsigned)((long long)a.blocks * B)), dim3(kBlock), params, 0,
+    const hipError_t e = hipLaunchKernel(fn, dim3((unsigned)grid), dim3(kBlock), params, 0,
                                          (hipStream_t)stream);
     if (e != hipSuccess) {
         kvattn_internal::set_last_hip_error((int)e);
