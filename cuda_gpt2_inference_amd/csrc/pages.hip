@@ -17,6 +17,8 @@ constexpr int kHd = 64;
 constexpr int kBlock = 256;
 constexpr int kMaxT = 1 << 23;
 
+int log2_or(int x) { return x > 0 && (x & (x - 1)) == 0 ? __builtin_ctz((unsigned)x) : -1; }
+
 int hip_status(hipError_t e) {
     if (e == hipSuccess) return KVATTN_OK;
     kvattn_internal::set_last_hip_error((int)e);
@@ -37,7 +39,9 @@ int hip_status(hipError_t e) {
 constexpr int kPoolHead = 0, kPoolCount = 1, kPoolTicket = 2, kPoolRing = 4;
 constexpr int kMaxRequests = 4096;
 constexpr int kRequestInts = 6;            // LDS words of a request
-constexpr int kReserveTokens = 1024;       // token rows a workgroup is launched for, up to
+constexpr int kReserveThreads = 1024;      // of a workgroup; kSmallThreads where one such is enough
+constexpr int kSmallThreads = 256;
+constexpr int kReserveTokens = 4096;       // token rows a workgroup is launched for, up to
 constexpr int kReserveMostBlocks = 256;    // so many workgroups
 constexpr int kRefused = 1 << 30;          // beside the positions a request keeps
 
@@ -54,6 +58,7 @@ struct ReserveArgs {
     int* positions;
     int* pool_next;
     int max_pages, R, num_pages, B, max_tokens;
+    int shift;                 // log2 of R, or -1
 };
 
 __device__ __forceinline__ int add_sat(int a, int b) {   // a, b >= 0
@@ -61,32 +66,48 @@ __device__ __forceinline__ int add_sat(int a, int b) {   // a, b >= 0
     return s > (unsigned)INT_MAX ? INT_MAX : (int)s;
 }
 
-// Exclusive prefix of v over the workgroup's threads, and its total.
-__device__ __forceinline__ int block_prefix(int v, int* wave_sums, int& total) {
-    const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
-    int in = v;
-#pragma unroll
-    for (int d = 1; d < kWave; d <<= 1) {
-        const int o = __shfl_up(in, d);
-        in = lane >= d ? add_sat(in, o) : in;
-    }
-    __syncthreads();
-    if (lane == kWave - 1) wave_sums[wave] = in;
-    __syncthreads();
-    int before = 0;
-    total = 0;
-#pragma unroll
-    for (int w = 0; w < kBlock / kWave; ++w) {
-        before = w < wave ? add_sat(before, wave_sums[w]) : before;
-        total = add_sat(total, wave_sums[w]);
-    }
-    const int up = __shfl_up(in, 1);
-    return add_sat(before, lane > 0 ? up : 0);
+// Inclusive prefix over the wave's lanes (saturating; values >= 0): rows of 16 by shifts, then the last
+// lane of the row before into rows 1 and 3, and lane 31 into the upper two.
+__device__ __forceinline__ int wave_prefix(int x) {
+    x = add_sat(x, __builtin_amdgcn_update_dpp(0, x, 0x111, 0xF, 0xF, true));   // row_shr:1, 2, 4, 8
+    x = add_sat(x, __builtin_amdgcn_update_dpp(0, x, 0x112, 0xF, 0xF, true));
+    x = add_sat(x, __builtin_amdgcn_update_dpp(0, x, 0x114, 0xF, 0xF, true));
+    x = add_sat(x, __builtin_amdgcn_update_dpp(0, x, 0x118, 0xF, 0xF, true));
+    x = add_sat(x, __builtin_amdgcn_update_dpp(0, x, 0x142, 0xA, 0xF, true));   // row_bcast:15
+    x = add_sat(x, __builtin_amdgcn_update_dpp(0, x, 0x143, 0xC, 0xF, true));   // row_bcast:31
+    return x;
 }
 
-// The last i of 0 .. n-1 with start[i] <= x (start[0] = 0): the owner of item x.
-__device__ __forceinline__ int owner(const int* start, int n, int x) {
-    int lo = 0, hi = n - 1;
+// Exclusive prefixes of kN values over the workgroup's threads, and their totals.  Subtraction undoes a
+// sum only where nothing was cut off, so the values themselves are shifted by a lane.
+template <int kThreads, int kN>
+__device__ __forceinline__ void block_prefix(const int (&v)[kN], int (&wave_sums)[kN][kThreads / kWave], int (&prefix)[kN],
+                                             int (&total)[kN]) {
+    const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+    int in[kN];
+#pragma unroll
+    for (int n = 0; n < kN; ++n) {
+        in[n] = wave_prefix(v[n]);
+        if (lane == kWave - 1) wave_sums[n][wave] = in[n];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int n = 0; n < kN; ++n) {
+        int before = 0, all = 0;
+#pragma unroll
+        for (int w = 0; w < kThreads / kWave; ++w) {
+            const int s = wave_sums[n][w];
+            before = w < wave ? add_sat(before, s) : before;
+            all = add_sat(all, s);
+        }
+        const int up = __shfl_up(in[n], 1);
+        prefix[n] = add_sat(before, lane > 0 ? up : 0);
+        total[n] = all;
+    }
+}
+
+// The last i of lo .. hi with start[i] <= x (start[lo] <= x): the owner of item x.
+__device__ __forceinline__ int owner(const int* start, int lo, int hi, int x) {
     while (lo < hi) {
         const int mid = (lo + hi + 1) >> 1;
         if (start[mid] <= x) lo = mid;
@@ -95,39 +116,55 @@ __device__ __forceinline__ int owner(const int* start, int n, int x) {
     return lo;
 }
 
-__global__ __launch_bounds__(kBlock) void reserve_kernel(ReserveArgs a) {
+template <int kThreads>
+__global__ __launch_bounds__(kThreads) void reserve_kernel(ReserveArgs a) {
     extern __shared__ int lds[];
-    __shared__ int wave_sums[kBlock / kWave];
-    __shared__ int shared_took, shared_turn;
+    __shared__ int asked_sums[2][kThreads / kWave], given_sums[1][kThreads / kWave];
+    __shared__ int shared_took, shared_turn, run_ends[2];
+    constexpr int kOwn = kThreads == kSmallThreads ? 1 : kMaxRequests / kThreads;   // requests a thread reads
     int* const tok = lds;                 // first token
     int* const take = tok + a.B;          // first of the pages it takes
     int* const give = take + a.B;         // first of the pages it gives back
     int* const have = give + a.B;         // pages it holds
     int* const want = have + a.B;         // pages it will hold (refused: those it holds)
     int* const kept = want + a.B;         // positions it keeps, and kRefused
+    const int tid = threadIdx.x;
     const int P = a.num_pages;
     const int head = (int)((unsigned)a.pool[kPoolHead] % (unsigned)P);
     const int count = min(max(a.pool[kPoolCount], 0), P);
     const long long most = (long long)a.max_pages * a.R;
-    const int each = (a.B + kBlock - 1) / kBlock, i0 = min((int)threadIdx.x * each, a.B), i1 = min(i0 + each, a.B);
-
+    auto pages_of = [&](int positions) {
+        return a.shift >= 0 ? (positions + a.R - 1) >> a.shift : (positions + a.R - 1) / a.R;
+    };
     // Tokens and pages asked for.  A request whose lengths make no sense asks for nothing.
-    int toks = 0, takes = 0;
-    for (int i = i0; i < i1; ++i) {
+    int hd_own[kOwn], kp_own[kOwn];
+#pragma unroll
+    for (int j = 0; j < kOwn; ++j) {
+        const int i = tid + j * kThreads;
+        if (i >= a.B) break;
         const int hd = a.held[i], kp = a.kept[i], fr = a.fresh[i];
+        hd_own[j] = hd;
+        kp_own[j] = kp;
         const bool ok = kp >= 0 && kp <= hd && hd <= most && fr >= 0 && (long long)kp + fr <= most;
-        have[i] = ok ? (hd + a.R - 1) / a.R : 0;
-        want[i] = ok ? (kp + fr + a.R - 1) / a.R : 0;
+        have[i] = ok ? pages_of(hd) : 0;
+        want[i] = ok ? pages_of(kp + fr) : 0;
         kept[i] = ok ? kp : kRefused;
         tok[i] = ok ? fr : 0;
-        toks = add_sat(toks, tok[i]);
-        takes = add_sat(takes, max(want[i] - have[i], 0));
     }
-    int all_toks, all_takes, all_gives;
-    int t = block_prefix(toks, wave_sums, all_toks), k = block_prefix(takes, wave_sums, all_takes);
+    if (tid == 0) shared_took = 0;
+    __syncthreads();
+    const int each = (a.B + kThreads - 1) / kThreads, i0 = min(tid * each, a.B), i1 = min(i0 + each, a.B);
+    int asked[2] = {0, 0}, before_me[2], all_asked[2];
+    for (int i = i0; i < i1; ++i) {
+        asked[0] = add_sat(asked[0], tok[i]);
+        asked[1] = add_sat(asked[1], max(want[i] - have[i], 0));
+    }
+    block_prefix<kThreads, 2>(asked, asked_sums, before_me, all_asked);
+    int t = before_me[0], k = before_me[1];
+    const int all_toks = all_asked[0];
     // Granted in request order while pages and token rows last: once one that takes pages is refused
     // for want of pages (or tokens), so is every later one that takes any, so pages taken have no gaps.
-    int gives = 0, took = 0;
+    int gives[1] = {0}, took = 0, gv[1], all_gives[1];
     for (int i = i0; i < i1; ++i) {
         const int fr = tok[i], tk = max(want[i] - have[i], 0);
         tok[i] = t;
@@ -140,73 +177,87 @@ __global__ __launch_bounds__(kBlock) void reserve_kernel(ReserveArgs a) {
             want[i] = have[i];
         }
         if (ok && tk > 0) took = k;
-        gives = add_sat(gives, max(have[i] - want[i], 0));
+        gives[0] = add_sat(gives[0], max(have[i] - want[i], 0));
     }
-    int gv = block_prefix(gives, wave_sums, all_gives);
-    for (int i = i0; i < i1; ++i) {
-        give[i] = gv;
-        gv = add_sat(gv, max(have[i] - want[i], 0));
-    }
-    if (threadIdx.x == 0) shared_took = 0;
-    __syncthreads();
     if (took > 0) atomicMax(&shared_took, took);
-    // Everything that another workgroup's outputs may overwrite has been read.
+    block_prefix<kThreads, 1>(gives, given_sums, gv, all_gives);
+    for (int i = i0; i < i1; ++i) {
+        give[i] = gv[0];
+        gv[0] = add_sat(gv[0], max(have[i] - want[i], 0));
+    }
+    // Everything that another workgroup's outputs may overwrite has been read.  Whose turn it is to write
+    // those is asked now and looked at last: the answer's way back is not waited for.
     wait_vm_stores();
     __syncthreads();
     const int all_took = shared_took;
-    if (threadIdx.x == 0) {
-        bool turn = true;
-        if (gridDim.x > 1) {
-            const unsigned seen = __hip_atomic_fetch_add((unsigned*)a.pool + kPoolTicket, 1u, __ATOMIC_RELAXED,
-                                                         __HIP_MEMORY_SCOPE_AGENT);
-            turn = seen == gridDim.x - 1;
-            if (turn)
-                __hip_atomic_store((unsigned*)a.pool + kPoolTicket, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        }
-        shared_turn = turn;
-    }
-    __syncthreads();
+    unsigned before = gridDim.x - 1;
+    if (gridDim.x > 1 && tid == 0)
+        before = __hip_atomic_fetch_add((unsigned*)a.pool + kPoolTicket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 
-    const int me = blockIdx.x * kBlock + threadIdx.x, step = gridDim.x * kBlock;
     int* const ring = a.pool + kPoolRing;
     auto ring_at = [&](int i) {           // entry i of the ring from its head on, i <= P
         const int at = head + i;
         return at >= P ? at - P : at;
     };
-    // Tokens.
+    // Tokens: a run of neighbours for every workgroup, whose owners lie between its ends'.
     const int n_tok = min(all_toks, a.max_tokens);
-    for (int x = me; x < n_tok; x += step) {
-        const int b = owner(tok, a.B, x);
-        const int kp = kept[b] & ~kRefused, pos = kp + (x - tok[b]), pi = pos / a.R;
-        if (a.positions) a.positions[x] = pos;
-        long long slot = -1;
-        if (!(kept[b] & kRefused)) {
-            const int page = pi < have[b] ? a.table[(size_t)b * a.max_pages + pi] : ring[ring_at(take[b] + pi - have[b])];
-            if (page >= 0 && page < P) slot = (long long)page * a.R + pos % a.R;
+    const int run = (n_tok + gridDim.x - 1) / gridDim.x;
+    const int x0 = min((int)blockIdx.x * run, n_tok), x1 = min(x0 + run, n_tok);
+    if (x0 < x1) {
+        int b0 = 0, b1 = a.B - 1;
+        if (gridDim.x > 1) {
+            if (tid < 2) run_ends[tid] = owner(tok, 0, a.B - 1, tid == 0 ? x0 : x1 - 1);
+            __syncthreads();
+            b0 = run_ends[0];
+            b1 = run_ends[1];
         }
-        a.slot_map[x] = slot;
+#pragma unroll 4
+        for (int x = x0 + tid; x < x1; x += kThreads) {
+            const int b = owner(tok, b0, b1, x);
+            const int kp = kept[b], pos = (kp & ~kRefused) + (x - tok[b]);
+            const int pi = a.shift >= 0 ? pos >> a.shift : pos / a.R;
+            if (a.positions) a.positions[x] = pos;
+            long long slot = -1;
+            if (!(kp & kRefused)) {
+                const int* const from = pi < have[b] ? a.table + (size_t)b * a.max_pages + pi
+                                                     : ring + ring_at(take[b] + pi - have[b]);
+                const int page = *from;
+                if (page >= 0 && page < P) slot = (long long)page * a.R + (pos - pi * a.R);
+            }
+            a.slot_map[x] = slot;
+        }
     }
-    // Pages taken.
-    for (int x = me; x < all_took; x += step) {
-        const int b = owner(take, a.B, x);
+    // Pages taken, from the last thread on, and given back, from the middle on: a small call's three
+    // kinds of work fall to different waves and wait side by side.
+    const int step = gridDim.x * kThreads, me = blockIdx.x * kThreads + tid;
+    for (int x = step - 1 - me; x < all_took; x += step) {
+        const int b = owner(take, 0, a.B - 1, x);
         a.table[(size_t)b * a.max_pages + have[b] + x - take[b]] = ring[ring_at(x)];
     }
-    // Pages given back.  (More than the ring has room for means a pool that was not this one's.)
-    const int n_give = min(all_gives, P - count);
-    for (int x = me; x < n_give; x += step) {
-        const int b = owner(give, a.B, x);
+    // (More given back than the ring has room for means a pool that was not this one's.)
+    const int n_give = min(all_gives[0], P - count);
+    for (int x = me >= step / 2 ? me - step / 2 : me + step - step / 2; x < n_give; x += step) {
+        const int b = owner(give, 0, a.B - 1, x);
         ring[ring_at(count + x)] = a.table[(size_t)b * a.max_pages + want[b] + x - give[b]];
     }
+    if (tid == 0) {
+        shared_turn = before == gridDim.x - 1;
+        if (shared_turn && gridDim.x > 1)
+            __hip_atomic_store((unsigned*)a.pool + kPoolTicket, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    __syncthreads();
     if (!shared_turn) return;
-    for (int i = threadIdx.x; i < a.B; i += kBlock) {
+#pragma unroll
+    for (int j = 0; j < kOwn; ++j) {
+        const int i = tid + j * kThreads;
+        if (i >= a.B) break;
         const bool ok = !(kept[i] & kRefused);
-        const int hd = a.held[i], kp = a.kept[i];
         const int fr = (i + 1 < a.B ? tok[i + 1] : all_toks) - tok[i];
-        a.held_out[i] = ok ? kp + fr : hd;
-        a.lens[i] = ok ? kp + fr : kp;
+        a.held_out[i] = ok ? kp_own[j] + fr : hd_own[j];
+        a.lens[i] = ok ? kp_own[j] + fr : kp_own[j];
         a.token_start[i] = tok[i];
     }
-    if (threadIdx.x == 0) {
+    if (tid == 0) {
         a.token_start[a.B] = all_toks;
         int* const next = a.pool_next ? a.pool_next : a.pool;
         next[kPoolHead] = ring_at(all_took);
@@ -408,7 +459,7 @@ __global__ __launch_bounds__(kBlock) void load_rows_kernel(RowsArgs a) {
 }
 
 int launch_rows(const void* fn, RowsArgs a, void* stream) {
-    a.shift = a.R > 0 && (a.R & (a.R - 1)) == 0 ? __builtin_ctz((unsigned)a.R) : -1;
+    a.shift = log2_or(a.R);
     const long long items = (long long)((a.n + 7) / 8) * 2 * a.NH;
     const long long grid = (items + kBlock / kWave - 1) / (kBlock / kWave);
     void* params[] = {&a};
@@ -490,19 +541,20 @@ int kvattn_paged_reserve(int* block_table, int max_pages, int page_rows, int num
         if ((uintptr_t)p & 3u) return KVATTN_ERR_MISALIGNED;
     if ((uintptr_t)slot_map & 7u) return KVATTN_ERR_MISALIGNED;
     ReserveArgs a{block_table, pool, held, kept, fresh, held_out, lens, token_start, slot_map, positions, pool_next,
-                  max_pages, page_rows, num_pages, B, max_tokens};
+                  max_pages, page_rows, num_pages, B, max_tokens, log2_or(page_rows)};
     const int lds = kRequestInts * B * (int)sizeof(int);
     static_assert(kRequestInts * kMaxRequests * sizeof(int) <= 128 * 1024, "LDS of a CU");
+    const bool small = B <= kSmallThreads && max_tokens <= 4 * kSmallThreads;
+    const int threads = small ? kSmallThreads : kReserveThreads;
+    const void* fn = small ? (const void*)&reserve_kernel<kSmallThreads> : (const void*)&reserve_kernel<kReserveThreads>;
     if (lds > 64 * 1024) {
-        const int st = hip_status(hipFuncSetAttribute((const void*)&reserve_kernel,
-                                                      hipFuncAttributeMaxDynamicSharedMemorySize, lds));
+        const int st = hip_status(hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, lds));
         if (st != KVATTN_OK) return st;
     }
     const long long blocks = ((long long)max_tokens + kReserveTokens - 1) / kReserveTokens;
-    const unsigned grid = (unsigned)(blocks < 1 ? 1 : blocks > kReserveMostBlocks ? kReserveMostBlocks : blocks);
+    const unsigned grid = (unsigned)(small || blocks < 1 ? 1 : blocks > kReserveMostBlocks ? kReserveMostBlocks : blocks);
     void* params[] = {&a};
-    return hip_status(hipLaunchKernel((const void*)&reserve_kernel, dim3(grid), dim3(kBlock), params, (size_t)lds,
-                                      (hipStream_t)stream));
+    return hip_status(hipLaunchKernel(fn, dim3(grid), dim3(threads), params, (size_t)lds, (hipStream_t)stream));
 }
 
 int kvattn_paged_store(void* pages, float* page_scales, int page_rows, int num_pages, const long long* slot_map,
