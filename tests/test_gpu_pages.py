@@ -282,3 +282,28 @@ def test_rows_captured(dev, kv):
         kvattn.paged_store(c2, qkv, slots, n, NH, HS, kv_dtype=kv)
         kvattn.paged_load(b2, c2, slots, n, NH, HS, kv_dtype=kv)
         assert torch.equal(b2, back)
+
+
+@pytest.mark.parametrize("kv", ["int4", "fp4"])
+def test_every_quotient_rounds_as_the_division(dev, kv):
+    """Codes of every pair of bf16 significands (a row's largest element and another) whose quotient can
+    reach a code of its own, in the middle of the range and at its ends: bit for bit the definition's."""
+    import torch
+    kvattn = _kv()
+    sig = 1 + np.arange(128) / 128.0
+    others = (sig[None, :] * 2.0 ** -np.arange(6)[:, None]).reshape(-1)       # 768 magnitudes, 1 .. 2^-5
+    rows = np.zeros((128, 13, 64), np.float32)
+    flat = np.concatenate([others, -others[:51]])                             # 13 * 63 = 819
+    rows[:, :, 1:] = flat.reshape(1, 13, 63)
+    rows[:, :, 0] = 2 * sig[:, None]                                          # the largest
+    for shift in (0, 80, -85, 118, -110):
+        x = (rows * np.float32(2.0) ** shift).reshape(-1, 64)
+        qkv = torch.zeros(x.shape[0], 3, 1, HS, dtype=torch.bfloat16, device=dev)
+        qkv[:, 1, 0] = torch.from_numpy(x).to(torch.bfloat16).to(dev)
+        n = x.shape[0]
+        pages, scales = _pool(kv, 1, 1, n, dev)
+        cache = kvattn.PagedCache(pages, None, 1, n, 1, scales)
+        kvattn.paged_store(cache, qkv, torch.arange(n, device=dev), n, 1, HS, kv_dtype=kv)
+        want, want_s = kv4ref.encode(qkv[:, 1, 0].float().cpu().numpy(), kv)
+        assert np.array_equal(scales[0, 0, 0].cpu().numpy(), want_s)
+        assert np.array_equal(pages[0, 0, 0].cpu().numpy(), want)
