@@ -49,8 +49,18 @@ constexpr float kQScale = 0.125f * 1.4426950408889634f;    // 1/sqrt(64) * log2(
 constexpr float kSlack = 8.0f;
 constexpr int kMaxT = 1 << 23;
 constexpr int kMaxSegments = 65535;        // the grid's third side
-constexpr int kWaves = 4;                  // waves of a workgroup
-constexpr int kFullGrid = 1024;            // workgroups that the GPU runs at once: four a CU
+// AUTO's shapes.  Up to one head a CU, workgroups of 8 waves, in as many segments as there are CUs; beyond,
+// 4 waves, in segments that fill four workgroups a CU, and with ragged lengths past 6144 positions of
+// about 32 tiles, so that the longest sequence is not waited for alone.  No segment is shorter than 16
+// tiles (a join of segments costs 1.5 to 2 us).  us per call, FP4 unless said, GPU time:
+//   12 heads of 1024 positions   8 waves 1 segment 5.0, 4 waves 1 / 4 segments 5.5 / 5.7
+//   12 heads of 8000             8 waves 8 / 4 / 1 segments 7.3 / 8.6 / 17.4, 4 waves 8 segments 7.9
+//   192 heads of 4096            8 waves 1 / 2 segments 12.4 / 15.0, 4 waves 4 / 1 segments 13.8 / 16.8
+//   288 ragged heads of up to 4096, 8 tokens   4 waves 3 / 1 segments 17.8 / 22.3, 8 waves 2 segments 17.1
+//   768 ragged heads of up to 8192, INT4       4 waves 4 / 1 segments 49.4 / 50.3, 8 waves 1 segment 50.7
+//   768 ragged heads of up to 1024             4 waves 1 / 2 segments 10.1 / 12.1, 8 waves 1 segment 11.1
+constexpr int kCUs = 256;
+constexpr int kSegTiles = 16;
 
 struct Args {
     const uint8_t* kv;
@@ -169,7 +179,8 @@ __global__ __launch_bounds__(kW * kWave) __attribute__((amdgpu_waves_per_eu(4)))
     // A lane scores kC positions of a tile for kS of the queries.
     constexpr int kC = kQ <= 4 ? 1 : 2, kS = kQ == 1 ? 1 : 4;
 
-    const int b = blockIdx.x, grp = a.groups == 1 ? 0 : blockIdx.y / a.NH, h = blockIdx.y - grp * a.NH, s = blockIdx.z;
+    // Heads lie next to each other in the grid, so that a long sequence's are spread over the XCDs.
+    const int b = blockIdx.y, grp = a.groups == 1 ? 0 : blockIdx.x / a.NH, h = blockIdx.x - grp * a.NH, s = blockIdx.z;
     int t0, n, total;
     if (a.start) {
         t0 = min(max(a.start[b], 0), a.num_tokens);
@@ -474,17 +485,18 @@ __global__ __launch_bounds__(kW * kWave) __attribute__((amdgpu_waves_per_eu(4)))
 }
 
 template <int kQ>
-const void* kernel_for(bool fp4) {
-    return fp4 ? (const void*)&attend4_kernel<true, kQ, kWaves> : (const void*)&attend4_kernel<false, kQ, kWaves>;
+const void* kernel_for(bool fp4, int waves) {
+    if (waves == 8) return fp4 ? (const void*)&attend4_kernel<true, kQ, 8> : (const void*)&attend4_kernel<false, kQ, 8>;
+    return fp4 ? (const void*)&attend4_kernel<true, kQ, 4> : (const void*)&attend4_kernel<false, kQ, 4>;
 }
 
 }  // namespace
 
 namespace kvattn_internal {
 
-int plan4(int heads, int maxT, int len_hint, int S, Plan4& p) {
+int plan4(int heads, int maxT, int len_hint, bool ragged, int S, Plan4& p) {
     const int tiles = ((len_hint >= 0 ? len_hint + 1 : maxT) + kTile - 1) / kTile;
-    p.waves = kWaves;
+    p.waves = heads <= kCUs ? 8 : 4;
     if (S > 0) {
         if (S > kMaxSegments) return KVATTN_ERR_SPLIT;
         p.S = S;
@@ -498,11 +510,11 @@ int plan4(int heads, int maxT, int len_hint, int S, Plan4& p) {
         p.S = (most + p.seg_tiles - 1) / p.seg_tiles;
         return p.S > kMaxSegments ? KVATTN_ERR_SPLIT : KVATTN_OK;
     }
-    // Enough workgroups to fill the GPU once, each with a tile or more for every wave.
-    p.S = kFullGrid / heads;
-    if (p.S > (tiles + kWaves - 1) / kWaves) p.S = (tiles + kWaves - 1) / kWaves;
-    if (p.S < 1) p.S = 1;
-    p.seg_tiles = (tiles + p.S - 1) / p.S;
+    p.S = p.waves == 8 ? kCUs / heads : 4 * kCUs / heads;
+    p.S = std::min(p.S, (tiles + kSegTiles - 1) / kSegTiles);
+    if (p.waves == 4 && ragged && tiles >= 96) p.S = std::max(p.S, tiles / 32);
+    p.S = std::max(1, std::min(p.S, kMaxSegments));
+    p.seg_tiles = kSegTiles;               // or ceil(tiles / S), on the device
     return KVATTN_OK;
 }
 
@@ -512,10 +524,11 @@ int attend4(const Attend4& c, bool launch) {
     const int most_new = c.start ? c.max_new : 1;
     const int per = most_new == 1 ? 1 : (most_new <= 4 ? 4 : 8);
     const int groups = (most_new + per - 1) / per;
-    const int st = plan4((int)std::min<long long>((long long)c.B * c.NH * groups, 1 << 30), c.maxT, c.len_hint, c.S, plan);
+    const int st = plan4((int)std::min<long long>((long long)c.B * c.NH * groups, 1 << 30), c.maxT, c.len_hint,
+                         c.start || c.lens_per_seq, c.S, plan);
     if (st != KVATTN_OK) return st;
     const long long rows = (long long)c.NH * groups;
-    if (rows > 65535 || rows * c.B * plan.S * plan.waves * kWave > 0xffffffffll) return KVATTN_ERR_SHAPE;
+    if (c.B > 65535 || rows * c.B * plan.S * plan.waves * kWave > 0xffffffffll) return KVATTN_ERR_SHAPE;
     Args a{};
     if (plan.S > 1) {
         if (!c.ws) return KVATTN_ERR_WORKSPACE;
@@ -549,9 +562,10 @@ int attend4(const Attend4& c, bool launch) {
     a.seg_tiles = plan.seg_tiles;
     a.num_tokens = c.num_tokens;
     const bool fp4 = c.kv_dtype == KVATTN_KV_FP4_E2M1;
-    const void* fn = per == 1 ? kernel_for<1>(fp4) : per == 4 ? kernel_for<4>(fp4) : kernel_for<8>(fp4);
+    const void* fn = per == 1 ? kernel_for<1>(fp4, plan.waves) : per == 4 ? kernel_for<4>(fp4, plan.waves)
+                                                                           : kernel_for<8>(fp4, plan.waves);
     void* params[] = {&a};
-    const hipError_t e = hipLaunchKernel(fn, dim3(c.B, (unsigned)rows, plan.S), dim3(plan.waves * kWave), params, 0,
+    const hipError_t e = hipLaunchKernel(fn, dim3((unsigned)rows, c.B, plan.S), dim3(plan.waves * kWave), params, 0,
                                          (hipStream_t)c.stream);
     if (e != hipSuccess) {
         set_last_hip_error((int)e);
