@@ -2872,6 +2872,7 @@ int check_common4(const void* qkv, const void* kv, const float* kv_scale, int B,
 int cache_write4(void* kv, float* kv_scale, const void* qkv, int B, int NH, int hs, int maxT, const int* d_cur_len,
                  int lens_per_seq, int kv_dtype, const CacheMap& cm, void* stream) {
     KV_TRY(check_common4(qkv, kv, kv_scale, B, NH, hs, maxT));
+    if (!d_cur_len) lens_per_seq = 0;      // the library's own length is one for the batch
     KV_TRY(resolve_len(d_cur_len));
     return kvattn_internal::append4(kv, kv_scale, qkv, B, NH, maxT, d_cur_len, lens_per_seq ? 1 : 0, cm.table,
                                     cm.max_pages, cm.page_rows, cm.num_pages, kv_dtype, stream);
@@ -2886,6 +2887,7 @@ int decode4(void* out, const void* qkv, const void* kv, const float* kv_scale, i
     if (!aligned16(out)) return KVATTN_ERR_MISALIGNED;
     if (len_hint < -1 || len_hint > maxT - 1) return KVATTN_ERR_LENGTH;
     if (strategy != KVATTN_AUTO && strategy != KVATTN_SPLIT_LASTBLOCK) return KVATTN_ERR_STRATEGY;
+    if (!d_cur_len) lens_per_seq = 0;      // the library's own length is one for the batch
     KV_TRY(resolve_len(d_cur_len));
     const kvattn_internal::Attend4 c{out, qkv, kv, kv_scale, cm.table, nullptr, d_cur_len, cm.max_pages, cm.page_rows,
                                      cm.num_pages, B, NH, maxT, B, 1, lens_per_seq ? 1 : 0, len_hint, S, kv_dtype,

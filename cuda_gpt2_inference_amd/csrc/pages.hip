@@ -227,6 +227,8 @@ __global__ __launch_bounds__(kThreads) void reserve_kernel(ReserveArgs a) {
             a.slot_map[x] = slot;
         }
     }
+    // Rows behind the last token, so that a step captured for max_tokens stores nothing for them.
+    for (int x = n_tok + blockIdx.x * kThreads + tid; x < a.max_tokens; x += gridDim.x * kThreads) a.slot_map[x] = -1;
     // Pages taken, from the last thread on, and given back, from the middle on: a small call's three
     // kinds of work fall to different waves and wait side by side.
     const int step = gridDim.x * kThreads, me = blockIdx.x * kThreads + tid;

@@ -10,11 +10,12 @@
  *   qkv       [B][3][NH][hs]             Q, K, V of the current token
  *   kv_cache  [2][B][NH][maxT][hs]       K block then V block; K(b,h,j) at
  *                                        ((b*NH+h)*maxT + j)*hs, V adds B*NH*maxT*hs
- *   kv_scale  [2][B][NH][maxT] float     per-row scales, 8-bit caches only
+ *   kv_scale  [2][B][NH][maxT] float     per-row scales, 8-bit and 4-bit caches only
  *   out       [B][NH][hs]
  *   part_out  [B][NH][S][hs] float, part_max / part_lse [B][NH][S] float
  * Element types: kv_dtype F32 -> qkv, kv_cache, out are float.  BF16 -> bfloat16.
  * INT8 / FP8_E4M3 -> kv_cache holds one byte per element, qkv and out are bfloat16.
+ * INT4 / FP4_E2M1 -> kv_cache holds half a byte per element, qkv and out are bfloat16.
  *
  * Lengths: the number of attended positions of sequence b is cur_len + 1 where cur_len
  * is read ON THE DEVICE when the kernels run: from d_cur_len[0] for every sequence, or
@@ -68,8 +69,10 @@ typedef enum kvattn_dtype {
     /* 4-bit caches: 32 bytes a row, channel 2i in the low half of byte i and 2i+1 in the high
      * half, one float scale a row (1/7 and 1/6 rounded to float); qkv and out are bf16.  No reference counterpart (its cache
      * types end at 8 bits).  Taken by kvattn_cache_write, kvattn_append, kvattn_decode,
-     * kvattn_append_decode, kvattn_plan and the kvattn_paged_* calls; the others return
-     * KVATTN_ERR_DTYPE. */
+     * kvattn_append_decode (two launches), kvattn_plan and the kvattn_paged_* calls; the others
+     * return KVATTN_ERR_DTYPE.  Attention over them has one strategy, KVATTN_SPLIT_LASTBLOCK
+     * (KVATTN_AUTO takes it), takes S > 0 and S < 0 (a multiple of 64) on paged caches too, needs
+     * no workspace where kvattn_plan reports one segment, and takes at most 65535 sequences. */
     KVATTN_KV_INT4 = 4,      /* scale = amax * (1/7); the half byte holds round(x / scale) + 8 */
     KVATTN_KV_FP4_E2M1 = 5   /* scale = amax * (1/6); sign and one of 0 .5 1 1.5 2 3 4 6,
                                 to nearest, ties to the even code */
@@ -390,10 +393,10 @@ int kvattn_paged_decode(void* out, const void* qkv, void* pages, float* page_sca
  *               number may be 0
  *   lens        [B] device: positions of sequence b, its new tokens among them; token i of n
  *               attends the first lens[b] - n + i + 1 of them (none: its output is zero)
- *   max_new     the most tokens of one sequence; with more, those beyond the next multiple of 8
- *               are left out
- * Rows of out behind token_start[B] are left as they were.  Values of token_start and lens are
- * clamped into [0, num_tokens] and [0, max_pages * page_rows].  Workspace:
+ *   max_new     the most tokens of one sequence (1, up to 4 and more take different kernels); a
+ *               sequence with more has the first max_new or more of them computed
+ * Rows of out behind token_start[B] are left as they were.  token_start must not decrease; it and
+ * lens are clamped into [0, num_tokens] and [0, max_pages * page_rows].  B <= 65535.  Workspace:
  * kvattn_workspace_bytes(num_tokens, NH, hs, max_pages * page_rows, S); S as in kvattn_decode with
  * a 4-bit cache.
  * No reference counterpart (the reference decodes one token at a time). */
@@ -420,11 +423,12 @@ int kvattn_paged_pool_init(int* pool, int num_pages, void* stream);
  *            ring, in request order, and entered behind the ones held; if negative, the last pages
  *            go back to the ring in the same order (to be taken by later calls).  Entries of
  *            block_table behind a request's pages are left as they were.
- *   held_out [B], lens [B]: kept + fresh.  Either may be its input (held, kept).
+ *   held_out [B], lens [B]: kept + fresh.  Either may be its own input (held, kept); apart from that
+ *            no output may share memory with an input or another output.
  *   token_start [B+1]: sums of fresh; tokens token_start[b] .. token_start[b+1]-1 are request b's
- *   slot_map [max_tokens]: page * page_rows + row of each token's position, for kvattn_paged_store
- *   positions [max_tokens] (may be NULL): each token's position
- *            Entries behind the last token are left as they were.
+ *   slot_map [max_tokens]: page * page_rows + row of each token's position, for kvattn_paged_store;
+ *            -1 behind the last token, so that a step captured for max_tokens tokens stores no more
+ *   positions [max_tokens] (may be NULL): each token's position; left as it was behind the last token
  *   pool_next [2] (may be NULL: the pool itself): the pool's first two words after the call.  With
  *            a buffer of its own the pool's words stay, so the call can be made again.
  * A request is refused, and keeps its pages and kept[b] positions (held_out = held, lens = kept), when

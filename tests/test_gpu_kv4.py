@@ -155,17 +155,17 @@ def test_decode_one_length_and_library_length(dev, kv):
     got = _decode(full, dev, q)
     full.lens = keep
     full.check(got, q, [(0, 0, 100), (1, 1, 1)], "clamped")
-    prev = torch.zeros(1, dtype=torch.int32)
     kvattn.set_cur_len(149)
     try:
         out = torch.empty(3, 2, HS, dtype=torch.bfloat16, device=dev)
         ws = kvattn.Workspace(3, 2, 200)
         q = case.queries(3)
-        kvattn.decode(out, _qkv(q, dev), _dev(case.packed, dev), 3, 2, HS, 200, kv_dtype=kv,
-                      kv_scale=_dev(case.scale, dev), **ws.kwargs())
-        case.check(out.float().cpu().numpy(), q, [(b, b, 150) for b in range(3)], "library length")
+        for per_seq in (False, True):      # the library holds one length, whatever is asked for
+            kvattn.decode(out, _qkv(q, dev), _dev(case.packed, dev), 3, 2, HS, 200, kv_dtype=kv,
+                          kv_scale=_dev(case.scale, dev), lens_per_seq=per_seq, **ws.kwargs())
+            case.check(out.float().cpu().numpy(), q, [(b, b, 150) for b in range(3)], "library length")
     finally:
-        kvattn.set_cur_len(int(prev[0]))
+        kvattn.set_cur_len(0)
 
 
 @pytest.mark.parametrize("kv", KV4)

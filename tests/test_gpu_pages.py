@@ -63,7 +63,7 @@ class Requests:
         assert np.array_equal(lens.cpu().numpy(), w[1])
         assert np.array_equal(start.cpu().numpy(), w[2])
         got, k = slots.cpu().numpy(), len(w[3])
-        assert np.array_equal(got[:k], w[3]) and (got[k:] == -9).all()
+        assert np.array_equal(got[:k], w[3]) and (got[k:most] == -1).all() and (got[max(most, k):] == -9).all()
         got = pos.cpu().numpy()
         if positions:
             assert np.array_equal(got[:k], w[4]) and (got[k:] == -9).all()
