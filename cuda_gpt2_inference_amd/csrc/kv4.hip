@@ -169,6 +169,9 @@ __device__ __forceinline__ float weight_of(float m, float M) { return m == -INFI
 // this keeps the compiler from moving one lane's reads over another's writes.
 __device__ __forceinline__ void lds_order() { asm volatile("" ::: "memory"); }
 
+// Keeps a wave's rare branch from becoming selects that every tile runs.
+__device__ __forceinline__ void stay_a_branch() { asm volatile(""); }
+
 // kQ: queries of a workgroup (1, 4 or 8); kW: its waves.
 template <bool kFp4, int kQ, int kW>
 __global__ __launch_bounds__(kW * kWave) __attribute__((amdgpu_waves_per_eu(4))) void attend4_kernel(Args a) {
@@ -250,6 +253,8 @@ __global__ __launch_bounds__(kW * kWave) __attribute__((amdgpu_waves_per_eu(4)))
         qa[0] = in_order<kFp4>(qp[0]);
         qa[1] = in_order<kFp4>(qp[1]);
     }
+    // Waited for here: left to the loop, their wait would hold up every tile for the next one's loads.
+    asm volatile("" : "+v"(qa[0]), "+v"(qa[1]));
     // INT4: the operand's codes are 8 too large, so every score starts at -8 times the sum of q.
     const Bf16x8 minus8 = (Bf16x8)(__bf16)(-8.0f);
     F32x4 s_init = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -260,11 +265,13 @@ __global__ __launch_bounds__(kW * kWave) __attribute__((amdgpu_waves_per_eu(4)))
     // Weights [query][upper, rest][place of a position]: with two positions a lane, those are neighbours.
     uint16_t* const lp = reinterpret_cast<uint16_t*>(lk);
     F32x4 acc[4] = {};                     // channels 16 c + 4 g + i of column col: query col % kQ
-    float m[kS], l[kS];                    // m: what the exponents are taken off, alike in a query's lanes
+    // m, alike in a query's lanes, is what the exponents are taken off (off: zero before the first score);
+    // limit: the score from which m follows.
+    float m[kS], off[kS], limit[kS], l[kS];
 #pragma unroll
     for (int i = 0; i < kS; ++i) {
-        m[i] = -INFINITY;
-        l[i] = 0.0f;
+        m[i] = limit[i] = -INFINITY;
+        off[i] = l[i] = 0.0f;
     }
     // Column col's weights: query col % kQ, part col / kQ (further columns repeat these).
     const int p_at = ((col & (kQ - 1)) * 2 + ((col / kQ) & 1)) * kTile + 8 * g;
@@ -321,15 +328,24 @@ __global__ __launch_bounds__(kW * kWave) __attribute__((amdgpu_waves_per_eu(4)))
         const bool masked = !there || pos + kTile > seen0;
         const int seen = there ? seen0 - pos - key0 + my_q : -kTile;     // query my_q + i sees position key0 + 32 j: seen + i > 32 j
         float sc[kC][kS];
-        bool grows = false;
 #pragma unroll
         for (int j = 0; j < kC; ++j)
 #pragma unroll
             for (int i = 0; i < kS; ++i) {
                 sc[j][i] = own[j][i] * ks[j];
-                if (masked) sc[j][i] = seen + i > 32 * j ? sc[j][i] : -INFINITY;
-                grows |= sc[j][i] > m[i] + kSlack;
             }
+        if (masked) {
+            stay_a_branch();
+#pragma unroll
+            for (int j = 0; j < kC; ++j)
+#pragma unroll
+                for (int i = 0; i < kS; ++i) sc[j][i] = seen + i > 32 * j ? sc[j][i] : -INFINITY;
+        }
+        bool grows = false;
+#pragma unroll
+        for (int j = 0; j < kC; ++j)
+#pragma unroll
+            for (int i = 0; i < kS; ++i) grows |= sc[j][i] > limit[i];
         // Exponents are taken off a maximum that may lag behind by kSlack: weights up to 2^kSlack lose
         // nothing, and after a wave's first tile this is rarely entered.
         if (__any(grows)) {
@@ -342,6 +358,8 @@ __global__ __launch_bounds__(kW * kWave) __attribute__((amdgpu_waves_per_eu(4)))
                 const float mn = fmaxf(m[i], top);
                 f[i] = weight_of(m[i], mn);
                 m[i] = mn;
+                off[i] = mn == -INFINITY ? 0.0f : mn;
+                limit[i] = mn + kSlack;
                 l[i] *= f[i];
             }
             float keep = f[0];
@@ -354,19 +372,28 @@ __global__ __launch_bounds__(kW * kWave) __attribute__((amdgpu_waves_per_eu(4)))
             for (int c = 0; c < 4; ++c) acc[c] *= keep;
         }
 #pragma unroll
+        for (int j = 0; j < kC; ++j)
+#pragma unroll
+            for (int i = 0; i < kS; ++i) {
+                // Not fused with the product that made the score: the largest one's difference is exact.
+#pragma clang fp contract(off)
+                const float p = exp2_fast(sc[j][i] - off[i]);
+                l[i] += p;
+                sc[j][i] = p * vs[j];
+            }
+        if (masked) {                      // a row that is not seen may have any scale
+            stay_a_branch();
+#pragma unroll
+            for (int j = 0; j < kC; ++j)
+#pragma unroll
+                for (int i = 0; i < kS; ++i) sc[j][i] = seen + i > 32 * j ? sc[j][i] : 0.0f;
+        }
+#pragma unroll
         for (int i = 0; i < kS; ++i) {
             uint32_t hi[kC], lo[kC];
 #pragma unroll
             for (int j = 0; j < kC; ++j) {
-                // Not fused with the product that made the score: the largest one's difference is exact.
-                float p;
-                {
-#pragma clang fp contract(off)
-                    p = exp2_fast(sc[j][i] - (m[i] == -INFINITY ? 0.0f : m[i]));
-                }
-                l[i] += p;
-                p *= vs[j];
-                if (masked) p = seen + i > 32 * j ? p : 0.0f;
+                const float p = sc[j][i];
                 hi[j] = __float_as_uint(p);
                 lo[j] = __float_as_uint(p - __uint_as_float(hi[j] & 0xffff0000u));
             }
