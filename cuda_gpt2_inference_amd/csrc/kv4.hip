@@ -61,6 +61,10 @@ constexpr int kMaxSegments = 65535;        // the grid's third side
 //   768 ragged heads of up to 1024             4 waves 1 / 2 segments 10.1 / 12.1, 8 waves 1 segment 11.1
 constexpr int kCUs = 256;
 constexpr int kSegTiles = 16;
+// A cache of more than these bytes is loaded as read only once (its scales are not: their lines are read in
+// parts).  64 sequences of 12 heads, us per call, with and without: 8192 ragged INT4 43.8 / 49.1, 4096 INT4
+// 39.9 / 45.4, 4096 ragged FP4 25.1 / 26.7; 16 of 4096 FP4 (57 MB) 12.6 / 11.8, 1 of 8000 7.7 / 7.4.
+constexpr long long kPositionBytes = 2 * (kRowBytes + 4), kCachedBytes = 128ll << 20;
 
 struct Args {
     const uint8_t* kv;
@@ -90,9 +94,11 @@ struct Raw {
 
 constexpr size_t kNoPage = ~(size_t)0;
 
-template <int kC>
-__device__ __forceinline__ Raw<kC> load_tile(const Args& a, size_t row0, int last, int lane, int key0) {
+template <int kC, bool kNt>
+__device__ __forceinline__ Raw<kC> load_tile(const Args& a, size_t row0, int last, int lane, int key0,
+                                              bool there) {
     Raw<kC> r;
+    r.there = there;
     const uint8_t* const k = a.kv + row0 * kRowBytes;
     const uint8_t* const v = k + a.v_rows * kRowBytes;
     const float* const s = a.sc + row0;
@@ -101,8 +107,8 @@ __device__ __forceinline__ Raw<kC> load_tile(const Args& a, size_t row0, int las
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
         const uint32_t at = (uint32_t)min((lane >> 1) + 32 * j, last) * kRowBytes + (lane & 1) * 16;
-        r.k[j] = load16<false>(k + at);
-        r.v[j] = load16<false>(v + at);
+        r.k[j] = load16<kNt>(k + at);
+        r.v[j] = load16<kNt>(v + at);
     }
 #pragma unroll
     for (int j = 0; j < kC; ++j) {
@@ -172,8 +178,8 @@ __device__ __forceinline__ void lds_order() { asm volatile("" ::: "memory"); }
 // Keeps a wave's rare branch from becoming selects that every tile runs.
 __device__ __forceinline__ void stay_a_branch() { asm volatile(""); }
 
-// kQ: queries of a workgroup (1, 4 or 8); kW: its waves.
-template <bool kFp4, int kQ, int kW>
+// kQ: queries of a workgroup (1, 4 or 8); kW: its waves; kNt: codes loaded as read only once.
+template <bool kFp4, int kQ, int kW, bool kNt>
 __global__ __launch_bounds__(kW * kWave) __attribute__((amdgpu_waves_per_eu(4))) void attend4_kernel(Args a) {
     __shared__ __align__(16) uint8_t lds[kW * kWaveLds];
     __shared__ float red_m[kW][kQ], red_l[kW][kQ];
@@ -218,41 +224,38 @@ __global__ __launch_bounds__(kW * kWave) __attribute__((amdgpu_waves_per_eu(4)))
         long long id = b;
         int in_page = pos;
         if (a.table) {
-            id = -1;
-            if (k0 + lane < mine) {
-                const int page = div_uniform(pos, a.R);
-                in_page = pos - page * a.R;
-                id = a.table[(size_t)b * a.max_pages + page];
-            }
-            if (id >= a.num_pages) id = -1;
+            const int page = div_uniform(pos, a.R);
+            in_page = pos - page * a.R;
+            id = a.table[(size_t)b * a.max_pages + min(page, a.max_pages - 1)];    // (lanes past the last tile)
         }
-        starts = id < 0 ? kNoPage : (size_t)(id * a.id_mul + h) * a.R + in_page;
+        const size_t start = (size_t)(id * a.id_mul + h) * a.R + in_page;
+        starts = a.table && (id < 0 || id >= a.num_pages) ? kNoPage : start;
     };
     auto start_of = [&](int k) {
         const int lo = __builtin_amdgcn_readlane((int)starts, k & (kWave - 1));
         const int hi = __builtin_amdgcn_readlane((int)(starts >> 32), k & (kWave - 1));
         return ((size_t)(unsigned)hi << 32) | (unsigned)lo;
     };
-    // The tile on its way.  (Two or three on their way, in registers, were 3 to 15 % slower.)
+    // The tile on its way.  Every tile's work asks for the next, behind the last a row again that is there: on a
+    // path without, the compiler would count on fewer loads in flight and wait for the newest.  (Two on their
+    // way, each waited for alone: 0 to 8 % slower.)
     Raw<kC> raw;
+    size_t row0 = 0;
     auto request = [&](int k) {
-        if (k >= mine) return;
         if ((k & (kWave - 1)) == 0) load_starts(k);
+        const size_t start = start_of(k);
         const int pos = (first + wave + k * kW) * kTile;
-        const size_t row0 = start_of(k);
-        raw = load_tile<kC>(a, row0 == kNoPage ? 0 : row0, min(kTile, rows - pos) - 1, lane, key0);
-        raw.there = row0 != kNoPage;
+        raw.there = k < mine && start != kNoPage;
+        if (raw.there) row0 = start;
+        raw = load_tile<kC, kNt>(a, row0, k < mine ? min(kTile, rows - pos) - 1 : 0, lane, key0, raw.there);
     };
-    request(0);
-
     // The left operand: row i is query i % kQ (the last one again past it).
-    Bf16x8 qa[2];
-    {
-        const int qi = min(col % kQ, nq - 1);
-        const uint4* qp = reinterpret_cast<const uint4*>(a.qkv + ((size_t)(t0 + q0 + qi) * 3 * a.NH + h) * kHd + 16 * g);
-        qa[0] = in_order<kFp4>(qp[0]);
-        qa[1] = in_order<kFp4>(qp[1]);
-    }
+    const int qi = min(col % kQ, nq - 1);
+    const uint4* const qp = reinterpret_cast<const uint4*>(a.qkv + ((size_t)(t0 + q0 + qi) * 3 * a.NH + h) * kHd + 16 * g);
+    const uint4 qw[2] = {qp[0], qp[1]};
+    lds_order();
+    request(0);
+    Bf16x8 qa[2] = {in_order<kFp4>(qw[0]), in_order<kFp4>(qw[1])};
     // Waited for here: left to the loop, their wait would hold up every tile for the next one's loads.
     asm volatile("" : "+v"(qa[0]), "+v"(qa[1]));
     // INT4: the operand's codes are 8 too large, so every score starts at -8 times the sum of q.
@@ -285,8 +288,9 @@ __global__ __launch_bounds__(kW * kWave) __attribute__((amdgpu_waves_per_eu(4)))
         float ks[kC], vs[kC];
 #pragma unroll
         for (int j = 0; j < kC; ++j) {
-            ks[j] = raw.ks[j] * kQScale;
-            vs[j] = raw.vs[j];
+            // (Copies that the compiler sees would share the next scales' registers, and be made at the tile's end.)
+            asm volatile("v_mov_b32 %0, %2\n\tv_mov_b32 %1, %3" : "=&v"(ks[j]), "=&v"(vs[j]) : "v"(raw.ks[j]), "v"(raw.vs[j]));
+            ks[j] *= kQScale;
         }
         lds_order();
 #pragma unroll
@@ -511,10 +515,14 @@ __global__ __launch_bounds__(kW * kWave) __attribute__((amdgpu_waves_per_eu(4)))
     }
 }
 
+template <int kQ, int kW>
+const void* kernel_for(bool fp4, bool nt) {
+    if (nt) return fp4 ? (const void*)&attend4_kernel<true, kQ, kW, true> : (const void*)&attend4_kernel<false, kQ, kW, true>;
+    return fp4 ? (const void*)&attend4_kernel<true, kQ, kW, false> : (const void*)&attend4_kernel<false, kQ, kW, false>;
+}
 template <int kQ>
-const void* kernel_for(bool fp4, int waves) {
-    if (waves == 8) return fp4 ? (const void*)&attend4_kernel<true, kQ, 8> : (const void*)&attend4_kernel<false, kQ, 8>;
-    return fp4 ? (const void*)&attend4_kernel<true, kQ, 4> : (const void*)&attend4_kernel<false, kQ, 4>;
+const void* kernel_for(bool fp4, int waves, bool nt) {
+    return waves == 8 ? kernel_for<kQ, 8>(fp4, nt) : kernel_for<kQ, 4>(fp4, nt);
 }
 
 }  // namespace
@@ -548,7 +556,7 @@ int plan4(int heads, int maxT, int len_hint, bool ragged, int S, Plan4& p) {
 int attend4(const Attend4& c, bool launch) {
     Plan4 plan;
     // Queries of a workgroup: the fewest that take a sequence's new tokens at once, up to eight.
-    const int most_new = c.start ? c.max_new : 1;
+    const int most_new = c.start ? std::min(c.max_new, c.num_tokens) : 1;
     const int per = most_new == 1 ? 1 : (most_new <= 4 ? 4 : 8);
     const int groups = (most_new + per - 1) / per;
     const int st = plan4((int)std::min<long long>((long long)c.B * c.NH * groups, 1 << 30), c.maxT, c.len_hint,
@@ -589,8 +597,11 @@ int attend4(const Attend4& c, bool launch) {
     a.seg_tiles = plan.seg_tiles;
     a.num_tokens = c.num_tokens;
     const bool fp4 = c.kv_dtype == KVATTN_KV_FP4_E2M1;
-    const void* fn = per == 1 ? kernel_for<1>(fp4, plan.waves) : per == 4 ? kernel_for<4>(fp4, plan.waves)
-                                                                           : kernel_for<8>(fp4, plan.waves);
+    long long positions = (long long)c.B * (c.len_hint >= 0 ? c.len_hint + 1 : c.maxT);
+    if (c.table) positions = std::min(positions, (long long)c.num_pages * c.page_rows);
+    const bool nt = positions > kCachedBytes / kPositionBytes / c.NH;
+    const void* fn = per == 1 ? kernel_for<1>(fp4, plan.waves, nt) : per == 4 ? kernel_for<4>(fp4, plan.waves, nt)
+                                                                              : kernel_for<8>(fp4, plan.waves, nt);
     void* params[] = {&a};
     const hipError_t e = hipLaunchKernel(fn, dim3((unsigned)rows, c.B, plan.S), dim3(plan.waves * kWave), params, 0,
                                          (hipStream_t)c.stream);

@@ -442,7 +442,8 @@ def paged_pool(num_pages, device="cuda", stream=None):
     if nbytes == 0:
         raise KvAttnError(ERR_SHAPE, "kvattn_paged_pool_bytes")
     pool = torch.empty(nbytes // 4, dtype=torch.int32, device=device)
-    _check(lib().kvattn_paged_pool_init(_ptr(pool), int(num_pages), _stream(stream)), "kvattn_paged_pool_init")
+    with torch.cuda.device(pool.device):
+        _check(lib().kvattn_paged_pool_init(_ptr(pool), int(num_pages), _stream(stream)), "kvattn_paged_pool_init")
     return pool
 
 

@@ -67,12 +67,13 @@ typedef enum kvattn_dtype {
     KVATTN_KV_INT8 = 2,      /* reference USE_KV_W8 + USE_INT8 (Makefile:80-82,100-106) */
     KVATTN_KV_FP8_E4M3 = 3,  /* reference USE_KV_W8 + USE_FP8 (Makefile:83-85,100-106) */
     /* 4-bit caches: 32 bytes a row, channel 2i in the low half of byte i and 2i+1 in the high
-     * half, one float scale a row (1/7 and 1/6 rounded to float); qkv and out are bf16.  No reference counterpart (its cache
-     * types end at 8 bits).  Taken by kvattn_cache_write, kvattn_append, kvattn_decode,
+     * half, one float scale a row (1/7 and 1/6 rounded to float); qkv and out are bf16.  No
+     * reference counterpart (its cache types end at 8 bits).  Taken by kvattn_cache_write, kvattn_append, kvattn_decode,
      * kvattn_append_decode (two launches), kvattn_plan and the kvattn_paged_* calls; the others
      * return KVATTN_ERR_DTYPE.  Attention over them has one strategy, KVATTN_SPLIT_LASTBLOCK
      * (KVATTN_AUTO takes it), takes S > 0 and S < 0 (a multiple of 64) on paged caches too, needs
-     * no workspace where kvattn_plan reports one segment, and takes at most 65535 sequences. */
+     * no workspace where kvattn_plan reports one segment and the batch has one length, and takes
+     * at most 65535 sequences. */
     KVATTN_KV_INT4 = 4,      /* scale = amax * (1/7); the half byte holds round(x / scale) + 8 */
     KVATTN_KV_FP4_E2M1 = 5   /* scale = amax * (1/6); sign and one of 0 .5 1 1.5 2 3 4 6,
                                 to nearest, ties to the even code */
@@ -393,8 +394,9 @@ int kvattn_paged_decode(void* out, const void* qkv, void* pages, float* page_sca
  *               number may be 0
  *   lens        [B] device: positions of sequence b, its new tokens among them; token i of n
  *               attends the first lens[b] - n + i + 1 of them (none: its output is zero)
- *   max_new     the most tokens of one sequence (1, up to 4 and more take different kernels); a
- *               sequence with more has the first max_new or more of them computed
+ *   max_new     the most tokens of one sequence (1, up to 4 and more take different kernels), or
+ *               any larger number; a sequence with more has the first max_new or more of them
+ *               computed
  * Rows of out behind token_start[B] are left as they were.  token_start must not decrease; it and
  * lens are clamped into [0, num_tokens] and [0, max_pages * page_rows].  B <= 65535.  Workspace:
  * kvattn_workspace_bytes(num_tokens, NH, hs, max_pages * page_rows, S); S as in kvattn_decode with
