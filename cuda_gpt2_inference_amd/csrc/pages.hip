@@ -449,6 +449,11 @@ __global__ __launch_bounds__(kBlock) void store_rows_kernel(RowsArgs a) {
     }
 }
 
+__device__ __forceinline__ void store16_nt(uint4* p, const uint4& v) {
+    typedef unsigned U32x4 __attribute__((ext_vector_type(4)));
+    __builtin_nontemporal_store(U32x4{v.x, v.y, v.z, v.w}, reinterpret_cast<U32x4*>(p));
+}
+
 template <int DT>
 __global__ __launch_bounds__(kBlock) void load_rows_kernel(RowsArgs a) {
     using F = Fmt<DT>;
@@ -480,7 +485,9 @@ __global__ __launch_bounds__(kBlock) void load_rows_kernel(RowsArgs a) {
 #pragma unroll
         for (int e = 0; e < 4; ++e)
             o[e] = f32_to_bf16(x[2 * e] * scale) | (uint32_t)f32_to_bf16(x[2 * e + 1] * scale) << 16;
-        *to = make_uint4(o[0], o[1], o[2], o[3]);
+        // Past the caches: what is loaded is mostly more than they hold (8192 tokens in and out 18.8 us without,
+        // 17.8 so; 160 tokens 4.9 both ways).  The same for what is stored costs 1.4 us.
+        store16_nt(to, make_uint4(o[0], o[1], o[2], o[3]));
     }
 }
 
