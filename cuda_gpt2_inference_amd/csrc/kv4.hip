@@ -52,15 +52,17 @@ constexpr int kMaxSegments = 65535;        // the grid's third side
 // AUTO's shapes.  Up to one head a CU, workgroups of 8 waves, in as many segments as there are CUs; beyond,
 // 4 waves, in segments that fill four workgroups a CU, and with ragged lengths past 6144 positions of
 // about 32 tiles, so that the longest sequence is not waited for alone.  No segment is shorter than 16
-// tiles (a join of segments costs 1.5 to 2 us).  us per call, FP4 unless said, GPU time:
-//   12 heads of 1024 positions   8 waves 1 segment 5.0, 4 waves 1 / 4 segments 5.5 / 5.7
-//   12 heads of 8000             8 waves 8 / 4 / 1 segments 7.3 / 8.6 / 17.4, 4 waves 8 segments 7.9
-//   192 heads of 4096            8 waves 1 / 2 segments 12.4 / 15.0, 4 waves 4 / 1 segments 13.8 / 16.8
-//   288 ragged heads of up to 4096, 8 tokens   4 waves 3 / 1 segments 17.8 / 22.3, 8 waves 2 segments 17.1
-//   768 ragged heads of up to 8192, INT4       4 waves 4 / 1 segments 49.4 / 50.3, 8 waves 1 segment 50.7
-//   768 ragged heads of up to 1024             4 waves 1 / 2 segments 10.1 / 12.1, 8 waves 1 segment 11.1
+// tiles (a join of segments costs 1 us and more), except where 4 waves split ragged lengths: the long
+// sequences' joins are waited for anyway, and the shorter ones end earlier.  us per call, FP4 unless said:
+//   12 heads of 1024 positions   8 waves 1 / 4 segments 4.7 / 5.8, 4 waves 1 / 4 segments 5.1 / 5.7
+//   12 heads of 8000             8 waves 8 / 4 / 1 segments 7.4 / 8.5 / 15.2, 4 waves 8 segments 7.8
+//   192 heads of 4096            8 waves 1 / 2 segments 11.8 / 14.7, 4 waves 4 / 1 segments 13.5 / 13.1
+//   288 ragged heads of up to 4096, 8 tokens   4 waves 3 segments 16.4, of 16 tiles at least 17.6, 1 18.3;
+//                                              8 waves 1 / 2 segments 16.2 / 16.8
+//   768 ragged heads of up to 8192, INT4       4 waves 4 / 1 segments 43.6 / 46.7, 8 waves 1 segment 46.3
+//   768 ragged heads of up to 1024             4 waves 1 / 2 segments 9.2 / 12.1, 8 waves 1 segment 11.0
 constexpr int kCUs = 256;
-constexpr int kSegTiles = 16;
+constexpr int kSegTiles = 16, kRaggedSegTiles = 4;
 // A cache of more than these bytes is loaded as read only once (its scales are not: their lines are read in
 // parts).  64 sequences of 12 heads, us per call, with and without: 8192 ragged INT4 43.8 / 49.1, 4096 INT4
 // 39.9 / 45.4, 4096 ragged FP4 25.1 / 26.7; 16 of 4096 FP4 (57 MB) 12.6 / 11.8, 1 of 8000 7.7 / 7.4.
@@ -207,8 +209,11 @@ __global__ __launch_bounds__(kW * kWave) __attribute__((amdgpu_waves_per_eu(4)))
     const int seen0 = total - n + q0 + 1;
     const int rows = max(seen0 + nq - 1, 0);
     const int tiles = (rows + kTile - 1) / kTile;
-    const int seg_tiles = max(a.seg_tiles, (tiles + a.S - 1) / a.S);
-    const int segs = max(1, (tiles + seg_tiles - 1) / seg_tiles);
+    int segs = 1, seg_tiles = tiles;
+    if (a.S > 1) {
+        seg_tiles = max(a.seg_tiles, (tiles + a.S - 1) / a.S);
+        segs = max(1, (tiles + seg_tiles - 1) / seg_tiles);
+    }
     if (s >= segs) return;
     const int first = s * seg_tiles, end = min(tiles, first + seg_tiles);
 
@@ -549,7 +554,8 @@ int plan4(int heads, int maxT, int len_hint, bool ragged, int S, Plan4& p) {
     p.S = std::min(p.S, (tiles + kSegTiles - 1) / kSegTiles);
     if (p.waves == 4 && ragged && tiles >= 96) p.S = std::max(p.S, tiles / 32);
     p.S = std::max(1, std::min(p.S, kMaxSegments));
-    p.seg_tiles = kSegTiles;               // or ceil(tiles / S), on the device
+    // Or ceil(tiles / S), on the device.
+    p.seg_tiles = p.waves == 4 && ragged && p.S > 1 ? kRaggedSegTiles : kSegTiles;
     return KVATTN_OK;
 }
 
