@@ -1,7 +1,7 @@
 // kv4.hip -- decode attention over a 4-bit KV cache on MI355X (gfx950), for one or several new
 // tokens of every sequence.
 //
-// A row costs 36 bytes, so at the memory's rate a wave has about 27 cycles for each: the products go
+// A row costs 36 bytes, so at the memory's rate a SIMD has about 17 cycles for each: the products go
 // to the matrix cores (16x16x32 bf16: codes and q are exact there, sums are float), which leaves the
 // vector units the codes' conversion and the softmax.  A wave walks tiles of 64 positions with an
 // online softmax.

@@ -53,7 +53,8 @@ def _key(row) -> str:
 
 
 OWN_KERNELS = ("split_kernel", "merge_kernel", "fused_single_kernel", "cache_write", "gemv_kernel", "gemm_kernel",
-               "gemm_tall_kernel", "set_len_kernel")
+               "gemm_tall_kernel", "set_len_kernel", "attend4_kernel", "reserve_kernel", "store_rows_kernel",
+               "load_rows_kernel", "verify_kernel")
 
 
 def _phases(d: str):
