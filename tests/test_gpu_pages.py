@@ -187,6 +187,57 @@ def test_reserve_captured(dev):
         torch.zeros(1000, device=dev).sum().item()
 
 
+def test_reserve_captured_many_requests(dev):
+    """A captured call whose requests need more LDS than a launch gets by itself, replayed in place."""
+    import torch
+    kvattn = _kv()
+    B, n, R, P, most = 3500, 2, 64, 6000, 40000
+    r = np.random.RandomState(4)
+    rq = Requests(dev, B, n, R, P)
+    z = lambda k, t=torch.int32: torch.zeros(k, dtype=t, device=dev)         # noqa: E731
+    kept, fresh, lens, start, slots = z(B), z(B), z(B), z(B + 1), z(most, torch.int64)
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        kvattn.paged_reserve(rq.cache, rq.pool, rq.d_held, kept, fresh, B, lens=lens, token_start=start, slot_map=slots,
+                             max_tokens=most)
+    for i in range(4):
+        k = np.where(r.rand(B) < 0.3, 0, rq.held)
+        f = np.minimum(r.randint(0, 20, B), n * R - k)
+        kept.copy_(_i32(k, dev))
+        fresh.copy_(_i32(f, dev))
+        graph.replay()
+        torch.cuda.synchronize()
+        w = rq.model.reserve(rq.table, R, rq.held, k, f, most)
+        rq.held = w[0]
+        assert np.array_equal(rq.d_table.cpu().numpy(), rq.table) and np.array_equal(rq.d_held.cpu().numpy(), w[0])
+        assert np.array_equal(lens.cpu().numpy(), w[1]) and np.array_equal(start.cpu().numpy(), w[2])
+        assert rq.pool[:4].tolist() == [rq.model.head, rq.model.count, 0, 0]
+        assert np.array_equal(slots[:len(w[3])].cpu().numpy(), w[3]) and (slots[len(w[3]):] == -1).all()
+
+
+def test_reserve_and_rows_on_another_stream(dev):
+    """Current stream not the default one: every call goes to it, in order."""
+    import torch
+    kvattn = _kv()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        B, n, R, P, NH = 6, 4, 64, 20, 3
+        rq = Requests(dev, B, n, R, P)
+        w = rq.step(np.zeros(B, np.int64), np.array([70, 0, 3, 64, 65, 128]), 400, in_place=False)
+        slots = torch.from_numpy(np.asarray(w[3], dtype=np.int64)).to(dev)
+        N = len(w[3])
+        pages, scales = _pool("bf16", P, NH, R, dev)
+        qkv = torch.randn(N, 3, NH, HS, device=dev).to(torch.bfloat16)
+        cache = kvattn.PagedCache(pages, None, n, R, P, scales)
+        kvattn.paged_store(cache, qkv, slots, N, NH, HS, kv_dtype="bf16")
+        back = torch.zeros(N, 2, NH, HS, dtype=torch.bfloat16, device=dev)
+        kvattn.paged_load(back, cache, slots, N, NH, HS, kv_dtype="bf16")
+        assert torch.equal(back, qkv[:, 1:])
+    torch.cuda.current_stream().wait_stream(side)
+
+
 # ------------------------------------------------------------------------------------
 # Rows by slot.
 # ------------------------------------------------------------------------------------

@@ -173,6 +173,30 @@ def test_wrong_starts_stay_inside(dev):
     assert np.array_equal(got[0], want[0]) and list(got[1]) == list(want[1]) + [0]
 
 
+@pytest.mark.parametrize("counts,V", [([5, 1, 0, 8], 50257), ([4] * 40, 3000), ([100, 3], 200)])
+def test_tokens_in_the_drafts_place(dev, counts, V):
+    """tokens may be draft_tokens, here on another stream than the default one."""
+    import torch
+    kvattn = _kv()
+    r = np.random.RandomState(14)
+    p, q, drafts, u, start = _case(r, counts, V, V, "f32", False, spare=2)
+    want = kv4ref.verify(p.astype(np.float64), q.astype(np.float64), drafts, u, start, V)
+    t = lambda x, d: torch.from_numpy(np.ascontiguousarray(x)).to(d).to(dev)      # noqa: E731
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        tokens, counted = t(drafts, torch.int32), torch.zeros(len(counts), dtype=torch.int32, device=dev)
+        nbytes = kvattn.verify_workspace_bytes(len(counts), V)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        kvattn.workspace_init(ws, nbytes)
+        kvattn.verify_drafts(tokens, counted, t(p, torch.float32), tokens, t(u, torch.float32), t(start, torch.int32), len(counts),
+                             len(u), V, draft_probs=t(q, torch.float32), workspace=ws, workspace_nbytes=nbytes)
+        got = tokens.cpu().numpy()
+    n = int(start[-1])
+    assert np.array_equal(got[:n], want[0][:n]) and np.array_equal(got[n:], drafts[n:])
+    assert np.array_equal(counted.cpu().numpy(), want[1])
+
+
 def test_repeats_and_capture(dev):
     """The workspace is left as it was; a captured call replayed on new numbers equals the eager one."""
     import torch
