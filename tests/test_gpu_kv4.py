@@ -468,23 +468,6 @@ def test_captured_step(dev, kv):
 
 
 @pytest.mark.parametrize("kv", KV4)
-def test_another_stream(dev, kv):
-    import torch
-    kvattn = _kv()
-    case = Case(kv, 1, 2, 700, [700], seed=32)
-    q = case.queries(1)
-    side = torch.cuda.Stream()
-    codes, scale, qkv = _dev(case.packed, dev), _dev(case.scale, dev), _qkv(q, dev)
-    cur = torch.tensor([699], dtype=torch.int32, device=dev)
-    ws = kvattn.Workspace(1, 2, 700)
-    out = torch.empty(1, 2, HS, dtype=torch.bfloat16, device=dev)
-    torch.cuda.synchronize()
-    kvattn.decode(out, qkv, codes, 1, 2, HS, 700, kv_dtype=kv, kv_scale=scale, cur_len=cur, stream=side, **ws.kwargs())
-    side.synchronize()
-    case.check(out.float().cpu().numpy(), q, [(0, 0, 700)], "side stream")
-
-
-@pytest.mark.parametrize("kv", KV4)
 def test_rows_past_32_bit_offsets(dev, kv):
     """Pages whose bytes lie beyond 4 GiB of the pool, and beyond 2^31 rows' worth of elements."""
     import torch

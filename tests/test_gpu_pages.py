@@ -216,28 +216,6 @@ def test_reserve_captured_many_requests(dev):
         assert np.array_equal(slots[:len(w[3])].cpu().numpy(), w[3]) and (slots[len(w[3]):] == -1).all()
 
 
-def test_reserve_and_rows_on_another_stream(dev):
-    """Current stream not the default one: every call goes to it, in order."""
-    import torch
-    kvattn = _kv()
-    side = torch.cuda.Stream()
-    side.wait_stream(torch.cuda.current_stream())
-    with torch.cuda.stream(side):
-        B, n, R, P, NH = 6, 4, 64, 20, 3
-        rq = Requests(dev, B, n, R, P)
-        w = rq.step(np.zeros(B, np.int64), np.array([70, 0, 3, 64, 65, 128]), 400, in_place=False)
-        slots = torch.from_numpy(np.asarray(w[3], dtype=np.int64)).to(dev)
-        N = len(w[3])
-        pages, scales = _pool("bf16", P, NH, R, dev)
-        qkv = torch.randn(N, 3, NH, HS, device=dev).to(torch.bfloat16)
-        cache = kvattn.PagedCache(pages, None, n, R, P, scales)
-        kvattn.paged_store(cache, qkv, slots, N, NH, HS, kv_dtype="bf16")
-        back = torch.zeros(N, 2, NH, HS, dtype=torch.bfloat16, device=dev)
-        kvattn.paged_load(back, cache, slots, N, NH, HS, kv_dtype="bf16")
-        assert torch.equal(back, qkv[:, 1:])
-    torch.cuda.current_stream().wait_stream(side)
-
-
 # ------------------------------------------------------------------------------------
 # Rows by slot.
 # ------------------------------------------------------------------------------------

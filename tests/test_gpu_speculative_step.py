@@ -140,3 +140,44 @@ def test_steps(dev, kv):
         kept = np.where(lens == kept + fresh, kept + counts, kept)
         kept = np.minimum(kept, held)
     assert refused > 0, "the pool is small enough that some step was refused"
+
+
+def test_pages_and_rows_on_another_stream(dev):
+    """Current stream not the default one: every call goes to it, in order."""
+    import torch
+    from cuda_gpt2_inference_amd import kvattn
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        fresh = [70, 0, 3, 64, 65, 128]
+        b, n, P, N = len(fresh), 4, 20, sum(fresh)
+        z = lambda *s, d=torch.int32: torch.zeros(s, dtype=d, device=dev)       # noqa: E731
+        cache = kvattn.PagedCache(z(P, 2, NH, R, HS, d=torch.bfloat16), z(b, n), n, R, P)
+        pool, lens, start, slots = kvattn.paged_pool(P, device=dev), z(b), z(b + 1), z(N, d=torch.int64)
+        kvattn.paged_reserve(cache, pool, z(b), z(b), torch.tensor(fresh, dtype=torch.int32, device=dev), b, lens=lens,
+                             token_start=start, slot_map=slots, max_tokens=N)
+        assert lens.tolist() == fresh and start[-1] == N and len(set(slots.tolist())) == N and slots.min() >= 0
+        qkv = torch.randn(N, 3, NH, HS, device=dev).to(torch.bfloat16)
+        kvattn.paged_store(cache, qkv, slots, N, NH, HS, kv_dtype="bf16")
+        back = torch.zeros(N, 2, NH, HS, dtype=torch.bfloat16, device=dev)
+        kvattn.paged_load(back, cache, slots, N, NH, HS, kv_dtype="bf16")
+        assert torch.equal(back, qkv[:, 1:])
+    torch.cuda.current_stream().wait_stream(side)
+
+
+@pytest.mark.parametrize("kv", ["int4", "fp4"])
+def test_decode_on_another_stream(dev, kv):
+    import torch
+    from cuda_gpt2_inference_amd import kvattn
+    from test_gpu_kv4 import Case, _dev, _qkv
+    case = Case(kv, 1, 2, 700, [700], seed=32)
+    q = case.queries(1)
+    side = torch.cuda.Stream()
+    codes, scale, qkv = _dev(case.packed, dev), _dev(case.scale, dev), _qkv(q, dev)
+    cur = torch.tensor([699], dtype=torch.int32, device=dev)
+    ws = kvattn.Workspace(1, 2, 700)
+    out = torch.empty(1, 2, HS, dtype=torch.bfloat16, device=dev)
+    torch.cuda.synchronize()
+    kvattn.decode(out, qkv, codes, 1, 2, HS, 700, kv_dtype=kv, kv_scale=scale, cur_len=cur, stream=side, **ws.kwargs())
+    side.synchronize()
+    case.check(out.float().cpu().numpy(), q, [(0, 0, 700)], "side stream")
