@@ -59,6 +59,7 @@ struct ReserveArgs {
     int* pool_next;
     int max_pages, R, num_pages, B, max_tokens;
     int shift;                 // log2 of R, or -1
+    int grid;                  // workgroups
 };
 
 __device__ __forceinline__ int add_sat(int a, int b) {   // a, b >= 0
@@ -78,31 +79,41 @@ __device__ __forceinline__ int wave_prefix(int x) {
     return x;
 }
 
+// A barrier for what was written to LDS: global reads and writes stay on their way (__syncthreads waits for them).
+__device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+// The largest over the wave's lanes (values >= 0), in every lane.
+__device__ __forceinline__ int wave_top(int x) {
+    x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x111, 0xF, 0xF, true));
+    x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x112, 0xF, 0xF, true));
+    x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x114, 0xF, 0xF, true));
+    x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x118, 0xF, 0xF, true));
+    x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x142, 0xA, 0xF, true));
+    x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x143, 0xC, 0xF, true));
+    return __builtin_amdgcn_readlane(x, kWave - 1);
+}
+
 // Exclusive prefixes of kN values over the workgroup's threads, and their totals.  Subtraction undoes a
 // sum only where nothing was cut off, so the values themselves are shifted by a lane.
 template <int kThreads, int kN>
 __device__ __forceinline__ void block_prefix(const int (&v)[kN], int (&wave_sums)[kN][kThreads / kWave], int (&prefix)[kN],
                                              int (&total)[kN]) {
-    const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+    const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     int in[kN];
 #pragma unroll
     for (int n = 0; n < kN; ++n) {
         in[n] = wave_prefix(v[n]);
         if (lane == kWave - 1) wave_sums[n][wave] = in[n];
     }
-    __syncthreads();
+    lds_barrier();
+    // The waves' sums: a prefix over the first lanes of every wave.
 #pragma unroll
     for (int n = 0; n < kN; ++n) {
-        int before = 0, all = 0;
-#pragma unroll
-        for (int w = 0; w < kThreads / kWave; ++w) {
-            const int s = wave_sums[n][w];
-            before = w < wave ? add_sat(before, s) : before;
-            all = add_sat(all, s);
-        }
+        const int upto = wave_prefix(lane < kThreads / kWave ? wave_sums[n][lane] : 0);
+        const int before = wave > 0 ? __builtin_amdgcn_readlane(upto, wave - 1) : 0;
         const int up = __shfl_up(in[n], 1);
         prefix[n] = add_sat(before, lane > 0 ? up : 0);
-        total[n] = all;
+        total[n] = __builtin_amdgcn_readlane(upto, kWave - 1);
     }
 }
 
@@ -116,12 +127,25 @@ __device__ __forceinline__ int owner(const int* start, int lo, int hi, int x) {
     return lo;
 }
 
-template <int kThreads>
+// The same for an x that the wave's lanes share, over all of n entries: 64 of them looked at at once.
+__device__ __forceinline__ int owner_of(const int* start, int n, int x) {
+    const int lane = threadIdx.x & (kWave - 1);
+    int lo = 0;
+    for (int step = n > kWave ? kWave : 1;; step = 1) {
+        const int i = lo + lane * step;
+        const unsigned long long at = __ballot(i < n && start[min(i, n - 1)] <= x);
+        lo += (63 - __clzll((long long)(at | 1))) * step;
+        if (step == 1) return lo;
+    }
+}
+
+// kOne: no more requests than threads, so that a thread's own one stays in its registers.
+template <int kThreads, bool kOne>
 __global__ __launch_bounds__(kThreads) void reserve_kernel(ReserveArgs a) {
     extern __shared__ int lds[];
     __shared__ int asked_sums[2][kThreads / kWave], given_sums[1][kThreads / kWave];
-    __shared__ int shared_took, shared_turn, run_ends[2];
-    constexpr int kOwn = kThreads == kSmallThreads ? 1 : kMaxRequests / kThreads;   // requests a thread reads
+    __shared__ int took_sums[kThreads / kWave], shared_turn;
+    constexpr int kOwn = kOne ? 1 : kMaxRequests / kThreads;   // requests a thread reads
     int* const tok = lds;                 // first token
     int* const take = tok + a.B;          // first of the pages it takes
     int* const give = take + a.B;         // first of the pages it gives back
@@ -136,8 +160,12 @@ __global__ __launch_bounds__(kThreads) void reserve_kernel(ReserveArgs a) {
     auto pages_of = [&](int positions) {
         return a.shift >= 0 ? (positions + a.R - 1) >> a.shift : (positions + a.R - 1) / a.R;
     };
-    // Tokens and pages asked for.  A request whose lengths make no sense asks for nothing.
+    // A request's tokens and pages; one whose lengths make no sense asks for nothing.
+    struct Request {
+        int tok, have, want, kept;
+    };
     int hd_own[kOwn], kp_own[kOwn];
+    Request own = {0, 0, 0, kRefused};
 #pragma unroll
     for (int j = 0; j < kOwn; ++j) {
         const int i = tid + j * kThreads;
@@ -146,18 +174,23 @@ __global__ __launch_bounds__(kThreads) void reserve_kernel(ReserveArgs a) {
         hd_own[j] = hd;
         kp_own[j] = kp;
         const bool ok = kp >= 0 && kp <= hd && hd <= most && fr >= 0 && (long long)kp + fr <= most;
-        have[i] = ok ? pages_of(hd) : 0;
-        want[i] = ok ? pages_of(kp + fr) : 0;
-        kept[i] = ok ? kp : kRefused;
-        tok[i] = ok ? fr : 0;
+        own = {ok ? fr : 0, ok ? pages_of(hd) : 0, ok ? pages_of(kp + fr) : 0, ok ? kp : kRefused};
+        have[i] = own.have;
+        if constexpr (!kOne) {
+            want[i] = own.want;
+            kept[i] = own.kept;
+            tok[i] = own.tok;
+        }
     }
-    if (tid == 0) shared_took = 0;
-    __syncthreads();
-    const int each = (a.B + kThreads - 1) / kThreads, i0 = min(tid * each, a.B), i1 = min(i0 + each, a.B);
+    // Then a run of requests for every thread (one: the same).
+    const int each = kOne ? 1 : (a.B + kThreads - 1) / kThreads, i0 = min(tid * each, a.B), i1 = min(i0 + each, a.B);
+    if constexpr (!kOne) lds_barrier();
+    auto request = [&](int i) { return kOne ? own : Request{tok[i], have[i], want[i], kept[i]}; };
     int asked[2] = {0, 0}, before_me[2], all_asked[2];
     for (int i = i0; i < i1; ++i) {
-        asked[0] = add_sat(asked[0], tok[i]);
-        asked[1] = add_sat(asked[1], max(want[i] - have[i], 0));
+        const Request r = request(i);
+        asked[0] = add_sat(asked[0], r.tok);
+        asked[1] = add_sat(asked[1], max(r.want - r.have, 0));
     }
     block_prefix<kThreads, 2>(asked, asked_sums, before_me, all_asked);
     int t = before_me[0], k = before_me[1];
@@ -166,32 +199,37 @@ __global__ __launch_bounds__(kThreads) void reserve_kernel(ReserveArgs a) {
     // for want of pages (or tokens), so is every later one that takes any, so pages taken have no gaps.
     int gives[1] = {0}, took = 0, gv[1], all_gives[1];
     for (int i = i0; i < i1; ++i) {
-        const int fr = tok[i], tk = max(want[i] - have[i], 0);
+        Request r = request(i);
+        const int tk = max(r.want - r.have, 0);
         tok[i] = t;
         take[i] = k;
-        t = add_sat(t, fr);
+        t = add_sat(t, r.tok);
         k = add_sat(k, tk);
-        const bool ok = !(kept[i] & kRefused) && (tk == 0 || k <= count) && (fr == 0 || t <= a.max_tokens);
+        const bool ok = !(r.kept & kRefused) && (tk == 0 || k <= count) && (r.tok == 0 || t <= a.max_tokens);
         if (!ok) {
-            kept[i] |= kRefused;
-            want[i] = have[i];
+            r.kept |= kRefused;
+            r.want = r.have;
         }
+        kept[i] = r.kept;
+        want[i] = r.want;
+        if constexpr (kOne) own = r;
         if (ok && tk > 0) took = k;
-        gives[0] = add_sat(gives[0], max(have[i] - want[i], 0));
+        gives[0] = add_sat(gives[0], max(r.have - r.want, 0));
     }
-    if (took > 0) atomicMax(&shared_took, took);
+    took = wave_top(took);
+    if ((tid & (kWave - 1)) == 0) took_sums[tid / kWave] = took;
     block_prefix<kThreads, 1>(gives, given_sums, gv, all_gives);
     for (int i = i0; i < i1; ++i) {
         give[i] = gv[0];
-        gv[0] = add_sat(gv[0], max(have[i] - want[i], 0));
+        if constexpr (!kOne) gv[0] = add_sat(gv[0], max(have[i] - want[i], 0));
     }
     // Everything that another workgroup's outputs may overwrite has been read.  Whose turn it is to write
     // those is asked now and looked at last: the answer's way back is not waited for.
     wait_vm_stores();
-    __syncthreads();
-    const int all_took = shared_took;
-    unsigned before = gridDim.x - 1;
-    if (gridDim.x > 1 && tid == 0)
+    lds_barrier();
+    const int all_took = wave_top((tid & (kWave - 1)) < kThreads / kWave ? took_sums[tid & (kWave - 1)] : 0);
+    unsigned before = 0;
+    if (tid == 0 && a.grid > 1)
         before = __hip_atomic_fetch_add((unsigned*)a.pool + kPoolTicket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 
     int* const ring = a.pool + kPoolRing;
@@ -201,15 +239,13 @@ __global__ __launch_bounds__(kThreads) void reserve_kernel(ReserveArgs a) {
     };
     // Tokens: a run of neighbours for every workgroup, whose owners lie between its ends'.
     const int n_tok = min(all_toks, a.max_tokens);
-    const int run = (n_tok + gridDim.x - 1) / gridDim.x;
+    const int run = (n_tok + a.grid - 1) / a.grid;
     const int x0 = min((int)blockIdx.x * run, n_tok), x1 = min(x0 + run, n_tok);
     if (x0 < x1) {
         int b0 = 0, b1 = a.B - 1;
-        if (gridDim.x > 1) {
-            if (tid < 2) run_ends[tid] = owner(tok, 0, a.B - 1, tid == 0 ? x0 : x1 - 1);
-            __syncthreads();
-            b0 = run_ends[0];
-            b1 = run_ends[1];
+        if (a.grid > 1) {
+            b0 = owner_of(tok, a.B, x0);
+            b1 = owner_of(tok, a.B, x1 - 1);
         }
 #pragma unroll 4
         for (int x = x0 + tid; x < x1; x += kThreads) {
@@ -228,10 +264,10 @@ __global__ __launch_bounds__(kThreads) void reserve_kernel(ReserveArgs a) {
         }
     }
     // Rows behind the last token, so that a step captured for max_tokens stores nothing for them.
-    for (int x = n_tok + blockIdx.x * kThreads + tid; x < a.max_tokens; x += gridDim.x * kThreads) a.slot_map[x] = -1;
+    for (int x = n_tok + blockIdx.x * kThreads + tid; x < a.max_tokens; x += a.grid * kThreads) a.slot_map[x] = -1;
     // Pages taken, from the last thread on, and given back, from the middle on: a small call's three
     // kinds of work fall to different waves and wait side by side.
-    const int step = gridDim.x * kThreads, me = blockIdx.x * kThreads + tid;
+    const int step = a.grid * kThreads, me = blockIdx.x * kThreads + tid;
     for (int x = step - 1 - me; x < all_took; x += step) {
         const int b = owner(take, 0, a.B - 1, x);
         a.table[(size_t)b * a.max_pages + have[b] + x - take[b]] = ring[ring_at(x)];
@@ -243,11 +279,12 @@ __global__ __launch_bounds__(kThreads) void reserve_kernel(ReserveArgs a) {
         ring[ring_at(count + x)] = a.table[(size_t)b * a.max_pages + want[b] + x - give[b]];
     }
     if (tid == 0) {
-        shared_turn = before == gridDim.x - 1;
-        if (shared_turn && gridDim.x > 1)
+        asm volatile("" : "+v"(before));      // not compared, and so waited for, before this
+        shared_turn = a.grid == 1 || before == (unsigned)a.grid - 1;
+        if (shared_turn && a.grid > 1)
             __hip_atomic_store((unsigned*)a.pool + kPoolTicket, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
-    __syncthreads();
+    lds_barrier();
     if (!shared_turn) return;
 #pragma unroll
     for (int j = 0; j < kOwn; ++j) {
@@ -574,20 +611,22 @@ int kvattn_paged_reserve(int* block_table, int max_pages, int page_rows, int num
         if ((uintptr_t)p & 3u) return KVATTN_ERR_MISALIGNED;
     if ((uintptr_t)slot_map & 7u) return KVATTN_ERR_MISALIGNED;
     ReserveArgs a{block_table, pool, held, kept, fresh, held_out, lens, token_start, slot_map, positions, pool_next,
-                  max_pages, page_rows, num_pages, B, max_tokens, log2_or(page_rows)};
+                  max_pages, page_rows, num_pages, B, max_tokens, log2_or(page_rows), 1};
     const int lds = kRequestInts * B * (int)sizeof(int);
     static_assert(kRequestInts * kMaxRequests * sizeof(int) <= 128 * 1024, "LDS of a CU");
     const bool small = B <= kSmallThreads && max_tokens <= 4 * kSmallThreads;
     const int threads = small ? kSmallThreads : kReserveThreads;
-    const void* fn = small ? (const void*)&reserve_kernel<kSmallThreads> : (const void*)&reserve_kernel<kReserveThreads>;
+    const void* fn = small ? (const void*)&reserve_kernel<kSmallThreads, true>
+                           : (B <= kReserveThreads ? (const void*)&reserve_kernel<kReserveThreads, true>
+                                                   : (const void*)&reserve_kernel<kReserveThreads, false>);
     if (lds > 64 * 1024) {
         const int st = hip_status(hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, lds));
         if (st != KVATTN_OK) return st;
     }
     const long long blocks = ((long long)max_tokens + kReserveTokens - 1) / kReserveTokens;
-    const unsigned grid = (unsigned)(small || blocks < 1 ? 1 : blocks > kReserveMostBlocks ? kReserveMostBlocks : blocks);
+    a.grid = (int)(small || blocks < 1 ? 1 : blocks > kReserveMostBlocks ? kReserveMostBlocks : blocks);
     void* params[] = {&a};
-    return hip_status(hipLaunchKernel(fn, dim3(grid), dim3(threads), params, (size_t)lds, (hipStream_t)stream));
+    return hip_status(hipLaunchKernel(fn, dim3(a.grid), dim3(threads), params, (size_t)lds, (hipStream_t)stream));
 }
 
 int kvattn_paged_store(void* pages, float* page_scales, int page_rows, int num_pages, const long long* slot_map,
