@@ -88,8 +88,9 @@ __device__ __forceinline__ void tile_probs(const void* p, size_t row0, int tile,
         }
 }
 
-// What a token weighs: a finite positive number, or nothing.
-__device__ __forceinline__ double mass(double w) { return w > 0.0 && w < INFINITY ? w : 0.0; }
+// What a token weighs: a positive number, or nothing; NaN, which what is not finite becomes (x + 0 x), nothing.
+__device__ __forceinline__ double finite(float x) { return (double)fmaf(x, 0.0f, x); }
+__device__ __forceinline__ double mass(double w) { return fmax(w, 0.0); }
 
 // Sums across lanes through DPP, as the float ones: a shuffle's trip through LDS in each of the six
 // steps of four sums added up to a microsecond.
@@ -182,11 +183,19 @@ __global__ __launch_bounds__(kBlock) void verify_kernel(VerifyArgs a) {
         double rest = 0.0, all = 0.0;
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-            const double w = (double)p[e];
+            const double w = finite(p[e]);
             all += mass(w);
-            // A draft without probabilities had it all, and leaves its own token nothing.
-            if (less_q) rest += mass(w - (double)q[e]);
-            else rest += token_at<false>(tile, e / 4, lane) + e % 4 == draft ? 0.0 : mass(w);
+            if (less_q) rest += mass(w - finite(q[e]));
+        }
+        // A draft without probabilities had it all, and leaves its own token nothing.
+        if (!less_q) {
+            rest = all;
+            if (draft >= 0 && draft / kTile == tile) {
+                rest = 0.0;
+#pragma unroll
+                for (int e = 0; e < 16; ++e)
+                    rest += token_at<false>(tile, e / 4, lane) + e % 4 == draft ? 0.0 : mass(finite(p[e]));
+            }
         }
         rest = wave_sum64(rest);
         all = wave_sum64(all);
@@ -254,24 +263,24 @@ __global__ __launch_bounds__(kBlock) void verify_kernel(VerifyArgs a) {
         float p[16], q[16];
         tile_probs<kF32, kVec, true>(a.p, row0, tile, a.V, lane, p);
         if (use_rest && less_q) tile_probs<kF32, kVec, true>(a.q, row0, tile, a.V, lane, q);
-        double w[16], mine = 0.0;
+        double upto[16], mine = 0.0;       // running sums of this lane's
+        bool some_at[16];
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-            w[e] = (double)p[e];
-            if (use_rest && less_q) w[e] -= (double)q[e];
-            w[e] = mass(w[e]);
-            if (use_rest && tile * kTile + lane * 16 + e == draft && !less_q) w[e] = 0.0;
-            mine += w[e];
+            double w = finite(p[e]);
+            if (use_rest && less_q) w -= finite(q[e]);
+            w = mass(w);
+            if (use_rest && tile * kTile + lane * 16 + e == draft && !less_q) w = 0.0;
+            some_at[e] = w > 0.0;
+            upto[e] = mine += w;
         }
-        double run = base + (wave_prefix64(mine) - mine);
+        base += wave_prefix64(mine) - mine;
         int hit = -1, last = -1;
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-            run += w[e];
-            if (w[e] > 0.0) {
-                last = tile * kTile + lane * 16 + e;
-                if (hit < 0 && run > aim) hit = last;
-            }
+        for (int e = 15; e >= 0; --e) {
+            const int v = tile * kTile + lane * 16 + e;
+            if (some_at[e] && last < 0) last = v;
+            if (some_at[e] && base + upto[e] > aim) hit = v;
         }
         const unsigned long long pass = __ballot(hit >= 0), some = __ballot(last >= 0);
         if (pass) drawn = __shfl(hit, __ffsll((long long)pass) - 1);
