@@ -12,8 +12,11 @@
 // sums, the tile).  Workgroups of a sequence run on one XCD, so that the values that each of them looks
 // up, and the tile that is read again, come from its L2.  One workgroup of 16 waves a sequence, whose
 // sums stay in LDS, saves the join's round trips but draws the row through one CU: 19 us against 8 for
-// one sequence, 32 against 13 for 64.  Workgroups of 4 / 8 / 16 waves: one sequence 6.7 / 7.1 / 7.6 us, 64
-// of them 12.1 / 11.5 / 10.7, 300 22.6 / 21.4 / 23.6.
+// one sequence, 32 against 13 for 64 (before the steps below).  A wave's arithmetic counts next to the round trips:
+// a weight of five instructions in place of eight, and the drawn token's tile divided among four
+// waves, took one sequence from 7.2 to 5.8 us, 64 from 11.3 to 10.2.  Workgroups of 4 / 8 / 16 waves:
+// one sequence 5.6 / 5.8 / 6.3 us, 64 of them 10.5 / 10.2 / 9.5, 300 19.6 / 19.2 / 20.8.  One / two workgroups
+// a CU: 64 10.6 / 10.5, 300 21.6 / 19.4.
 #include <hip/hip_runtime.h>
 
 #include "kvattn.h"
@@ -28,9 +31,11 @@ namespace {
 constexpr int kBlock = 512;
 constexpr int kWaves = kBlock / kWave;
 constexpr int kTile = 16 * kWave;         // tokens of a wave's tile: 16 a lane
+constexpr int kRuns = 4;                  // runs of a tile: neighbouring tokens of all lanes
+static_assert(kWaves >= kRuns && kTile == kRuns * 4 * kWave, "a wave for every run");
 constexpr int kMaxVocab = 1 << 24;
 constexpr int kMaxSequences = 1 << 16;
-constexpr int kFillBlocks = 256;          // workgroups that keep the memory busy, one a CU
+constexpr int kFillBlocks = 512;          // workgroups that keep the memory busy, two a CU
 
 struct VerifyArgs {
     int* tokens;
@@ -64,28 +69,32 @@ __device__ __forceinline__ void probs4(const void* p, size_t row0, int v, float*
     }
 }
 
-// A lane's 16 probabilities of a tile: kNear: 16 neighbours, else four runs of four, each run next to
-// the neighbouring lanes'.  Zero past the vocabulary.  The branch is the wave's, so that all of the
-// tile's loads are on their way at once.
-template <bool kNear>
-__device__ __forceinline__ int token_at(int tile, int j, int lane) {
-    return tile * kTile + (kNear ? lane * 16 + j * 4 : (j * kWave + lane) * 4);
-}
-template <bool kF32, bool kVec, bool kNear>
-__device__ __forceinline__ void tile_probs(const void* p, size_t row0, int tile, int V, int lane, float (&x)[16]) {
+// A lane's probabilities of a tile: four neighbours from token_at on in each of its four runs, where they
+// lie next to the neighbouring lanes'.  Zero past the vocabulary.  The branch is the wave's, so that all
+// of the loads are on their way at once.
+__device__ __forceinline__ int token_at(int tile, int run, int lane) { return tile * kTile + (run * kWave + lane) * 4; }
+template <bool kF32, bool kVec>
+__device__ __forceinline__ void run_probs(const void* p, size_t row0, int tile, int run, int V, int lane, float* x) {
+    const int v0 = token_at(tile, run, lane);
     if (kVec && tile * kTile + kTile <= V) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) probs4<kF32>(p, row0, token_at<kNear>(tile, j, lane), x + 4 * j);
+        probs4<kF32>(p, row0, v0, x);
         return;
     }
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
+    for (int i = 0; i < 4; ++i) {
+        const float w = prob<kF32>(p, row0 + min(v0 + i, V - 1));
+        x[i] = v0 + i < V ? w : 0.0f;
+    }
+}
+template <bool kF32, bool kVec>
+__device__ __forceinline__ void tile_probs(const void* p, size_t row0, int tile, int V, int lane, float (&x)[16]) {
+    if (kVec && tile * kTile + kTile <= V) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int v = token_at<kNear>(tile, j, lane) + i;
-            const float w = prob<kF32>(p, row0 + min(v, V - 1));
-            x[4 * j + i] = v < V ? w : 0.0f;
-        }
+        for (int j = 0; j < 4; ++j) probs4<kF32>(p, row0, token_at(tile, j, lane), x + 4 * j);
+        return;
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) run_probs<kF32, false>(p, row0, tile, j, V, lane, x + 4 * j);
 }
 
 // What a token weighs: a positive number, or nothing; NaN, which what is not finite becomes (x + 0 x), nothing.
@@ -140,6 +149,7 @@ __device__ __forceinline__ double get64(const double* p) {
 template <bool kF32, bool kVec>
 __global__ __launch_bounds__(kBlock) void verify_kernel(VerifyArgs a) {
     __shared__ int is_last;
+    __shared__ double run_sums[kRuns];
     const int slot = xcd_slot(blockIdx.x, a.blocks), b = slot / a.blocks, blk = slot - b * a.blocks;
     if (b >= a.B) return;
     const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
@@ -152,12 +162,13 @@ __global__ __launch_bounds__(kBlock) void verify_kernel(VerifyArgs a) {
     const float u_last = a.u[t0 + n - 1];  // a number that no draft is held against
     // The first row whose draft is not accepted (the last row has none): 64 rows at a time, a lane
     // each.  The comparison is exact: products of two floats fit a double.
-    int row = n - 1;
+    int row = n - 1, draft = -1;
     for (int i0 = 0; i0 < n - 1; i0 += kWave) {
         const int i = i0 + lane;
         bool no = false;
+        int x = -1;
         if (i < n - 1) {
-            const int x = a.drafts[t0 + i];
+            x = a.drafts[t0 + i];
             const size_t at = (size_t)(t0 + i) * a.row + x;
             no = !(x >= 0 && x < a.V);
             if (!no) {
@@ -167,19 +178,20 @@ __global__ __launch_bounds__(kBlock) void verify_kernel(VerifyArgs a) {
         }
         const unsigned long long refused = __ballot(no);
         if (refused) {
-            row = i0 + __ffsll((long long)refused) - 1;
+            const int at = __ffsll((long long)refused) - 1;
+            row = i0 + at;
+            draft = __builtin_amdgcn_readlane(x, at);
             break;
         }
     }
     const bool refused = row < n - 1;
-    const int draft = refused ? a.drafts[t0 + row] : -1;
     const bool less_q = refused && a.q;
     const size_t row0 = (size_t)(t0 + row) * a.row;
 
     for (int tile = blk * kWaves + wave; tile < a.tiles; tile += a.blocks * kWaves) {
         float p[16], q[16];
-        tile_probs<kF32, kVec, false>(a.p, row0, tile, a.V, lane, p);
-        if (less_q) tile_probs<kF32, kVec, false>(a.q, row0, tile, a.V, lane, q);
+        tile_probs<kF32, kVec>(a.p, row0, tile, a.V, lane, p);
+        if (less_q) tile_probs<kF32, kVec>(a.q, row0, tile, a.V, lane, q);
         double rest = 0.0, all = 0.0;
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
@@ -194,7 +206,7 @@ __global__ __launch_bounds__(kBlock) void verify_kernel(VerifyArgs a) {
                 rest = 0.0;
 #pragma unroll
                 for (int e = 0; e < 16; ++e)
-                    rest += token_at<false>(tile, e / 4, lane) + e % 4 == draft ? 0.0 : mass(finite(p[e]));
+                    rest += token_at(tile, e / 4, lane) + e % 4 == draft ? 0.0 : mass(finite(p[e]));
             }
         }
         rest = wave_sum64(rest);
@@ -215,7 +227,7 @@ __global__ __launch_bounds__(kBlock) void verify_kernel(VerifyArgs a) {
     }
     __syncthreads();
     if (!is_last) return;
-    if (wave != 0) return;
+    if (wave >= kRuns) return;
 
     // Totals, and which weights count: where a refused draft leaves nothing (p = q), p's own.
     const double* const s = a.sums + (size_t)b * a.tiles * 2;
@@ -243,7 +255,7 @@ __global__ __launch_bounds__(kBlock) void verify_kernel(VerifyArgs a) {
     int drawn = -1;
     if (total > 0.0) {
         // The first tile whose running sum passes the aim (rounding may leave none: the last that weighs
-        // anything), then the first token in it likewise.
+        // anything), then the first run of it, then the first token likewise.
         int tile = -1;
         double base = 0.0, before = 0.0;
         for (int t1 = 0; t1 < a.tiles; t1 += kWave) {
@@ -260,31 +272,51 @@ __global__ __launch_bounds__(kBlock) void verify_kernel(VerifyArgs a) {
             if (pass) break;
             before = __shfl(upto, kWave - 1);
         }
-        float p[16], q[16];
-        tile_probs<kF32, kVec, true>(a.p, row0, tile, a.V, lane, p);
-        if (use_rest && less_q) tile_probs<kF32, kVec, true>(a.q, row0, tile, a.V, lane, q);
-        double upto[16], mine = 0.0;       // running sums of this lane's
-        bool some_at[16];
+        // Every wave takes one of the tile's runs; the one that the aim falls into goes on.
+        float p[4], q[4];
+        run_probs<kF32, kVec>(a.p, row0, tile, wave, a.V, lane, p);
+        if (use_rest && less_q) run_probs<kF32, kVec>(a.q, row0, tile, wave, a.V, lane, q);
+        const int v0 = token_at(tile, wave, lane);
+        double w[4], mine = 0.0;
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-            double w = finite(p[e]);
-            if (use_rest && less_q) w -= finite(q[e]);
-            w = mass(w);
-            if (use_rest && tile * kTile + lane * 16 + e == draft && !less_q) w = 0.0;
-            some_at[e] = w > 0.0;
-            upto[e] = mine += w;
+        for (int i = 0; i < 4; ++i) {
+            w[i] = finite(p[i]);
+            if (use_rest && less_q) w[i] -= finite(q[i]);
+            w[i] = use_rest && !less_q && v0 + i == draft ? 0.0 : mass(w[i]);
+            mine += w[i];
         }
-        base += wave_prefix64(mine) - mine;
+        const double sum = wave_prefix64(mine);
+        if (lane == kWave - 1) run_sums[wave] = sum;
+        __syncthreads();
+        int run = -1;
+        double run0 = 0.0;
+        bool passed = false;
+#pragma unroll
+        for (int j = 0; j < kRuns; ++j) {
+            const double r = run_sums[j];
+            if (r > 0.0 && !passed) {
+                run = j;
+                run0 = base;
+                passed = base + r > aim;
+            }
+            base += r;
+        }
+        if (wave != run) return;
+        double upto = run0 + (sum - mine);
         int hit = -1, last = -1;
 #pragma unroll
-        for (int e = 15; e >= 0; --e) {
-            const int v = tile * kTile + lane * 16 + e;
-            if (some_at[e] && last < 0) last = v;
-            if (some_at[e] && base + upto[e] > aim) hit = v;
+        for (int i = 0; i < 4; ++i) {
+            upto += w[i];
+            if (w[i] > 0.0) {
+                last = v0 + i;
+                if (hit < 0 && upto > aim) hit = last;
+            }
         }
         const unsigned long long pass = __ballot(hit >= 0), some = __ballot(last >= 0);
         if (pass) drawn = __shfl(hit, __ffsll((long long)pass) - 1);
         else if (some) drawn = __shfl(last, 63 - __clzll((long long)some));
+    } else if (wave != 0) {
+        return;
     }
     for (int i = lane; i < n; i += kWave) a.tokens[t0 + i] = i < row ? a.drafts[t0 + i] : (i == row ? drawn : -1);
     if (lane == 0) a.count[b] = row + (drawn >= 0 ? 1 : 0);
