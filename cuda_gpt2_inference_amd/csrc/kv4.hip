@@ -45,6 +45,7 @@ constexpr int kTile = 64;                  // positions of a tile
 constexpr int kRowBytes = 32;
 constexpr int kTileBytes = kTile * kRowBytes;
 constexpr int kWaveLds = 2 * kTileBytes;   // K (then the weights), V
+constexpr int kOutPad = kHd + 4;            // floats from one query's outputs to the next in LDS: other banks
 constexpr float kQScale = 0.125f * 1.4426950408889634f;    // 1/sqrt(64) * log2(e)
 constexpr float kSlack = 8.0f;
 constexpr int kMaxT = 1 << 23;
@@ -186,7 +187,7 @@ __global__ __launch_bounds__(kW * kWave) __attribute__((amdgpu_waves_per_eu(4)))
     __shared__ __align__(16) uint8_t lds[kW * kWaveLds];
     __shared__ float red_m[kW][kQ], red_l[kW][kQ];
     __shared__ int is_last;
-    static_assert(kQ * kHd * 4 <= kWaveLds && kQ * 2 * kTile * 2 <= kTileBytes, "outputs and weights take a tile's place");
+    static_assert(kQ * kOutPad * 4 <= kWaveLds && kQ * 2 * kTile * 2 <= kTileBytes, "outputs and weights take a tile's place");
     // A lane scores kC positions of a tile for kS of the queries.
     constexpr int kC = kQ <= 4 ? 1 : 2, kS = kQ == 1 ? 1 : 4;
 
@@ -438,7 +439,7 @@ __global__ __launch_bounds__(kW * kWave) __attribute__((amdgpu_waves_per_eu(4)))
         for (int i = 0; i < 4; ++i)
             acc[c][i] += kQ == 1 ? dpp<kDppQuadXor1>(acc[c][i])
                                  : (kQ == 4 ? dpp<kDppRowRor4>(acc[c][i]) : dpp<kDppRowRor8>(acc[c][i]));
-        if (col < kQ) *reinterpret_cast<F32x4*>(ro + col * kHd + 16 * c + 4 * g) = acc[c];
+        if (col < kQ) *reinterpret_cast<F32x4*>(ro + col * kOutPad + 16 * c + 4 * g) = acc[c];
     }
 #pragma unroll
     for (int i = 0; i < kS; ++i) {
@@ -459,7 +460,7 @@ __global__ __launch_bounds__(kW * kWave) __attribute__((amdgpu_waves_per_eu(4)))
         for (int w = 0; w < kW; ++w) {
             const float f = weight_of(red_m[w][qq], M);
             L += f * red_l[w][qq];
-            o += f * reinterpret_cast<const float*>(lds + w * kWaveLds)[e];
+            o += f * reinterpret_cast<const float*>(lds + w * kWaveLds)[qq * kOutPad + ch];
         }
         const size_t head = (tok0 + qq) * a.NH + h;
         if (segs == 1) {
