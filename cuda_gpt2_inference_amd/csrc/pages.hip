@@ -144,7 +144,7 @@ __device__ __forceinline__ int owner_of(const int* start, int n, int x) {
 // kWaves: no more than lanes, and every wave does all of them for itself, with a copy in LDS of its own,
 // so that nobody waits for anybody (24 requests 4.1 us, 3.7 so).
 enum Each { kMany, kOne, kWaves };
-template <int kThreads, Each kEach>
+template <int kThreads, int kEach>
 __global__ __launch_bounds__(kThreads) void reserve_kernel(ReserveArgs a) {
     extern __shared__ int lds[];
     __shared__ int asked_sums[2][kThreads / kWave], given_sums[1][kThreads / kWave];
