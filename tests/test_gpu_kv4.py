@@ -238,22 +238,22 @@ def test_paged_decode_tokens(dev, kv, counts, S):
 
 
 @pytest.mark.parametrize("kv", KV4)
-@pytest.mark.parametrize("counts", [[1, 1, 1], [2, 4, 0], [3, 8, 1]])
+@pytest.mark.parametrize("counts", [[1, 1, 1], [2, 4, 0], [3, 8, 1], [1] * 140, [3, 0, 1, 2] * 35, [5, 1] * 70])
 def test_paged_decode_tokens_large_pool(dev, kv, counts):
     """A pool of more than 128 MiB, of which the loads are others (as read only once), and room for 320000
     positions a sequence; no bound on the tokens of one."""
     import torch
     kvattn = _kv()
     R, NH, P, room = 64, 2, 15000, 5000
-    case = Case(kv, 3, NH, 256, [256, 65, 130], seed=16)
-    N = sum(counts)
+    B, N = len(counts), sum(counts)
+    case = Case(kv, B, NH, 256, ([256, 65, 130] + [9 + i for i in range(B)])[:B], seed=16)
     q = case.queries(N)
     small, table = case.paged(R, dev)
     front = P - small.num_pages             # the rows lie in the last pages
     pages = torch.full((P, 2, NH, R, HS // 2), 0xFF, dtype=torch.uint8, device=dev)
     scales = torch.full((P, 2, NH, R), float("nan"), dtype=torch.float32, device=dev)
     pages[front:], scales[front:] = small.pages, small.page_scales
-    wide = np.full((3, room), -1, dtype=np.int32)
+    wide = np.full((B, room), -1, dtype=np.int32)
     wide[:, :table.shape[1]] = table + front
     cache = kvattn.PagedCache(pages, _dev(wide, dev), room, R, P, scales)
     start = np.concatenate([[0], np.cumsum(counts)]).astype(np.int32)
@@ -261,7 +261,7 @@ def test_paged_decode_tokens_large_pool(dev, kv, counts):
     ws = kvattn.Workspace(N, NH, room * R)
     for most in (max(counts), 2 ** 31 - 1):
         out = torch.full((N, NH, HS), 7.0, dtype=torch.bfloat16, device=dev)
-        kvattn.paged_decode_tokens(out, _qkv(q, dev), cache, _dev(start, dev), _dev(np.array(case.lens, np.int32), dev), 3, N,
+        kvattn.paged_decode_tokens(out, _qkv(q, dev), cache, _dev(start, dev), _dev(np.array(case.lens, np.int32), dev), B, N,
                                    NH, HS, kv_dtype=kv, max_new=most, **ws.kwargs())
         case.check(out.float().cpu().numpy(), q, tokens, f"counts {counts} most {most}")
 

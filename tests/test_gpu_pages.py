@@ -74,6 +74,7 @@ class Requests:
 
 @pytest.mark.parametrize("B,n,R,P,top,most", [
     (1, 1, 1, 1, 1, 1), (1, 8, 64, 8, 300, 300), (5, 4, 64, 12, 90, 200), (64, 16, 64, 300, 8, 512),
+    (65, 16, 64, 300, 8, 512), (200, 8, 64, 400, 6, 1000),
     (257, 12, 96, 900, 400, 30000), (1000, 33, 64, 9000, 300, 200000), (4096, 4, 128, 5000, 200, 100000),
 ])
 @pytest.mark.parametrize("in_place", [True, False])
