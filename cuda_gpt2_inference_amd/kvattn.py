@@ -168,6 +168,26 @@ def _ptr(x) -> Optional[int]:
     return x.data_ptr()
 
 
+class _Calls:
+    """The entry points that return a status, bound at their first use: each takes tensors, addresses, integers
+    and None as they are (_pycall.Call; without it ctypes, and _ptr for every argument)."""
+
+    def __getattr__(self, name):
+        fn = getattr(lib(), name)
+        try:
+            from ._pycall import Call
+        except ImportError:
+            def call(*args):
+                return fn(*map(_ptr, args))
+        else:
+            call = Call(ctypes.cast(fn, _vp).value, len(SIGNATURES[name][1]))
+        setattr(self, name, call)
+        return call
+
+
+_call = _Calls()
+
+
 # The handle of torch's current stream on the current device.  torch.cuda.current_stream() builds
 # a Stream object for it, 2.8 us of an eager call's 8.3 us; the handle alone takes 0.1 us.
 _current_stream = None
@@ -224,8 +244,8 @@ def set_cur_len_async(cur_len: int, d_cur_len=None, stream=None) -> None:
 def kv_cache_write(kv_cache, qkv, B, NH, hs, maxT, *, kv_dtype, kv_scale=None, cur_len=None,
                    lens_per_seq=False, stream=None) -> None:
     """Append the current token's K/V (reference kv_cache_write_kernel[_w8])."""
-    _check(lib().kvattn_cache_write(_ptr(kv_cache), _ptr(kv_scale), _ptr(qkv), B, NH, hs, maxT,
-                                    _ptr(cur_len), int(bool(lens_per_seq)), kv_dtype_code(kv_dtype),
+    _check(_call.kvattn_cache_write(kv_cache, kv_scale, qkv, B, NH, hs, maxT, cur_len,
+                                    int(bool(lens_per_seq)), kv_dtype_code(kv_dtype),
                                     _stream(stream)), "kvattn_cache_write")
 
 
@@ -327,8 +347,8 @@ def decode(out, qkv, kv_cache, B, NH, hs, maxT, *, kv_dtype, kv_scale=None, cur_
            lens_per_seq=False, len_hint=-1, workspace=None, workspace_nbytes=0, S=0, strategy="auto",
            stream=None) -> None:
     """One decode-attention call with an explicit strategy (kvattn_decode)."""
-    _check(lib().kvattn_decode(_ptr(out), _ptr(qkv), _ptr(kv_cache), _ptr(kv_scale), B, NH, hs, maxT,
-                               _ptr(cur_len), int(bool(lens_per_seq)), int(len_hint), _ptr(workspace),
+    _check(_call.kvattn_decode(out, qkv, kv_cache, kv_scale, B, NH, hs, maxT,
+                               cur_len, int(bool(lens_per_seq)), int(len_hint), workspace,
                                int(workspace_nbytes), int(S), strategy_code(strategy),
                                kv_dtype_code(kv_dtype), _stream(stream)), "kvattn_decode")
 
@@ -347,8 +367,8 @@ def append_decode(out, qkv, kv_cache, B, NH, hs, maxT, *, kv_dtype, kv_scale=Non
                   lens_per_seq=False, len_hint=-1, workspace=None, workspace_nbytes=0, S=0, strategy="auto",
                   stream=None) -> None:
     """kv_cache_write + decode in one launch (kvattn_append_decode)."""
-    _check(lib().kvattn_append_decode(_ptr(out), _ptr(qkv), _ptr(kv_cache), _ptr(kv_scale), B, NH, hs, maxT,
-                                      _ptr(cur_len), int(bool(lens_per_seq)), int(len_hint), _ptr(workspace),
+    _check(_call.kvattn_append_decode(out, qkv, kv_cache, kv_scale, B, NH, hs, maxT,
+                                      cur_len, int(bool(lens_per_seq)), int(len_hint), workspace,
                                       int(workspace_nbytes), int(S), strategy_code(strategy),
                                       kv_dtype_code(kv_dtype), _stream(stream)), "kvattn_append_decode")
 
@@ -400,14 +420,14 @@ class PagedCache:
         return self.max_pages * self.page_rows
 
     def _args(self):
-        return (_ptr(self.pages), _ptr(self.page_scales), _ptr(self.block_table), self.max_pages, self.page_rows,
+        return (self.pages, self.page_scales, self.block_table, self.max_pages, self.page_rows,
                 self.num_pages)
 
 
 def paged_cache_write(cache: PagedCache, qkv, B, NH, hs, *, kv_dtype, cur_len=None, lens_per_seq=False,
                       stream=None) -> None:
     """kv_cache_write into a paged cache (kvattn_paged_cache_write)."""
-    _check(lib().kvattn_paged_cache_write(*cache._args(), _ptr(qkv), B, NH, hs, _ptr(cur_len),
+    _check(_call.kvattn_paged_cache_write(*cache._args(), qkv, B, NH, hs, cur_len,
                                           int(bool(lens_per_seq)), kv_dtype_code(kv_dtype), _stream(stream)),
            "kvattn_paged_cache_write")
 
@@ -417,8 +437,8 @@ def paged_decode(out, qkv, cache: PagedCache, B, NH, hs, *, kv_dtype, cur_len=No
                  stream=None) -> None:
     """decode / append_decode on a paged cache (kvattn_paged_decode)."""
     p = cache._args()
-    _check(lib().kvattn_paged_decode(_ptr(out), _ptr(qkv), p[0], p[1], p[2], p[3], p[4], p[5], B, NH, hs,
-                                     _ptr(cur_len), int(bool(lens_per_seq)), int(len_hint), _ptr(workspace),
+    _check(_call.kvattn_paged_decode(out, qkv, p[0], p[1], p[2], p[3], p[4], p[5], B, NH, hs,
+                                     cur_len, int(bool(lens_per_seq)), int(len_hint), workspace,
                                      int(workspace_nbytes), int(S), strategy_code(strategy),
                                      kv_dtype_code(kv_dtype), int(bool(append)), _stream(stream)),
            "kvattn_paged_decode")
@@ -428,10 +448,10 @@ def paged_decode_tokens(out, qkv, cache: PagedCache, token_start, lens, B, num_t
                         workspace=None, workspace_nbytes=0, S=0, stream=None) -> None:
     """Attention of several new tokens of every sequence over a paged 4-bit cache that holds their rows
     (kvattn_paged_decode_tokens); the workspace is that of num_tokens sequences."""
-    _check(lib().kvattn_paged_decode_tokens(_ptr(out), _ptr(qkv), _ptr(cache.pages), _ptr(cache.page_scales),
-                                            _ptr(cache.block_table), cache.max_pages, cache.page_rows, cache.num_pages,
-                                            _ptr(token_start), _ptr(lens), B, num_tokens, int(max_new), NH, hs,
-                                            _ptr(workspace), int(workspace_nbytes), int(S), kv_dtype_code(kv_dtype),
+    _check(_call.kvattn_paged_decode_tokens(out, qkv, cache.pages, cache.page_scales, cache.block_table,
+                                            cache.max_pages, cache.page_rows, cache.num_pages, token_start, lens, B,
+                                            num_tokens, int(max_new), NH, hs, workspace, int(workspace_nbytes),
+                                            int(S), kv_dtype_code(kv_dtype),
                                             _stream(stream)), "kvattn_paged_decode_tokens")
 
 
@@ -451,24 +471,24 @@ def paged_reserve(cache: PagedCache, pool, held, kept, fresh, B, *, lens, token_
                   held_out=None, positions=None, pool_next=None, stream=None) -> None:
     """Pages, token offsets, slot map and positions of a step from what every request holds, keeps and
     adds (kvattn_paged_reserve).  held_out None: held is updated in place."""
-    _check(lib().kvattn_paged_reserve(_ptr(cache.block_table), cache.max_pages, cache.page_rows, cache.num_pages,
-                                      _ptr(pool), _ptr(held), _ptr(kept), _ptr(fresh), B, int(max_tokens),
-                                      _ptr(held if held_out is None else held_out), _ptr(lens), _ptr(token_start),
-                                      _ptr(slot_map), _ptr(positions), _ptr(pool_next), _stream(stream)),
+    _check(_call.kvattn_paged_reserve(cache.block_table, cache.max_pages, cache.page_rows, cache.num_pages,
+                                      pool, held, kept, fresh, B, int(max_tokens),
+                                      held if held_out is None else held_out, lens, token_start, slot_map,
+                                      positions, pool_next, _stream(stream)),
            "kvattn_paged_reserve")
 
 
 def paged_store(cache: PagedCache, qkv, slot_map, num_tokens, NH, hs, *, kv_dtype, stream=None) -> None:
     """K and V of a batch of tokens into the pool by slot (kvattn_paged_store)."""
-    _check(lib().kvattn_paged_store(_ptr(cache.pages), _ptr(cache.page_scales), cache.page_rows, cache.num_pages,
-                                    _ptr(slot_map), _ptr(qkv), num_tokens, NH, hs, kv_dtype_code(kv_dtype),
+    _check(_call.kvattn_paged_store(cache.pages, cache.page_scales, cache.page_rows, cache.num_pages,
+                                    slot_map, qkv, num_tokens, NH, hs, kv_dtype_code(kv_dtype),
                                     _stream(stream)), "kvattn_paged_store")
 
 
 def paged_load(kv, cache: PagedCache, slot_map, num_tokens, NH, hs, *, kv_dtype, stream=None) -> None:
     """Rows of the pool by slot into kv [num_tokens][2][NH][hs] (kvattn_paged_load)."""
-    _check(lib().kvattn_paged_load(_ptr(kv), _ptr(cache.pages), _ptr(cache.page_scales), cache.page_rows,
-                                   cache.num_pages, _ptr(slot_map), num_tokens, NH, hs, kv_dtype_code(kv_dtype),
+    _check(_call.kvattn_paged_load(kv, cache.pages, cache.page_scales, cache.page_rows,
+                                   cache.num_pages, slot_map, num_tokens, NH, hs, kv_dtype_code(kv_dtype),
                                    _stream(stream)), "kvattn_paged_load")
 
 
@@ -482,10 +502,10 @@ def verify_drafts(tokens, counts, target_probs, draft_tokens, uniform, token_sta
                   stream=None) -> None:
     """Accepts drafted tokens against the target's probabilities and draws the next one
     (kvattn_verify_drafts).  draft_probs None: drafts without probabilities."""
-    _check(lib().kvattn_verify_drafts(_ptr(tokens), _ptr(counts), _ptr(target_probs), _ptr(draft_probs),
-                                      _ptr(draft_tokens), _ptr(uniform), _ptr(token_start), B, num_tokens, V,
+    _check(_call.kvattn_verify_drafts(tokens, counts, target_probs, draft_probs,
+                                      draft_tokens, uniform, token_start, B, num_tokens, V,
                                       V if row_stride is None else int(row_stride), kv_dtype_code(dtype),
-                                      _ptr(workspace), int(workspace_nbytes), _stream(stream)), "kvattn_verify_drafts")
+                                      workspace, int(workspace_nbytes), _stream(stream)), "kvattn_verify_drafts")
 
 
 class Workspace:
