@@ -50,7 +50,8 @@ constexpr float kQScale = 0.125f * 1.4426950408889634f;    // 1/sqrt(64) * log2(
 constexpr float kSlack = 8.0f;
 constexpr int kMaxT = 1 << 23;
 constexpr int kMaxSegments = 65535;        // the grid's third side
-// AUTO's shapes.  Up to one head a CU, workgroups of 8 waves, in as many segments as there are CUs; beyond,
+// AUTO's shapes.  Up to one head a CU (two where eight queries share a pass, whose heads take longer),
+// workgroups of 8 waves, in as many segments as there are CUs; beyond,
 // 4 waves, in segments that fill four workgroups a CU, and with ragged lengths past 6144 positions of
 // about 32 tiles, so that the longest sequence is not waited for alone.  No segment is shorter than 16
 // tiles (a join of segments costs 1 us and more), except where 4 waves split ragged lengths: the long
@@ -58,8 +59,11 @@ constexpr int kMaxSegments = 65535;        // the grid's third side
 //   12 heads of 1024 positions   8 waves 1 / 4 segments 4.7 / 5.8, 4 waves 1 / 4 segments 5.1 / 5.7
 //   12 heads of 8000             8 waves 8 / 4 / 1 segments 7.4 / 8.5 / 15.2, 4 waves 8 segments 7.8
 //   192 heads of 4096            8 waves 1 / 2 segments 11.8 / 14.7, 4 waves 4 / 1 segments 13.5 / 13.1
-//   288 ragged heads of up to 4096, 8 tokens   4 waves 3 segments 16.4, of 16 tiles at least 17.6, 1 18.3;
-//                                              8 waves 1 / 2 segments 16.2 / 16.8
+//   288 ragged heads of up to 4096, 8 tokens   8 waves 1 / 2 segments 16.1 / 16.8; 4 waves 3 segments 16.7,
+//                                              of 16 tiles at least 17.6, 1 18.3
+//   360 ragged heads of up to 2048, 8 tokens   8 waves 13.3, 4 waves 14.1
+//   288 ragged heads of up to 4096, 1 token    4 waves 3 segments 14.1, 8 waves 1 segment 14.6
+//   480 ragged heads of up to 1024, 4 tokens, INT4   4 waves 9.8, 8 waves 10.4
 //   768 ragged heads of up to 8192, INT4       4 waves 4 / 1 segments 43.6 / 46.7, 8 waves 1 segment 46.3
 //   768 ragged heads of up to 1024             4 waves 1 / 2 segments 9.2 / 12.1, 8 waves 1 segment 11.0
 constexpr int kCUs = 256;
@@ -535,9 +539,9 @@ const void* kernel_for(bool fp4, int waves, bool nt) {
 
 namespace kvattn_internal {
 
-int plan4(int heads, int maxT, int len_hint, bool ragged, int S, Plan4& p) {
+int plan4(int heads, int queries, int maxT, int len_hint, bool ragged, int S, Plan4& p) {
     const int tiles = ((len_hint >= 0 ? len_hint + 1 : maxT) + kTile - 1) / kTile;
-    p.waves = heads <= kCUs ? 8 : 4;
+    p.waves = heads <= (queries == 8 ? 2 : 1) * kCUs ? 8 : 4;
     if (S > 0) {
         if (S > kMaxSegments) return KVATTN_ERR_SPLIT;
         p.S = S;
@@ -551,7 +555,7 @@ int plan4(int heads, int maxT, int len_hint, bool ragged, int S, Plan4& p) {
         p.S = (most + p.seg_tiles - 1) / p.seg_tiles;
         return p.S > kMaxSegments ? KVATTN_ERR_SPLIT : KVATTN_OK;
     }
-    p.S = p.waves == 8 ? kCUs / heads : 4 * kCUs / heads;
+    p.S = p.waves == 8 ? std::max(1, kCUs / heads) : 4 * kCUs / heads;
     p.S = std::min(p.S, (tiles + kSegTiles - 1) / kSegTiles);
     if (p.waves == 4 && ragged && tiles >= 96) p.S = std::max(p.S, tiles / 32);
     p.S = std::max(1, std::min(p.S, kMaxSegments));
@@ -566,7 +570,7 @@ int attend4(const Attend4& c, bool launch) {
     const int most_new = c.start ? std::min(c.max_new, c.num_tokens) : 1;
     const int per = most_new == 1 ? 1 : (most_new <= 4 ? 4 : 8);
     const int groups = (most_new + per - 1) / per;
-    const int st = plan4((int)std::min<long long>((long long)c.B * c.NH * groups, 1 << 30), c.maxT, c.len_hint,
+    const int st = plan4((int)std::min<long long>((long long)c.B * c.NH * groups, 1 << 30), per, c.maxT, c.len_hint,
                          c.start || c.lens_per_seq, c.S, plan);
     if (st != KVATTN_OK) return st;
     const long long rows = (long long)c.NH * groups;

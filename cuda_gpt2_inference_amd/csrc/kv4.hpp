@@ -39,7 +39,7 @@ __attribute__((visibility("hidden"))) int attend4(const Attend4& c, bool launch)
 struct Plan4 {
     int waves, S, seg_tiles;
 };
-__attribute__((visibility("hidden"))) int plan4(int heads, int maxT, int len_hint, bool ragged, int S,
+__attribute__((visibility("hidden"))) int plan4(int heads, int queries, int maxT, int len_hint, bool ragged, int S,
                                                  Plan4& p);
 
 // The append into a 4-bit cache: K and V of one token a sequence (pages.hip).

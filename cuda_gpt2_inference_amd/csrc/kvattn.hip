@@ -3153,7 +3153,7 @@ int kvattn_plan(int B, int NH, int hs, int maxT, int len_hint, int S, int strate
         if (len_hint < -1 || len_hint > maxT - 1) return KVATTN_ERR_LENGTH;
         if (strategy != KVATTN_AUTO && strategy != KVATTN_SPLIT_LASTBLOCK) return KVATTN_ERR_STRATEGY;
         kvattn_internal::Plan4 p4{};
-        KV_TRY(kvattn_internal::plan4(B * NH, maxT, len_hint, false, S, p4));
+        KV_TRY(kvattn_internal::plan4(B * NH, 1, maxT, len_hint, false, S, p4));
         *strategy_out = KVATTN_SPLIT_LASTBLOCK;
         *segments_out = p4.S;
         *seg_rows_out = S > 0 ? 0 : p4.seg_tiles * kMinSegRows;
