@@ -238,7 +238,8 @@ def test_paged_decode_tokens(dev, kv, counts, S):
 
 
 @pytest.mark.parametrize("kv", KV4)
-@pytest.mark.parametrize("counts", [[1, 1, 1], [2, 4, 0], [3, 8, 1], [1] * 140, [3, 0, 1, 2] * 35, [5, 1] * 70])
+@pytest.mark.parametrize("counts", [[1, 1, 1], [2, 4, 0], [3, 8, 1], [1] * 140, [3, 0, 1, 2] * 35, [5, 1] * 70,
+                                    [5, 0, 1] * 90])
 def test_paged_decode_tokens_large_pool(dev, kv, counts):
     """A pool of more than 128 MiB, of which the loads are others (as read only once), and room for 320000
     positions a sequence; no bound on the tokens of one."""
