@@ -339,7 +339,9 @@ int kvattn_verify_drafts(int* tokens, int* counts, const void* target_probs, con
                          int V, long long row_stride, int dtype, void* workspace, size_t workspace_bytes, void* stream) {
     if (dtype != KVATTN_KV_F32 && dtype != KVATTN_KV_BF16) return KVATTN_ERR_DTYPE;
     if (B < 1 || B > kMaxSequences || V < 1 || V > kMaxVocab || num_tokens < 0 || row_stride < V) return KVATTN_ERR_SHAPE;
-    if (!tokens || !counts || !target_probs || !draft_tokens || !uniform || !token_start) return KVATTN_ERR_NULL_POINTER;
+    if (!counts || !token_start) return KVATTN_ERR_NULL_POINTER;
+    // (Nothing of an array without elements is looked at, and its address may be none.)
+    if (num_tokens > 0 && (!tokens || !target_probs || !draft_tokens || !uniform)) return KVATTN_ERR_NULL_POINTER;
     const size_t size = dtype == KVATTN_KV_F32 ? 4 : 2;
     if (((uintptr_t)target_probs % size) || ((uintptr_t)draft_probs % size) || ((uintptr_t)tokens & 3u) ||
         ((uintptr_t)counts & 3u) || ((uintptr_t)draft_tokens & 3u) || ((uintptr_t)uniform & 3u) ||

@@ -224,3 +224,12 @@ def test_repeats_and_capture(dev):
         want = kv4ref.verify(p.astype(np.float64), q.astype(np.float64), drafts, u, start, V)
         assert np.array_equal(tokens.cpu().numpy(), want[0]) and np.array_equal(counts.cpu().numpy(), want[1])
         assert not ws[:256].any()
+
+
+@pytest.mark.parametrize("B,V", [(1, 100), (5, 50257), (600, 9000)])
+def test_batch_without_tokens(dev, B, V):
+    """Arrays of no elements (their address is none): every count is zero."""
+    p = np.zeros((0, V), np.float32)
+    for q in (p, None):
+        tokens, counts = _run(dev, p, q, np.zeros(0), np.zeros(0), np.zeros(B + 1), V)
+        assert tokens.size == 0 and not counts.any()

@@ -119,6 +119,14 @@ def test_verify_refusals(kw, status):
     assert _status("kvattn_verify_drafts", VERIFY, kw) == status
 
 
+def test_verify_of_no_tokens_needs_no_arrays_of_them():
+    none = dict(tokens=None, p=None, q=None, drafts=None, u=None, ws=None)     # refused for its workspace alone
+    assert _status("kvattn_verify_drafts", VERIFY, {**none, "n": 0}) == 7
+    assert _status("kvattn_verify_drafts", VERIFY, {**none, "n": 1}) == 1
+    assert _status("kvattn_verify_drafts", VERIFY, {**none, "n": 0, "counts": None}) == 1
+    assert _status("kvattn_verify_drafts", VERIFY, {**none, "n": 0, "start": None}) == 1
+
+
 def test_verify_workspace_bytes():
     kv = _kv()
     assert kv.verify_workspace_bytes(1, 1) == 512
