@@ -253,6 +253,13 @@ __global__ __launch_bounds__(kBlock) void verify_kernel(VerifyArgs a) {
     const double total = use_rest ? rest : all;
     const double aim = (double)u_last * total;
     int drawn = -1;
+    // The sums are left at zero, as the counter is, once all four waves have read them: where they lie,
+    // a call of another B or V has its counters.
+    auto leave_zero = [&] {
+        __syncthreads();
+        double* const z = a.sums + (size_t)b * a.tiles * 2;
+        for (int t = threadIdx.x; t < 2 * a.tiles; t += kRuns * kWave) put64(z + t, 0.0);
+    };
     if (total > 0.0) {
         // The first tile whose running sum passes the aim (rounding may leave none: the last that weighs
         // anything), then the first run of it, then the first token likewise.
@@ -287,7 +294,7 @@ __global__ __launch_bounds__(kBlock) void verify_kernel(VerifyArgs a) {
         }
         const double sum = wave_prefix64(mine);
         if (lane == kWave - 1) run_sums[wave] = sum;
-        __syncthreads();
+        leave_zero();
         int run = -1;
         double run0 = 0.0;
         bool passed = false;
@@ -315,8 +322,9 @@ __global__ __launch_bounds__(kBlock) void verify_kernel(VerifyArgs a) {
         const unsigned long long pass = __ballot(hit >= 0), some = __ballot(last >= 0);
         if (pass) drawn = __shfl(hit, __ffsll((long long)pass) - 1);
         else if (some) drawn = __shfl(last, 63 - __clzll((long long)some));
-    } else if (wave != 0) {
-        return;
+    } else {
+        leave_zero();
+        if (wave != 0) return;
     }
     for (int i = lane; i < n; i += kWave) a.tokens[t0 + i] = i < row ? a.drafts[t0 + i] : (i == row ? drawn : -1);
     if (lane == 0) a.count[b] = row + (drawn >= 0 ? 1 : 0);

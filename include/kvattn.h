@@ -473,8 +473,10 @@ int kvattn_paged_load(void* kv, const void* pages, const float* page_scales, int
  *               (dtype KVATTN_KV_F32) or bf16 (KVATTN_KV_BF16); NaN, infinite and negative ones weigh
  *               nothing in a draw.  draft_probs NULL: drafts without probabilities (q = 1 at the draft)
  *   draft_tokens  ids outside [0, V) are refused
- *   workspace   kvattn_verify_workspace_bytes(B, V) bytes, 256-byte aligned, zeroed once
- *               (kvattn_workspace_init).  Calls sharing a workspace must be ordered.
+ *   workspace   kvattn_verify_workspace_bytes(B, V) bytes or more, 256-byte aligned, zeroed once
+ *               (kvattn_workspace_init); every call leaves it zero again, so a buffer of the largest
+ *               size serves calls of any B and V.  Calls sharing it must be ordered, and only calls
+ *               of this entry point may.
  * No reference counterpart (the reference samples one token at a time on the host). */
 size_t kvattn_verify_workspace_bytes(int B, int V);
 int kvattn_verify_drafts(int* tokens, int* counts, const void* target_probs, const void* draft_probs,

@@ -233,3 +233,57 @@ def test_batch_without_tokens(dev, B, V):
     for q in (p, None):
         tokens, counts = _run(dev, p, q, np.zeros(0), np.zeros(0), np.zeros(B + 1), V)
         assert tokens.size == 0 and not counts.any()
+
+
+def test_one_workspace_for_batches_of_every_size(dev):
+    """One buffer, zeroed once and sized for the largest, serves calls of any B and V in any order: what one
+    leaves in it is no other's business (V from 8193 on takes several workgroups a sequence)."""
+    import torch
+    kvattn = _kv()
+    calls = [(64, 50257), (96, 20000), (300, 9000), (500, 8200), (5, 50257), (1, 100000), (64, 300), (129, 8193), (513, 9000),
+             (2, 70000), (96, 20000)]
+    nbytes = max(kvattn.verify_workspace_bytes(B, V) for B, V in calls)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    kvattn.workspace_init(ws, nbytes)
+    r = np.random.RandomState(21)
+    for B, V in calls:
+        counts = np.where(np.arange(B) % 3 == 0, 2, 1)
+        counts[B // 2] = B > 1 and V % 2                  # one without tokens
+        case = _case(r, counts, V, V, "f32", B % 2 == 0)
+        _check(dev, case, V, ws=ws)
+        assert not ws.any(), (B, V)
+
+
+def test_two_captured_calls_share_a_workspace(dev):
+    """Graphs of different batches over one workspace, replayed in turn."""
+    import torch
+    kvattn = _kv()
+    r = np.random.RandomState(22)
+    t = lambda x, d: torch.from_numpy(np.ascontiguousarray(x)).to(d).to(dev)      # noqa: E731
+    shapes = [(64, 20000), (80, 16400)]
+    nbytes = max(kvattn.verify_workspace_bytes(B, V) for B, V in shapes)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    kvattn.workspace_init(ws, nbytes)
+    held = []
+    for B, V in shapes:
+        p, q, drafts, u, start = _case(r, [2] * B, V, V, "f32", False)
+        d = dict(p=t(p, torch.float32), q=t(q, torch.float32), drafts=t(drafts, torch.int32), u=t(u, torch.float32),
+                 start=t(start, torch.int32), tokens=torch.full((2 * B,), -2, dtype=torch.int32, device=dev),
+                 counts=torch.full((B,), -2, dtype=torch.int32, device=dev), host=(p, q, drafts, start, V))
+        graph = torch.cuda.CUDAGraph()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph):
+            kvattn.verify_drafts(d["tokens"], d["counts"], d["p"], d["drafts"], d["u"], d["start"], B, 2 * B, V,
+                                 draft_probs=d["q"], workspace=ws, workspace_nbytes=nbytes)
+        held.append((graph, d))
+    for i in range(3):
+        for graph, d in held:
+            u = r.rand(d["u"].numel()).astype(np.float32)
+            d["u"].copy_(t(u, torch.float32))
+            d["tokens"].fill_(-2)
+            d["counts"].fill_(-2)
+            graph.replay()
+            torch.cuda.synchronize()
+            p, q, drafts, start, V = d["host"]
+            want = kv4ref.verify(p.astype(np.float64), q.astype(np.float64), drafts, u, start, V)
+            assert np.array_equal(d["tokens"].cpu().numpy(), want[0]) and np.array_equal(d["counts"].cpu().numpy(), want[1])
