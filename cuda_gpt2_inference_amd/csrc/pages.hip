@@ -364,6 +364,7 @@ __device__ __forceinline__ uint32_t codes4(const float (&x)[8], float scale) {
         for (int i = 0; i < 8; ++i) {
             const float q = x[i] * r;
             y[i] = fmaf(fmaf(-q, scale, x[i]), r, q);
+            if constexpr (DT == KVATTN_KV_FP4_E2M1) y[i] = copysignf(y[i], x[i]);   // -0: its remainder is +0
         }
     } else {
         const bool live = scale > 0.0f;

@@ -337,3 +337,28 @@ def test_every_quotient_rounds_as_the_division(dev, kv):
         want, want_s = kv4ref.encode(qkv[:, 1, 0].float().cpu().numpy(), kv)
         assert np.array_equal(scales[0, 0, 0].cpu().numpy(), want_s)
         assert np.array_equal(pages[0, 0, 0].cpu().numpy(), want)
+
+
+@pytest.mark.parametrize("kv", ["int4", "fp4"])
+@pytest.mark.parametrize("beside", ["plain", "zeros", "nan"])
+def test_negative_zero_keeps_its_code(dev, kv, beside):
+    """-0 (and a negative value that rounds to no magnitude) has the code that the definition gives it, whatever rows
+    its wave's other tokens are."""
+    import torch
+    kvattn = _kv()
+    r = np.random.RandomState(3)
+    x = r.standard_normal((8, HS)).astype(np.float32)
+    x[:, ::3] = -0.0
+    x[:, 1::7] = 0.0
+    x[:, 2::9] = -1e-6
+    if beside == "zeros":
+        x[3] = 0.0
+    elif beside == "nan":
+        x[3, 5] = np.nan
+    qkv = torch.zeros(8, 3, 1, HS, dtype=torch.bfloat16, device=dev)
+    qkv[:, 1, 0] = torch.from_numpy(x).to(torch.bfloat16).to(dev)
+    pages, scales = _pool(kv, 1, 1, 64, dev)
+    kvattn.paged_store(kvattn.PagedCache(pages, None, 1, 64, 1, scales), qkv, torch.arange(8, device=dev), 8, 1, HS, kv_dtype=kv)
+    want, want_s = kv4ref.encode(qkv[:, 1, 0].float().cpu().numpy(), kv)
+    assert np.array_equal(scales[0, 0, 0, :8].cpu().numpy(), want_s)
+    assert np.array_equal(pages[0, 0, 0, :8].cpu().numpy(), want)
