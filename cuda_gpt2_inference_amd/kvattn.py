@@ -169,18 +169,22 @@ def _ptr(x) -> Optional[int]:
 
 
 class _Calls:
-    """The entry points that return a status, bound at their first use: each takes tensors, addresses, integers
-    and None as they are (_pycall.Call; without it ctypes, and _ptr for every argument)."""
+    """The entry points that return a status, bound at their first use: each takes tensors, addresses and None as
+    they are where it has a pointer, and an integer's value where it has an integer (_pycall.Call; without it
+    ctypes, and _ptr for every pointer).  What is no integer there is a ctypes.ArgumentError."""
 
     def __getattr__(self, name):
         fn = getattr(lib(), name)
+        kinds = SIGNATURES[name][1]
         try:
             from ._pycall import Call
         except ImportError:
             def call(*args):
-                return fn(*map(_ptr, args))
+                if len(args) != len(kinds):
+                    raise TypeError(f"{len(kinds)} positional arguments expected, {len(args)} given")
+                return fn(*[_ptr(x) if k is _vp else x for k, x in zip(kinds, args)])
         else:
-            call = Call(ctypes.cast(fn, _vp).value, len(SIGNATURES[name][1]))
+            call = Call(ctypes.cast(fn, _vp).value, len(kinds), sum(1 << i for i, k in enumerate(kinds) if k is not _vp))
         setattr(self, name, call)
         return call
 

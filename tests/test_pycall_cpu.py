@@ -107,3 +107,80 @@ def test_wrappers_without_the_extension(monkeypatch):
     with pytest.raises(kvattn.KvAttnError) as e:
         kvattn.paged_store(cache, x, None, 1, 1, 64, kv_dtype="bf16", stream=0)
     assert e.value.status in (kvattn.ERR_SHAPE, kvattn.ERR_NULL_POINTER)
+
+
+def _calls(monkeypatch, extension):
+    import sys
+    kvattn = _kv()
+    if not extension:
+        monkeypatch.setitem(sys.modules, "cuda_gpt2_inference_amd._pycall", None)
+    monkeypatch.setattr(kvattn, "_call", kvattn._Calls())
+    return kvattn
+
+
+@pytest.mark.parametrize("extension", [True, False])
+def test_integers_are_values(monkeypatch, extension):
+    """Where an entry point has an integer, every argument gives what it gives through ctypes: the value of a tensor of
+    one integer (never its address), and a refusal for what is no integer."""
+    import torch
+    kvattn = _calls(monkeypatch, extension)
+    kinds_of_int = [torch.tensor(4), torch.tensor([0, 5])[-1], torch.tensor([3]), np.int64(-7), np.array(6), True, 2 ** 40 + 1,
+                    torch.zeros(3, dtype=torch.int32), torch.tensor(4.0), None, 4.0, "4", object()]
+    for name in ("kvattn_cache_write", "kvattn_decode", "kvattn_append_decode", "kvattn_paged_cache_write",
+                 "kvattn_paged_decode", "kvattn_paged_decode_tokens", "kvattn_paged_reserve", "kvattn_paged_store",
+                 "kvattn_paged_load", "kvattn_verify_drafts"):
+        kinds = kvattn.SIGNATURES[name][1]
+        for i, k in enumerate(kinds):
+            if k is kvattn._vp:
+                continue
+            for x in kinds_of_int:
+                # Every other integer fits, and the pointers are missing: refused, by the sizes or for a pointer.
+                args = [None if t is kvattn._vp else 64 for t in kinds]
+                args[i] = x
+                try:
+                    want = getattr(kvattn.lib(), name)(*args)
+                except ctypes.ArgumentError:
+                    with pytest.raises(ctypes.ArgumentError):
+                        getattr(kvattn._call, name)(*args)
+                    continue
+                assert want != kvattn.OK and getattr(kvattn._call, name)(*args) == want, (name, i, x)
+
+
+@pytest.mark.parametrize("extension", [True, False])
+def test_counts_of_wrappers_are_values(monkeypatch, extension):
+    """The statuses tell whether a count arrived: -1 is refused as a size before the missing pointer is."""
+    import torch
+    kvattn = _calls(monkeypatch, extension)
+    x = torch.zeros(64, dtype=torch.int32)
+    cache = kvattn.PagedCache(x, x, 1, 64, 1, x)
+    for n, status in ((torch.tensor([0, -1])[-1], kvattn.ERR_SHAPE), (torch.tensor(2), kvattn.ERR_NULL_POINTER)):
+        for call in (lambda: kvattn.decode(None, None, None, n, 1, 64, 64, kv_dtype="bf16", stream=0),
+                     lambda: kvattn.append_decode(None, None, None, 1, n, 64, 64, kv_dtype="bf16", stream=0),
+                     lambda: kvattn.kv_cache_write(None, None, 1, 1, 64, n, kv_dtype="bf16", stream=0),
+                     lambda: kvattn.paged_decode(None, None, cache, n, 1, 64, kv_dtype="bf16", stream=0),
+                     lambda: kvattn.paged_decode_tokens(None, x, cache, x, x, 1, n, 1, 64, kv_dtype="int4", max_new=1, stream=0),
+                     lambda: kvattn.paged_store(cache, None, x, n, 1, 64, kv_dtype="bf16", stream=0),
+                     lambda: kvattn.verify_drafts(x, x, None, x, x, x, 1, n, 8, stream=0)):
+            with pytest.raises(kvattn.KvAttnError) as e:
+                call()
+            assert e.value.status == status
+
+
+def test_integers_by_bit():
+    import torch
+    from cuda_gpt2_inference_amd._pycall import Call
+    got = []
+
+    def seen(*words):
+        got[:] = words
+        return 0
+    fn = ctypes.CFUNCTYPE(ctypes.c_int, *[_W] * 24)(seen)
+    call = Call(ctypes.cast(fn, ctypes.c_void_p).value, 24, 0b101 | 1 << 23)
+    x = torch.zeros(2)
+    assert call(np.int64(-7), x, torch.tensor(9), *[x] * 20, 2 ** 64 + 3) == 0
+    assert got == [-7, x.data_ptr(), 9] + [x.data_ptr()] * 20 + [3]
+    for i in (0, 2, 23):
+        args = [1] * 24
+        args[i] = x
+        with pytest.raises(ctypes.ArgumentError, match=f"argument {i + 1}:"):
+            call(*args)
