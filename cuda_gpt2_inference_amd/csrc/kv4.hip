@@ -88,6 +88,7 @@ struct Args {
     size_t v_rows;             // rows from a head's K block to its V block
     int id_mul, R;             // a head's block of page (or sequence) id starts at row (id * id_mul + h) * R
     int max_pages, num_pages, lens_per_seq, NH, maxT, groups, S, seg_tiles, num_tokens;
+    int line;                  // groups in one line: the number of sequences, else 0
 };
 
 // A tile on its way: 16-byte chunks lane and lane + 64 of K and V, and the scales of the kC positions
@@ -182,6 +183,24 @@ __device__ __forceinline__ float weight_of(float m, float M) { return m == -INFI
 // this keeps the compiler from moving one lane's reads over another's writes.
 __device__ __forceinline__ void lds_order() { asm volatile("" ::: "memory"); }
 
+// Groups of kQ queries in one line, as many as the tokens can fill: sequence b's first is start[b] / kQ + b, and as
+// its n tokens make at most start[b + 1] / kQ - start[b] / kQ + 1 of them, no two sequences meet, and all of them end
+// before B + num_tokens / kQ.  The last sequence that begins at or before the slot, 64 looked at at once, and
+// the group of it (negative: none).
+template <int kQ>
+__device__ __forceinline__ int sequence_at(const Args& a, int slot, int lane, int& grp) {
+    auto first = [&](int b) { return min(max(a.start[b], 0), a.num_tokens) / kQ + b; };
+    int b = 0;
+    for (int step = a.line > kWave * kWave ? kWave * kWave : a.line > kWave ? kWave : 1;; step /= kWave) {
+        const int i = b + lane * step;
+        const unsigned long long at = __ballot(i < a.line && first(min(i, a.line - 1)) <= slot);
+        b += (63 - __clzll((long long)(at | 1))) * step;
+        if (step == 1) break;
+    }
+    grp = slot - first(b);
+    return b;
+}
+
 // Keeps a wave's rare branch from becoming selects that every tile runs.
 __device__ __forceinline__ void stay_a_branch() { asm volatile(""); }
 
@@ -196,7 +215,14 @@ __global__ __launch_bounds__(kW * kWave) __attribute__((amdgpu_waves_per_eu(4)))
     constexpr int kC = kQ <= 4 ? 1 : 2, kS = kQ == 1 ? 1 : 4;
 
     // Heads lie next to each other in the grid, so that a long sequence's are spread over the XCDs.
-    const int b = blockIdx.y, grp = a.groups == 1 ? 0 : blockIdx.x / a.NH, h = blockIdx.x - grp * a.NH, s = blockIdx.z;
+    int b = blockIdx.y, grp = a.groups == 1 ? 0 : blockIdx.x / a.NH;
+    const int h = blockIdx.x - grp * a.NH, s = blockIdx.z;
+    if constexpr (kQ == 8) {
+        if (a.line) {
+            b = sequence_at<kQ>(a, grp, threadIdx.x & (kWave - 1), grp);
+            if (grp < 0) return;
+        }
+    }
     int t0, n, total;
     if (a.start) {
         t0 = min(max(a.start[b], 0), a.num_tokens);
@@ -569,12 +595,18 @@ int attend4(const Attend4& c, bool launch) {
     // Queries of a workgroup: the fewest that take a sequence's new tokens at once, up to eight.
     const int most_new = c.start ? std::min(c.max_new, c.num_tokens) : 1;
     const int per = most_new == 1 ? 1 : (most_new <= 4 ? 4 : 8);
+    // A grid row for every sequence's groups, or all groups in a line where that is shorter: past eight tokens max_new
+    // says little about most sequences.  12 heads, us per call, line / rows: 24 ragged sequences of up to 4096,
+    // 0 to 8 tokens, max_new 17 / 32 / any 21.0 / 24.6, 20.7 / 20.1, 20.6 / 24.2; 256 of up to 512 16 / 24 / any
+    // 24.8 / 26.3, 24.8 / 23.3, 24.6 / 159; 64 of up to 1024, one of them with 200 tokens 14.5 / 20.1.
     const int groups = (most_new + per - 1) / per;
-    const int st = plan4((int)std::min<long long>((long long)c.B * c.NH * groups, 1 << 30), per, c.maxT, c.len_hint,
-                         c.start || c.lens_per_seq, c.S, plan);
+    const long long line = c.B + c.num_tokens / per, each = (long long)c.B * groups;
+    const bool in_line = per == 8 && each > line;
+    const long long heads = (in_line ? line : each) * c.NH;
+    const int st = plan4((int)std::min<long long>(heads, 1 << 30), per, c.maxT, c.len_hint, c.start || c.lens_per_seq,
+                         c.S, plan);
     if (st != KVATTN_OK) return st;
-    const long long rows = (long long)c.NH * groups;
-    if (c.B > 65535 || rows * c.B * plan.S * plan.waves * kWave > 0xffffffffll) return KVATTN_ERR_SHAPE;
+    if (c.B > 65535 || heads * plan.S * plan.waves * kWave > 0xffffffffll) return KVATTN_ERR_SHAPE;
     Args a{};
     if (plan.S > 1) {
         if (!c.ws) return KVATTN_ERR_WORKSPACE;
@@ -604,6 +636,7 @@ int attend4(const Attend4& c, bool launch) {
     a.NH = c.NH;
     a.maxT = c.maxT;
     a.groups = groups;
+    a.line = in_line ? c.B : 0;
     a.S = plan.S;
     a.seg_tiles = plan.seg_tiles;
     a.num_tokens = c.num_tokens;
@@ -614,8 +647,8 @@ int attend4(const Attend4& c, bool launch) {
     const void* fn = per == 1 ? kernel_for<1>(fp4, plan.waves, nt) : per == 4 ? kernel_for<4>(fp4, plan.waves, nt)
                                                                               : kernel_for<8>(fp4, plan.waves, nt);
     void* params[] = {&a};
-    const hipError_t e = hipLaunchKernel(fn, dim3((unsigned)rows, c.B, plan.S), dim3(plan.waves * kWave), params, 0,
-                                         (hipStream_t)c.stream);
+    const hipError_t e = hipLaunchKernel(fn, in_line ? dim3((unsigned)heads, 1, plan.S) : dim3(c.NH * groups, c.B, plan.S),
+                                         dim3(plan.waves * kWave), params, 0, (hipStream_t)c.stream);
     if (e != hipSuccess) {
         set_last_hip_error((int)e);
         return KVATTN_ERR_HIP;

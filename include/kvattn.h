@@ -394,9 +394,9 @@ int kvattn_paged_decode(void* out, const void* qkv, void* pages, float* page_sca
  *               number may be 0
  *   lens        [B] device: positions of sequence b, its new tokens among them; token i of n
  *               attends the first lens[b] - n + i + 1 of them (none: its output is zero)
- *   max_new     the most tokens of one sequence (1, up to 4 and more take different kernels), or
- *               any larger number; a sequence with more has the first max_new or more of them
- *               computed
+ *   max_new     the most tokens of one sequence (1, up to 4, up to 8 and more take different
+ *               launches), or any larger number; a sequence with more has the first max_new or more
+ *               of them computed
  * Rows of out behind token_start[B] are left as they were.  token_start must not decrease; it and
  * lens are clamped into [0, num_tokens] and [0, max_pages * page_rows].  B <= 65535.  Workspace:
  * kvattn_workspace_bytes(num_tokens, NH, hs, max_pages * page_rows, S); S as in kvattn_decode with

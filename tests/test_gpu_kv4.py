@@ -268,6 +268,38 @@ def test_paged_decode_tokens_large_pool(dev, kv, counts):
 
 
 @pytest.mark.parametrize("kv", KV4)
+@pytest.mark.parametrize("B,counts,lead", [(3, [1, 0, 2], 20), (64, [3, 0, 9, 1], 0), (65, [8], 5), (300, [0, 0, 0, 17], 9),
+                                           (4096, [4, 0, 8, 1, 7], 0), (4097, [1, 0, 0], 8), (5000, [3, 2, 4], 100),
+                                           (1024, [8], 0)])
+@pytest.mark.parametrize("S", [0, 2])
+def test_paged_decode_tokens_of_any_number(dev, kv, B, counts, lead, S):
+    """max_new that says nothing, over batches of every size: sequences share their first pages, as prompts may, and
+    the tokens may begin behind rows of another use, which are left as they were."""
+    import torch
+    kvattn = _kv()
+    R, n, own = 64, 2, 16
+    case = Case(kv, own, 2, n * R, [128, 70, 64, 9] * 4, seed=17)
+    counts = (counts * B)[:B]
+    counts[B // 2] = 23                             # one with three groups
+    start = lead + np.concatenate([[0], np.cumsum(counts)]).astype(np.int32)
+    N, spare = int(start[-1]), 3
+    q = case.queries(N + spare)
+    few, table = case.paged(R, dev)
+    cache = kvattn.PagedCache(few.pages, _dev(table[np.arange(B) % own], dev), n, R, few.num_pages, few.page_scales)
+    lens = np.array(case.lens, np.int32)[np.arange(B) % own]
+    ws = kvattn.Workspace(N + spare, 2, n * R)
+    tokens = [(start[b] + i, b % own, lens[b] - c + i + 1) for b, c in enumerate(counts) for i in range(c)]
+    for most in (23, 2 ** 31 - 1):
+        out = torch.full((N + spare, 2, HS), 7.0, dtype=torch.bfloat16, device=dev)
+        kvattn.paged_decode_tokens(out, _qkv(q, dev), cache, _dev(start, dev), _dev(lens, dev), B, N + spare, 2, HS, kv_dtype=kv,
+                                   max_new=most, S=S, **ws.kwargs())
+        got = out.float().cpu().numpy()
+        assert (got[:lead] == 7.0).all() and (got[N:] == 7.0).all() and not (got[lead:N] == 7.0).all(-1).any()
+        case.check(got, q, tokens[::1 + len(tokens) // 1500], f"B {B} most {most}")
+        case.check(got, q, [t for t in tokens if t[0] >= start[B // 2] and t[0] < start[B // 2 + 1]], f"B {B} most {most}")
+
+
+@pytest.mark.parametrize("kv", KV4)
 def test_tokens_see_nothing_of_later_ones(dev, kv):
     """A later draft's row of infinite or NaN scale leaves the tokens before it as they are; tokens
     before the first position attend nothing and give zero."""

@@ -39,6 +39,13 @@ def test_decode_tokens_refusals(kw, status):
     assert _status("kvattn_paged_decode_tokens", TOKENS, kw) == status
 
 
+@pytest.mark.parametrize("B,n,NH", [(1024, 8192, 12), (4096, 16384, 12), (65535, 1 << 18, 25), (1, 1 << 20, 12)])
+@pytest.mark.parametrize("max_new", [9, 64, 8192, 2 ** 31 - 1])
+def test_decode_tokens_takes_any_max_new(B, n, NH, max_new):
+    """The number of tokens bounds the grid; refused here for the missing workspace of two segments alone."""
+    assert _status("kvattn_paged_decode_tokens", TOKENS, dict(B=B, n=n, NH=NH, max_new=max_new, S=2, ws=None)) == 7
+
+
 DECODE = dict(out=A, qkv=A, kv=A, scale=A, B=1, NH=12, hs=64, maxT=4096, cur=A, per_seq=0, hint=-1, ws=None, wsb=0, S=4,
               strategy=0, dt=4, stream=None)
 
