@@ -142,6 +142,67 @@ def test_steps(dev, kv):
     assert refused > 0, "the pool is small enough that some step was refused"
 
 
+def _next_kept(lens, kept, fresh, counts):
+    """What a request keeps after a step: a granted one its tokens up to the last emitted one's place, a refused one,
+    for whose rows the step's other calls computed nothing that counts, what it had."""
+    import torch
+    return torch.where(lens == kept + fresh, kept + counts, kept)
+
+
+def _last(lens, kept, fresh, counts):
+    return lens - fresh + counts                    # right for the granted ones alone
+
+
+@pytest.mark.parametrize("rule", [_next_kept, _last])
+@pytest.mark.parametrize("kv", ["int4", "fp4"])
+def test_refused_requests_lose_nothing(dev, kv, rule):
+    """Steps whose next kept positions are computed on the device, over a pool that is too small: every position that
+    was kept holds the row that was accepted for it, however often its request was refused since.  (A rule that
+    takes the rows of refused requests for accepted ones is caught.)"""
+    import torch
+    r = np.random.RandomState(41)
+    s = Server(dev, kv, 2)
+    rows = [[] for _ in range(B)]                   # (step, token row) of every kept position
+    log, refused, wrong = [], 0, False
+    kept = torch.zeros(B, dtype=torch.int32, device=dev)
+    for step in range(100):
+        wrong = kept.tolist() != [len(x) for x in rows]
+        if wrong:
+            break
+        if step in (60, 80):
+            kept[step // 20], rows[step // 20] = 0, []          # one ends, and its pages go to others
+        k = kept.cpu().numpy()
+        fresh = np.minimum(r.randint(1, 5, B), MAX_PAGES * R - k)
+        qkv = r.standard_normal((MAX_TOKENS, 3, NH, HS)).astype(np.float32)
+        q = np.full((MAX_TOKENS, V), 1 / V, np.float32)
+        _load(s, k, fresh, qkv, q, r.randint(0, V, MAX_TOKENS), 0.2 * r.rand(MAX_TOKENS).astype(np.float32))
+        s.issue()
+        start = np.concatenate([[0], np.cumsum(fresh)])
+        granted, counts = (s.lens == kept + s.fresh).cpu().numpy(), s.counts.cpu().numpy()
+        refused += int((~granted).sum())
+        log.append(torch.from_numpy(qkv[:, 1:]).to(torch.bfloat16).float().numpy())
+        for b in np.nonzero(granted)[0]:
+            rows[b] += [(step, start[b] + i) for i in range(counts[b])]
+        kept = rule(s.lens, kept, s.fresh, s.counts)
+    if rule is _last:
+        assert wrong
+        return
+    assert not wrong and refused > 5 and sum(map(len, rows)) > 100
+    k = kept.cpu().numpy()
+    table = s.cache.block_table.cpu().numpy()
+    for b in range(B):
+        assert len(rows[b]) == k[b] <= int(s.held[b])
+        if not rows[b]:
+            continue
+        pos = np.arange(k[b])
+        slots = torch.from_numpy(table[b, pos // R].astype(np.int64) * R + pos % R).to(dev)
+        back = torch.zeros(k[b], 2, NH, HS, dtype=torch.bfloat16, device=dev)
+        s.kvattn.paged_load(back, s.cache, slots, int(k[b]), NH, HS, kv_dtype=kv)
+        codes, scale = kv4ref.encode(np.stack([log[t][row] for t, row in rows[b]]), kv)
+        want = kv4ref.decode(codes, np.ones_like(scale), kv).astype(np.float32) * scale[..., None]
+        assert torch.equal(back.cpu(), torch.from_numpy(want).to(torch.bfloat16)), b
+
+
 def test_pages_and_rows_on_another_stream(dev):
     """Current stream not the default one: every call goes to it, in order."""
     import torch
