@@ -267,7 +267,9 @@ int kvattn_set_merge_poll_limit(int polls);
  * (lens_per_seq == 0).  A call with per-sequence lengths takes the same plan, except where
  * this one streams a BF16 or INT8 cache through the split + merge kernels (there AUTO keeps
  * its general plan: the last-block merge, or split + merge over segments of up to 512
- * rows), and for many heads of 257 to 1024 positions, whose bounds on the heads differ.  Its
+ * rows), for many heads of 257 to 1024 positions, whose bounds on the heads differ, and for more
+ * than 256 heads of a 4-bit cache, which per-sequence lengths of up to 6144 and more positions
+ * (maxT, or the hint) split into more and shorter segments.  Its
  * workspace may then differ from the reported one too: S == 0 in kvattn_workspace_bytes is
  * enough for every call.  No reference counterpart: it exposes the AUTO choice, which the reference makes
  * inline in its caller (inference_gpt2_opt.cu:247,304,331: fused_single below a length

@@ -187,6 +187,38 @@ def test_paged_decode(dev, kv, R):
 
 
 @pytest.mark.parametrize("kv", KV4)
+@pytest.mark.parametrize("B,NH,n", [(260, 4, 96), (260, 4, 95), (129, 2, 96), (128, 2, 128), (300, 1, 200)])
+def test_workspace_of_ragged_batches(dev, kv, B, NH, n):
+    """The plan is that of one length for the batch: its workspace serves such a batch.  Per-sequence lengths of many
+    heads may need more; the workspace for every choice (S = 0) serves them too."""
+    import torch
+    kvattn = _kv()
+    R = 64
+    case = Case(kv, 3, NH, n * R, [n * R, 1, 300], seed=18)
+    few, table = case.paged(R, dev)
+    own = np.arange(B) % 3
+    cache = kvattn.PagedCache(few.pages, _dev(table[own], dev), n, R, few.num_pages, few.page_scales)
+    q = case.queries(B)
+    lens = np.array(case.lens, np.int32)[own]
+    planned = kvattn.plan(B, NH, HS, n * R, kv_dtype=kv)[1]
+    tokens = [(b, b % 3, int(lens[b])) for b in range(0, B, 7)]
+
+    def call(S, cur, per_seq):
+        out = torch.full((B, NH, HS), 7.0, dtype=torch.bfloat16, device=dev)
+        ws = kvattn.Workspace(B, NH, n * R, S)
+        kvattn.paged_decode(out, _qkv(q, dev), cache, B, NH, HS, kv_dtype=kv, cur_len=cur, lens_per_seq=per_seq, **ws.kwargs())
+        return out.float().cpu().numpy()
+    case.check(call(0, _dev(lens - 1, dev), True), q, tokens, "ragged")
+    case.check(call(planned, _dev(np.array([299], np.int32), dev), False), q, [(b, b % 3, 300) for b in range(0, B, 21)], "one")
+    if B * NH > 256 and n >= 96 and n // 32 > planned:
+        with pytest.raises(kvattn.KvAttnError) as e:
+            call(planned, _dev(lens - 1, dev), True)
+        assert e.value.status == kvattn.ERR_WORKSPACE
+    else:
+        case.check(call(planned, _dev(lens - 1, dev), True), q, tokens, "ragged, as planned")
+
+
+@pytest.mark.parametrize("kv", KV4)
 def test_bad_pages_are_skipped(dev, kv):
     """Positions of table entries outside the pool do not count; a sequence with none left gives zero."""
     import torch
