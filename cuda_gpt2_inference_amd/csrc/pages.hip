@@ -44,6 +44,7 @@ constexpr int kReserveThreads = 1024;      // of a workgroup; kSmallThreads wher
 constexpr int kSmallThreads = 256;
 constexpr int kReserveTokens = 4096;       // token rows a workgroup is launched for, up to
 constexpr int kReserveMostBlocks = 256;    // so many workgroups
+constexpr int kMostTokens = 1 << 30;       // a step of every workgroup's threads beyond is still an int
 constexpr int kRefused = 1 << 30;          // beside the positions a request keeps
 
 struct ReserveArgs {
@@ -612,7 +613,7 @@ int kvattn_paged_reserve(int* block_table, int max_pages, int page_rows, int num
                          const int* kept, const int* fresh, int B, int max_tokens, int* held_out, int* lens,
                          int* token_start, long long* slot_map, int* positions, int* pool_next, void* stream) {
     if (B < 1 || B > kMaxRequests || max_pages < 1 || page_rows < 1 || num_pages < 1 || num_pages > (1 << 28) ||
-        (long long)max_pages * page_rows > kMaxT || max_tokens < 0)
+        (long long)max_pages * page_rows > kMaxT || max_tokens < 0 || max_tokens > kMostTokens)
         return KVATTN_ERR_SHAPE;
     if (!block_table || !pool || !held || !kept || !fresh || !held_out || !lens || !token_start ||
         (!slot_map && max_tokens > 0))
