@@ -35,6 +35,7 @@ constexpr int kRuns = 4;                  // runs of a tile: neighbouring tokens
 static_assert(kWaves >= kRuns && kTile == kRuns * 4 * kWave, "a wave for every run");
 constexpr int kMaxVocab = 1 << 24;
 constexpr int kMaxSequences = 1 << 16;
+constexpr int kMostTokens = 1 << 30;      // a wave's next 64 drafts beyond are still an int
 constexpr int kFillBlocks = 512;          // workgroups that keep the memory busy, two a CU
 
 struct VerifyArgs {
@@ -346,7 +347,8 @@ int kvattn_verify_drafts(int* tokens, int* counts, const void* target_probs, con
                          const int* draft_tokens, const float* uniform, const int* token_start, int B, int num_tokens,
                          int V, long long row_stride, int dtype, void* workspace, size_t workspace_bytes, void* stream) {
     if (dtype != KVATTN_KV_F32 && dtype != KVATTN_KV_BF16) return KVATTN_ERR_DTYPE;
-    if (B < 1 || B > kMaxSequences || V < 1 || V > kMaxVocab || num_tokens < 0 || row_stride < V) return KVATTN_ERR_SHAPE;
+    if (B < 1 || B > kMaxSequences || V < 1 || V > kMaxVocab || num_tokens < 0 || num_tokens > kMostTokens || row_stride < V)
+        return KVATTN_ERR_SHAPE;
     if (!counts || !token_start) return KVATTN_ERR_NULL_POINTER;
     // (Nothing of an array without elements is looked at, and its address may be none.)
     if (num_tokens > 0 && (!tokens || !target_probs || !draft_tokens || !uniform)) return KVATTN_ERR_NULL_POINTER;

@@ -472,7 +472,7 @@ int kvattn_paged_load(void* kv, const void* pages, const float* page_scales, int
  * tokens [num_tokens] (may be draft_tokens): accepted drafts, the drawn token, -1 behind it; counts
  * [B]: accepted plus drawn.  A row without any mass draws nothing (counts: accepted alone).  A sequence without tokens
  * has count 0; rows behind token_start[B] are left as they were.  num_tokens may be 0: then counts and
- * token_start alone are needed.
+ * token_start alone are needed.  B <= 65536, V <= 2^24, num_tokens <= 2^30.
  *   target_probs, draft_probs  [num_tokens] rows of V probabilities, row_stride elements apart, float
  *               (dtype KVATTN_KV_F32) or bf16 (KVATTN_KV_BF16); NaN, infinite and negative ones weigh
  *               nothing in a draw.  draft_probs NULL: drafts without probabilities (q = 1 at the draft)

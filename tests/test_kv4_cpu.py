@@ -92,6 +92,7 @@ def test_counts_whose_indices_would_overflow():
     """Refused before the GPU: a thread's walk past its last row would leave 31 bits."""
     for n in (2 ** 30 + 1, 2 ** 31 - 1):
         assert _status("kvattn_paged_reserve", RESERVE, dict(most=n)) == 4
+        assert _status("kvattn_verify_drafts", VERIFY, dict(n=n)) == 4
 
 
 def test_pool_calls():
