@@ -568,7 +568,7 @@ int rows_call(const void* fn, void* act, void* pages, float* scales, int page_ro
               const long long* slots, int n, int NH, int hs, int dt, void* stream) {
     if (hs != kHd) return KVATTN_ERR_HEAD_DIM;
     if (n < 1 || NH < 1 || page_rows < 1 || page_rows > kMaxT || num_pages < 1) return KVATTN_ERR_SHAPE;
-    if ((long long)n * NH > (1ll << 27)) return KVATTN_ERR_SHAPE;
+    if (NH > (1 << 24) || (long long)n * NH > (1ll << 27)) return KVATTN_ERR_SHAPE;
     if (!fn) return KVATTN_ERR_DTYPE;
     if (!act || !pages || !slots) return KVATTN_ERR_NULL_POINTER;
     const bool coded = dt != KVATTN_KV_F32 && dt != KVATTN_KV_BF16;

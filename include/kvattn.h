@@ -451,7 +451,7 @@ int kvattn_paged_reserve(int* block_table, int max_pages, int page_rows, int num
 /* K and V rows of num_tokens tokens, from qkv [num_tokens][3][NH][hs], into the pool at slots
  * slot_map[t] = page * page_rows + row, for every kv_dtype, as kvattn_paged_cache_write writes a
  * row.  Slots outside [0, num_pages * page_rows) are skipped; the others must differ from one
- * another. */
+ * another.  num_tokens * NH <= 2^27, NH <= 2^24. */
 int kvattn_paged_store(void* pages, float* page_scales, int page_rows, int num_pages, const long long* slot_map,
                        const void* qkv, int num_tokens, int NH, int hs, int kv_dtype, void* stream);
 

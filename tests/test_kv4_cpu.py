@@ -95,6 +95,14 @@ def test_counts_whose_indices_would_overflow():
         assert _status("kvattn_verify_drafts", VERIFY, dict(n=n)) == 4
 
 
+def test_rows_of_more_heads_than_a_grid_takes():
+    """2^24 heads, as everywhere: few tokens of more would have more threads than a grid counts."""
+    order = ("act", "pages", "scales", "R", "P", "slots", "n", "NH", "hs", "dt", "stream")
+    for n, NH in ((1, 1 << 25), (4, 1 << 25), (1, 1 << 27), (1, (1 << 24) + 1), (9, 1 << 24)):
+        assert _status("kvattn_paged_store", ROWS, dict(n=n, NH=NH)) == 4
+        assert _status("kvattn_paged_load", {k: ROWS[k] for k in order}, dict(n=n, NH=NH)) == 4
+
+
 def test_pool_calls():
     kv = _kv()
     L = kv.lib()
