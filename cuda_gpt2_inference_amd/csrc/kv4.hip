@@ -50,6 +50,7 @@ constexpr float kQScale = 0.125f * 1.4426950408889634f;    // 1/sqrt(64) * log2(
 constexpr float kSlack = 8.0f;
 constexpr int kMaxT = 1 << 23;
 constexpr int kMaxSegments = 65535;        // the grid's third side
+constexpr int kMostWaves = (1 << 26) - 1;  // of a grid: 2^32 threads are too many
 // AUTO's shapes.  Up to one head a CU (two where eight queries share a pass, whose heads take longer),
 // workgroups of 8 waves, in as many segments as there are CUs; beyond,
 // 4 waves, in segments that fill four workgroups a CU, and with ragged lengths past 6144 positions of
@@ -584,7 +585,7 @@ int plan4(int heads, int queries, int maxT, int len_hint, bool ragged, int S, Pl
     p.S = p.waves == 8 ? std::max(1, kCUs / heads) : 4 * kCUs / heads;
     p.S = std::min(p.S, (tiles + kSegTiles - 1) / kSegTiles);
     if (p.waves == 4 && ragged && tiles >= 96) p.S = std::max(p.S, tiles / 32);
-    p.S = std::max(1, std::min(p.S, kMaxSegments));
+    p.S = std::max(1, std::min({p.S, kMaxSegments, kMostWaves / p.waves / heads}));
     // Or ceil(tiles / S), on the device.
     p.seg_tiles = p.waves == 4 && ragged && p.S > 1 ? kRaggedSegTiles : kSegTiles;
     return KVATTN_OK;
@@ -606,7 +607,7 @@ int attend4(const Attend4& c, bool launch) {
     const int st = plan4((int)std::min<long long>(heads, 1 << 30), per, c.maxT, c.len_hint, c.start || c.lens_per_seq,
                          c.S, plan);
     if (st != KVATTN_OK) return st;
-    if (c.B > 65535 || heads * plan.S * plan.waves * kWave > 0xffffffffll) return KVATTN_ERR_SHAPE;
+    if (c.B > 65535 || heads * plan.S * plan.waves > kMostWaves) return KVATTN_ERR_SHAPE;
     Args a{};
     if (plan.S > 1) {
         if (!c.ws) return KVATTN_ERR_WORKSPACE;

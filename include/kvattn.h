@@ -400,7 +400,8 @@ int kvattn_paged_decode(void* out, const void* qkv, void* pages, float* page_sca
  *               launches), or any larger number; a sequence with more has the first max_new or more
  *               of them computed
  * Rows of out behind token_start[B] are left as they were.  token_start must not decrease; it and
- * lens are clamped into [0, num_tokens] and [0, max_pages * page_rows].  B <= 65535.  Workspace:
+ * lens are clamped into [0, num_tokens] and [0, max_pages * page_rows].  B <= 65535; B * NH,
+ * num_tokens * NH and, where max_new > 8, (B + num_tokens / 8) * NH below 2^24.  Workspace:
  * kvattn_workspace_bytes(num_tokens, NH, hs, max_pages * page_rows, S); S as in kvattn_decode with
  * a 4-bit cache.
  * No reference counterpart (the reference decodes one token at a time). */

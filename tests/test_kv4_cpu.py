@@ -46,6 +46,14 @@ def test_decode_tokens_takes_any_max_new(B, n, NH, max_new):
     assert _status("kvattn_paged_decode_tokens", TOKENS, dict(B=B, n=n, NH=NH, max_new=max_new, S=2, ws=None)) == 7
 
 
+@pytest.mark.parametrize("B,NH,n,max_new", [(342, 12, 400, 8), (342, 12, 400, 1), (4096, 12, 8192, 100), (4096, 12, 4096, 2)])
+def test_widest_tables_are_taken(B, NH, n, max_new):
+    """Tables of 2^23 positions a sequence: the segments that the library picks fit a grid (refused here for the missing
+    workspace alone)."""
+    kw = dict(B=B, NH=NH, n=n, max_new=max_new, max_pages=1 << 17, ws=None)
+    assert _status("kvattn_paged_decode_tokens", TOKENS, kw) == 7
+
+
 DECODE = dict(out=A, qkv=A, kv=A, scale=A, B=1, NH=12, hs=64, maxT=4096, cur=A, per_seq=0, hint=-1, ws=None, wsb=0, S=4,
               strategy=0, dt=4, stream=None)
 
