@@ -534,8 +534,10 @@ __global__ __launch_bounds__(kBlock) void load_rows_kernel(RowsArgs a) {
 #pragma unroll
         for (int e = 0; e < 4; ++e)
             o[e] = f32_to_bf16(x[2 * e] * scale) | (uint32_t)f32_to_bf16(x[2 * e + 1] * scale) << 16;
-        // Past the caches: what is loaded is mostly more than they hold (8192 tokens in and out 18.8 us without,
-        // 17.8 so; 160 tokens 4.9 both ways).  The same for what is stored costs 1.4 us.
+        // Past the caches: what is loaded is mostly more than they hold.  12 heads of FP4, us without / so: the load alone,
+        // 160 tokens 2.4 / 2.4, 4000 6.1 / 5.6, 8192 9.5 / 8.1; stored and loaded, 160 4.8 / 4.8, 8192 18.7 / 17.5; loaded and
+        // read by the next kernel, 160 4.4 / 4.6, 1000 6.2 / 6.5, 4000 13.8 / 12.5, 8192 19.5 / 19.8.  The same for
+        // what is stored costs 1.4 us.
         store16_nt(to, make_uint4(o[0], o[1], o[2], o[3]));
     }
 }

@@ -562,3 +562,22 @@ def test_rows_past_32_bit_offsets(dev, kv):
     assert torch.equal(pages[P - 1, :, :, 1000:1003].permute(2, 0, 1, 3).cpu(), torch.from_numpy(c))
     want = (kv4ref.decode(c, np.ones_like(s), kv).astype(np.float32) * s[..., None])
     assert torch.equal(back.cpu(), torch.from_numpy(want).to(torch.bfloat16))
+
+
+@pytest.mark.parametrize("T,n", [(1, 1), (64, 1), (999, 1), (999, 5), (2048, 8), (4097, 1)])
+def test_int4_within_its_operands_bound(dev, monkeypatch, T, n):
+    """The INT4 operand is code + 8, of magnitude 1 to 15: the bound of sums over such terms, half as wide as one for
+    another operand's 31."""
+    import torch
+    kvattn = _kv()
+    monkeypatch.setitem(kv4ref.BIAS, "int4", 8.0)
+    maxT = -(-T // 64) * 64
+    case = Case("int4", 2, 3, maxT, [T, max(n, T // 2)], seed=T + n, sharp=2.0)
+    cache, _ = case.paged(64, dev)
+    q = case.queries(2 * n)
+    out = torch.empty(2 * n, 3, HS, dtype=torch.bfloat16, device=dev)
+    ws = kvattn.Workspace(2 * n, 3, maxT)
+    kvattn.paged_decode_tokens(out, _qkv(q, dev), cache, _dev(np.array([0, n, 2 * n], np.int32), dev),
+                               _dev(np.array(case.lens, np.int32), dev), 2, 2 * n, 3, HS, kv_dtype="int4", max_new=n, **ws.kwargs())
+    tokens = [(b * n + i, b, case.lens[b] - n + i + 1) for b in range(2) for i in range(n)]
+    case.check(out.float().cpu().numpy(), q, tokens, f"T {T} n {n}")
