@@ -442,7 +442,8 @@ int kvattn_paged_pool_init(int* pool, int num_pages, void* stream);
  * 0 <= kept <= held, 0 <= fresh, kept + fresh <= max_pages * page_rows; it counts as having no
  * tokens.  A granted request is told by lens[b] == kept[b] + fresh[b].  A refused one's token rows
  * stay among token_start's, and what attention and verification of the step write for them means
- * nothing: its kept is the next step's again.  Table entries outside [0, num_pages) give slot -1 and go back to the ring as they are.
+ * nothing: its kept is the next step's again.  Table entries outside [0, num_pages) give slot -1 and
+ * go back to the ring as they are.
  * B <= 4096, max_tokens <= 2^30.  Calls on one pool must be ordered. */
 int kvattn_paged_reserve(int* block_table, int max_pages, int page_rows, int num_pages, int* pool,
                          const int* held, const int* kept, const int* fresh, int B, int max_tokens,
