@@ -21,41 +21,12 @@
 // So a load takes row lane / 4, chunk lane % 4, and ds_bpermute moves the four dwords to the
 // operand's lane.
 #include "fc.hpp"
+#include "matrix.hpp"
 
 #include <algorithm>
 #include <type_traits>
 
 namespace {
-
-typedef __bf16 Bf16x8 __attribute__((ext_vector_type(8)));
-typedef uint32_t U32x4 __attribute__((ext_vector_type(4)));
-typedef float F32x4 __attribute__((ext_vector_type(4)));
-
-// A lane's 16-byte chunk of 8-bit codes as 16 bf16 values, two MFMA operands of 8.  Every code
-// is exact in bf16: INT8 has at most 7 significant bits and a sign (-128 = -2^7), E4M3 four.
-template <bool kFp8>
-__device__ __forceinline__ void codes_to_bf16(U32x4 w, Bf16x8 (&o)[2]) {
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        uint32_t p[4];
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const uint32_t c = w[2 * h + i];
-            if constexpr (kFp8) {
-                p[2 * i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c, 1.0f, false));
-                p[2 * i + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c, 1.0f, true));
-            } else {
-                float f[4];
-#pragma unroll
-                for (int k = 0; k < 4; ++k) f[k] = (float)(int8_t)(c >> (8 * k));
-                // The high halves of two floats whose low halves are zero.
-                p[2 * i] = __builtin_amdgcn_perm(__float_as_uint(f[1]), __float_as_uint(f[0]), 0x07060302u);
-                p[2 * i + 1] = __builtin_amdgcn_perm(__float_as_uint(f[3]), __float_as_uint(f[2]), 0x07060302u);
-            }
-        }
-        o[h] = __builtin_bit_cast(Bf16x8, U32x4{p[0], p[1], p[2], p[3]});
-    }
-}
 
 __device__ __forceinline__ U32x4 ld16(const uint8_t* p) { return *reinterpret_cast<const U32x4*>(p); }
 

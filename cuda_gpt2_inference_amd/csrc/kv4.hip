@@ -29,16 +29,12 @@
 
 #include "lanes.hpp"
 #include "layout.hpp"
+#include "matrix.hpp"
 
 namespace {
 
 using kvattn_internal::Attend4;
 using kvattn_internal::Plan4;
-
-typedef __bf16 Bf16x8 __attribute__((ext_vector_type(8)));
-typedef uint32_t U32x4 __attribute__((ext_vector_type(4)));
-typedef int I32x2 __attribute__((ext_vector_type(2)));
-typedef float F32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kHd = 64;
 constexpr int kTile = 64;                  // positions of a tile
@@ -128,62 +124,6 @@ __device__ __forceinline__ Raw<kC> load_tile(const Args& a, size_t row0, int las
     return r;
 }
 
-// Eight 4-bit codes as a matrix-core operand.  FP4: the values, in order.  INT4: 8 + code, which the
-// callers take off again: a half byte alone in a byte is an E4M3 number 2^-9 times it, and one
-// instruction makes bf16 of two; in the order 0 2 4 6 1 3 5 7.
-template <bool kFp4>
-__device__ __forceinline__ Bf16x8 operand(uint32_t w) {
-    U32x4 d;
-    if constexpr (kFp4) {
-        d[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, 1.0f, 0));
-        d[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, 1.0f, 1));
-        d[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, 1.0f, 2));
-        d[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, 1.0f, 3));
-    } else {
-        const uint32_t even = w & 0x0F0F0F0Fu, odd = (w >> 4) & 0x0F0F0F0Fu;
-        d[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(even, 512.0f, false));
-        d[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(even, 512.0f, true));
-        d[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(odd, 512.0f, false));
-        d[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(odd, 512.0f, true));
-    }
-    return __builtin_bit_cast(Bf16x8, d);
-}
-
-// The place of code r of eight in operand().
-template <bool kFp4>
-__device__ __forceinline__ int place(int r) { return kFp4 ? r : ((r & 1) << 2) + (r >> 1); }
-
-// Eight bf16 values in the order of operand()'s.
-template <bool kFp4>
-__device__ __forceinline__ Bf16x8 in_order(const uint4& w) {
-    U32x4 d = {w.x, w.y, w.z, w.w};
-    if constexpr (!kFp4) {
-        d[0] = (w.x & 0xffffu) | (w.y << 16);
-        d[1] = (w.z & 0xffffu) | (w.w << 16);
-        d[2] = (w.x >> 16) | (w.y & 0xffff0000u);
-        d[3] = (w.z >> 16) | (w.w & 0xffff0000u);
-    }
-    return __builtin_bit_cast(Bf16x8, d);
-}
-
-__device__ __forceinline__ F32x4 mfma(Bf16x8 a, Bf16x8 b, F32x4 c) {
-    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
-}
-
-__device__ __forceinline__ void put(float* p, float v) {
-    __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-}
-__device__ __forceinline__ float get(const float* p) {
-    return __hip_atomic_load(const_cast<float*>(p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-}
-
-// exp2(m - M) with an empty side (m = -inf) weighing nothing.
-__device__ __forceinline__ float weight_of(float m, float M) { return m == -INFINITY ? 0.0f : exp2_fast(m - M); }
-
-// The wave's LDS operations run in order, so what its lanes hand one another there needs no barrier;
-// this keeps the compiler from moving one lane's reads over another's writes.
-__device__ __forceinline__ void lds_order() { asm volatile("" ::: "memory"); }
-
 // Groups of kQ queries in one line, as many as the tokens can fill: sequence b's first is start[b] / kQ + b, and as
 // its n tokens make at most start[b + 1] / kQ - start[b] / kQ + 1 of them, no two sequences meet, and all of them end
 // before B + num_tokens / kQ.  The last sequence that begins at or before the slot, 64 looked at at once, and
@@ -201,9 +141,6 @@ __device__ __forceinline__ int sequence_at(const Args& a, int slot, int lane, in
     grp = slot - first(b);
     return b;
 }
-
-// Keeps a wave's rare branch from becoming selects that every tile runs.
-__device__ __forceinline__ void stay_a_branch() { asm volatile(""); }
 
 // kQ: queries of a workgroup (1, 4 or 8); kW: its waves; kNt: codes loaded as read only once.
 template <bool kFp4, int kQ, int kW, bool kNt>

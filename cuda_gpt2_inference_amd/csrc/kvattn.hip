@@ -42,6 +42,7 @@
 #include "kv4.hpp"
 #include "kvattn.h"
 #include "lanes.hpp"
+#include "tree.hpp"
 
 namespace {
 
@@ -3013,6 +3014,26 @@ int kvattn_paged_decode_tokens(void* out, const void* qkv, const void* pages, co
                                      num_pages, B, NH, maxT, num_tokens, max_new, 1, -1, S, kv_dtype, workspace,
                                      workspace_bytes, stream};
     return kvattn_internal::attend4(c, true);
+}
+
+int kvattn_paged_decode_tree(void* out, const void* qkv, const void* pages, const float* page_scales,
+                             const int* block_table, int max_pages, int page_rows, int num_pages,
+                             const int* token_start, const int* lens, const unsigned long long* masks, int mask_words,
+                             int B, int num_tokens, int max_new, int NH, int hs, void* workspace,
+                             size_t workspace_bytes, int S, int kv_dtype, void* stream) {
+    int maxT = 0;
+    KV_TRY(check_paged(block_table, max_pages, page_rows, num_pages, NH, maxT));
+    KV_TRY(check_common(qkv, pages, page_scales, B, NH, hs, maxT, is_4bit(kv_dtype) ? (int)KVATTN_KV_INT8 : kv_dtype));
+    if (num_tokens < 1 || max_new < 1 || (long long)num_tokens * NH > (1ll << 24)) return KVATTN_ERR_SHAPE;
+    if (mask_words < 1 || mask_words > kvattn_internal::kMaxMaskWords || std::min(max_new, num_tokens) > 64 * mask_words)
+        return KVATTN_ERR_SHAPE;
+    if (!out || !token_start || !lens || !masks) return KVATTN_ERR_NULL_POINTER;
+    if (!aligned16(out) || ((uintptr_t)token_start & 3u) || ((uintptr_t)lens & 3u) || ((uintptr_t)masks & 7u))
+        return KVATTN_ERR_MISALIGNED;
+    const kvattn_internal::AttendTree c{out, qkv, pages, page_scales, block_table, token_start, lens, masks, mask_words,
+                                        max_pages, page_rows, num_pages, B, NH, maxT, num_tokens, max_new, S, kv_dtype,
+                                        workspace, workspace_bytes, stream};
+    return kvattn_internal::attend_tree(c);
 }
 
 int kvattn_forward_small(void* out, const void* qkv, const void* kv_cache, const float* kv_scale, int B, int NH,

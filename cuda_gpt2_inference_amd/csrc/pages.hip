@@ -550,6 +550,83 @@ int launch_rows(const void* fn, RowsArgs a, void* stream) {
     return hip_status(hipLaunchKernel(fn, dim3((unsigned)grid), dim3(kBlock), params, 0, (hipStream_t)stream));
 }
 
+// A tree's accepted path next to the prefix: the row of path[d] to the place of the sequence's d-th new token.  Eight
+// lanes have a row, as above; a sequence's (part, head) is one such group's, which goes along the path: what is
+// written at d is read at d or before, as path[d] >= d and the path only grows.  So loads of eight steps, then their stores.
+struct KeepArgs {
+    uint8_t* kv;
+    float* scale;
+    const long long* slots;
+    const int* path;
+    const int* start;
+    int R, num_pages, B, num_tokens, NH, shift;
+};
+
+template <int DT>
+__global__ __launch_bounds__(kBlock) void keep_rows_kernel(KeepArgs a) {
+    using F = Fmt<DT>;
+    const int lane = threadIdx.x & (kWave - 1), c = lane & 7, group = lane & 56;
+    const long long item = (long long)blockIdx.x * (kBlock / 8) + threadIdx.x / 8;
+    const int b = (int)(item / (2 * a.NH)), ph = (int)(item - (long long)b * 2 * a.NH), part = ph >= a.NH, h = ph - part * a.NH;
+    const bool live = b < a.B;
+    int t0 = 0, n = 0;
+    if (live) {
+        t0 = min(max(a.start[b], 0), a.num_tokens);
+        n = min(max(a.start[b + 1], t0), a.num_tokens) - t0;
+    }
+    auto row_of = [&](long long slot) {
+        if (slot < 0 || slot >= (long long)a.num_pages * a.R) return -1ll;
+        const long long page = a.shift >= 0 ? slot >> a.shift : slot / a.R;
+        return (page * 2 * a.NH + (long long)part * a.NH + h) * a.R + (slot - page * a.R);
+    };
+    // (The wave's groups go on together until the longest path ends.)
+    bool more = live;
+    for (int d0 = 0; __any(more); d0 += 8) {
+        const int d = d0 + c;
+        long long from = -1, to = -1;
+        bool ok = false;
+        if (more && d < n) {
+            const int at = a.path[t0 + d], last = d > 0 ? a.path[t0 + d - 1] : -1;
+            ok = at >= d && at < n && at > last;
+            if (ok && at != d) {
+                from = row_of(a.slots[t0 + at]);
+                to = row_of(a.slots[t0 + d]);
+            }
+        }
+        const uint32_t steps = (uint32_t)(__ballot(ok) >> group) & 0xffu;
+        const int len = __builtin_ctz(~steps);         // steps of this group until its path ends
+        if (c >= len || from < 0 || to < 0 || from == to) from = -1;
+        more = more && len == 8;
+        uint4 x0[8], x1[8];
+        float sc[8];
+        long long src[8], dst[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            src[j] = __shfl(from, group + j);
+            dst[j] = __shfl(to, group + j);
+            if (src[j] < 0) continue;
+            const uint8_t* const p = a.kv + (src[j] * 8 + c) * F::kBytes;
+            if constexpr (F::kBytes >= 16) x0[j] = *reinterpret_cast<const uint4*>(p);
+            if constexpr (F::kBytes == 32) x1[j] = reinterpret_cast<const uint4*>(p)[1];
+            if constexpr (F::kBytes == 8) *reinterpret_cast<uint2*>(&x0[j]) = *reinterpret_cast<const uint2*>(p);
+            if constexpr (F::kBytes == 4) x0[j].x = *reinterpret_cast<const uint32_t*>(p);
+            if constexpr (F::kCoded) sc[j] = a.scale[src[j]];
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            if (src[j] < 0) continue;
+            uint8_t* const p = a.kv + (dst[j] * 8 + c) * F::kBytes;
+            if constexpr (F::kBytes >= 16) *reinterpret_cast<uint4*>(p) = x0[j];
+            if constexpr (F::kBytes == 32) reinterpret_cast<uint4*>(p)[1] = x1[j];
+            if constexpr (F::kBytes == 8) *reinterpret_cast<uint2*>(p) = *reinterpret_cast<const uint2*>(&x0[j]);
+            if constexpr (F::kBytes == 4) *reinterpret_cast<uint32_t*>(p) = x0[j].x;
+            if constexpr (F::kCoded) {
+                if (c == 0) a.scale[dst[j]] = sc[j];
+            }
+        }
+    }
+}
+
 template <template <int> class K>
 const void* by_type(int dt) {
     switch (dt) {
@@ -564,6 +641,7 @@ const void* by_type(int dt) {
 }
 template <int DT> struct StoreFn { static const void* fn() { return (const void*)&store_rows_kernel<DT, true>; } };
 template <int DT> struct LoadFn { static const void* fn() { return (const void*)&load_rows_kernel<DT>; } };
+template <int DT> struct KeepFn { static const void* fn() { return (const void*)&keep_rows_kernel<DT>; } };
 
 // Checks shared by paged_store and paged_load, then the launch.
 int rows_call(const void* fn, void* act, void* pages, float* scales, int page_rows, int num_pages,
@@ -656,6 +734,29 @@ int kvattn_paged_load(void* kv, const void* pages, const float* page_scales, int
                       const long long* slot_map, int num_tokens, int NH, int hs, int kv_dtype, void* stream) {
     return rows_call(by_type<LoadFn>(kv_dtype), kv, (void*)pages, (float*)page_scales, page_rows, num_pages, slot_map,
                      num_tokens, NH, hs, kv_dtype, stream);
+}
+
+int kvattn_paged_keep(void* pages, float* page_scales, int page_rows, int num_pages, const long long* slot_map,
+                      const int* path, const int* token_start, int B, int num_tokens, int NH, int hs, int kv_dtype,
+                      void* stream) {
+    if (hs != kHd) return KVATTN_ERR_HEAD_DIM;
+    if (B < 1 || num_tokens < 0 || num_tokens > kMostTokens || NH < 1 || page_rows < 1 || page_rows > kMaxT || num_pages < 1 ||
+        (long long)B * NH > (1ll << 24))
+        return KVATTN_ERR_SHAPE;
+    const void* fn = by_type<KeepFn>(kv_dtype);
+    if (!fn) return KVATTN_ERR_DTYPE;
+    if (num_tokens == 0) return KVATTN_OK;
+    if (!pages || !slot_map || !path || !token_start) return KVATTN_ERR_NULL_POINTER;
+    const bool coded = kv_dtype != KVATTN_KV_F32 && kv_dtype != KVATTN_KV_BF16;
+    if (coded && !page_scales) return KVATTN_ERR_DTYPE;
+    if (((uintptr_t)pages & 15u) || ((uintptr_t)slot_map & 7u) || ((uintptr_t)path & 3u) || ((uintptr_t)token_start & 3u) ||
+        ((uintptr_t)page_scales & 3u))
+        return KVATTN_ERR_MISALIGNED;
+    KeepArgs a{(uint8_t*)pages, page_scales, slot_map, path, token_start, page_rows, num_pages, B, num_tokens, NH,
+               log2_or(page_rows)};
+    const long long grid = ((long long)B * 2 * NH + kBlock / 8 - 1) / (kBlock / 8);
+    void* params[] = {&a};
+    return hip_status(hipLaunchKernel(fn, dim3((unsigned)grid), dim3(kBlock), params, 0, (hipStream_t)stream));
 }
 
 }  // extern "C"

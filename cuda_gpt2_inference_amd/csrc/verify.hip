@@ -1,6 +1,9 @@
 // verify.hip -- verification of drafted tokens on MI355X (gfx950): a sequence's drafts are accepted
 // one after another while r q(x) < p(x), and the token behind the last accepted one is drawn from
 // max(0, p - q) where a draft was refused, from p where none was, by the inverse of the running sum.
+// Of a tree of drafts, a token's children are tried in their order while r < the sum of p over those tried: the
+// inverse of p's running sum with the children's tokens first, whatever the tree was made from; behind the last
+// accepted token the rest of that sum, p without its children, is drawn from.
 //
 // Only one row of p and one of q a sequence is read whole (2 x 200 KB at GPT-2's vocabulary): which
 // one follows from a few single values, which every wave looks up for itself.  The row is cut into
@@ -21,10 +24,7 @@
 
 #include "kvattn.h"
 #include "lanes.hpp"
-
-namespace kvattn_internal {
-void set_last_hip_error(int e);   // kvattn.hip: read back by kvattn_last_hip_error
-}
+#include "tree.hpp"
 
 namespace {
 
@@ -50,7 +50,15 @@ struct VerifyArgs {
     unsigned* counters;
     size_t row;                           // elements from one row to the next
     int B, num_tokens, V, tiles, blocks;  // blocks: workgroups of a sequence
+    // A tree of drafts (drafts: every token's own).
+    const int* parents;
+    const float* draw;
+    const int* lens;
+    int* path;
+    int* kept;
 };
+using kvattn_internal::kMaxTree;
+constexpr int kTreeLanes = kMaxTree / kWave;   // tokens of a tree a lane holds
 
 template <bool kF32>
 __device__ __forceinline__ float prob(const void* p, size_t i) {
@@ -147,24 +155,101 @@ __device__ __forceinline__ double get64(const double* p) {
     return __hip_atomic_load(const_cast<double*>(p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
-template <bool kF32, bool kVec>
+// The walk down a tree of n tokens, by every wave for itself: path gets the accepted tokens' numbers, the root's
+// first, out the tokens of the last one's children.  -> the path's length less one, and the children's number.
+struct Walk {
+    int depth, children;
+};
+template <bool kF32>
+__device__ __forceinline__ Walk walk_tree(const VerifyArgs& a, int t0, int n, int lane, int* path, int* out) {
+    int parent[kTreeLanes], token[kTreeLanes];
+    float mass_of[kTreeLanes], u[kTreeLanes];
+    const int rounds = (min(n, kMaxTree) + kWave - 1) / kWave;
+#pragma unroll
+    for (int r = 0; r < kTreeLanes; ++r) {
+        parent[r] = -1;
+        token[r] = -1;
+        mass_of[r] = u[r] = 0.0f;
+        const int i = lane + kWave * r;
+        if (r < rounds && i > 0 && i < n) {
+            const int p = a.parents[t0 + i];
+            token[r] = a.drafts[t0 + i];
+            if (p >= 0 && p < i) {
+                parent[r] = p;
+                u[r] = a.u[t0 + p];
+                if (token[r] >= 0 && token[r] < a.V)
+                    mass_of[r] = prob<kF32>(a.p, (size_t)(t0 + p) * a.row + token[r]);
+            }
+        }
+    }
+    Walk w{0, 0};
+    int at = 0;
+    if (lane == 0) path[0] = 0;
+    for (;;) {
+        double upto = 0.0;
+        int next = -1;
+        w.children = 0;
+#pragma unroll
+        for (int r = 0; r < kTreeLanes; ++r) {
+            if (r >= rounds || next >= 0) break;
+            for (unsigned long long left = __ballot(parent[r] == at); left; left &= left - 1) {
+                const int j = __ffsll((long long)left) - 1;
+                const int x = __builtin_amdgcn_readlane(token[r], j);
+                // A token that an earlier child is has no mass left.
+                bool again = false;
+#pragma unroll
+                for (int q = 0; q <= r; ++q) {
+                    unsigned long long same = __ballot(parent[q] == at && token[q] == x);
+                    if (q == r) same &= (1ull << j) - 1;
+                    again |= same != 0;
+                }
+                if (lane == 0) out[w.children] = x;
+                ++w.children;
+                if (again) continue;
+                const float p = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(mass_of[r]), j));
+                upto += mass(finite(p));
+                if ((double)__uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(u[r]), j)) < upto) {
+                    next = j + kWave * r;
+                    break;
+                }
+            }
+        }
+        if (next < 0) return w;
+        at = next;
+        ++w.depth;
+        if (lane == 0) path[w.depth] = at;
+    }
+}
+
+template <bool kF32, bool kVec, bool kTree>
 __global__ __launch_bounds__(kBlock) void verify_kernel(VerifyArgs a) {
     __shared__ int is_last;
     __shared__ double run_sums[kRuns];
+    // Of a tree, every wave's own.
+    __shared__ int paths[kTree ? kWaves : 1][kTree ? kMaxTree : 1], outs[kTree ? kWaves : 1][kTree ? kMaxTree : 1];
     const int slot = xcd_slot(blockIdx.x, a.blocks), b = slot / a.blocks, blk = slot - b * a.blocks;
     if (b >= a.B) return;
     const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
     const int t0 = min(max(a.start[b], 0), a.num_tokens);
     const int n = min(max(a.start[b + 1], t0), a.num_tokens) - t0;
     if (n == 0) {
-        if (blk == 0 && threadIdx.x == 0) a.count[b] = 0;
+        if (blk == 0 && threadIdx.x == 0) {
+            a.count[b] = 0;
+            if (kTree && a.kept) a.kept[b] = a.lens[b];
+        }
         return;
     }
-    const float u_last = a.u[t0 + n - 1];  // a number that no draft is held against
+    const float u_last = kTree ? a.draw[b] : a.u[t0 + n - 1];  // a number that no draft is held against
     // The first row whose draft is not accepted (the last row has none): 64 rows at a time, a lane
     // each.  The comparison is exact: products of two floats fit a double.
     int row = n - 1, draft = -1;
-    for (int i0 = 0; i0 < n - 1; i0 += kWave) {
+    Walk walk{0, 0};
+    const int* const out = outs[kTree ? wave : 0];
+    if constexpr (kTree) {
+        walk = walk_tree<kF32>(a, t0, n, lane, paths[wave], outs[wave]);
+        row = paths[wave][walk.depth];
+    }
+    for (int i0 = 0; i0 < (kTree ? 0 : n - 1); i0 += kWave) {
         const int i = i0 + lane;
         bool no = false;
         int x = -1;
@@ -185,7 +270,7 @@ __global__ __launch_bounds__(kBlock) void verify_kernel(VerifyArgs a) {
             break;
         }
     }
-    const bool refused = row < n - 1;
+    const bool refused = !kTree && row < n - 1;
     const bool less_q = refused && a.q;
     const size_t row0 = (size_t)(t0 + row) * a.row;
 
@@ -208,6 +293,22 @@ __global__ __launch_bounds__(kBlock) void verify_kernel(VerifyArgs a) {
 #pragma unroll
                 for (int e = 0; e < 16; ++e)
                     rest += token_at(tile, e / 4, lane) + e % 4 == draft ? 0.0 : mass(finite(p[e]));
+            }
+        }
+        // Nor do a tree's children that were tried.
+        if constexpr (kTree) {
+            bool some = false;
+            for (int c = 0; c < walk.children; ++c) {
+                const int x = out[c];
+                if (x < 0 || x / kTile != tile) continue;
+                some = true;
+#pragma unroll
+                for (int e = 0; e < 16; ++e) p[e] = token_at(tile, e / 4, lane) + e % 4 == x ? 0.0f : p[e];
+            }
+            if (some) {
+                rest = 0.0;
+#pragma unroll
+                for (int e = 0; e < 16; ++e) rest += mass(finite(p[e]));
             }
         }
         rest = wave_sum64(rest);
@@ -291,6 +392,9 @@ __global__ __launch_bounds__(kBlock) void verify_kernel(VerifyArgs a) {
             w[i] = finite(p[i]);
             if (use_rest && less_q) w[i] -= finite(q[i]);
             w[i] = use_rest && !less_q && v0 + i == draft ? 0.0 : mass(w[i]);
+            if constexpr (kTree) {
+                for (int c = 0; c < (use_rest ? walk.children : 0); ++c) w[i] = v0 + i == out[c] ? 0.0 : w[i];
+            }
             mine += w[i];
         }
         const double sum = wave_prefix64(mine);
@@ -327,12 +431,76 @@ __global__ __launch_bounds__(kBlock) void verify_kernel(VerifyArgs a) {
         leave_zero();
         if (wave != 0) return;
     }
+    if constexpr (kTree) {
+        const int* const path = paths[wave];
+        // (tokens may be the drafts: all are read first.)
+        int accepted[kTreeLanes];
+#pragma unroll
+        for (int r = 0; r < kTreeLanes; ++r) {
+            const int i = lane + kWave * r;
+            accepted[r] = i < walk.depth ? a.drafts[t0 + path[i + 1]] : (i == walk.depth ? drawn : -1);
+        }
+        for (int i = lane + kMaxTree; i < n; i += kWave) a.path[t0 + i] = a.tokens[t0 + i] = -1;
+#pragma unroll
+        for (int r = 0; r < kTreeLanes; ++r) {
+            const int i = lane + kWave * r;
+            if (i >= n) break;
+            a.tokens[t0 + i] = accepted[r];
+            a.path[t0 + i] = i <= walk.depth ? path[i] : -1;
+        }
+        if (lane == 0) {
+            a.count[b] = walk.depth + (drawn >= 0 ? 1 : 0);
+            if (a.kept) a.kept[b] = max(a.lens[b] - n, 0) + walk.depth + 1;
+        }
+        return;
+    }
     for (int i = lane; i < n; i += kWave) a.tokens[t0 + i] = i < row ? a.drafts[t0 + i] : (i == row ? drawn : -1);
     if (lane == 0) a.count[b] = row + (drawn >= 0 ? 1 : 0);
 }
 
 int tiles_of(int V) { return (V + kTile - 1) / kTile; }
 size_t up256(size_t x) { return (x + 255) / 256 * 256; }
+
+template <bool kF32, bool kTree>
+const void* kernel_for(bool vec) {
+    return vec ? (const void*)&verify_kernel<kF32, true, kTree> : (const void*)&verify_kernel<kF32, false, kTree>;
+}
+
+// Checks shared by the two entry points, then the launch.
+int verify_call(VerifyArgs a, long long row_stride, int dtype, void* workspace, size_t workspace_bytes, void* stream) {
+    const int B = a.B, V = a.V;
+    if (dtype != KVATTN_KV_F32 && dtype != KVATTN_KV_BF16) return KVATTN_ERR_DTYPE;
+    if (B < 1 || B > kMaxSequences || V < 1 || V > kMaxVocab || a.num_tokens < 0 || a.num_tokens > kMostTokens || row_stride < V)
+        return KVATTN_ERR_SHAPE;
+    if (!a.count || !a.start) return KVATTN_ERR_NULL_POINTER;
+    // (Nothing of an array without elements is looked at, and its address may be none.)
+    if (a.num_tokens > 0 && (!a.tokens || !a.p || !a.drafts || !a.u)) return KVATTN_ERR_NULL_POINTER;
+    const size_t size = dtype == KVATTN_KV_F32 ? 4 : 2;
+    if (((uintptr_t)a.p % size) || ((uintptr_t)a.q % size) || ((uintptr_t)a.tokens & 3u) || ((uintptr_t)a.count & 3u) ||
+        ((uintptr_t)a.drafts & 3u) || ((uintptr_t)a.u & 3u) || ((uintptr_t)a.start & 3u) || ((uintptr_t)workspace & 255u))
+        return KVATTN_ERR_MISALIGNED;
+    if (!workspace || workspace_bytes < kvattn_verify_workspace_bytes(B, V)) return KVATTN_ERR_WORKSPACE;
+    a.counters = (unsigned*)workspace;
+    a.sums = (double*)((uint8_t*)workspace + up256((size_t)B * sizeof(unsigned)));
+    a.row = (size_t)row_stride;
+    a.tiles = tiles_of(V);
+    const int most = (a.tiles + kWaves - 1) / kWaves;      // one tile a wave
+    const int few = (kFillBlocks + B - 1) / B;
+    a.blocks = most < few ? most : few;
+    // Four probabilities in one load where every row starts on such a boundary.
+    const bool vec = row_stride % 4 == 0 && ((uintptr_t)a.p % (4 * size)) == 0 && ((uintptr_t)a.q % (4 * size)) == 0;
+    const void* fn;
+    if (a.parents) fn = dtype == KVATTN_KV_F32 ? kernel_for<true, true>(vec) : kernel_for<false, true>(vec);
+    else fn = dtype == KVATTN_KV_F32 ? kernel_for<true, false>(vec) : kernel_for<false, false>(vec);
+    const long long grid = 8ll * ((B + 7) / 8) * a.blocks;      // whole rounds of the eight XCDs
+    void* params[] = {&a};
+    const hipError_t e = hipLaunchKernel(fn, dim3((unsigned)grid), dim3(kBlock), params, 0, (hipStream_t)stream);
+    if (e != hipSuccess) {
+        kvattn_internal::set_last_hip_error((int)e);
+        return KVATTN_ERR_HIP;
+    }
+    return KVATTN_OK;
+}
 
 }  // namespace
 
@@ -346,18 +514,6 @@ size_t kvattn_verify_workspace_bytes(int B, int V) {
 int kvattn_verify_drafts(int* tokens, int* counts, const void* target_probs, const void* draft_probs,
                          const int* draft_tokens, const float* uniform, const int* token_start, int B, int num_tokens,
                          int V, long long row_stride, int dtype, void* workspace, size_t workspace_bytes, void* stream) {
-    if (dtype != KVATTN_KV_F32 && dtype != KVATTN_KV_BF16) return KVATTN_ERR_DTYPE;
-    if (B < 1 || B > kMaxSequences || V < 1 || V > kMaxVocab || num_tokens < 0 || num_tokens > kMostTokens || row_stride < V)
-        return KVATTN_ERR_SHAPE;
-    if (!counts || !token_start) return KVATTN_ERR_NULL_POINTER;
-    // (Nothing of an array without elements is looked at, and its address may be none.)
-    if (num_tokens > 0 && (!tokens || !target_probs || !draft_tokens || !uniform)) return KVATTN_ERR_NULL_POINTER;
-    const size_t size = dtype == KVATTN_KV_F32 ? 4 : 2;
-    if (((uintptr_t)target_probs % size) || ((uintptr_t)draft_probs % size) || ((uintptr_t)tokens & 3u) ||
-        ((uintptr_t)counts & 3u) || ((uintptr_t)draft_tokens & 3u) || ((uintptr_t)uniform & 3u) ||
-        ((uintptr_t)token_start & 3u) || ((uintptr_t)workspace & 255u))
-        return KVATTN_ERR_MISALIGNED;
-    if (!workspace || workspace_bytes < kvattn_verify_workspace_bytes(B, V)) return KVATTN_ERR_WORKSPACE;
     VerifyArgs a{};
     a.tokens = tokens;
     a.count = counts;
@@ -366,31 +522,37 @@ int kvattn_verify_drafts(int* tokens, int* counts, const void* target_probs, con
     a.drafts = draft_tokens;
     a.u = uniform;
     a.start = token_start;
-    a.counters = (unsigned*)workspace;
-    a.sums = (double*)((uint8_t*)workspace + up256((size_t)B * sizeof(unsigned)));
-    a.row = (size_t)row_stride;
     a.B = B;
     a.num_tokens = num_tokens;
     a.V = V;
-    a.tiles = tiles_of(V);
-    const int most = (a.tiles + kWaves - 1) / kWaves;      // one tile a wave
-    const int few = (kFillBlocks + B - 1) / B;
-    a.blocks = most < few ? most : few;
-    // Four probabilities in one load where every row starts on such a boundary.
-    const bool vec = row_stride % 4 == 0 && ((uintptr_t)target_probs % (4 * size)) == 0 &&
-                     ((uintptr_t)draft_probs % (4 * size)) == 0;
-    const void* fn = dtype == KVATTN_KV_F32
-                         ? (vec ? (const void*)&verify_kernel<true, true> : (const void*)&verify_kernel<true, false>)
-                         : (vec ? (const void*)&verify_kernel<false, true> : (const void*)&verify_kernel<false, false>);
-    const long long grid = 8ll * ((B + 7) / 8) * a.blocks;      // whole rounds of the eight XCDs
-    void* params[] = {&a};
-    const hipError_t e = hipLaunchKernel(fn, dim3((unsigned)grid), dim3(kBlock), params, 0,
-                                         (hipStream_t)stream);
-    if (e != hipSuccess) {
-        kvattn_internal::set_last_hip_error((int)e);
-        return KVATTN_ERR_HIP;
-    }
-    return KVATTN_OK;
+    return verify_call(a, row_stride, dtype, workspace, workspace_bytes, stream);
+}
+
+int kvattn_verify_tree(int* tokens, int* path, int* counts, int* kept, const void* target_probs, const int* tree_tokens,
+                       const int* parents, const float* uniform, const float* draw, const int* token_start,
+                       const int* lens, int B, int num_tokens, int V, long long row_stride, int dtype, void* workspace,
+                       size_t workspace_bytes, void* stream) {
+    static const int none = 0;
+    if (kept && !lens) return KVATTN_ERR_NULL_POINTER;
+    if (num_tokens > 0 && (!path || !parents || !draw)) return KVATTN_ERR_NULL_POINTER;
+    if (((uintptr_t)path & 3u) || ((uintptr_t)kept & 3u) || ((uintptr_t)parents & 3u) || ((uintptr_t)draw & 3u) || ((uintptr_t)lens & 3u))
+        return KVATTN_ERR_MISALIGNED;
+    VerifyArgs a{};
+    a.tokens = tokens;
+    a.count = counts;
+    a.p = target_probs;
+    a.drafts = tree_tokens;
+    a.u = uniform;
+    a.start = token_start;
+    a.B = B;
+    a.num_tokens = num_tokens;
+    a.V = V;
+    a.parents = parents ? parents : &none;     // (not read without tokens)
+    a.draw = draw;
+    a.lens = lens;
+    a.path = path;
+    a.kept = kept;
+    return verify_call(a, row_stride, dtype, workspace, workspace_bytes, stream);
 }
 
 }  // extern "C"

@@ -118,6 +118,17 @@ SIGNATURES = {
     "kvattn_paged_load": (_i, [_vp, _vp, _vp, _i, _i, _vp, _i, _i, _i, _i, _vp]),
     "kvattn_verify_workspace_bytes": (_sz, [_i, _i]),
     "kvattn_verify_drafts": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _ll, _i, _vp, _sz, _vp]),
+    "kvattn_tree_masks": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _i, _i, _vp]),
+    "kvattn_paged_decode_tree": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _i, _i, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _vp,
+                                      _sz, _i, _i, _vp]),
+    "kvattn_paged_keep": (_i, [_vp, _vp, _i, _i, _vp, _vp, _vp, _i, _i, _i, _i, _i, _vp]),
+    "kvattn_verify_tree": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _ll, _i, _vp, _sz,
+                                _vp]),
+    "kvattn_process_logits": (_i, [_vp, _vp, _vp, _vp, _i, _i, _i, _ll, _ll, _i, _i, _i, _vp]),
+    "kvattn_w4_bytes": (_sz, [_i, _i, _i]),
+    "kvattn_w4_pack": (_i, [_vp, _vp, _vp, _i, _i, _i, _i, _vp]),
+    "kvattn_w4_quantize": (_i, [_vp, _vp, _i, _i, _i, _i, _i, _vp]),
+    "kvattn_gemv_w4": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _vp]),
 }
 
 
@@ -510,6 +521,108 @@ def verify_drafts(tokens, counts, target_probs, draft_tokens, uniform, token_sta
                                       draft_tokens, uniform, token_start, B, num_tokens, V,
                                       V if row_stride is None else int(row_stride), kv_dtype_code(dtype),
                                       workspace, int(workspace_nbytes), _stream(stream)), "kvattn_verify_drafts")
+
+
+def tree_masks(masks, parents, token_start, B, num_tokens, *, positions=None, lens=None, mask_words=1, stream=None) -> None:
+    """Masks (and positions) of trees of drafted tokens from every token's parent (kvattn_tree_masks)."""
+    _check(_call.kvattn_tree_masks(masks, positions, parents, token_start, lens, B, num_tokens, int(mask_words),
+                                   _stream(stream)), "kvattn_tree_masks")
+
+
+def paged_decode_tree(out, qkv, cache: PagedCache, token_start, lens, masks, B, num_tokens, NH, hs, *, kv_dtype, max_new,
+                      mask_words=1, workspace=None, workspace_nbytes=0, S=0, stream=None) -> None:
+    """Attention of trees of drafted tokens over a paged cache that holds their rows (kvattn_paged_decode_tree); the
+    workspace is that of num_tokens sequences."""
+    _check(_call.kvattn_paged_decode_tree(out, qkv, cache.pages, cache.page_scales, cache.block_table, cache.max_pages,
+                                          cache.page_rows, cache.num_pages, token_start, lens, masks, int(mask_words), B,
+                                          num_tokens, int(max_new), NH, hs, workspace, int(workspace_nbytes), int(S),
+                                          kv_dtype_code(kv_dtype), _stream(stream)), "kvattn_paged_decode_tree")
+
+
+def paged_keep(cache: PagedCache, slot_map, path, token_start, B, num_tokens, NH, hs, *, kv_dtype, stream=None) -> None:
+    """K and V rows of the accepted paths to where the next step needs them (kvattn_paged_keep)."""
+    _check(_call.kvattn_paged_keep(cache.pages, cache.page_scales, cache.page_rows, cache.num_pages, slot_map, path,
+                                   token_start, B, num_tokens, NH, hs, kv_dtype_code(kv_dtype), _stream(stream)),
+           "kvattn_paged_keep")
+
+
+def verify_tree(tokens, path, counts, target_probs, tree_tokens, parents, uniform, draw, token_start, B, num_tokens, V, *,
+                lens=None, kept=None, row_stride=None, dtype="f32", workspace=None, workspace_nbytes=0,
+                stream=None) -> None:
+    """Accepts a path of a tree of drafted tokens against the target's probabilities and draws the next token
+    (kvattn_verify_tree); the workspace is verify_drafts'."""
+    _check(_call.kvattn_verify_tree(tokens, path, counts, kept, target_probs, tree_tokens, parents, uniform, draw,
+                                    token_start, lens, B, num_tokens, V, V if row_stride is None else int(row_stride),
+                                    kv_dtype_code(dtype), workspace, int(workspace_nbytes), _stream(stream)),
+           "kvattn_verify_tree")
+
+
+class _LogitRules(ctypes.Structure):
+    """kvattn_logit_rules."""
+    _fields_ = [(name, _vp) for name in (
+        "history", "history_len", "prompt_len", "tokens", "masks", "repetition", "frequency", "presence", "bias_start",
+        "bias_ids", "bias", "allowed", "allowed_of", "temperature")] + [
+        (name, _i) for name in ("max_history", "mask_words", "num_bias", "max_bias", "num_allowed", "allowed_stride")]
+
+
+class LogitRules:
+    """Rules on logits for process_logits: the fields of kvattn_logit_rules by name, device tensors and integers.  Made
+    once; the tensors are kept, and may be written between calls."""
+
+    def __init__(self, **rules):
+        self._struct = _LogitRules()
+        names = dict(_LogitRules._fields_)
+        for name, x in rules.items():
+            if name not in names:
+                raise TypeError(f"LogitRules: no rule {name!r}")
+            setattr(self._struct, name, _ptr(x) if names[name] is _vp else int(x))
+        self._tensors = rules
+        self.address = ctypes.addressof(self._struct)
+
+
+def process_logits(out, logits, rules: Optional[LogitRules], token_start, B, rows, V, *, row_stride=None, out_stride=None,
+                   dtype="f32", out_dtype=None, probs=True, stream=None) -> None:
+    """Penalties, biases and grammar masks on rows of logits, as probabilities (or, probs False, as logits)
+    (kvattn_process_logits).  out_dtype None: dtype."""
+    _check(_call.kvattn_process_logits(out, logits, None if rules is None else rules.address, token_start, B, rows, V,
+                                       V if row_stride is None else int(row_stride),
+                                       V if out_stride is None else int(out_stride), kv_dtype_code(dtype),
+                                       kv_dtype_code(dtype if out_dtype is None else out_dtype), int(bool(probs)),
+                                       _stream(stream)), "kvattn_process_logits")
+
+
+def w4_bytes(M, K, group) -> int:
+    """Bytes of an M x K matrix of 4-bit weights as gemv_w4 reads it."""
+    return int(lib().kvattn_w4_bytes(M, K, group))
+
+
+def _w4_buffer(M, K, group, like):
+    import torch
+    nbytes = w4_bytes(M, K, group)
+    if nbytes == 0:
+        raise KvAttnError(ERR_SHAPE, "kvattn_w4_bytes")
+    return torch.empty(nbytes, dtype=torch.uint8, device=like.device)
+
+
+def w4_pack(codes, scales, M, K, group, *, w_dtype, out=None, stream=None):
+    """4-bit codes [M][K/2] and bf16 scales [M][K/group] laid out for gemv_w4 (kvattn_w4_pack)."""
+    out = _w4_buffer(M, K, group, codes) if out is None else out
+    _check(_call.kvattn_w4_pack(out, codes, scales, M, K, int(group), kv_dtype_code(w_dtype), _stream(stream)), "kvattn_w4_pack")
+    return out
+
+
+def w4_quantize(W, M, K, group, *, w_dtype, src_dtype="bf16", out=None, stream=None):
+    """W [M][K] coded in 4 bits and laid out for gemv_w4 (kvattn_w4_quantize)."""
+    out = _w4_buffer(M, K, group, W) if out is None else out
+    _check(_call.kvattn_w4_quantize(out, W, M, K, int(group), kv_dtype_code(src_dtype), kv_dtype_code(w_dtype),
+                                    _stream(stream)), "kvattn_w4_quantize")
+    return out
+
+
+def gemv_w4(out, w4, x, B, M, K, *, group, w_dtype, bias=None, pre_gelu=None, gelu=False, out_dtype="bf16", stream=None) -> None:
+    """Fully connected layer on 4-bit weights with a scale for every group (kvattn_gemv_w4)."""
+    _check(_call.kvattn_gemv_w4(out, pre_gelu, w4, x, bias, B, M, K, int(group), kv_dtype_code(w_dtype),
+                                kv_dtype_code(out_dtype), int(bool(gelu)), _stream(stream)), "kvattn_gemv_w4")
 
 
 class Workspace:

@@ -411,6 +411,53 @@ int kvattn_paged_decode_tokens(void* out, const void* qkv, const void* pages, co
                                int NH, int hs, void* workspace, size_t workspace_bytes, int S, int kv_dtype,
                                void* stream);
 
+/* ---- Trees of drafted tokens ------------------------------------------------------------
+ * A sequence's new tokens may be the nodes of a tree: token 0 its root (the last token that was
+ * accepted), every other one a draft behind its parent, an earlier token of the sequence.  Their rows
+ * are in the cache already (kvattn_paged_store: token i's at position lens[b] - n + i), but a token
+ * attends the positions before the tree and its own branch alone.  A chain of drafts is the tree whose
+ * token i has the parent i - 1.  Up to 256 tokens a sequence.  No reference counterpart (the reference
+ * decodes one token at a time).
+ *   token_start [B+1] device: as in kvattn_paged_decode_tokens; a sequence may have no tokens
+ *   parents [num_tokens] device: index of the parent among the sequence's tokens; what is negative or
+ *           not below the token's own index counts as none (the token follows the cached prefix)
+ *   masks [num_tokens][mask_words] device, 64-bit words, mask_words 1 to 4: bit i % 64 of word i / 64:
+ *           the token attends token i of its sequence */
+
+/* The masks of trees (a token's ancestors and itself), made once a step and read by every layer.
+ *   positions [num_tokens] (may be NULL): every token's position for its embedding, lens[b] - n + its
+ *             depth (0 where that is negative); lens [B] as in kvattn_paged_decode_tokens, needed for
+ *             positions alone
+ * Tokens from 64 * mask_words on get an empty mask, and the position of a root.  Rows behind
+ * token_start[B] are left as they were.  B >= 1, num_tokens <= 2^30 (0: nothing is done). */
+int kvattn_tree_masks(unsigned long long* masks, int* positions, const int* parents, const int* token_start,
+                      const int* lens, int B, int num_tokens, int mask_words, void* stream);
+
+/* Attention of trees' tokens over a paged cache of any kv_dtype (F32: qkv and out float, else bf16).
+ * Token i of sequence b's n attends the first lens[b] - n positions and those new tokens j whose
+ * position lens[b] - n + j is in [0, lens[b]) and whose bit its mask has, of whatever shape the masks
+ * are; one that attends nothing gets zeros.  K and V of positions that a token does not attend never
+ * reach its output, also where they are infinite or NaN.  A table entry outside the pool: its positions
+ * are skipped.  The cache is read once for 64 tokens of a sequence (32 for F32, INT8, FP8, INT4 and FP4).
+ *   max_new  the most tokens of one sequence, at most 64 * mask_words (or num_tokens is); a sequence with
+ *            more has the first max_new or more of them computed
+ * Other arguments, limits and the workspace as in kvattn_paged_decode_tokens; B <= 65535. */
+int kvattn_paged_decode_tree(void* out, const void* qkv, const void* pages, const float* page_scales,
+                             const int* block_table, int max_pages, int page_rows, int num_pages,
+                             const int* token_start, const int* lens, const unsigned long long* masks, int mask_words,
+                             int B, int num_tokens, int max_new, int NH, int hs, void* workspace,
+                             size_t workspace_bytes, int S, int kv_dtype, void* stream);
+
+/* After kvattn_verify_tree: K and V rows of every sequence's accepted path to where the next step needs
+ * them, behind the prefix.  Row slot_map[token_start[b] + path[d]] goes to slot_map[token_start[b] + d],
+ * codes and scales as they are, for every d from 0 until path[d] (entry token_start[b] + d of path) is not above
+ * path[d - 1], not below d, or not one of the sequence's tokens.  Steps with a slot outside the pool are
+ * skipped; a sequence's slots, and those of different sequences, must differ.  Every kv_dtype.
+ * B * NH <= 2^24. */
+int kvattn_paged_keep(void* pages, float* page_scales, int page_rows, int num_pages, const long long* slot_map,
+                      const int* path, const int* token_start, int B, int num_tokens, int NH, int hs, int kv_dtype,
+                      void* stream);
+
 /* ---- Pages from request lengths --------------------------------------------------------
  * The bookkeeping of a paged cache, on the device: no length, table or page count goes through the
  * host, so a captured step allocates too.  No reference counterpart (the reference has one
@@ -490,6 +537,72 @@ int kvattn_verify_drafts(int* tokens, int* counts, const void* target_probs, con
                          int num_tokens, int V, long long row_stride, int dtype, void* workspace,
                          size_t workspace_bytes, void* stream);
 
+/* Verification of a tree of drafts.  Row t of target_probs is the distribution behind tree token t.  From a
+ * sequence's token 0 on, the children of the token reached are tried in the order of their indices: the
+ * first one whose running sum of target_probs[t][child's token] passes uniform[t] is accepted and reached
+ * next.  (A token that an earlier child is too, an id outside [0, V) and what is not a positive finite
+ * number weigh nothing.)  Where none is accepted, the next token is drawn from row t without the tokens
+ * of t's children, or where nothing is left without them from all of row t: the lowest token whose
+ * running sum passes draw[b] times the total.  Sums are 64 bits wide.  The tokens that come out are the
+ * target's, whatever the tree was made from (uniform and draw are independent of it).
+ *   tokens [num_tokens] (may be tree_tokens): accepted tokens, the drawn one, -1 behind it
+ *   path [num_tokens]: the root's index 0, then the accepted tokens' among the sequence's, -1 behind: the rows that
+ *            kvattn_paged_keep keeps
+ *   counts [B]: accepted plus drawn (a row without any mass draws nothing)
+ *   kept [B] (may be NULL): lens[b] - n + 1 + accepted, the next step's kept of kvattn_paged_reserve; of a
+ *            sequence without tokens lens[b].  lens [B], needed for kept alone, as in kvattn_tree_masks.
+ *            A request that kvattn_paged_reserve refused keeps what it kept, which the caller sets again
+ *   tree_tokens [num_tokens]: every tree token's id (a root's is not read)
+ *   uniform [num_tokens], draw [B]: numbers in [0, 1)
+ * Tokens of a sequence from the 256th on are not looked at.  Other arguments, limits and the workspace as in
+ * kvattn_verify_drafts, which may share the workspace. */
+int kvattn_verify_tree(int* tokens, int* path, int* counts, int* kept, const void* target_probs, const int* tree_tokens,
+                       const int* parents, const float* uniform, const float* draw, const int* token_start,
+                       const int* lens, int B, int num_tokens, int V, long long row_stride, int dtype, void* workspace,
+                       size_t workspace_bytes, void* stream);
+
+/* ---- Rules on logits -------------------------------------------------------------------
+ * What a sequence's logits go through before a token is chosen.  Device arrays; NULL: no such rule.
+ * "Held" are the tokens of the sequence's history and, for a row of a tree, of the row's branch (the
+ * tokens whose bits the row's mask has: its ancestors and itself). */
+typedef struct kvattn_logit_rules {
+    const int* history;          /* [B][max_history] ids; others than 0 .. V - 1 are passed over */
+    const int* history_len;      /* [B] of them in use */
+    const int* prompt_len;       /* [B] the first of them that are the prompt's: held, but not generated */
+    const int* tokens;           /* [rows] id of every row's own token, with masks */
+    const unsigned long long* masks;   /* [rows][mask_words] as in kvattn_tree_masks */
+    const float* repetition;     /* [B] x of a held token: x / repetition where x > 0, else x * repetition */
+    const float* frequency;      /* [B] subtracted for every time a token was generated */
+    const float* presence;       /* [B] subtracted once where it was */
+    const int* bias_start;       /* [B+1] sequence b's entries of bias_ids and bias */
+    const int* bias_ids;         /* [num_bias] */
+    const float* bias;           /* [num_bias] added; of an id listed twice the last entry holds */
+    const unsigned* allowed;     /* [num_allowed][allowed_stride] bit v % 32 of word v / 32: v is allowed; others: -inf */
+    const int* allowed_of;       /* [rows] a row's line of allowed; outside [0, num_allowed): all are.  NULL: line `row` */
+    const float* temperature;    /* [B] of the probabilities; not above 0: the likeliest token, the lowest of several */
+    int max_history;             /* up to 32768 */
+    int mask_words;              /* 1 to 4 */
+    int num_bias, max_bias;      /* entries in all, and most of one sequence (further ones are passed over; up to 32768) */
+    int num_allowed, allowed_stride;   /* words */
+} kvattn_logit_rules;
+
+/* The rules on rows of V logits, in the order above, in float: repetition, frequency and presence, bias, allowed.
+ *   probs 0: the logits (-inf where not allowed); 1: softmax(x / temperature), as kvattn_verify_drafts and
+ *            kvattn_verify_tree take it; a row that allows nothing becomes zeros, one with a NaN or +inf that is
+ *            allowed NaN where it is not zero
+ *   rules    host struct, read by the call (the arrays it names are read when the kernel runs); NULL: none
+ *   token_start [B+1] device: rows token_start[b] .. token_start[b+1]-1 are sequence b's; rows behind token_start[B]
+ *            are left as they were.  NULL: row b is sequence b's (rows == B)
+ *   dtype, out_dtype  KVATTN_KV_F32 or KVATTN_KV_BF16; out may be logits where the types and strides are the same.
+ *            What lies behind a row's V elements is neither read nor written
+ * V <= 2^18, rows <= 2^21, B <= 2^20.  KVATTN_ERR_LDS: the table of named tokens does not fit in LDS
+ * (V / 8 bytes for the map, V / 16, V / 8 with allowed, 4 bytes, with biases 8, for each of
+ * min(V, max_history + 64 mask_words + max_bias) entries, in 156 KB).
+ * No reference counterpart (the reference takes the argmax or samples on the host, without rules). */
+int kvattn_process_logits(void* out, const void* logits, const kvattn_logit_rules* rules, const int* token_start,
+                          int B, int rows, int V, long long row_stride, long long out_stride, int dtype, int out_dtype,
+                          int probs, void* stream);
+
 /* The decode step's fully connected layer, used after the attention for the output
  * projection: for b < B, m < M
  *   pre = w_scale[m] * sum_k W[m][k] * x[b][k] + bias[m]      (w_scale: 8-bit weights only)
@@ -548,6 +661,27 @@ int kvattn_gemv_qkv_append(void* qkv, const void* W, const float* w_scale, const
                            float* kv_scale, int maxT, const int* d_cur_len, int lens_per_seq,
                            int w_dtype, int kv_dtype, void* workspace, size_t workspace_bytes,
                            void* stream);
+
+/* ---- 4-bit weights with a scale for every group --------------------------------------------
+ * kvattn_gemv_ex on INT4 or FP4_E2M1 codes whose scales are bf16, one for every `group` (32, 64 or 128)
+ * neighbours of a row: weight [m][k] = code * scale[m][k / group], codes as in the 4-bit caches (INT4: half byte - 8,
+ * here -8 too; FP4: sign and one of 0 .5 1 1.5 2 3 4 6).  K is a multiple of group, K <= 2^20, M any.
+ * No reference counterpart (its weights end at 8 bits, with one scale a row).
+ * Weights are laid out once for the kernels: w4, 16-byte aligned, of kvattn_w4_bytes(M, K, group) bytes (0: such a
+ * matrix is refused); what is in it depends on M, K and group. */
+size_t kvattn_w4_bytes(int M, int K, int group);
+
+/* Lays out codes [M][K / 2] bytes (column 2i in the low half of byte i, 16-byte aligned) and scales [M][K / group] bf16. */
+int kvattn_w4_pack(void* w4, const void* codes, const void* scales, int M, int K, int group, int w_dtype, void* stream);
+
+/* Codes and lays out W [M][K], float or bf16 (src_dtype): scale = bf16(largest magnitude / 7, FP4: / 6), codes of w / scale
+ * to nearest, ties to even, within -7 .. 7 (FP4: -6 .. 6). */
+int kvattn_w4_quantize(void* w4, const void* W, int M, int K, int group, int src_dtype, int w_dtype, void* stream);
+
+/* out[b][m] = act(sum_k weight[m][k] x[b][k] + bias[m]) with FP32 sums; x, bias (may be NULL) bf16, out and pre_gelu
+ * (may be NULL) float or bf16 by out_dtype; gelu as in kvattn_gemv.  Any B, on the matrix cores. */
+int kvattn_gemv_w4(void* out, void* pre_gelu, const void* w4, const void* x, const void* bias, int B, int M, int K,
+                   int group, int w_dtype, int out_dtype, int gelu, void* stream);
 
 #ifdef __cplusplus
 }
