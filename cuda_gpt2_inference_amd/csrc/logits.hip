@@ -5,12 +5,17 @@
 //   x  -= frequency * count + (count > 0 ? presence : 0)                               (count: times generated)
 //   x  += bias;   x = -inf where the grammar forbids the token
 //
-// A row is one workgroup's: it is read once, stays in registers between the maximum, the sum and the quotient, and is
-// written once.  What a sequence holds is a list of ids, so the tokens that any rule names are few against the
-// vocabulary: they are set bits of a map in LDS (a bit a token), and a token's place among the set bits, from a
-// prefix sum over the map's words, is its entry in a table of counts and biases.  A row's four neighbouring
-// tokens look at four bits, and only where one is set at the table.  The row of a token of a tree holds its branch
-// too (the bits of its mask), so every row builds its own table.
+// A row is read once, stays in registers between the maximum, the sum and the quotient, and is written once.  What a
+// sequence holds is a list of ids, so the tokens that any rule names are few against the vocabulary: they are set bits of
+// a map in LDS (a bit a token), and a token's place among the set bits, from a prefix sum over the map's words, is its
+// entry in a table: a thread for every entry works its logit out.  A row's four neighbouring tokens look at four
+// bits, and only where one is set at the table.  The row of a token of a tree holds its branch too (the bits of its mask),
+// so every row builds its own table.
+//
+// A row on one CU takes the CU's time for its arithmetic (a dozen instructions a token and the table: 18 us for one row of
+// 50257), so few rows are cut into slices, a workgroup each.  Of probabilities the slices of a row exchange their maxima
+// and sums as tagged words in the workspace, while all of them are on the GPU; a slice that waits in vain works the
+// missing ones out itself.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -20,14 +25,16 @@
 
 namespace {
 
-constexpr int kThreads = 1024;
-constexpr int kWaves = kThreads / kWave;
 constexpr int kRun = 4;                        // neighbouring tokens of a thread
-constexpr int kStep = kThreads * kRun;         // tokens from one run of a thread to its next
+constexpr int kSliceThreads = 512, kRowThreads = 1024;     // of a slice's workgroup, of a whole row's
+constexpr int kMostSlices = 64;                // of a row whose slices exchange words: a lane each
+constexpr int kTogether = 512;                 // workgroups of kSliceThreads that run at once: two a CU
 constexpr int kMaxVocab = 1 << 18;
 constexpr int kMaxRows = 1 << 21;              // workgroups of a grid: 2^32 threads are too many
 constexpr int kMaxSequences = 1 << 20;
+constexpr int kIds = 8, kNamed = 2;             // ids and named tokens of a thread that are asked for ahead
 constexpr int kLdsMost = 156 * 1024;           // a CU's, less what is static here
+constexpr int kLdsTogether = 76 * 1024;        // two workgroups a CU
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct LogitArgs {
@@ -37,6 +44,10 @@ struct LogitArgs {
     kvattn_logit_rules r;
     size_t in_row, out_row;
     int B, rows, V, words, entries;            // words of the map; entries of the table
+    int slices, slice;                         // of a row, tokens of one
+    unsigned long long* exchange;              // [rows][slices][2] tagged words
+    int polls;
+    bool vec;                                  // rows start on boundaries of a run
 };
 
 template <bool kF32>
@@ -45,9 +56,10 @@ __device__ __forceinline__ float logit(const void* p, size_t i) {
     else return bf16_to_f32(reinterpret_cast<const uint16_t*>(p)[i]);
 }
 
-template <bool kF32, bool kVec>
-__device__ __forceinline__ void load_run(const void* p, size_t row0, int v, int V, float (&x)[kRun]) {
-    if (kVec && v + kRun <= V) {
+// vec: rows start on boundaries of a run.
+template <bool kF32>
+__device__ __forceinline__ void load_run(const void* p, size_t row0, int v, int V, bool vec, float (&x)[kRun]) {
+    if (vec && v + kRun <= V) {
         if constexpr (kF32) {
             const float4 w = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(p) + row0 + v);
             x[0] = w.x; x[1] = w.y; x[2] = w.z; x[3] = w.w;
@@ -61,9 +73,9 @@ __device__ __forceinline__ void load_run(const void* p, size_t row0, int v, int 
     for (int i = 0; i < kRun; ++i) x[i] = v + i < V ? logit<kF32>(p, row0 + min(v + i, V - 1)) : -INFINITY;
 }
 
-template <bool kF32, bool kVec>
-__device__ __forceinline__ void store_run(void* p, size_t row0, int v, int V, const float (&x)[kRun]) {
-    if (kVec && v + kRun <= V) {
+template <bool kF32>
+__device__ __forceinline__ void store_run(void* p, size_t row0, int v, int V, bool vec, const float (&x)[kRun]) {
+    if (vec && v + kRun <= V) {
         if constexpr (kF32) {
             *reinterpret_cast<float4*>(reinterpret_cast<float*>(p) + row0 + v) = make_float4(x[0], x[1], x[2], x[3]);
         } else {
@@ -92,27 +104,32 @@ __device__ __forceinline__ int sequence_of(const int* start, int B, int row, int
     return b;
 }
 
-// A number that orders as the float does.
-__device__ __forceinline__ uint32_t ordered(float x) {
-    const uint32_t u = __float_as_uint(x);
-    return u & 0x80000000u ? ~u : u | 0x80000000u;
-}
-
 // kRuns: runs of a thread that are kept in registers; 0: of a longer row none is, and each pass reads it again.
-template <bool kInF32, bool kOutF32, bool kVec, bool kProbs, int kRuns>
-__global__ __launch_bounds__(kThreads) void logits_kernel(LogitArgs a) {
-    extern __shared__ uint32_t lds[];          // map, its allowed tokens, prefixes (16 bits), counts, biases
+// kShare: the row's probabilities are those of several workgroups.
+template <bool kInF32, bool kOutF32, bool kProbs, int kThreads, int kRuns, bool kShare>
+__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(4))) void logits_kernel(LogitArgs a) {
+    constexpr int kWaves = kThreads / kWave, kStep = kThreads * kRun;      // tokens from one run of a thread to its next
+    static_assert(!kShare || (kProbs && kRuns > 0), "slices in registers");
+    extern __shared__ uint32_t lds[];          // map, allowed tokens, named tokens, counts, biases, prefixes (16 bits)
     __shared__ uint32_t wave_words[kWaves];
-    __shared__ float wave_floats[kWaves];
+    __shared__ float wave_floats[2][kWaves];
     __shared__ unsigned long long wave_keys[kWaves];
-    const int row = blockIdx.x, tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave;
+    __shared__ float slice_top[kMostSlices], slice_sum[kMostSlices];       // (sum: of the likeliest token alone, its number)
+    __shared__ unsigned long long missing_at;
+    const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave;
+    const int row = a.slices > 1 ? blockIdx.x / a.slices : blockIdx.x;
+    const int own = a.slices > 1 ? blockIdx.x - row * a.slices : 0;
     constexpr int kHeld = kRuns ? kRuns : 1;
     float x[kHeld][kRun];
     const size_t in0 = (size_t)row * a.in_row, out0 = (size_t)row * a.out_row;
-    if constexpr (kRuns > 0) {
+    int v0 = own * a.slice, v1 = min(a.V, v0 + a.slice);      // this workgroup's tokens
+    auto load = [&] {
+        if constexpr (kRuns > 0) {
 #pragma unroll
-        for (int j = 0; j < kRuns; ++j) load_run<kInF32, kVec>(a.x, in0, tid * kRun + j * kStep, a.V, x[j]);
-    }
+            for (int j = 0; j < kRuns; ++j) load_run<kInF32>(a.x, in0, v0 + tid * kRun + j * kStep, v1, a.vec, x[j]);
+        }
+    };
+    load();
     int b = row, t0 = row;
     if (a.start) {
         if (row >= a.start[a.B]) return;       // behind the last token
@@ -120,45 +137,67 @@ __global__ __launch_bounds__(kThreads) void logits_kernel(LogitArgs a) {
         t0 = min(max(a.start[b], 0), row);
     }
 
+    // What the sequence holds is asked for before its length is known (places behind it are not looked at).
+    const bool table = a.entries > 0;
+    const int* const history = a.r.history + (size_t)b * a.r.max_history;
+    int ids[kIds];
+    if (a.r.history) {
+#pragma unroll
+        for (int k = 0; k < kIds; ++k) ids[k] = k * kThreads < a.r.max_history ? history[min(tid + k * kThreads, a.r.max_history - 1)] : -1;
+    }
+    const float temperature = a.r.temperature ? a.r.temperature[b] : 1.0f;
     uint32_t* const map = lds;
     uint32_t* const allowed = map + a.words;
-    uint16_t* const before = reinterpret_cast<uint16_t*>(allowed + (a.r.allowed ? a.words : 0));
-    uint32_t* const count = reinterpret_cast<uint32_t*>(before) + (a.words + 1) / 2;
+    uint32_t* const names = allowed + (a.r.allowed ? a.words : 0);
+    uint32_t* const count = names + a.entries;
     uint32_t* const bias_at = count + a.entries;
-    const bool table = a.entries > 0;
-    bool grammar = false;
-    if (a.r.allowed) {
-        const int of = a.r.allowed_of ? a.r.allowed_of[row] : row;
-        grammar = of >= 0 && of < a.r.num_allowed;
-        if (grammar)
-            for (int w = tid; w < a.words; w += kThreads) allowed[w] = a.r.allowed[(size_t)of * a.r.allowed_stride + w];
-    }
+    uint16_t* const before = reinterpret_cast<uint16_t*>(bias_at + (a.r.bias_start ? a.entries : 0));
+    int line = -1;
+    if (a.r.allowed) line = a.r.allowed_of ? a.r.allowed_of[row] : row;
+    const bool grammar = a.r.allowed && line >= 0 && line < a.r.num_allowed;
+
+    int held = 0, prompt = 0, branch = -1, bias0 = 0, biases = 0;
+    float repetition = 1.0f, frequency = 0.0f, presence = 0.0f;
     if (table) {
-        const int held = a.r.history ? min(max(a.r.history_len[b], 0), a.r.max_history) : 0;
-        const int prompt = a.r.prompt_len ? a.r.prompt_len[b] : 0;
-        const int* const history = a.r.history + (size_t)b * a.r.max_history;
+        held = a.r.history ? min(max(a.r.history_len[b], 0), a.r.max_history) : 0;
+        prompt = a.r.prompt_len ? a.r.prompt_len[b] : 0;
+        if (a.r.repetition) repetition = a.r.repetition[b];
+        if (a.r.frequency) frequency = a.r.frequency[b];
+        if (a.r.presence) presence = a.r.presence[b];
         // This thread's token of the row's branch, and the sequence's biases.
-        int branch = -1;
-        if (a.r.tokens && tid < 64 * a.r.mask_words && t0 + tid < a.rows) {
-            if ((a.r.masks[(size_t)row * a.r.mask_words + (tid >> 6)] >> (tid & 63)) & 1) branch = a.r.tokens[t0 + tid];
+        if (a.r.tokens && tid < 64 * a.r.mask_words) {
+            const int its = a.r.tokens[min(t0 + tid, a.rows - 1)];
+            if (t0 + tid < a.rows && (a.r.masks[(size_t)row * a.r.mask_words + (tid >> 6)] >> (tid & 63)) & 1) branch = its;
         }
-        int bias0 = 0, biases = 0;
         if (a.r.bias_start) {
             bias0 = min(max(a.r.bias_start[b], 0), a.r.num_bias);
             biases = min(min(max(a.r.bias_start[b + 1], bias0), a.r.num_bias) - bias0, a.r.max_bias);
         }
-        for (int w = tid; w < a.words; w += kThreads) map[w] = 0;
+    }
+    // Allowed and named tokens of v0 .. v1 - 1.
+    auto build = [&] {
+        const int first = v0 >> 5, words = (v1 - v0 + 31) >> 5;
+        if (grammar)
+            for (int w = tid; w < words; w += kThreads) allowed[w] = a.r.allowed[(size_t)line * a.r.allowed_stride + first + w];
+        if (!table) return;
+        for (int w = tid; w < words; w += kThreads) map[w] = 0;
         __syncthreads();
-        auto known = [&](int id) { return id >= 0 && id < a.V; };
-        auto mark = [&](int id) {
-            if (known(id)) atomicOr(map + (id >> 5), 1u << (id & 31));
+        auto known = [&](int id) { return id >= v0 && id < v1; };
+        auto each_held = [&](auto&& f) {
+#pragma unroll
+            for (int k = 0; k < kIds; ++k)
+                if (tid + k * kThreads < held) f(ids[k], tid + k * kThreads);
+            for (int i = tid + kIds * kThreads; i < held; i += kThreads) f(history[i], i);
         };
-        for (int i = tid; i < held; i += kThreads) mark(history[i]);
+        auto mark = [&](int id) {              // (text repeats itself: mostly it is marked)
+            if (known(id) && !((map[(id - v0) >> 5] >> (id & 31)) & 1)) atomicOr(map + ((id - v0) >> 5), 1u << (id & 31));
+        };
+        each_held([&](int id, int) { mark(id); });
         mark(branch);
         for (int i = tid; i < biases; i += kThreads) mark(a.r.bias_ids[bias0 + i]);
         __syncthreads();
         // Set bits before every word: a thread's words, then the threads'.
-        const int per = (a.words + kThreads - 1) / kThreads, w0 = min(tid * per, a.words), w1 = min(w0 + per, a.words);
+        const int per = (words + kThreads - 1) / kThreads, w0 = min(tid * per, words), w1 = min(w0 + per, words);
         uint32_t mine = 0;
         for (int w = w0; w < w1; ++w) mine += __popc(map[w]);
         uint32_t upto = mine;
@@ -177,54 +216,66 @@ __global__ __launch_bounds__(kThreads) void logits_kernel(LogitArgs a) {
         }
         for (int w = w0; w < w1; ++w) {
             before[w] = (uint16_t)at;
-            at += __popc(map[w]);
+            for (uint32_t bits = map[w]; bits; bits &= bits - 1) names[at++] = v0 + 32 * w + __builtin_ctz(bits);
         }
         for (uint32_t e = tid; e < all; e += kThreads) {
             count[e] = 0;
             if (a.r.bias_start) bias_at[e] = 0;
         }
         __syncthreads();
-        auto entry = [&](int id) { return before[id >> 5] + __popc(map[id >> 5] & ((1u << (id & 31)) - 1)); };
+        // The named tokens' logits are asked for while they are counted.
+        float named[kNamed];
+#pragma unroll
+        for (int k = 0; k < kNamed; ++k) named[k] = tid + k * kThreads < all ? logit<kInF32>(a.x, in0 + names[tid + k * kThreads]) : 0.0f;
+        auto entry = [&](int id) { return before[(id - v0) >> 5] + __popc(map[(id - v0) >> 5] & ((1u << (id & 31)) - 1)); };
         // Times held in the lower half, times of those in the prompt in the upper: at most 2^15 each.
-        for (int i = tid; i < held; i += kThreads) {
-            const int id = history[i];
+        each_held([&](int id, int i) {
             if (known(id)) atomicAdd(count + entry(id), i < prompt ? 0x10001u : 1u);
-        }
+        });
         if (known(branch)) atomicAdd(count + entry(branch), 1u);
         for (int i = tid; i < biases; i += kThreads) {
             const int id = a.r.bias_ids[bias0 + i];
             if (known(id)) atomicMax(bias_at + entry(id), (uint32_t)(bias0 + i + 1));   // of an id listed twice the last
         }
-    }
-    const float repetition = a.r.repetition ? a.r.repetition[b] : 1.0f;
-    const float frequency = a.r.frequency ? a.r.frequency[b] : 0.0f, presence = a.r.presence ? a.r.presence[b] : 0.0f;
-    if (table || a.r.allowed) __syncthreads();
-
+        __syncthreads();
+        // A thread for every named token: its logit takes its count's place.
+        auto adjust = [&](uint32_t e, float z) {
+#pragma clang fp contract(off)
+            const uint32_t c = count[e];
+            const float made = (float)((c & 0xffffu) - (c >> 16));
+            if (c) z = z > 0.0f ? z / repetition : z * repetition;
+            z = z - (frequency * made + (made > 0.0f ? presence : 0.0f));
+            if (a.r.bias_start) {
+                const uint32_t from = bias_at[e];
+                if (from) z = z + a.r.bias[from - 1];
+            }
+            count[e] = __float_as_uint(z);
+        };
+#pragma unroll
+        for (int k = 0; k < kNamed; ++k)
+            if (tid + k * kThreads < all) adjust(tid + k * kThreads, named[k]);
+        for (uint32_t e = tid + kNamed * kThreads; e < all; e += kThreads) adjust(e, logit<kInF32>(a.x, in0 + names[e]));
+    };
     auto rules = [&](int v, float (&y)[kRun]) {
-        if (v >= a.V) return;
+        if (v >= v1) return;
+        const int w = (v - v0) >> 5;
         if (table) {
-            const uint32_t bits = (map[v >> 5] >> (v & 31)) & 15u;
+            const uint32_t word = map[w], bits = (word >> (v & 31)) & 15u;
             if (bits) {
+                // (Entries of the run are neighbours; those before its first bit and behind its last are read for nothing.)
+                uint32_t e = before[w] + __popc(word & ((1u << (v & 31)) - 1));
+                uint32_t z[kRun];
 #pragma unroll
                 for (int i = 0; i < kRun; ++i) {
-#pragma clang fp contract(off)
-                    if (!((bits >> i) & 1)) continue;
-                    const uint32_t e = before[v >> 5] + __popc(map[v >> 5] & ((1u << ((v + i) & 31)) - 1));
-                    const uint32_t c = count[e];
-                    const float made = (float)((c & 0xffffu) - (c >> 16));
-                    float z = y[i];
-                    if (c) z = z > 0.0f ? z / repetition : z * repetition;
-                    z = z - (frequency * made + (made > 0.0f ? presence : 0.0f));
-                    if (a.r.bias_start) {
-                        const uint32_t at = bias_at[e];
-                        if (at) z = z + a.r.bias[at - 1];
-                    }
-                    y[i] = z;
+                    z[i] = count[e];
+                    if (i + 1 < kRun) e = min(e + ((bits >> i) & 1), (uint32_t)a.entries - 1);
                 }
+#pragma unroll
+                for (int i = 0; i < kRun; ++i) y[i] = (bits >> i) & 1 ? __uint_as_float(z[i]) : y[i];
             }
         }
         if (grammar) {
-            const uint32_t ok = allowed[v >> 5] >> (v & 31);
+            const uint32_t ok = allowed[w] >> (v & 31);
 #pragma unroll
             for (int i = 0; i < kRun; ++i) y[i] = (ok >> i) & 1 ? y[i] : -INFINITY;
         }
@@ -233,98 +284,206 @@ __global__ __launch_bounds__(kThreads) void logits_kernel(LogitArgs a) {
     auto each = [&](auto&& f) {
         if constexpr (kRuns > 0) {
 #pragma unroll
-            for (int j = 0; j < kRuns; ++j) f(tid * kRun + j * kStep, x[j]);
+            for (int j = 0; j < kRuns; ++j) f(v0 + tid * kRun + j * kStep, x[j]);
         } else {
-            for (int v = tid * kRun; v < a.V; v += kStep) {
-                load_run<kInF32, kVec>(a.x, in0, v, a.V, x[0]);
+            for (int v = v0 + tid * kRun; v < v1; v += kStep) {
+                load_run<kInF32>(a.x, in0, v, v1, a.vec, x[0]);
                 rules(v, x[0]);
                 f(v, x[0]);
             }
         }
     };
-    if constexpr (kRuns > 0) {
+    auto apply = [&] {
+        build();
+        if (table || a.r.allowed) __syncthreads();
+        if constexpr (kRuns > 0) {
 #pragma unroll
-        for (int j = 0; j < kRuns; ++j) rules(tid * kRun + j * kStep, x[j]);
-    }
-    if constexpr (!kProbs) {
-        each([&](int v, float (&y)[kRun]) { store_run<kOutF32, kVec>(a.out, out0, v, a.V, y); });
-        return;
-    }
-    float top = -INFINITY;
-    each([&](int, float (&y)[kRun]) {
-#pragma unroll
-        for (int i = 0; i < kRun; ++i) top = fmaxf(top, y[i]);
-    });
-    top = wave_max(top);
-    if (lane == 0) wave_floats[wave] = top;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < kWaves; ++w) top = fmaxf(top, wave_floats[w]);
-    const float temperature = a.r.temperature ? a.r.temperature[b] : 1.0f;
-    if (!(temperature > 0.0f) || top == -INFINITY) {
-        // The likeliest token alone, the lowest of several; nothing where no token is left.
-        unsigned long long best = 0;
-        each([&](int v, float (&y)[kRun]) {
-#pragma unroll
-            for (int i = 0; i < kRun; ++i) {
-                const unsigned long long key = (unsigned long long)ordered(y[i]) << 32 | (0xffffffffu - (uint32_t)(v + i));
-                if (y[i] == top && v + i < a.V && key > best) best = key;
-            }
-        });
-#pragma unroll
-        for (int d = 1; d < kWave; d *= 2) {
-            const unsigned long long o = __shfl_xor(best, d);
-            best = o > best ? o : best;
+            for (int j = 0; j < kRuns; ++j) rules(v0 + tid * kRun + j * kStep, x[j]);
         }
-        if (lane == 0) wave_keys[wave] = best;
-        __syncthreads();
-#pragma unroll
-        for (int w = 0; w < kWaves; ++w) best = wave_keys[w] > best ? wave_keys[w] : best;
-        const int token = top == -INFINITY ? -1 : (int)(0xffffffffu - (uint32_t)best);
-        each([&](int v, float (&y)[kRun]) {
-#pragma unroll
-            for (int i = 0; i < kRun; ++i) y[i] = v + i == token ? 1.0f : 0.0f;
-            store_run<kOutF32, kVec>(a.out, out0, v, a.V, y);
-        });
+    };
+    apply();
+    if constexpr (!kProbs) {
+        each([&](int v, float (&y)[kRun]) { store_run<kOutF32>(a.out, out0, v, v1, a.vec, y); });
         return;
     }
+    const bool likeliest = !(temperature > 0.0f);
     const float scale = kLog2e / temperature;
+    float top = -INFINITY, sum = 0.0f;         // of this workgroup's tokens
+    int token = -1;                            // its likeliest, the lowest of several
     auto weigh = [&](float (&y)[kRun]) {
 #pragma unroll
         for (int i = 0; i < kRun; ++i) y[i] = exp2_fast((y[i] - top) * scale);
     };
-    float sum = 0.0f;
-    each([&](int, float (&y)[kRun]) {
-        weigh(y);
-        sum += (y[0] + y[1]) + (y[2] + y[3]);
-    });
-    sum = wave_sum(sum);
-    __syncthreads();                           // (the maxima have been read)
-    if (lane == 0) wave_floats[wave] = sum;
-    __syncthreads();
-    sum = 0.0f;
+    // The tokens' maximum, and the sum of their weights against it (in their places), or which one is the largest.
+    auto reduce = [&] {
+        top = -INFINITY;
+        each([&](int, float (&y)[kRun]) {
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) sum += wave_floats[w];
-    const float one = 1.0f / sum;
+            for (int i = 0; i < kRun; ++i) top = fmaxf(top, y[i]);
+        });
+        top = wave_max(top);
+        if (lane == 0) wave_floats[0][wave] = top;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) top = fmaxf(top, wave_floats[0][w]);
+        if (likeliest || top == -INFINITY) {
+            unsigned long long best = 0;
+            each([&](int v, float (&y)[kRun]) {
+#pragma unroll
+                for (int i = 0; i < kRun; ++i) {
+                    const unsigned long long key = 0xffffffffu - (uint32_t)(v + i);
+                    if (y[i] == top && v + i < v1 && key > best) best = key;
+                }
+            });
+#pragma unroll
+            for (int d = 1; d < kWave; d *= 2) {
+                const unsigned long long o = __shfl_xor(best, d);
+                best = o > best ? o : best;
+            }
+            if (lane == 0) wave_keys[wave] = best;
+            __syncthreads();
+#pragma unroll
+            for (int w = 0; w < kWaves; ++w) best = wave_keys[w] > best ? wave_keys[w] : best;
+            token = top == -INFINITY ? -1 : (int)(0xffffffffu - (uint32_t)best);
+            sum = 0.0f;
+        } else {
+            sum = 0.0f;
+            each([&](int, float (&y)[kRun]) {
+                weigh(y);
+                sum += (y[0] + y[1]) + (y[2] + y[3]);
+            });
+            sum = wave_sum(sum);
+            if (lane == 0) wave_floats[1][wave] = sum;
+            __syncthreads();
+            sum = 0.0f;
+#pragma unroll
+            for (int w = 0; w < kWaves; ++w) sum += wave_floats[1][w];
+        }
+    };
+    reduce();
+    float one = 1.0f / sum;                    // what a weight is multiplied with
+    bool none = top == -INFINITY;
+    if constexpr (kShare) {
+        // A slice's words: its maximum; its sum, or its likeliest token.
+        unsigned long long* const words = a.exchange + (size_t)row * a.slices * 2;
+        const uint32_t tag = call_tag();
+        if (tid == 0) {
+            publish_word(words + 2 * own, tagged_word(top, tag), false);
+            publish_word(words + 2 * own + 1, tagged_word(likeliest ? __int_as_float(token) : sum, tag), false);
+        }
+        if (wave == 0) {
+            unsigned long long w0 = 0, w1 = 0;
+            bool ok = false;
+            for (int r = 0; r < a.polls; ++r) {
+                if (!ok) {
+                    w0 = get_word(words + 2 * min(lane, a.slices - 1));
+                    w1 = get_word(words + 2 * min(lane, a.slices - 1) + 1);
+                    ok = word_is(w0, tag) && word_is(w1, tag);
+                }
+                if (__all(ok)) break;
+            }
+            if (lane == own) {                 // (also where nothing was waited for)
+                ok = true;
+                w0 = tagged_word(top, tag);
+                w1 = tagged_word(likeliest ? __int_as_float(token) : sum, tag);
+            }
+            slice_top[lane] = word_value(w0);
+            slice_sum[lane] = word_value(w1);
+            const unsigned long long out = __ballot(!ok && lane < a.slices);
+            if (lane == 0) missing_at = out;
+        }
+        __syncthreads();
+        // Slices that have not come are worked out here, then this one again.
+        unsigned long long missing = missing_at;
+        if (missing) {
+            missing |= 1ull << own;
+            const int order_own = own;
+            while (missing) {
+                const unsigned long long others = missing & ~(1ull << order_own);
+                const int s = others ? __ffsll((long long)others) - 1 : order_own;
+                missing &= ~(1ull << s);
+                v0 = s * a.slice;
+                v1 = min(a.V, v0 + a.slice);
+                __syncthreads();
+                load();
+                apply();
+                reduce();
+                if (tid == 0) {
+                    slice_top[s] = top;
+                    slice_sum[s] = likeliest ? __int_as_float(token) : sum;
+                }
+                __syncthreads();
+            }
+        }
+        // A lane for every slice.
+        const float its_top = lane < a.slices ? slice_top[lane] : -INFINITY, its_sum = slice_sum[lane];
+        const float all = wave_max(its_top);
+        none = all == -INFINITY;
+        if (likeliest) {
+            const unsigned long long at = __ballot(its_top == all);
+            token = __builtin_amdgcn_readlane(__float_as_int(its_sum), __ffsll((long long)(at | 1ull << 63)) - 1);
+        } else {
+            // (A slice that allows nothing has a sum of zero, and its maximum may not be taken a difference of.)
+            const float total = wave_sum(its_top == -INFINITY ? 0.0f : exp2_fast((its_top - all) * scale) * its_sum);
+            one = (top == -INFINITY ? 0.0f : exp2_fast((top - all) * scale)) / total;
+        }
+    }
+    if (likeliest || none) {
+        // The likeliest token alone; nothing where no token is left.
+        each([&](int v, float (&y)[kRun]) {
+#pragma unroll
+            for (int i = 0; i < kRun; ++i) y[i] = !none && v + i == token ? 1.0f : 0.0f;
+            store_run<kOutF32>(a.out, out0, v, v1, a.vec, y);
+        });
+        return;
+    }
+    const bool empty = top == -INFINITY;       // (of a slice: its logits were left as they are)
     each([&](int v, float (&y)[kRun]) {
         if constexpr (kRuns == 0) weigh(y);
         // (A forbidden token has none, also where the others' is NaN.)
 #pragma unroll
-        for (int i = 0; i < kRun; ++i) y[i] = y[i] == 0.0f ? 0.0f : y[i] * one;
-        store_run<kOutF32, kVec>(a.out, out0, v, a.V, y);
+        for (int i = 0; i < kRun; ++i) y[i] = empty || y[i] == 0.0f ? 0.0f : y[i] * one;
+        store_run<kOutF32>(a.out, out0, v, v1, a.vec, y);
     });
 }
 
-template <bool kInF32, bool kOutF32, bool kVec, bool kProbs>
-const void* kernel_for(int V) {
-    if (V <= 4 * kStep) return (const void*)&logits_kernel<kInF32, kOutF32, kVec, kProbs, 4>;
-    if (V <= 13 * kStep) return (const void*)&logits_kernel<kInF32, kOutF32, kVec, kProbs, 13>;
-    return (const void*)&logits_kernel<kInF32, kOutF32, kVec, kProbs, 0>;
+// How a call runs: threads and runs of a workgroup, its slices of a row.
+struct LogitPlan {
+    const void* fn;
+    int threads, tokens, slices;               // tokens of a slice
+};
+template <bool kInF32, bool kOutF32, bool kProbs, int kRuns>
+LogitPlan slices_plan(int V) {
+    const int tokens = kSliceThreads * kRun * kRuns, slices = (V + tokens - 1) / tokens;
+    const void* fn = (const void*)&logits_kernel<kInF32, kOutF32, kProbs, kSliceThreads, kRuns, false>;
+    if constexpr (kProbs) {
+        if (slices > 1) fn = (const void*)&logits_kernel<kInF32, kOutF32, kProbs, kSliceThreads, kRuns, true>;
+    }
+    return {fn, kSliceThreads, tokens, slices};
 }
-template <bool kInF32, bool kOutF32>
-const void* kernel_for(int V, bool vec, bool probs) {
-    if (vec) return probs ? kernel_for<kInF32, kOutF32, true, true>(V) : kernel_for<kInF32, kOutF32, true, false>(V);
-    return probs ? kernel_for<kInF32, kOutF32, false, true>(V) : kernel_for<kInF32, kOutF32, false, false>(V);
+template <bool kInF32, bool kOutF32, bool kProbs>
+LogitPlan plan_for(int rows, int V, bool share) {
+    constexpr int kToken = kSliceThreads * kRun;
+    auto fits = [&](int runs) {
+        const long long slices = (V + kToken * runs - 1) / (kToken * runs);
+        if (!kProbs) return rows * slices <= kTogether + kTogether / 4;
+        return slices == 1 || (share && slices <= kMostSlices && rows * slices <= kTogether);
+    };
+    if (fits(1)) return slices_plan<kInF32, kOutF32, kProbs, 1>(V);
+    if (fits(2)) return slices_plan<kInF32, kOutF32, kProbs, 2>(V);
+    if (fits(4)) return slices_plan<kInF32, kOutF32, kProbs, 4>(V);
+    if (!kProbs || fits(8)) return slices_plan<kInF32, kOutF32, kProbs, 8>(V);
+    if constexpr (kProbs) {
+        if (fits(13)) return slices_plan<kInF32, kOutF32, kProbs, 13>(V);
+        constexpr int kRowToken = kRowThreads * kRun;
+        if (V <= 13 * kRowToken) return {(const void*)&logits_kernel<kInF32, kOutF32, true, kRowThreads, 13, false>, kRowThreads, V, 1};
+    }
+    return {(const void*)&logits_kernel<kInF32, kOutF32, true, kRowThreads, 0, false>, kRowThreads, V, 1};
+}
+template <bool kInF32>
+LogitPlan plan_for(int rows, int V, bool out_f32, bool probs, bool share) {
+    if (out_f32) return probs ? plan_for<kInF32, true, true>(rows, V, share) : plan_for<kInF32, true, false>(rows, V, share);
+    return probs ? plan_for<kInF32, false, true>(rows, V, share) : plan_for<kInF32, false, false>(rows, V, share);
 }
 
 int hip_status(hipError_t e) {
@@ -334,6 +493,8 @@ int hip_status(hipError_t e) {
 }
 
 }  // namespace
+
+extern "C" size_t kvattn_logits_workspace_bytes(void) { return (size_t)kTogether * 2 * sizeof(unsigned long long); }
 
 extern "C" int kvattn_process_logits(void* out, const void* logits, const kvattn_logit_rules* rules,
                                      const int* token_start, int B, int rows, int V, long long row_stride,
@@ -360,7 +521,8 @@ extern "C" int kvattn_process_logits(void* out, const void* logits, const kvattn
                            r.temperature, r.bias_start, r.bias_ids, r.bias, r.allowed, r.allowed_of};
     for (const void* p : words)
         if ((uintptr_t)p & 3u) return KVATTN_ERR_MISALIGNED;
-    if (((uintptr_t)r.masks & 7u) || ((uintptr_t)logits % in) || ((uintptr_t)out % res)) return KVATTN_ERR_MISALIGNED;
+    if (r.workspace && r.workspace_bytes < kvattn_logits_workspace_bytes()) return KVATTN_ERR_WORKSPACE;
+    if (((uintptr_t)r.workspace & 7u) || ((uintptr_t)r.masks & 7u) || ((uintptr_t)logits % in) || ((uintptr_t)out % res)) return KVATTN_ERR_MISALIGNED;
     if (r.bias_start && (r.num_bias == 0 || r.max_bias == 0)) r.bias_start = nullptr;
     a.out = out;
     a.x = logits;
@@ -370,19 +532,36 @@ extern "C" int kvattn_process_logits(void* out, const void* logits, const kvattn
     a.B = B;
     a.rows = rows;
     a.V = V;
-    a.words = (V + 31) / 32;
-    // Every entry is another token: a row has no more of them than of these.
-    a.entries = std::min(V, (r.history ? r.max_history : 0) + (branches ? 64 * r.mask_words : 0) + (r.bias_start ? r.max_bias : 0));
-    const size_t lds = (size_t)a.words * (r.allowed ? 8 : 4) + (size_t)(a.words + 1) / 2 * 4 + (size_t)a.entries * (r.bias_start ? 8 : 4);
+    // Every entry is another token: a workgroup has no more of them than of these.
+    const int named = (r.history ? r.max_history : 0) + (branches ? 64 * r.mask_words : 0) + (r.bias_start ? r.max_bias : 0);
+    const auto lds_of = [&](int tokens) {
+        a.words = (std::min(V, tokens) + 31) / 32;
+        a.entries = std::min(std::min(V, tokens), named);
+        return (size_t)a.words * (r.allowed ? 8 : 4) + (size_t)(a.words + 1) / 2 * 4 + (size_t)a.entries * (r.bias_start ? 12 : 8);
+    };
+    a.vec = row_stride % kRun == 0 && out_stride % kRun == 0 && ((uintptr_t)logits % (kRun * in)) == 0 &&
+            ((uintptr_t)out % (kRun * res)) == 0;
+    const bool out_f32 = out_dtype == KVATTN_KV_F32;
+    const auto plan = [&](bool share) {
+        return dtype == KVATTN_KV_F32 ? plan_for<true>(rows, V, out_f32, probs != 0, share) : plan_for<false>(rows, V, out_f32, probs != 0, share);
+    };
+    LogitPlan p = plan(r.workspace != nullptr);
+    size_t lds = lds_of(p.tokens);
+    if (probs && p.slices > 1 && lds > kLdsTogether) {     // they would not run at once
+        p = plan(false);
+        lds = lds_of(p.tokens);
+    }
     if (lds > kLdsMost) return KVATTN_ERR_LDS;
-    const bool vec = row_stride % kRun == 0 && out_stride % kRun == 0 && ((uintptr_t)logits % (kRun * in)) == 0 &&
-                     ((uintptr_t)out % (kRun * res)) == 0;
-    const void* fn = dtype == KVATTN_KV_F32 ? (out_dtype == KVATTN_KV_F32 ? kernel_for<true, true>(V, vec, probs != 0) : kernel_for<true, false>(V, vec, probs != 0))
-                                            : (out_dtype == KVATTN_KV_F32 ? kernel_for<false, true>(V, vec, probs != 0) : kernel_for<false, false>(V, vec, probs != 0));
-    if (lds > 64 * 1024 - 512) {
-        const int st = hip_status(hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, kLdsMost));
+    a.slices = p.slices;
+    a.slice = p.tokens;
+    a.exchange = (unsigned long long*)r.workspace;
+    a.polls = kvattn_internal::merge_poll_limit();
+    if (lds > 60 * 1024) {
+        const int st = hip_status(hipFuncSetAttribute(p.fn, hipFuncAttributeMaxDynamicSharedMemorySize, kLdsMost));
         if (st != KVATTN_OK) return st;
     }
+    const long long grid = (long long)rows * p.slices;
+    if (grid * p.threads >= (1ll << 32)) return KVATTN_ERR_SHAPE;
     void* params[] = {&a};
-    return hip_status(hipLaunchKernel(fn, dim3((unsigned)rows), dim3(kThreads), params, lds, (hipStream_t)stream));
+    return hip_status(hipLaunchKernel(p.fn, dim3((unsigned)grid), dim3(p.threads), params, lds, (hipStream_t)stream));
 }

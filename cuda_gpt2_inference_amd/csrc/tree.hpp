@@ -28,4 +28,5 @@ struct AttendTree {
 __attribute__((visibility("hidden"))) int attend_tree(const AttendTree& c);
 
 void set_last_hip_error(int e);   // kvattn.hip: read back by kvattn_last_hip_error
+int merge_poll_limit();           // kvattn.hip: kvattn_set_merge_poll_limit's bound
 }  // namespace kvattn_internal

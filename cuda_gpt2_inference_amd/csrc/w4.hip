@@ -9,11 +9,17 @@
 //
 // Weights are laid out once, in the order in which lanes need them: 16 rows x 128 columns are one block of 1 KB,
 // lane 16 g + r's 16 bytes of which are columns 32 j + 8 g .. + 7 of row r in dword j, so that product j is columns 32 j ..
-// 32 j + 31, a group or a part of one, and a load of the block is contiguous.  Scales of a block lie in the order in
-// which results have rows (lane 16 g + r: rows 4 g .. 4 g + 3).
+// 32 j + 31, a group or a part of one, and a load of the block is contiguous.  (INT4: in the order from which operand()
+// makes columns in theirs.)  Weights are the products' right operand, so that of a result lane 16 g + r has weight row r
+// for vectors 4 g .. 4 g + 3: one scale a lane, and INT4's -8 times the vectors' sums as four neighbouring floats.  (As
+// the left one: 64 vectors x 50304 x 768 15.4 us.)
+//
+// Vectors go through LDS: loaded directly in the operands' order, neighbouring lanes would be in different rows, and
+// a load takes 64 cycles in place of 16.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "fc.hpp"
 #include "matrix.hpp"
@@ -23,7 +29,8 @@ namespace {
 constexpr int kRows = 16, kCols = 128;         // of a block
 constexpr int kBlockBytes = kRows * kCols / 2;
 constexpr int kW4Waves = 8;
-
+constexpr int kTallGroups = 256;               // workgroups: one a CU
+constexpr size_t kTallLds = 152 * 1024;
 // Where a matrix's blocks and scales lie.
 struct W4Shape {
     int M, K, group, tiles, steps, groups;     // row tiles, blocks of a row tile, groups of a block
@@ -49,11 +56,93 @@ struct W4Args {
     int B, M, K, steps, gelu;
 };
 
-// kGroups: groups of a block; kRT, kNT: row tiles and tiles of 16 vectors of a workgroup, whose waves split the columns.
-template <bool kFp4, int kGroups, int kRT, int kNT, bool kOutF32>
+// A lane's scales of a block.
+template <int kGroups> struct Scales {
+    uint32_t w[kGroups == 4 ? 2 : 1];
+    __device__ __forceinline__ void load(const uint8_t* p) {
+        if constexpr (kGroups == 4) {
+            const uint2 v = *reinterpret_cast<const uint2*>(p);
+            w[0] = v.x;
+            w[1] = v.y;
+        } else if constexpr (kGroups == 2) {
+            w[0] = *reinterpret_cast<const uint32_t*>(p);
+        } else {
+            w[0] = *reinterpret_cast<const uint16_t*>(p);
+        }
+    }
+    __device__ __forceinline__ float of(int q) const { return q & 1 ? bf16_hi(w[q / 2]) : bf16_lo(w[q / 2]); }
+};
+
+// A block's vectors in LDS: 256 bytes a vector, 16-byte chunks turned by the vector's number, so that the lanes that read one
+// chunk of 16 vectors find them in different banks.
+__device__ __forceinline__ int x_at(int vec, int chunk) { return vec * 256 + ((chunk ^ (vec & 15)) << 4); }
+
+// The products of a block, 16 rows x 16 kNT vectors, added to acc.  x(j, q): vectors' operand of product q.  INT4: the
+// operand's codes are 8 too large, so -8 times the vectors goes into a group's sum too; start(j, q), if given, has it.
+// kRT row tiles share the vectors' operands.
+struct NoStart {};
+template <bool kFp4, int kGroups, int kNT, int kRT, typename X, typename S = NoStart>
+__device__ __forceinline__ void block_products(const uint4 (&w)[kRT], const Scales<kGroups> (&sc)[kRT], X&& x,
+                                               F32x4 (&acc)[kRT][kNT], S start = {}) {
+    constexpr int kPer = 4 / kGroups;          // products of a group
+    constexpr bool kMinus = !kFp4 && std::is_same<S, NoStart>::value;
+    const Bf16x8 minus8 = (Bf16x8)(__bf16)(-8.0f);
+#pragma unroll
+    for (int q = 0; q < kGroups; ++q) {
+        F32x4 d[kRT][kNT];
+#pragma unroll
+        for (int j = 0; j < kNT; ++j) {
+            F32x4 d0 = {0.0f, 0.0f, 0.0f, 0.0f};
+            if constexpr (!kFp4 && !kMinus) d0 = start(j, q);
+#pragma unroll
+            for (int i = 0; i < kRT; ++i) d[i][j] = d0;
+        }
+#pragma unroll
+        for (int p = 0; p < kPer; ++p) {
+            Bf16x8 op[kRT];
+#pragma unroll
+            for (int i = 0; i < kRT; ++i) {
+                const uint32_t c[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
+                op[i] = operand<kFp4>(c[q * kPer + p]);
+            }
+#pragma unroll
+            for (int j = 0; j < kNT; ++j) {
+                const Bf16x8 v = x(j, q * kPer + p);
+#pragma unroll
+                for (int i = 0; i < kRT; ++i) {
+                    if constexpr (kMinus) d[i][j] = mfma(v, minus8, d[i][j]);
+                    d[i][j] = mfma(v, op[i], d[i][j]);
+                }
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < kRT; ++i) {
+            const float f = sc[i].of(q);
+#pragma unroll
+            for (int j = 0; j < kNT; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[i][j][e] = fmaf(d[i][j][e], f, acc[i][j][e]);
+        }
+    }
+}
+
+// One output through the epilogue.
+template <bool kOutF32>
+__device__ __forceinline__ void finish(const W4Args& a, int b, int m, float pre) {
+    const size_t o = (size_t)b * a.M + m;
+    if (a.pre_gelu) store_res<kOutF32>(a.pre_gelu, o, pre);
+    if (a.gelu) pre = gelu_tanh(pre);
+    store_res<kOutF32>(a.out, o, pre);
+}
+
+// Waves of a workgroup split the columns of kRT row tiles, for kNT tiles of 16 vectors, of which 4 kQ are there at most: four
+// vectors a load, 16 lanes each, past the last one that one again.  (A load that only some calls need, behind a branch, is
+// waited for before the next: 64 vectors 49 us in place of 10.)  kGroups: groups of a block.
+template <bool kFp4, int kGroups, int kRT, int kNT, int kQ, bool kOutF32>
 __global__ __launch_bounds__(kW4Waves * kWave) void gemv_w4_kernel(W4Args a) {
-    constexpr int kPitch = kRT * kRows + 4;    // floats; keeps 16-byte stores aligned and spreads the banks
-    extern __shared__ float red[];             // [waves][kNT * 16][kPitch]
+    constexpr int kPitch = kRT * kRows + 4;    // floats; spreads the banks
+    constexpr int kXBytes = kNT * 16 * 256, kWaveLds = std::max(kXBytes, kNT * 16 * kPitch * 4);
+    extern __shared__ __align__(16) uint8_t lds[];     // a wave's vectors of a block, then [waves][kNT * 16][kPitch] sums
     const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int col = lane & 15, g = lane >> 4;
     const int tiles = (a.M + kRows - 1) / kRows;
@@ -66,101 +155,212 @@ __global__ __launch_bounds__(kW4Waves * kWave) void gemv_w4_kernel(W4Args a) {
     for (int i = 0; i < kRT; ++i) {
         const size_t block = (size_t)min(tile0 + i, tiles - 1) * a.steps;
         wp[i] = a.w + block * kBlockBytes + lane * 16;
-        sp[i] = a.scales + block * kScaleBytes + g * 8 * kGroups;
+        sp[i] = a.scales + block * kScaleBytes + col * 2 * kGroups;
     }
-    const uint16_t* xp[kNT];
-#pragma unroll
-    for (int j = 0; j < kNT; ++j) xp[j] = a.x + (size_t)min(b0 + 16 * j + col, a.B - 1) * a.K + 8 * g;
-
-    F32x4 acc[kRT][kNT] = {};
-    const F32x4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
-    const Bf16x8 minus8 = (Bf16x8)(__bf16)(-8.0f);
-    for (int s = s0; s < s1; ++s) {
+    struct Block {
         uint4 w[kRT];
-        uint2 sc[kRT][kGroups];
+        Scales<kGroups> sc[kRT];
+        uint4 x[kQ];
+    };
+    auto load = [&](Block& t, int s) {
 #pragma unroll
         for (int i = 0; i < kRT; ++i) {
-            w[i] = load16(wp[i] + (size_t)s * kBlockBytes);
-#pragma unroll
-            for (int q = 0; q < kGroups; ++q) sc[i][q] = *reinterpret_cast<const uint2*>(sp[i] + (size_t)s * kScaleBytes + 8 * q);
+            t.w[i] = load16(wp[i] + (size_t)s * kBlockBytes);
+            t.sc[i].load(sp[i] + (size_t)s * kScaleBytes);
         }
-        Bf16x8 x[kNT][4];
-        F32x4 init[kNT][kGroups];
+        const int k = min(s * kCols + 8 * col, a.K - 8);
 #pragma unroll
-        for (int j = 0; j < kNT; ++j) {
+        for (int q = 0; q < kQ; ++q) t.x[q] = *reinterpret_cast<const uint4*>(a.x + (size_t)min(b0 + 4 * q + g, a.B - 1) * a.K + k);
+    };
+    uint8_t* const xs = lds + wave * kWaveLds;
+    F32x4 acc[kRT][kNT] = {};
+    Block t;
+    if (s0 < s1) load(t, s0);
+    for (int s = s0; s < s1; ++s) {
+        const bool in = s * kCols + 8 * col < a.K;     // what is past the row's end is zero
+        lds_order();
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const int k = s * kCols + 32 * q + 8 * g;
-                uint4 v = *reinterpret_cast<const uint4*>(xp[j] + min(s * kCols + 32 * q, a.K - 32));
-                if (k >= a.K) v = make_uint4(0, 0, 0, 0);
-                x[j][q] = in_order<kFp4>(v);
-            }
-            // INT4: the operand's codes are 8 too large, so a group's sum starts at -8 times that of x.
-#pragma unroll
-            for (int q = 0; q < kGroups; ++q) {
-                init[j][q] = zero;
-                if constexpr (!kFp4) {
-#pragma unroll
-                    for (int p = 0; p < 4 / kGroups; ++p) init[j][q] = mfma(minus8, x[j][q * (4 / kGroups) + p], init[j][q]);
-                }
-            }
-        }
+        for (int q = 0; q < kQ; ++q) *reinterpret_cast<uint4*>(xs + x_at(4 * q + g, col)) = in ? t.x[q] : make_uint4(0, 0, 0, 0);
+        lds_order();
+        uint4 w[kRT];
+        Scales<kGroups> sc[kRT];
 #pragma unroll
         for (int i = 0; i < kRT; ++i) {
-            const uint32_t c[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
-#pragma unroll
-            for (int q = 0; q < kGroups; ++q) {
-                F32x4 d[kNT];
-#pragma unroll
-                for (int j = 0; j < kNT; ++j) d[j] = init[j][q];
-#pragma unroll
-                for (int p = 0; p < 4 / kGroups; ++p) {
-                    const int at = q * (4 / kGroups) + p;
-                    const Bf16x8 op = operand<kFp4>(c[at]);
-#pragma unroll
-                    for (int j = 0; j < kNT; ++j) d[j] = mfma(op, x[j][at], d[j]);
-                }
-                const float f[4] = {bf16_lo(sc[i][q].x), bf16_hi(sc[i][q].x), bf16_lo(sc[i][q].y), bf16_hi(sc[i][q].y)};
-#pragma unroll
-                for (int j = 0; j < kNT; ++j)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) acc[i][j][e] = fmaf(d[j][e], f[e], acc[i][j][e]);
-            }
+            w[i] = t.w[i];
+            sc[i] = t.sc[i];
         }
+        if (s + 1 < s1) load(t, s + 1);
+        auto x_of = [&](int j, int q) { return *reinterpret_cast<const Bf16x8*>(xs + x_at(16 * j + col, 4 * q + g)); };
+        block_products<kFp4, kGroups, kNT, kRT>(w, sc, x_of, acc);
+        lds_order();
     }
-    // Lane 16 g + c holds rows 4 g .. 4 g + 3 of vector c.
+    // Lane 16 g + c holds weight row c for vectors 4 g .. 4 g + 3.
+    lds_order();
 #pragma unroll
     for (int i = 0; i < kRT; ++i)
 #pragma unroll
         for (int j = 0; j < kNT; ++j)
-            *reinterpret_cast<F32x4*>(red + (size_t)((wave * kNT + j) * 16 + col) * kPitch + 16 * i + 4 * g) = acc[i][j];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) reinterpret_cast<float*>(xs)[(16 * j + 4 * g + e) * kPitch + 16 * i + col] = acc[i][j][e];
     __syncthreads();
     for (int e = threadIdx.x; e < kRT * kRows * kNT * 16; e += kW4Waves * kWave) {
         const int mm = e % (kRT * kRows), bb = e / (kRT * kRows), m = tile0 * kRows + mm, b = b0 + bb;
         if (m >= a.M || b >= a.B) continue;
         float v[kW4Waves];
 #pragma unroll
-        for (int w = 0; w < kW4Waves; ++w) v[w] = red[(size_t)(w * kNT * 16 + bb) * kPitch + mm];
+        for (int w = 0; w < kW4Waves; ++w) v[w] = reinterpret_cast<const float*>(lds + w * kWaveLds)[bb * kPitch + mm];
 #pragma unroll
         for (int d = 1; d < kW4Waves; d *= 2)
 #pragma unroll
             for (int w = 0; w + d < kW4Waves; w += 2 * d) v[w] += v[w + d];
-        float pre = v[0] + (a.bias ? bf16_to_f32(a.bias[m]) : 0.0f);
-        const size_t o = (size_t)b * a.M + m;
-        if (a.pre_gelu) store_res<kOutF32>(a.pre_gelu, o, pre);
-        if (a.gelu) pre = gelu_tanh(pre);
-        store_res<kOutF32>(a.out, o, pre);
+        finish<kOutF32>(a, b, m, v[0] + (a.bias ? bf16_to_f32(a.bias[m]) : 0.0f));
     }
 }
 
-template <bool kFp4, int kGroups, int kRT, int kNT>
-const void* kernel_for(bool out_f32) {
-    return out_f32 ? (const void*)&gemv_w4_kernel<kFp4, kGroups, kRT, kNT, true> : (const void*)&gemv_w4_kernel<kFp4, kGroups, kRT, kNT, false>;
+// Tall matrices: a workgroup, one a CU, keeps its 16 kNT vectors in LDS for their whole length, and each of its waves takes
+// whole row tiles, with no sum across waves.  INT4: -8 times the vectors' sums over every group are made once, too.
+// (Two row tiles a wave, of half as many waves: the same time.)
+constexpr int kTallW4Waves = 16, kTallW4Steps = 3;     // blocks of a load, two of which are in flight
+template <bool kFp4, int kGroups, int kNT, bool kOutF32>
+__global__ __launch_bounds__(kTallW4Waves * kWave) void gemv_w4_tall_kernel(W4Args a, int groups) {
+    constexpr int kT = kTallW4Steps, kWaves = kTallW4Waves, kScaleBytes = 32 * kGroups;
+    extern __shared__ __align__(16) uint8_t lds[];     // [steps][kNT * 16][256], then [steps * kGroups][kNT * 16] floats
+    const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const int col = lane & 15, g = lane >> 4;
+    const int tiles = (a.M + kRows - 1) / kRows;
+    const int grp = blockIdx.x, b0 = blockIdx.y * 16 * kNT;
+    const int tile0 = (int)((long long)tiles * grp / groups), tile1 = (int)((long long)tiles * (grp + 1) / groups);
+    float* const sums = reinterpret_cast<float*>(lds + (size_t)a.steps * kNT * 16 * 256);
+    struct Block {
+        uint4 w[kT][1];
+        Scales<kGroups> sc[kT][1];
+    };
+    const int chunks = (a.steps + kT - 1) / kT;
+    int ltile = tile0 + wave, lchunk = 0;              // what is loaded next
+    auto next = [&](Block& t) {
+        if (ltile >= tile1) return false;
+#pragma unroll
+        for (int u = 0; u < kT; ++u) {
+            const int s = min(lchunk * kT + u, a.steps - 1);
+            const size_t block = (size_t)ltile * a.steps + s;
+            t.w[u][0] = load16(a.w + block * kBlockBytes + lane * 16);
+            t.sc[u][0].load(a.scales + block * kScaleBytes + col * 2 * kGroups);
+        }
+        if (++lchunk == chunks) {
+            lchunk = 0;
+            ltile += kWaves;
+        }
+        return true;
+    };
+    Block t0, t1;
+    const bool busy = next(t0);
+    bool more = next(t1);
+    // Vectors to LDS, four a load.
+    const int quads = min(4 * kNT, (min(a.B - b0, 16 * kNT) + 3) / 4), pieces = a.steps * quads;
+    constexpr int kAhead = 6;
+    for (int i0 = wave; i0 < pieces; i0 += kWaves * kAhead) {
+        uint4 v[kAhead];
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) {
+            const int i = min(i0 + k * kWaves, pieces - 1), s = i / quads, q = i - s * quads;
+            v[k] = *reinterpret_cast<const uint4*>(a.x + (size_t)min(b0 + 4 * q + g, a.B - 1) * a.K + min(s * kCols + 8 * col, a.K - 8));
+        }
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) {
+            const int i = i0 + k * kWaves;
+            if (i >= pieces) break;
+            const int s = i / quads, q = i - s * quads;
+            *reinterpret_cast<uint4*>(lds + (size_t)s * kNT * 16 * 256 + x_at(4 * q + g, col)) =
+                s * kCols + 8 * col < a.K ? v[k] : make_uint4(0, 0, 0, 0);
+        }
+    }
+    __syncthreads();
+    auto x_of = [&](int s, int j, int q) {
+        return *reinterpret_cast<const Bf16x8*>(lds + (size_t)s * kNT * 16 * 256 + x_at(16 * j + col, 4 * q + g));
+    };
+    if constexpr (!kFp4) {
+        const F32x4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
+        const Bf16x8 minus8 = (Bf16x8)(__bf16)(-8.0f);
+        for (int i = wave; i < a.steps * kNT; i += kWaves) {
+            const int s = i / kNT, j = i - s * kNT;
+#pragma unroll
+            for (int q = 0; q < kGroups; ++q) {
+                F32x4 d = zero;
+#pragma unroll
+                for (int p = 0; p < 4 / kGroups; ++p) d = mfma(x_of(s, j, q * (4 / kGroups) + p), minus8, d);
+                if (col == 0) *reinterpret_cast<F32x4*>(sums + ((s * kGroups + q) * kNT + j) * 16 + 4 * g) = d;
+            }
+        }
+        __syncthreads();
+    }
+    if (!busy) return;
+    int tile = tile0 + wave, chunk = 0;                // what is worked on
+    F32x4 acc[1][kNT] = {};
+    auto consume = [&](const Block& t) {
+#pragma unroll
+        for (int u = 0; u < kT; ++u) {
+            const int s = chunk * kT + u;
+            if (s >= a.steps) break;
+            block_products<kFp4, kGroups, kNT, 1>(t.w[u], t.sc[u], [&](int j, int q) { return x_of(s, j, q); }, acc, [&](int j, int q) {
+                return *reinterpret_cast<const F32x4*>(sums + ((s * kGroups + q) * kNT + j) * 16 + 4 * g);
+            });
+        }
+        if (++chunk < chunks) return;
+        const int m = tile * kRows + col;
+        const float bias = a.bias ? bf16_to_f32(a.bias[min(m, a.M - 1)]) : 0.0f;
+        const int left = m < a.M ? a.B - b0 - 4 * g : 0;       // vectors from this lane's first on
+        if (a.gelu || a.pre_gelu) {
+#pragma unroll
+            for (int j = 0; j < kNT; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (16 * j + e < left) finish<kOutF32>(a, b0 + 16 * j + 4 * g + e, m, acc[0][j][e] + bias);
+        } else {
+            size_t o = (size_t)(b0 + 4 * g) * a.M + m;
+#pragma unroll
+            for (int j = 0; j < kNT; ++j) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (16 * j + e < left) store_res<kOutF32>(a.out, o + (size_t)e * a.M, acc[0][j][e] + bias);
+                o += (size_t)16 * a.M;
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < kNT; ++j) acc[0][j] = F32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        chunk = 0;
+        tile += kWaves;
+    };
+    while (true) {
+        consume(t0);
+        if (!more) break;
+        more = next(t0);
+        consume(t1);
+        if (!more) break;
+        more = next(t1);
+    }
 }
-template <int kRT, int kNT>
-const void* kernel_for(bool fp4, int groups, bool out_f32) {
-    if (fp4) return groups == 4 ? kernel_for<true, 4, kRT, kNT>(out_f32) : groups == 2 ? kernel_for<true, 2, kRT, kNT>(out_f32) : kernel_for<true, 1, kRT, kNT>(out_f32);
-    return groups == 4 ? kernel_for<false, 4, kRT, kNT>(out_f32) : groups == 2 ? kernel_for<false, 2, kRT, kNT>(out_f32) : kernel_for<false, 1, kRT, kNT>(out_f32);
+
+template <bool kFp4, int kGroups, int kNT, bool kOutF32>
+const void* kernel_for(int row_tiles, int B) {
+    if (row_tiles == 0) return (const void*)&gemv_w4_tall_kernel<kFp4, kGroups, kNT, kOutF32>;
+    if (kNT == 1 && B <= 4) {
+        return row_tiles == 1 ? (const void*)&gemv_w4_kernel<kFp4, kGroups, 1, kNT, 1, kOutF32>
+                              : (const void*)&gemv_w4_kernel<kFp4, kGroups, 2, kNT, 1, kOutF32>;
+    }
+    return row_tiles == 1 ? (const void*)&gemv_w4_kernel<kFp4, kGroups, 1, kNT, 4 * kNT, kOutF32>
+                          : (const void*)&gemv_w4_kernel<kFp4, kGroups, 2, kNT, 4 * kNT, kOutF32>;
+}
+template <bool kFp4, int kGroups, int kNT>
+const void* kernel_for(int row_tiles, int B, bool out_f32) {
+    return out_f32 ? kernel_for<kFp4, kGroups, kNT, true>(row_tiles, B) : kernel_for<kFp4, kGroups, kNT, false>(row_tiles, B);
+}
+template <int kNT>
+const void* kernel_for(bool fp4, int groups, int row_tiles, int B, bool out_f32) {
+    if (fp4)
+        return groups == 4 ? kernel_for<true, 4, kNT>(row_tiles, B, out_f32)
+                           : groups == 2 ? kernel_for<true, 2, kNT>(row_tiles, B, out_f32) : kernel_for<true, 1, kNT>(row_tiles, B, out_f32);
+    return groups == 4 ? kernel_for<false, 4, kNT>(row_tiles, B, out_f32)
+                       : groups == 2 ? kernel_for<false, 2, kNT>(row_tiles, B, out_f32) : kernel_for<false, 1, kNT>(row_tiles, B, out_f32);
 }
 
 // ------------------------------------------------------------------------------------
@@ -174,18 +374,26 @@ __device__ __forceinline__ size_t dword_at(const W4Shape& s, int m, int k) {
 }
 __device__ __forceinline__ size_t scale_at(const W4Shape& s, int m, int k) {
     const size_t block = (size_t)(m / kRows) * s.steps + k / kCols;
-    const int r = m % kRows;
-    return block * (16 * s.groups) + (r / 4) * 4 * s.groups + (k % kCols / s.group) * 4 + r % 4;
+    return block * (kRows * s.groups) + (m % kRows) * s.groups + k % kCols / s.group;
+}
+
+// Eight codes, the first in the lowest half byte, in the order that operand() takes.
+__device__ __forceinline__ uint32_t in_layout(uint32_t w, bool int4) {
+    if (!int4) return w;
+    uint32_t o = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o |= ((w >> (4 * i)) & 15u) << (8 * i) | ((w >> (16 + 4 * i)) & 15u) << (8 * i + 4);
+    return o;
 }
 
 // A thread for every dword of the layout; what is behind the matrix's end is zero.
 __global__ __launch_bounds__(256) void pack_w4_kernel(uint32_t* w4, uint16_t* out_scales, const uint32_t* codes, const uint16_t* scales,
-                                                      W4Shape s, uint32_t none) {
+                                                      W4Shape s, int int4) {
     const long long words = (long long)s.tiles * kRows * s.steps * (kCols / 8);
     for (long long e = (long long)blockIdx.x * 256 + threadIdx.x; e < words; e += (long long)gridDim.x * 256) {
         const int per = s.steps * (kCols / 8), m = (int)(e / per), k = (int)(e - (long long)m * per) * 8;
         const bool in = m < s.M && k < s.K;
-        w4[dword_at(s, m, k)] = in ? codes[((size_t)m * s.K + k) / 8] : none;
+        w4[dword_at(s, m, k)] = in_layout(in ? codes[((size_t)m * s.K + k) / 8] : int4 ? 0x88888888u : 0u, int4);
         if (k % s.group == 0) out_scales[scale_at(s, m, k)] = in ? scales[(size_t)m * (s.K / s.group) + k / s.group] : 0;
     }
 }
@@ -223,7 +431,7 @@ __global__ __launch_bounds__(256) void quantize_w4_kernel(uint32_t* w4, uint16_t
                 }
                 w |= c << (4 * i);
             }
-            w4[dword_at(s, m, k0 + i0)] = w;
+            w4[dword_at(s, m, k0 + i0)] = in_layout(w, !kFp4);
         }
     }
 }
@@ -251,10 +459,10 @@ int kvattn_w4_pack(void* w4, const void* codes, const void* scales, int M, int K
     if (!shape_of(M, K, group, s)) return KVATTN_ERR_SHAPE;
     if (!w4 || !codes || !scales) return KVATTN_ERR_NULL_POINTER;
     if (((uintptr_t)w4 & 15u) || ((uintptr_t)codes & 15u) || ((uintptr_t)scales & 1u)) return KVATTN_ERR_MISALIGNED;
-    uint32_t none = w_dtype == KVATTN_KV_INT4 ? 0x88888888u : 0u;
+    int int4 = w_dtype == KVATTN_KV_INT4;
     uint8_t* sc = (uint8_t*)w4 + s.scales_at();
     const long long words = (long long)s.tiles * kRows * s.steps * (kCols / 8);
-    void* params[] = {&w4, &sc, &codes, &scales, &s, &none};
+    void* params[] = {&w4, &sc, &codes, &scales, &s, &int4};
     return hip_status(hipLaunchKernel((const void*)&pack_w4_kernel, dim3((unsigned)std::min<long long>((words + 255) / 256, 1 << 20)),
                                       dim3(256), params, 0, (hipStream_t)stream));
 }
@@ -288,12 +496,30 @@ int kvattn_gemv_w4(void* out, void* pre_gelu, const void* w4, const void* x, con
              B, M, K, s.steps, gelu ? 1 : 0};
     const bool fp4 = w_dtype == KVATTN_KV_FP4_E2M1, f32 = out_dtype == KVATTN_KV_F32;
     const int nt = B <= 16 ? 1 : B <= 32 ? 2 : 4;
-    const void* fn = nt == 1 ? kernel_for<1, 1>(fp4, s.groups, f32) : nt == 2 ? kernel_for<1, 2>(fp4, s.groups, f32) : kernel_for<1, 4>(fp4, s.groups, f32);
+    const size_t x_lds = (size_t)s.steps * nt * 16 * (256 + 4 * s.groups);
+    // Two row tiles a workgroup halve the vectors' loads where enough workgroups are left, and 64 vectors the registers for
+    // it are missing; tall matrices keep their vectors in LDS, few vectors from more rows on.  us per call (graph), INT4, groups of 64, one / two row
+    // tiles / vectors in LDS:
+    //   1 vector    8192 x 8192 9.1 / 8.9      12000 x 1024 3.4 / 3.7 / 5.5   20000 x 1024 5.1 / 5.4 / 6.7   50304 x 768 9.6 / 9.2 / 7.5
+    //   16          4096 x 4096 4.6 / 6.4       8192 x 8192 13.5 / 10.4       12000 x 1024 4.8 / 4.1 / 6.8   20000 x 1024 5.9 / 5.6 / 7.6
+    //   26          6400 x 1600 7.2 / 5.5
+    //   32          4096 x 4096 6.1 / 8.4      12000 x 1024 7.6 / 7.1 / 8.0   20000 x 1024 11.7 / 9.9 / 9.0
+    //   64          6400 x 1600 11.9 / 16.6    12000 x 1024 12.5 / 21.4 / 13.7   20000 x 1024 20.4 / 31.6 / 14.8   50304 x 768 49 / 63 / 15.4
+    int row_tiles = nt < 4 && s.tiles >= (nt == 1 ? 512 : 320) ? 2 : 1;
+    if (s.tiles >= (nt == 1 ? 2048 : 1024) && x_lds <= kTallLds) row_tiles = 0;
+    const void* fn = nt == 1 ? kernel_for<1>(fp4, s.groups, row_tiles, B, f32)
+                             : nt == 2 ? kernel_for<2>(fp4, s.groups, row_tiles, B, f32) : kernel_for<4>(fp4, s.groups, row_tiles, B, f32);
     const long long cols = (B + 16 * nt - 1) / (16 * nt);
     if (cols > 65535) return KVATTN_ERR_SHAPE;
-    const size_t lds = (size_t)kW4Waves * nt * 16 * (kRows + 4) * sizeof(float);
-    void* params[] = {&a};
-    return hip_status(hipLaunchKernel(fn, dim3((unsigned)s.tiles, (unsigned)cols), dim3(kW4Waves * kWave), params, lds, (hipStream_t)stream));
+    int groups = kTallGroups;
+    const int grid = row_tiles ? (s.tiles + row_tiles - 1) / row_tiles : groups, waves = row_tiles ? kW4Waves : kTallW4Waves;
+    const size_t lds = row_tiles ? (size_t)kW4Waves * nt * 16 * std::max(256, (row_tiles * kRows + 4) * 4) : x_lds;
+    if (lds > 64 * 1024) {
+        const int st = hip_status(hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024));
+        if (st != KVATTN_OK) return st;
+    }
+    void* params[] = {&a, &groups};
+    return hip_status(hipLaunchKernel(fn, dim3((unsigned)grid, (unsigned)cols), dim3(waves * kWave), params, lds, (hipStream_t)stream));
 }
 
 }  // extern "C"

@@ -124,6 +124,7 @@ SIGNATURES = {
     "kvattn_paged_keep": (_i, [_vp, _vp, _i, _i, _vp, _vp, _vp, _i, _i, _i, _i, _i, _vp]),
     "kvattn_verify_tree": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _ll, _i, _vp, _sz,
                                 _vp]),
+    "kvattn_logits_workspace_bytes": (_sz, []),
     "kvattn_process_logits": (_i, [_vp, _vp, _vp, _vp, _i, _i, _i, _ll, _ll, _i, _i, _i, _vp]),
     "kvattn_w4_bytes": (_sz, [_i, _i, _i]),
     "kvattn_w4_pack": (_i, [_vp, _vp, _vp, _i, _i, _i, _i, _vp]),
@@ -562,15 +563,22 @@ class _LogitRules(ctypes.Structure):
     _fields_ = [(name, _vp) for name in (
         "history", "history_len", "prompt_len", "tokens", "masks", "repetition", "frequency", "presence", "bias_start",
         "bias_ids", "bias", "allowed", "allowed_of", "temperature")] + [
-        (name, _i) for name in ("max_history", "mask_words", "num_bias", "max_bias", "num_allowed", "allowed_stride")]
+        (name, _i) for name in ("max_history", "mask_words", "num_bias", "max_bias", "num_allowed", "allowed_stride")] + [
+        ("workspace", _vp), ("workspace_bytes", _sz)]
 
 
 class LogitRules:
     """Rules on logits for process_logits: the fields of kvattn_logit_rules by name, device tensors and integers.  Made
-    once; the tensors are kept, and may be written between calls."""
+    once; the tensors are kept, and may be written between calls.  Without a workspace of the caller's, rules with tensors
+    bring their own, so calls with one LogitRules must be ordered."""
 
     def __init__(self, **rules):
         self._struct = _LogitRules()
+        like = next((x for x in rules.values() if hasattr(x, "device")), None)
+        if "workspace" not in rules and like is not None and like.is_cuda:
+            import torch
+            nbytes = int(lib().kvattn_logits_workspace_bytes())
+            rules = dict(rules, workspace=torch.zeros(nbytes, dtype=torch.uint8, device=like.device), workspace_bytes=nbytes)
         names = dict(_LogitRules._fields_)
         for name, x in rules.items():
             if name not in names:

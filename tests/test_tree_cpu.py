@@ -88,6 +88,7 @@ LOGITS = dict(out=A, x=A, rules=None, start=A, B=2, rows=4, V=100, row=100, out_
     ({}, dict(bias_start=A, num_bias=3, max_bias=40000, bias_ids=A, bias=A), 4),
     ({}, dict(allowed=A, num_allowed=0, allowed_stride=4), 4), ({}, dict(allowed=A, num_allowed=2, allowed_stride=3), 4),
     ({}, dict(temperature=A + 1), 2), ({}, dict(repetition=A + 2), 2),
+    ({}, dict(workspace=A, workspace_bytes=64), 7), ({}, dict(workspace=A + 4, workspace_bytes=1 << 20), 2),
     (dict(V=1 << 18, row=1 << 18, out_row=1 << 18), dict(history=A, history_len=A, max_history=32768, bias_start=A, bias_ids=A, bias=A,
                                                          num_bias=32768, max_bias=32768), 10)])
 def test_process_logits(kw, rules, status):
@@ -102,7 +103,7 @@ def test_process_logits(kw, rules, status):
 def test_logit_rules_of_no_such_name():
     with pytest.raises(TypeError):
         _kv().LogitRules(histroy=A)
-    assert ctypes.sizeof(_kv()._LogitRules) == 14 * 8 + 6 * 4
+    assert ctypes.sizeof(_kv()._LogitRules) == 14 * 8 + 6 * 4 + 16
 
 
 GEMV = dict(out=A, pre=None, w4=A, x=A, bias=None, B=1, M=10, K=256, group=64, w=4, out_dtype=1, gelu=0, stream=None)
