@@ -12,9 +12,13 @@
 // in a sum is free, so a lane's eight places of step s are positions 32 s + 4 g .. + 3 and 32 s + 16 + 4 g .. + 3,
 // and V, which is needed channel-major, is read from LDS by the transposing reads (ds_read_b64_tr_b16, b8, b4)
 // in that order.
-//   Types.  BF16 rows are operands as they are; 8-bit and 4-bit codes are exact in bf16, and their scales go to
-//   the scores and the weights in float.  FP32 rows take 16x16x4 float products.  Weights in bf16 are two
-//   halves, upper and rest (2^-14), so that a sharp head's output is rounded once.
+//   Types.  BF16 rows are operands as they are; 8-bit and 4-bit codes are exact in bf16 and in float16, and their
+//   scales go to the scores and the weights in float.  FP32 rows take 16x16x4 float products.  Weights are rounded
+//   finer than the outputs (2^-8), since one bf16 would round a sharp head's output twice: over BF16 rows a weight is two
+//   bf16 halves, upper and rest (2^-14); over codes one float16 (2^-11) of the weight times its row's scale, in a unit
+//   that the wave's largest scale so far sets (a power of two; float16 then holds weights down to 2^-29 of the largest
+//   possible, and a smaller one's error is 2^-18 of it times the largest scale at most).  With two halves over codes
+//   too: INT4, 24 sequences of up to 4096, 32 tokens each, 26.5 us.
 //   Masks.  Only tiles that reach the new tokens look at any.  There a value that one query must not see may be
 //   infinite or NaN, which a weight of zero does not take out of a product: such a tile, found by looking at its V
 //   rows, has its outputs summed on the vector units, position by position.
@@ -26,6 +30,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "lanes.hpp"
 #include "layout.hpp"
@@ -45,7 +50,7 @@ constexpr float kQScale = 0.125f * 1.4426950408889634f;    // 1/sqrt(64) * log2(
 constexpr float kSlack = 8.0f;
 constexpr int kMaxSegments = 65535;        // the grid's third side
 constexpr int kMostWaves = (1 << 26) - 1;  // of a grid: 2^32 threads are too many
-constexpr int kCUs = 256;
+constexpr int kCUs = 256, kFewHeads = 32;
 
 template <int DT> struct Kv {
     static constexpr bool kF32 = DT == KVATTN_KV_F32;
@@ -58,6 +63,7 @@ template <int DT> struct Kv {
     static constexpr bool kCoded = k8 || k4;
     static constexpr int kRow = kF32 ? 256 : kBf16 ? 128 : k8 ? 64 : 32;      // bytes
     static constexpr int kChunks = kRow / 16;
+    static constexpr int kPos = kF32 ? 16 : kBf16 ? 32 : 64;                  // positions of a wave's tile: up to 8 KB
     static constexpr bool kMayBeInfinite = kF32 || kBf16 || kFp8;             // (FP8 has a NaN)
     // Where chunk c of a row lies among the row's chunks in LDS, so that the rows that are read together
     // lie in different banks.
@@ -121,16 +127,28 @@ __device__ __forceinline__ bool not_finite(const uint4& v) {
     return bad;
 }
 
-// kG: groups of 16 queries a workgroup may hold; kW: its waves; kPos: positions of a wave's tile.
-template <int DT, int kG, int kW, int kPos>
-__global__ __launch_bounds__(kW * kWave) __attribute__((amdgpu_waves_per_eu(2))) void tree_kernel(TreeArgs a) {
+// Four neighbouring outputs; a query that attends nothing has none.
+template <bool kF32>
+__device__ __forceinline__ void store_out(uint8_t* out, size_t at, float L, F32x4 o) {
+    o = L == 0.0f ? F32x4{0.0f, 0.0f, 0.0f, 0.0f} : o / L;
+    if constexpr (kF32) {
+        *reinterpret_cast<F32x4*>(out + at * 4) = o;
+    } else {
+        *reinterpret_cast<uint2*>(out + at * 2) =
+            make_uint2(f32_to_bf16(o[0]) | (uint32_t)f32_to_bf16(o[1]) << 16, f32_to_bf16(o[2]) | (uint32_t)f32_to_bf16(o[3]) << 16);
+    }
+}
+
+// kG: groups of 16 queries a workgroup may hold; kW: its waves.
+template <int DT, int kG, int kW>
+__global__ __launch_bounds__(kW * kWave) __attribute__((amdgpu_waves_per_eu(kG == 1 ? 3 : 2))) void tree_kernel(TreeArgs a) {
     using T = Kv<DT>;
-    constexpr int kT = kPos / 16;                              // groups of 16 positions of a tile
+    constexpr int kPos = T::kPos, kT = kPos / 16;              // positions of a wave's tile, groups of 16 of them
     constexpr int kTileBytes = kPos * T::kRow;
     constexpr int kLoads = kTileBytes / 1024;                  // 16-byte chunks a lane, of K and of V
     constexpr int kScales = T::kCoded ? 2 * kPos * 4 : 0;
     constexpr int kWaveLds = std::max(2 * kTileBytes + kScales, kQ * kOutPad * 4);
-    static_assert(kPos == 64 || (kPos == 32 && !T::kCoded), "a lane holds one position's scales");
+    static_assert(kPos == 64 || !T::kCoded, "a lane holds one position's scales");
     static_assert(kTileBytes % 1024 == 0 && kWaveLds % 16 == 0, "whole loads");
     __shared__ __align__(16) uint8_t lds[kW * kWaveLds];
     __shared__ float red_m[kW][kQ], red_l[kW][kQ];
@@ -212,6 +230,9 @@ __global__ __launch_bounds__(kW * kWave) __attribute__((amdgpu_waves_per_eu(2)))
             qw[i][u] = *reinterpret_cast<const uint4*>(qp + (T::kCoded ? 32 * g + 16 * u : 64 * u + 16 * g));
     }
     if (mine > 0) request(0);
+    unsigned long long mask0[kG];          // the first word of each query's mask
+#pragma unroll
+    for (int i = 0; i < kG; ++i) mask0[i] = a.masks[(size_t)(t0 + q0 + min(kQ * i + col, nq - 1)) * a.words];
     Bf16x8 qa[kG][2];
     float q_init[kG] = {};                 // INT4: the operand's codes are 8 too large, so a score starts at -8 sum q
     if constexpr (!T::kF32) {
@@ -233,6 +254,7 @@ __global__ __launch_bounds__(kW * kWave) __attribute__((amdgpu_waves_per_eu(2)))
     float* const ls = reinterpret_cast<float*>(lv + kTileBytes);
     F32x4 acc[kG][4] = {};                 // channels 16 c + 4 g + i of query col
     F32x4 acc8[kG] = {};                   // INT4: 8 sum of the weights, taken off at the end
+    float unit = 0.0f, per_unit = 0.0f;    // codes: of the weights
     float m[kG], off[kG], limit[kG], l[kG];
 #pragma unroll
     for (int i = 0; i < kG; ++i) {
@@ -263,8 +285,23 @@ __global__ __launch_bounds__(kW * kWave) __attribute__((amdgpu_waves_per_eu(2)))
             *reinterpret_cast<uint4*>(lv + at) = rv[j];
         }
         if constexpr (T::kCoded) {
+            // The weights' unit: a power of two not below the largest scale, followed where that has grown fourfold.
+            const float size = fabsf(rvs);
+            const float most = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(wave_max(size < INFINITY ? size : 0.0f))));
+            if (most > 4.0f * unit) {
+                const int e = min(max((int)(__float_as_uint(most) >> 23) + 1, 27), 254);
+                const float grown = __uint_as_float((uint32_t)e << 23), f = unit / grown;
+                unit = grown;
+                per_unit = __uint_as_float((uint32_t)(259 - e) << 23);      // 32 / unit
+#pragma unroll
+                for (int i = 0; i < kG; ++i) {
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) acc[i][c] *= f;
+                    if constexpr (T::kInt4) acc8[i] *= f;
+                }
+            }
             ls[lane] = rks * kQScale;
-            ls[kPos + lane] = rvs;
+            ls[kPos + lane] = rvs * per_unit;
         }
         lds_order();
         if (k + 1 < mine) request(k + 1);
@@ -283,175 +320,161 @@ __global__ __launch_bounds__(kW * kWave) __attribute__((amdgpu_waves_per_eu(2)))
             for (int i = 0; i < kG; ++i) {
                 const size_t tok = t0 + q0 + min(kQ * i + col, nq - 1);
                 const unsigned long long* const mp = a.masks + tok * a.words;
-                auto word = [&](int w) { return w < 0 ? ~0ull : w < a.words ? mp[w] : 0ull; };
+                auto word = [&](int w) { return w < 0 ? ~0ull : w == 0 ? mask0[i] : w < a.words ? mp[w] : 0ull; };
                 unsigned long long v = word(w0) >> sh;
                 if (sh) v |= word(w0 + 1) << (64 - sh);
                 vis[i] = v & live;
             }
         }
 
-        // K's operands.
-        Bf16x8 ka[T::kF32 ? 1 : kT][2];
-        U32x4 kf[T::kF32 ? kT : 1][4];
-#pragma unroll
-        for (int t = 0; t < kT; ++t) {
-            const int row = 16 * t + col;
-            if constexpr (T::kF32) {
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    kf[t][j] = *reinterpret_cast<const U32x4*>(lk + row * T::kRow + 16 * T::chunk_at(row, 4 * j + g));
-            } else if constexpr (T::kBf16) {
-#pragma unroll
-                for (int u = 0; u < 2; ++u)
-                    ka[t][u] = *reinterpret_cast<const Bf16x8*>(lk + row * T::kRow + 16 * T::chunk_at(row, 4 * u + g));
-            } else if constexpr (T::k8) {
-                codes_to_bf16<T::kFp8>(*reinterpret_cast<const U32x4*>(lk + row * T::kRow + 16 * T::chunk_at(row, g)), ka[t]);
-            } else {
-                const uint2 w = *reinterpret_cast<const uint2*>(lk + row * T::kRow + 8 * g);
-                ka[t][0] = operand<T::kFp4>(w.x);
-                ka[t][1] = operand<T::kFp4>(w.y);
-            }
-        }
-        // V's operands, transposed: step u's places of channels 16 c + col.
-        constexpr int kU = kPos / 32;
-        Bf16x8 va[4][kU];
-        if constexpr (!T::kF32) {
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                if constexpr (T::kBf16) {
-                    typedef short S16x4 __attribute__((ext_vector_type(4)));
-                    typedef short S16x8 __attribute__((ext_vector_type(8)));
-#pragma unroll
-                    for (int u = 0; u < kU; ++u) {
-                        S16x4 part[2];
-#pragma unroll
-                        for (int e = 0; e < 2; ++e) {
-                            const int row = 32 * u + 16 * e + 4 * g + (col >> 2);
-                            part[e] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                                (__attribute__((address_space(3))) S16x4*)(lv + row * T::kRow +
-                                    16 * T::chunk_at(row, 2 * c + ((col >> 1) & 1)) + 8 * (col & 1)));
-                        }
-                        va[c][u] = __builtin_bit_cast(Bf16x8, __builtin_shufflevector(part[0], part[1], 0, 1, 2, 3, 4, 5, 6, 7));
-                    }
-                } else if constexpr (T::k8) {
-                    I32x2 part[2];
-#pragma unroll
-                    for (int u = 0; u < 2; ++u) {
-                        const int e = col >> 1, row = 32 * u + 16 * (e >> 2) + 4 * g + (e & 3);
-                        part[u] = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
-                            (__attribute__((address_space(3))) I32x2*)(lv + row * T::kRow + 16 * T::chunk_at(row, c) + 8 * (col & 1)));
-                    }
-                    codes_to_bf16<T::kFp8>(U32x4{(uint32_t)part[0][0], (uint32_t)part[0][1], (uint32_t)part[1][0], (uint32_t)part[1][1]}, va[c]);
-                } else {
-                    const int e = place<T::kFp4>(col & 7), row = 32 * (col >> 3) + 16 * (e >> 2) + 4 * g + (e & 3);
-                    const I32x2 w = __builtin_amdgcn_ds_read_tr4_b64_v2i32(
-                        (__attribute__((address_space(3))) I32x2*)(lv + row * T::kRow + 8 * c));
-                    va[c][0] = operand<T::kFp4>((uint32_t)w[0]);
-                    va[c][1] = operand<T::kFp4>((uint32_t)w[1]);
-                }
-            }
-        }
-        F32x4 ks[T::kCoded ? kT : 1], vs[T::kCoded ? kT : 1];
-        if constexpr (T::kCoded) {
+        // The tile's work for kN groups: K's operands meet every group's queries as they are read, V's every group's
+        // weights, so that neither is held.
+        auto work = [&](auto groups) {
+            constexpr int kN = decltype(groups)::value, kU = kPos >= 32 ? kPos / 32 : 1;      // steps of 32 positions
+            F32x4 p[kN][kT];
 #pragma unroll
             for (int t = 0; t < kT; ++t) {
-                ks[t] = *reinterpret_cast<const F32x4*>(ls + 16 * t + 4 * g);
-                vs[t] = *reinterpret_cast<const F32x4*>(ls + kPos + 16 * t + 4 * g);
-            }
-        }
-        lds_order();
-
+                const int row = 16 * t + col;
 #pragma unroll
-        for (int i = 0; i < kG; ++i) {
-            if (i >= ng) break;
-            F32x4 p[kT];
-#pragma unroll
-            for (int t = 0; t < kT; ++t) {
-                p[t] = F32x4{q_init[i], q_init[i], q_init[i], q_init[i]};
+                for (int i = 0; i < kN; ++i) p[i][t] = F32x4{q_init[i], q_init[i], q_init[i], q_init[i]};
                 if constexpr (T::kF32) {
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
-                        const uint32_t qv[4] = {qw[i][j].x, qw[i][j].y, qw[i][j].z, qw[i][j].w};
+                        const U32x4 kf = *reinterpret_cast<const U32x4*>(lk + row * T::kRow + 16 * T::chunk_at(row, 4 * j + g));
 #pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            p[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kf[t][j][e]), __uint_as_float(qv[e]),
-                                                                        p[t], 0, 0, 0);
+                        for (int i = 0; i < kN; ++i) {
+                            const uint32_t qv[4] = {qw[i][j].x, qw[i][j].y, qw[i][j].z, qw[i][j].w};
+#pragma unroll
+                            for (int e = 0; e < 4; ++e)
+                                p[i][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kf[e]), __uint_as_float(qv[e]), p[i][t], 0, 0, 0);
+                        }
                     }
                 } else {
-                    p[t] = mfma(ka[t][0], qa[i][0], p[t]);
-                    p[t] = mfma(ka[t][1], qa[i][1], p[t]);
-                }
+                    Bf16x8 ka[2];
+                    if constexpr (T::kBf16) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    if constexpr (T::kCoded) p[t][e] *= ks[t][e];
-                    else p[t][e] *= kQScale;
+                        for (int u = 0; u < 2; ++u)
+                            ka[u] = *reinterpret_cast<const Bf16x8*>(lk + row * T::kRow + 16 * T::chunk_at(row, 4 * u + g));
+                    } else if constexpr (T::k8) {
+                        codes_to_bf16<T::kFp8>(*reinterpret_cast<const U32x4*>(lk + row * T::kRow + 16 * T::chunk_at(row, g)), ka);
+                    } else {
+                        const uint2 w = *reinterpret_cast<const uint2*>(lk + row * T::kRow + 8 * g);
+                        ka[0] = operand<T::kFp4>(w.x);
+                        ka[1] = operand<T::kFp4>(w.y);
+                    }
+#pragma unroll
+                    for (int i = 0; i < kN; ++i) {
+                        p[i][t] = mfma(ka[0], qa[i][0], p[i][t]);
+                        p[i][t] = mfma(ka[1], qa[i][1], p[i][t]);
+                    }
                 }
+                if constexpr (T::kCoded) {
+                    const F32x4 ks = *reinterpret_cast<const F32x4*>(ls + 16 * t + 4 * g);
+#pragma unroll
+                    for (int i = 0; i < kN; ++i) p[i][t] *= ks;
+                } else {
+#pragma unroll
+                    for (int i = 0; i < kN; ++i) p[i][t] *= kQScale;
+                }
+                if constexpr (kN > 1) lds_order();     // (else all of it is read ahead, into registers that are not there)
             }
-            const unsigned long long seen = vis[i] >> (4 * g);
-            if (tail) {
-                stay_a_branch();
+            // Softmax; the weights as operands (F32: in place).
+            typedef typename std::conditional<T::kCoded, F16x8, Bf16x8>::type Weights;
+            Weights wh[T::kF32 ? 1 : kN][kU], wl[T::kBf16 ? kN : 1][kU];
+#pragma unroll
+            for (int i = 0; i < kN; ++i) {
+                const unsigned long long seen = vis[i] >> (4 * g);
+                if (tail) {
+                    stay_a_branch();
+#pragma unroll
+                    for (int t = 0; t < kT; ++t)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) p[i][t][e] = (seen >> (16 * t + e)) & 1 ? p[i][t][e] : -INFINITY;
+                }
+                float top = p[i][0][0];
 #pragma unroll
                 for (int t = 0; t < kT; ++t)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) p[t][e] = (seen >> (16 * t + e)) & 1 ? p[t][e] : -INFINITY;
-            }
-            float top = p[0][0];
+                    for (int e = 0; e < 4; ++e) top = fmaxf(top, p[i][t][e]);
+                // Exponents are taken off a maximum that may lag behind by kSlack: weights up to 2^kSlack lose
+                // nothing, and after a wave's first tile this is rarely entered.
+                if (__any(top > limit[i])) {
+                    top = op_xor32<true>(op_xor16<true>(top));
+                    const float mn = fmaxf(m[i], top);
+                    const float f = weight_of(m[i], mn);
+                    m[i] = mn;
+                    off[i] = mn == -INFINITY ? 0.0f : mn;
+                    limit[i] = mn + kSlack;
+                    l[i] *= f;
 #pragma unroll
-            for (int t = 0; t < kT; ++t)
+                    for (int c = 0; c < 4; ++c) acc[i][c] *= f;
+                    if constexpr (T::kInt4) acc8[i] *= f;
+                }
 #pragma unroll
-                for (int e = 0; e < 4; ++e) top = fmaxf(top, p[t][e]);
-            // Exponents are taken off a maximum that may lag behind by kSlack: weights up to 2^kSlack lose
-            // nothing, and after a wave's first tile this is rarely entered.
-            if (__any(top > limit[i])) {
-                top = op_xor32<true>(op_xor16<true>(top));
-                const float mn = fmaxf(m[i], top);
-                const float f = weight_of(m[i], mn);
-                m[i] = mn;
-                off[i] = mn == -INFINITY ? 0.0f : mn;
-                limit[i] = mn + kSlack;
-                l[i] *= f;
+                for (int t = 0; t < kT; ++t) {
+                    F32x4 vs = {1.0f, 1.0f, 1.0f, 1.0f};
+                    if constexpr (T::kCoded) vs = *reinterpret_cast<const F32x4*>(ls + kPos + 16 * t + 4 * g);
 #pragma unroll
-                for (int c = 0; c < 4; ++c) acc[i][c] *= f;
-                if constexpr (T::kInt4) acc8[i] *= f;
-            }
-#pragma unroll
-            for (int t = 0; t < kT; ++t)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    // Not fused with the product that made the score: the largest one's difference is exact.
+                    for (int e = 0; e < 4; ++e) {
+                        // Not fused with the product that made the score: the largest one's difference is exact.
 #pragma clang fp contract(off)
-                    const float w = exp2_fast(p[t][e] - off[i]);
-                    l[i] += w;
-                    p[t][e] = w;
-                    if constexpr (T::kCoded) p[t][e] = w * vs[t][e];
+                        const float w = exp2_fast(p[i][t][e] - off[i]);
+                        l[i] += w;
+                        p[i][t][e] = T::kCoded ? w * vs[e] : w;
+                    }
                 }
-            if (T::kCoded && tail) {           // a row that is not seen may have any scale
-                stay_a_branch();
+                if (T::kCoded && tail) {       // a row that is not seen may have any scale
+                    stay_a_branch();
 #pragma unroll
-                for (int t = 0; t < kT; ++t)
+                    for (int t = 0; t < kT; ++t)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) p[t][e] = (seen >> (16 * t + e)) & 1 ? p[t][e] : 0.0f;
-            }
-            if (T::kMayBeInfinite && bad) {
-                stay_a_branch();
-                // Position 16 t + 4 gg + e: its weight of query col is in lane 16 gg + col.
+                        for (int e = 0; e < 4; ++e) p[i][t][e] = (seen >> (16 * t + e)) & 1 ? p[i][t][e] : 0.0f;
+                }
+                if (T::kMayBeInfinite && bad) {
+                    stay_a_branch();
+                    // The group's weights [query][position] in K's place, then position by position.
+                    static_assert(kQ * kPos * 4 <= kTileBytes || !T::kMayBeInfinite, "weights take K's place");
+                    float* const lp = reinterpret_cast<float*>(lk) + col * kPos;
+                    lds_order();
 #pragma unroll
-                for (int t = 0; t < kT; ++t)
+                    for (int t = 0; t < kT; ++t) *reinterpret_cast<F32x4*>(lp + 16 * t + 4 * g) = p[i][t];
+                    lds_order();
+#pragma unroll 1
+                    for (int row = 0; row < kPos; ++row) {
+                        const float w = lp[row];
+                        if ((vis[i] >> row) & 1) {
 #pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        for (int gg = 0; gg < 4; ++gg) {
-                            const int row = 16 * t + 4 * gg + e;
-                            const float w = __shfl(p[t][e], 16 * gg + col);
-                            if ((vis[i] >> row) & 1) {
+                            for (int c = 0; c < 4; ++c)
 #pragma unroll
-                                for (int c = 0; c < 4; ++c)
-#pragma unroll
-                                    for (int x = 0; x < 4; ++x)
-                                        acc[i][c][x] += w * element<T::kMayBeInfinite ? DT : KVATTN_KV_F32>(lv, row, 16 * c + 4 * g + x);
-                            }
+                                for (int x = 0; x < 4; ++x)
+                                    acc[i][c][x] += w * element<T::kMayBeInfinite ? DT : KVATTN_KV_F32>(lv, row, 16 * c + 4 * g + x);
                         }
-                continue;
+                    }
+                    lds_order();
+                } else if constexpr (T::kCoded) {
+#pragma unroll
+                    for (int u = 0; u < kU; ++u)
+#pragma unroll
+                        for (int x = 0; x < 8; ++x) wh[i][u][x] = (_Float16)p[i][2 * u + x / 4][x % 4];
+                } else if constexpr (T::kBf16) {
+#pragma unroll
+                    for (int u = 0; u < kU; ++u) {
+                        U32x4 hi, lo;
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {          // places 2 j and 2 j + 1
+                            const float p0 = p[i][2 * u + j / 2][2 * (j % 2)], p1 = p[i][2 * u + j / 2][2 * (j % 2) + 1];
+                            const uint32_t b0 = __float_as_uint(p0), b1 = __float_as_uint(p1);
+                            hi[j] = __builtin_amdgcn_perm(b1, b0, 0x07060302u);
+                            const float r0 = p0 - __uint_as_float(b0 & 0xffff0000u), r1 = p1 - __uint_as_float(b1 & 0xffff0000u);
+                            lo[j] = __builtin_amdgcn_perm(__float_as_uint(r1), __float_as_uint(r0), 0x07060302u);
+                        }
+                        wh[i][u] = __builtin_bit_cast(Bf16x8, hi);
+                        wl[i][u] = __builtin_bit_cast(Bf16x8, lo);
+                    }
+                }
             }
+            if (T::kMayBeInfinite && bad) return;
+            // V's operands, transposed: step u's places of channels 16 c + col.
             if constexpr (T::kF32) {
 #pragma unroll
                 for (int t = 0; t < kT; ++t)
@@ -462,35 +485,62 @@ __global__ __launch_bounds__(kW * kWave) __attribute__((amdgpu_waves_per_eu(2)))
                         for (int c = 0; c < 4; ++c) {
                             const float v = *reinterpret_cast<const float*>(lv + row * T::kRow + 16 * T::chunk_at(row, 4 * c + (col >> 2)) +
                                                                             4 * (col & 3));
-                            acc[i][c] = __builtin_amdgcn_mfma_f32_16x16x4f32(v, p[t][e], acc[i][c], 0, 0, 0);
+#pragma unroll
+                            for (int i = 0; i < kN; ++i) acc[i][c] = __builtin_amdgcn_mfma_f32_16x16x4f32(v, p[i][t][e], acc[i][c], 0, 0, 0);
                         }
                     }
             } else {
-                const Bf16x8 eight = (Bf16x8)(__bf16)8.0f;
+                if constexpr (T::kInt4) {
 #pragma unroll
-                for (int u = 0; u < kU; ++u) {
-                    U32x4 hi, lo;
+                    for (int i = 0; i < kN; ++i)
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {              // places 2 j and 2 j + 1
-                        const float p0 = p[2 * u + j / 2][2 * (j % 2)], p1 = p[2 * u + j / 2][2 * (j % 2) + 1];
-                        const uint32_t b0 = __float_as_uint(p0), b1 = __float_as_uint(p1);
-                        hi[j] = __builtin_amdgcn_perm(b1, b0, 0x07060302u);
-                        const float r0 = p0 - __uint_as_float(b0 & 0xffff0000u), r1 = p1 - __uint_as_float(b1 & 0xffff0000u);
-                        lo[j] = __builtin_amdgcn_perm(__float_as_uint(r1), __float_as_uint(r0), 0x07060302u);
-                    }
-                    const Bf16x8 ph = __builtin_bit_cast(Bf16x8, hi), pl = __builtin_bit_cast(Bf16x8, lo);
+                        for (int u = 0; u < kU; ++u) acc8[i] = mfma((F16x8)(_Float16)8.0f, wh[i][u], acc8[i]);
+                }
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        acc[i][c] = mfma(va[c][u], ph, acc[i][c]);
-                        acc[i][c] = mfma(va[c][u], pl, acc[i][c]);
+                for (int c = 0; c < 4; ++c) {
+                    Weights va[kU];
+                    if constexpr (T::kBf16) {
+                        typedef short S16x4 __attribute__((ext_vector_type(4)));
+#pragma unroll
+                        for (int u = 0; u < kU; ++u) {
+                            S16x4 part[2];
+#pragma unroll
+                            for (int e = 0; e < 2; ++e) {
+                                const int row = 32 * u + 16 * e + 4 * g + (col >> 2);
+                                part[e] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                    (__attribute__((address_space(3))) S16x4*)(lv + row * T::kRow +
+                                        16 * T::chunk_at(row, 2 * c + ((col >> 1) & 1)) + 8 * (col & 1)));
+                            }
+                            va[u] = __builtin_bit_cast(Bf16x8, __builtin_shufflevector(part[0], part[1], 0, 1, 2, 3, 4, 5, 6, 7));
+                        }
+                    } else if constexpr (T::k8) {
+#pragma unroll
+                        for (int u = 0; u < 2; ++u) {
+                            const int e = col >> 1, row = 32 * u + 16 * (e >> 2) + 4 * g + (e & 3);
+                            const I32x2 w = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
+                                (__attribute__((address_space(3))) I32x2*)(lv + row * T::kRow + 16 * T::chunk_at(row, c) + 8 * (col & 1)));
+                            va[u] = codes_to_f16<T::kFp8>((uint32_t)w[0], (uint32_t)w[1]);
+                        }
+                    } else {
+                        const int e = place<T::kFp4>(col & 7), row = 32 * (col >> 3) + 16 * (e >> 2) + 4 * g + (e & 3);
+                        const I32x2 w = __builtin_amdgcn_ds_read_tr4_b64_v2i32(
+                            (__attribute__((address_space(3))) I32x2*)(lv + row * T::kRow + 8 * c));
+                        va[0] = operand16<T::kFp4>((uint32_t)w[0]);
+                        va[1] = operand16<T::kFp4>((uint32_t)w[1]);
                     }
-                    if constexpr (T::kInt4) {
-                        acc8[i] = mfma(eight, ph, acc8[i]);
-                        acc8[i] = mfma(eight, pl, acc8[i]);
-                    }
+#pragma unroll
+                    for (int i = 0; i < kN; ++i)
+#pragma unroll
+                        for (int u = 0; u < kU; ++u) {
+                            acc[i][c] = mfma(va[u], wh[i][u], acc[i][c]);
+                            if constexpr (T::kBf16) acc[i][c] = mfma(va[u], wl[i][u], acc[i][c]);
+                        }
+                    if constexpr (kN > 1) lds_order();     // (else all of it is read ahead, into registers that are not there)
                 }
             }
-        }
+        };
+        if (kG == 1 || ng == 1) work(std::integral_constant<int, 1>{});
+        else work(std::integral_constant<int, kG>{});
         lds_order();
     }
 
@@ -506,6 +556,7 @@ __global__ __launch_bounds__(kW * kWave) __attribute__((amdgpu_waves_per_eu(2)))
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
             if constexpr (T::kInt4) acc[i][c] -= acc8[i];
+            if constexpr (T::kCoded) acc[i][c] *= unit * 0.03125f;
             *reinterpret_cast<F32x4*>(ro + col * kOutPad + 16 * c + 4 * g) = acc[i][c];
         }
         const float sum = op_xor32<false>(op_xor16<false>(l[i]));
@@ -528,17 +579,10 @@ __global__ __launch_bounds__(kW * kWave) __attribute__((amdgpu_waves_per_eu(2)))
             }
             const size_t head = (tok0 + kQ * i + qq) * a.NH + h;
             if (segs == 1) {
-                o = L == 0.0f ? F32x4{0.0f, 0.0f, 0.0f, 0.0f} : o / L;
-                if constexpr (T::kF32) {
-                    *reinterpret_cast<F32x4*>(a.out + (head * kHd + ch) * 4) = o;
-                } else {
-                    *reinterpret_cast<uint2*>(a.out + (head * kHd + ch) * 2) =
-                        make_uint2(f32_to_bf16(o[0]) | (uint32_t)f32_to_bf16(o[1]) << 16, f32_to_bf16(o[2]) | (uint32_t)f32_to_bf16(o[3]) << 16);
-                }
+                store_out<T::kF32>(a.out, head * kHd + ch, L, o);
             } else {
                 const size_t slot = head * a.S + s;
-#pragma unroll
-                for (int x = 0; x < kVec; ++x) put(a.part_out + slot * kHd + ch + x, o[x]);
+                put4(a.part_out + slot * kHd + ch, o);
                 if (ch == 0) {
                     put(a.part_max + slot, M);
                     put(a.part_lse + slot, L);
@@ -593,26 +637,14 @@ __global__ __launch_bounds__(kW * kWave) __attribute__((amdgpu_waves_per_eu(2)))
             }
             M = top;
         }
-        o = L == 0.0f ? F32x4{0.0f, 0.0f, 0.0f, 0.0f} : o / L;
-        if constexpr (T::kF32) {
-            *reinterpret_cast<F32x4*>(a.out + (head * kHd + ch) * 4) = o;
-        } else {
-            *reinterpret_cast<uint2*>(a.out + (head * kHd + ch) * 2) =
-                make_uint2(f32_to_bf16(o[0]) | (uint32_t)f32_to_bf16(o[1]) << 16, f32_to_bf16(o[2]) | (uint32_t)f32_to_bf16(o[3]) << 16);
-        }
+        store_out<T::kF32>(a.out, head * kHd + ch, L, o);
     }
 }
 
-// Groups of 16 queries that a workgroup holds at most: the registers of FP32 rows leave room for two.
-template <int DT> constexpr int kMostGroups = Kv<DT>::kF32 ? 2 : 4;
-
 template <int DT>
-const void* kernel_for(int groups) {
-    constexpr int kWide = Kv<DT>::kF32 ? 32 : 64;      // positions of a tile where registers allow
-    if (groups == 1) return (const void*)&tree_kernel<DT, 1, 4, kWide>;
-    if (groups == 2) return (const void*)&tree_kernel<DT, 2, 4, kWide>;
-    if constexpr (kMostGroups<DT> >= 4) return (const void*)&tree_kernel<DT, 4, 4, Kv<DT>::kBf16 ? 32 : 64>;
-    return nullptr;
+const void* kernel_for(int queries, int waves) {
+    if (waves == 8) return queries == kQ ? (const void*)&tree_kernel<DT, 1, 8> : (const void*)&tree_kernel<DT, 2, 8>;
+    return queries == kQ ? (const void*)&tree_kernel<DT, 1, 4> : (const void*)&tree_kernel<DT, 2, 4>;
 }
 
 // ------------------------------------------------------------------------------------
@@ -678,12 +710,22 @@ namespace kvattn_internal {
 
 int attend_tree(const AttendTree& c) {
     const int most_new = std::min(c.max_new, c.num_tokens);
-    const int most_groups = c.kv_dtype == KVATTN_KV_F32 ? kMostGroups<KVATTN_KV_F32> : kMostGroups<KVATTN_KV_BF16>;
-    const int want = (most_new + kQ - 1) / kQ;
-    const int groups = std::min(most_groups, want <= 2 ? want : 4);
-    const int passes = (want + groups - 1) / groups;
+    const int queries = most_new <= kQ ? kQ : 2 * kQ;      // of a workgroup
+    const int passes = (most_new + queries - 1) / queries;
     const long long heads = (long long)c.B * c.NH * passes;
-    constexpr int kWaves = 4;
+    // Workgroups of 8 waves where there are few; else 4, in segments of one length (maxT over their number, so that a short
+    // sequence has fewer) that make as many workgroups as run at once, none shorter than 256 positions (8 waves over codes:
+    // 1024, a tile each for two rounds).  us per call, positions of a segment : us:
+    //   BF16  1 x 12 heads of 1000, 26 tokens   8 waves 256: 9.7, 512: 10.8, one 10.6; 4 waves 256: 10.4, one 13.2
+    //   BF16  1 x 12 of 8000, 16                8 waves 512: 11.4, 1024: 10.9, 256: 14.8; 4 waves 512: 11.3
+    //   FP4   1 x 12 of 1000, 7                 8 waves one 6.4, 256: 7.6; 4 waves one 7.0
+    //   FP8   3 x 25 of 1999, 7                 4 waves 256: 9.4, 512: 10.1, one 13.1; 8 waves one 10.4
+    //   BF16  8 x 12 ragged of up to 2048, 16   4 waves 256: 9.3, 512: 10.2, one 14.2; 8 waves 11
+    //   INT8  8 x 12 ragged of up to 4096, 64   4 waves 1024: 20.6, 512: 24.5, 2048: 23.2; 8 waves one 24.7
+    //   INT4 24 x 12 ragged of up to 4096, 32   4 waves 2048: 24.1, one 26.5, 1024: 28.6; 8 waves one 23.0
+    //   BF16 16 x 12 ragged of up to 8192, 64   4 waves 2048: 46.2, 4096: 47.8, one 72; 8 waves one 47.4
+    //   FP8  64 x 12 ragged of up to 1024, 16   4 waves one 16.4, 512: 24
+    const int waves = heads <= kFewHeads ? 8 : 4;
     const int tiles = (c.maxT + kSeg - 1) / kSeg;
     int S = 1, seg_tiles = 1;
     if (c.S > 0) {
@@ -695,10 +737,12 @@ int attend_tree(const AttendTree& c) {
         S = (tiles + seg_tiles - 1) / seg_tiles;
         if (S > kMaxSegments) return KVATTN_ERR_SPLIT;
     } else {
-        seg_tiles = 8;
-        S = (int)std::max<long long>(1, std::min<long long>({2 * kCUs / heads, (tiles + seg_tiles - 1) / seg_tiles, kMaxSegments}));
+        const bool coded = c.kv_dtype != KVATTN_KV_F32 && c.kv_dtype != KVATTN_KV_BF16;
+        const int least = waves == 8 && coded ? 16 : 4;
+        S = (int)std::max<long long>(1, std::min<long long>({3 * kCUs / heads, (tiles + least - 1) / least, 16}));
+        seg_tiles = (tiles + S - 1) / S;
     }
-    if (c.B > 65535 || heads * S * kWaves > kMostWaves) return KVATTN_ERR_SHAPE;
+    if (c.B > 65535 || heads * S * waves > kMostWaves) return KVATTN_ERR_SHAPE;
     TreeArgs a{};
     if (S > 1) {
         if (!c.ws) return KVATTN_ERR_WORKSPACE;
@@ -731,15 +775,15 @@ int attend_tree(const AttendTree& c) {
     a.num_tokens = c.num_tokens;
     const void* fn = nullptr;
     switch (c.kv_dtype) {
-        case KVATTN_KV_F32: fn = kernel_for<KVATTN_KV_F32>(groups); break;
-        case KVATTN_KV_BF16: fn = kernel_for<KVATTN_KV_BF16>(groups); break;
-        case KVATTN_KV_INT8: fn = kernel_for<KVATTN_KV_INT8>(groups); break;
-        case KVATTN_KV_FP8_E4M3: fn = kernel_for<KVATTN_KV_FP8_E4M3>(groups); break;
-        case KVATTN_KV_INT4: fn = kernel_for<KVATTN_KV_INT4>(groups); break;
-        default: fn = kernel_for<KVATTN_KV_FP4_E2M1>(groups); break;
+        case KVATTN_KV_F32: fn = kernel_for<KVATTN_KV_F32>(queries, waves); break;
+        case KVATTN_KV_BF16: fn = kernel_for<KVATTN_KV_BF16>(queries, waves); break;
+        case KVATTN_KV_INT8: fn = kernel_for<KVATTN_KV_INT8>(queries, waves); break;
+        case KVATTN_KV_FP8_E4M3: fn = kernel_for<KVATTN_KV_FP8_E4M3>(queries, waves); break;
+        case KVATTN_KV_INT4: fn = kernel_for<KVATTN_KV_INT4>(queries, waves); break;
+        default: fn = kernel_for<KVATTN_KV_FP4_E2M1>(queries, waves); break;
     }
     void* params[] = {&a};
-    return hip_status(hipLaunchKernel(fn, dim3(c.NH * passes, c.B, S), dim3(kWaves * kWave), params, 0, (hipStream_t)c.stream));
+    return hip_status(hipLaunchKernel(fn, dim3(c.NH * passes, c.B, S), dim3(waves * kWave), params, 0, (hipStream_t)c.stream));
 }
 
 }  // namespace kvattn_internal

@@ -91,8 +91,11 @@ def attend(q, k, v, seen, kscale, vscale, kv):
     Scores: 64 products, exact for bf16 q and codes, a float rounding each for F32, summed in float in any order: 70
     roundings of 2^-24 of the sum of magnitudes, in which an INT4 code counts 15 + 8 (the operand adds 8, and -8 times
     the sum of q starts the sum); two roundings of the scale's product; the exponent's difference rounds once more.  A
-    weight is exp2 of that (2^-22 for the instruction), cut to two bf16 halves (2^-14).  Sums: a rounding for each
-    32 rows of a product, the joins of waves and segments, the total's division; then half a step of the output."""
+    weight is exp2 of that (2^-22 for the instruction); over BF16 rows it is cut to two bf16 halves (2^-14), over codes its
+    product with the row's scale is rounded to float16: half a step, 2^-11 of it (float16 keeps 10 bits behind the first),
+    or, below 2^-14 in the wave's unit, 2^-25: the unit is the largest scale over 32 to 128, so 2^-18 of w times that
+    scale over the codes.  Sums: a rounding for each 32 rows of a product, the joins of waves and segments, the total's
+    division; then half a step of the output."""
     n = len(seen)
     if n == 0:
         return np.zeros(HS), np.full(HS, 2.0 ** -126)
@@ -104,7 +107,7 @@ def attend(q, k, v, seen, kscale, vscale, kv):
     more = 23.0 if kv == "int4" else 0.0
     mag = (np.abs(k) @ np.abs(q)).max() + more * np.abs(q).sum() * (kscale[seen].max() if more else 0.0)
     es = 2 * 74 * 2.0 ** -24 * mag * 0.125 * LOG2E
-    rel_w = (0.0 if kv == "f32" else 2.0 ** -14) + 2.0 ** -21 + 2 * math.log(2) * es
+    rel_w = {"f32": 0.0, "bf16": 2.0 ** -14}.get(kv, 2.0 ** -11) + 2.0 ** -21 + 2 * math.log(2) * es
     size = np.abs(v).max() + more * (vscale[seen].max() if more else 0.0)
     steps = (n / 4 + 24) * 2.0 ** -24 if kv == "f32" else (n / 32 + 24) * 2.0 ** -24
     half = HALF_STEP["f32" if kv == "f32" else "bf16"]
