@@ -2,8 +2,11 @@
 // type, and the trees' masks.
 //
 // A sequence's n new tokens are nodes of a tree; their K and V rows are the cache's last n.  Token i attends the
-// prefix before them and the new tokens whose bits its mask has (itself and its ancestors).  So a pass over the
-// cache serves all of a tree's tokens: up to 64 of them share a workgroup's tile of 64 positions.
+// prefix before them and the new tokens whose bits its mask has (itself and its ancestors).  A workgroup serves 16 of a
+// tree's tokens, the columns of a product; those of larger trees run side by side, so that what one loads the others
+// find in the caches.  (Two or four groups of 16 in one workgroup take registers that other workgroups hide latency
+// with: BF16, 26 tokens over 1000 positions 9.6 us in place of 7.6, INT4 64 x 64 tokens 43.4 and 41.0, 16 x 64 over
+// 8192 46.0 and 46.6.)
 //
 // Both products go to the matrix cores, scores as S^T = K Q^T and outputs as O^T = V^T P^T.  Of S^T lane
 // 16 g + c holds positions 16 t + 4 g .. + 3 of query c.  That makes everything the softmax does (maximum, sum,
@@ -139,9 +142,9 @@ __device__ __forceinline__ void store_out(uint8_t* out, size_t at, float L, F32x
     }
 }
 
-// kG: groups of 16 queries a workgroup may hold; kW: its waves.
-template <int DT, int kG, int kW>
-__global__ __launch_bounds__(kW * kWave) __attribute__((amdgpu_waves_per_eu(kG == 1 ? 3 : 2))) void tree_kernel(TreeArgs a) {
+// kW: waves of a workgroup.
+template <int DT, int kW>
+__global__ __launch_bounds__(kW * kWave) __attribute__((amdgpu_waves_per_eu(3))) void tree_kernel(TreeArgs a) {
     using T = Kv<DT>;
     constexpr int kPos = T::kPos, kT = kPos / 16;              // positions of a wave's tile, groups of 16 of them
     constexpr int kTileBytes = kPos * T::kRow;
@@ -158,9 +161,9 @@ __global__ __launch_bounds__(kW * kWave) __attribute__((amdgpu_waves_per_eu(kG =
     const int t0 = min(max(a.start[b], 0), a.num_tokens);
     const int n = min(max(a.start[b + 1], t0), a.num_tokens) - t0;
     const int total = min(max(a.lens[b], 0), a.maxT);
-    const int q0 = grp * kQ * kG;
+    const int q0 = grp * kQ;
     if (q0 >= n) return;
-    const int nq = min(kQ * kG, n - q0), ng = (nq + kQ - 1) / kQ;
+    const int nq = min(kQ, n - q0);
     const int base = total - n;                                // position of new token 0
     const int seg_count = (total + kSeg - 1) / kSeg;
     int segs = 1, seg_tiles = seg_count;
@@ -218,49 +221,37 @@ __global__ __launch_bounds__(kW * kWave) __attribute__((amdgpu_waves_per_eu(kG =
         }
     };
 
-    // Queries: column c is query c of a group (the last one again past it), in the order of K's operands.
+    // Queries: column c is query c (the last one again past it), in the order of K's operands.
     constexpr int kQu = T::kF32 ? 4 : 2;                       // 16-byte pieces of a lane
-    uint4 qw[kG][kQu];
+    const size_t my_tok = (size_t)t0 + q0 + min(col, nq - 1);
+    const unsigned long long* const my_mask = a.masks + my_tok * a.words;
+    uint4 qw[kQu];
 #pragma unroll
-    for (int i = 0; i < kG; ++i) {
-        const size_t tok = t0 + q0 + min(kQ * i + col, nq - 1);
-        const uint8_t* const qp = a.qkv + (tok * 3 * a.NH + h) * kHd * (T::kF32 ? 4 : 2);
-#pragma unroll
-        for (int u = 0; u < kQu; ++u)
-            qw[i][u] = *reinterpret_cast<const uint4*>(qp + (T::kCoded ? 32 * g + 16 * u : 64 * u + 16 * g));
-    }
+    for (int u = 0; u < kQu; ++u)
+        qw[u] = *reinterpret_cast<const uint4*>(a.qkv + (my_tok * 3 * a.NH + h) * kHd * (T::kF32 ? 4 : 2) +
+                                                (T::kCoded ? 32 * g + 16 * u : 64 * u + 16 * g));
     if (mine > 0) request(0);
-    unsigned long long mask0[kG];          // the first word of each query's mask
-#pragma unroll
-    for (int i = 0; i < kG; ++i) mask0[i] = a.masks[(size_t)(t0 + q0 + min(kQ * i + col, nq - 1)) * a.words];
-    Bf16x8 qa[kG][2];
-    float q_init[kG] = {};                 // INT4: the operand's codes are 8 too large, so a score starts at -8 sum q
+    const unsigned long long mask0 = my_mask[0];
+    Bf16x8 qa[2];
+    float q_init = 0.0f;                   // INT4: the operand's codes are 8 too large, so a score starts at -8 sum q
     if constexpr (!T::kF32) {
-        const Bf16x8 minus8 = (Bf16x8)(__bf16)(-8.0f);
 #pragma unroll
-        for (int i = 0; i < kG; ++i) {
-#pragma unroll
-            for (int u = 0; u < 2; ++u)
-                qa[i][u] = T::kInt4 ? in_order<false>(qw[i][u]) : __builtin_bit_cast(Bf16x8, qw[i][u]);
-            if constexpr (T::kInt4) {
-                const F32x4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
-                q_init[i] = mfma(minus8, qa[i][1], mfma(minus8, qa[i][0], zero))[0];
-            }
+        for (int u = 0; u < 2; ++u) qa[u] = T::kInt4 ? in_order<false>(qw[u]) : __builtin_bit_cast(Bf16x8, qw[u]);
+        if constexpr (T::kInt4) {
+            const Bf16x8 minus8 = (Bf16x8)(__bf16)(-8.0f);
+            const F32x4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
+            q_init = mfma(minus8, qa[1], mfma(minus8, qa[0], zero))[0];
         }
     }
 
     uint8_t* const lk = lds + wave * kWaveLds;
     uint8_t* const lv = lk + kTileBytes;
     float* const ls = reinterpret_cast<float*>(lv + kTileBytes);
-    F32x4 acc[kG][4] = {};                 // channels 16 c + 4 g + i of query col
-    F32x4 acc8[kG] = {};                   // INT4: 8 sum of the weights, taken off at the end
+    F32x4 acc[4] = {};                     // channels 16 c + 4 g + i of query col
+    F32x4 acc8 = {};                       // INT4: 8 sum of the weights, taken off at the end
     float unit = 0.0f, per_unit = 0.0f;    // codes: of the weights
-    float m[kG], off[kG], limit[kG], l[kG];
-#pragma unroll
-    for (int i = 0; i < kG; ++i) {
-        m[i] = limit[i] = -INFINITY;
-        off[i] = l[i] = 0.0f;
-    }
+    // off: what the exponents are taken off (zero before the first score); limit: the score from which m follows.
+    float m = -INFINITY, limit = -INFINITY, off = 0.0f, l = 0.0f;
 
     for (int k = 0; k < mine; ++k) {
         const int pos = pos_of(k);
@@ -294,11 +285,8 @@ __global__ __launch_bounds__(kW * kWave) __attribute__((amdgpu_waves_per_eu(kG =
                 unit = grown;
                 per_unit = __uint_as_float((uint32_t)(259 - e) << 23);      // 32 / unit
 #pragma unroll
-                for (int i = 0; i < kG; ++i) {
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) acc[i][c] *= f;
-                    if constexpr (T::kInt4) acc8[i] *= f;
-                }
+                for (int c = 0; c < 4; ++c) acc[c] *= f;
+                if constexpr (T::kInt4) acc8 *= f;
             }
             ls[lane] = rks * kQScale;
             ls[kPos + lane] = rvs * per_unit;
@@ -307,286 +295,235 @@ __global__ __launch_bounds__(kW * kWave) __attribute__((amdgpu_waves_per_eu(kG =
         if (k + 1 < mine) request(k + 1);
         if (!here) continue;                   // its page is not in the pool
 
-        // Positions that a query of each group sees, one bit each.
-        unsigned long long vis[kG];
-#pragma unroll
-        for (int i = 0; i < kG; ++i) vis[i] = ~0ull;
+        // Positions that the query sees, one bit each.
+        unsigned long long vis = ~0ull;
         if (tail) {
             stay_a_branch();
             const int d = pos - base, w0 = d >> 6, sh = d & 63;      // (d may be negative: words before the first are the prefix)
             const int left = total - pos;
-            const unsigned long long live = left >= 64 ? ~0ull : (1ull << left) - 1;
-#pragma unroll
-            for (int i = 0; i < kG; ++i) {
-                const size_t tok = t0 + q0 + min(kQ * i + col, nq - 1);
-                const unsigned long long* const mp = a.masks + tok * a.words;
-                auto word = [&](int w) { return w < 0 ? ~0ull : w == 0 ? mask0[i] : w < a.words ? mp[w] : 0ull; };
-                unsigned long long v = word(w0) >> sh;
-                if (sh) v |= word(w0 + 1) << (64 - sh);
-                vis[i] = v & live;
-            }
+            auto word = [&](int w) { return w < 0 ? ~0ull : w == 0 ? mask0 : w < a.words ? my_mask[w] : 0ull; };
+            vis = word(w0) >> sh;
+            if (sh) vis |= word(w0 + 1) << (64 - sh);
+            vis &= left >= 64 ? ~0ull : (1ull << left) - 1;
         }
+        const unsigned long long seen = vis >> (4 * g);
 
-        // The tile's work for kN groups: K's operands meet every group's queries as they are read, V's every group's
-        // weights, so that neither is held.
-        auto work = [&](auto groups) {
-            constexpr int kN = decltype(groups)::value, kU = kPos >= 32 ? kPos / 32 : 1;      // steps of 32 positions
-            F32x4 p[kN][kT];
+        // Scores.
+        F32x4 p[kT];
 #pragma unroll
-            for (int t = 0; t < kT; ++t) {
-                const int row = 16 * t + col;
-#pragma unroll
-                for (int i = 0; i < kN; ++i) p[i][t] = F32x4{q_init[i], q_init[i], q_init[i], q_init[i]};
-                if constexpr (T::kF32) {
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const U32x4 kf = *reinterpret_cast<const U32x4*>(lk + row * T::kRow + 16 * T::chunk_at(row, 4 * j + g));
-#pragma unroll
-                        for (int i = 0; i < kN; ++i) {
-                            const uint32_t qv[4] = {qw[i][j].x, qw[i][j].y, qw[i][j].z, qw[i][j].w};
-#pragma unroll
-                            for (int e = 0; e < 4; ++e)
-                                p[i][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kf[e]), __uint_as_float(qv[e]), p[i][t], 0, 0, 0);
-                        }
-                    }
-                } else {
-                    Bf16x8 ka[2];
-                    if constexpr (T::kBf16) {
-#pragma unroll
-                        for (int u = 0; u < 2; ++u)
-                            ka[u] = *reinterpret_cast<const Bf16x8*>(lk + row * T::kRow + 16 * T::chunk_at(row, 4 * u + g));
-                    } else if constexpr (T::k8) {
-                        codes_to_bf16<T::kFp8>(*reinterpret_cast<const U32x4*>(lk + row * T::kRow + 16 * T::chunk_at(row, g)), ka);
-                    } else {
-                        const uint2 w = *reinterpret_cast<const uint2*>(lk + row * T::kRow + 8 * g);
-                        ka[0] = operand<T::kFp4>(w.x);
-                        ka[1] = operand<T::kFp4>(w.y);
-                    }
-#pragma unroll
-                    for (int i = 0; i < kN; ++i) {
-                        p[i][t] = mfma(ka[0], qa[i][0], p[i][t]);
-                        p[i][t] = mfma(ka[1], qa[i][1], p[i][t]);
-                    }
-                }
-                if constexpr (T::kCoded) {
-                    const F32x4 ks = *reinterpret_cast<const F32x4*>(ls + 16 * t + 4 * g);
-#pragma unroll
-                    for (int i = 0; i < kN; ++i) p[i][t] *= ks;
-                } else {
-#pragma unroll
-                    for (int i = 0; i < kN; ++i) p[i][t] *= kQScale;
-                }
-                if constexpr (kN > 1) lds_order();     // (else all of it is read ahead, into registers that are not there)
-            }
-            // Softmax; the weights as operands (F32: in place).
-            typedef typename std::conditional<T::kCoded, F16x8, Bf16x8>::type Weights;
-            Weights wh[T::kF32 ? 1 : kN][kU], wl[T::kBf16 ? kN : 1][kU];
-#pragma unroll
-            for (int i = 0; i < kN; ++i) {
-                const unsigned long long seen = vis[i] >> (4 * g);
-                if (tail) {
-                    stay_a_branch();
-#pragma unroll
-                    for (int t = 0; t < kT; ++t)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) p[i][t][e] = (seen >> (16 * t + e)) & 1 ? p[i][t][e] : -INFINITY;
-                }
-                float top = p[i][0][0];
-#pragma unroll
-                for (int t = 0; t < kT; ++t)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) top = fmaxf(top, p[i][t][e]);
-                // Exponents are taken off a maximum that may lag behind by kSlack: weights up to 2^kSlack lose
-                // nothing, and after a wave's first tile this is rarely entered.
-                if (__any(top > limit[i])) {
-                    top = op_xor32<true>(op_xor16<true>(top));
-                    const float mn = fmaxf(m[i], top);
-                    const float f = weight_of(m[i], mn);
-                    m[i] = mn;
-                    off[i] = mn == -INFINITY ? 0.0f : mn;
-                    limit[i] = mn + kSlack;
-                    l[i] *= f;
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) acc[i][c] *= f;
-                    if constexpr (T::kInt4) acc8[i] *= f;
-                }
-#pragma unroll
-                for (int t = 0; t < kT; ++t) {
-                    F32x4 vs = {1.0f, 1.0f, 1.0f, 1.0f};
-                    if constexpr (T::kCoded) vs = *reinterpret_cast<const F32x4*>(ls + kPos + 16 * t + 4 * g);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        // Not fused with the product that made the score: the largest one's difference is exact.
-#pragma clang fp contract(off)
-                        const float w = exp2_fast(p[i][t][e] - off[i]);
-                        l[i] += w;
-                        p[i][t][e] = T::kCoded ? w * vs[e] : w;
-                    }
-                }
-                if (T::kCoded && tail) {       // a row that is not seen may have any scale
-                    stay_a_branch();
-#pragma unroll
-                    for (int t = 0; t < kT; ++t)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) p[i][t][e] = (seen >> (16 * t + e)) & 1 ? p[i][t][e] : 0.0f;
-                }
-                if (T::kMayBeInfinite && bad) {
-                    stay_a_branch();
-                    // The group's weights [query][position] in K's place, then position by position.
-                    static_assert(kQ * kPos * 4 <= kTileBytes || !T::kMayBeInfinite, "weights take K's place");
-                    float* const lp = reinterpret_cast<float*>(lk) + col * kPos;
-                    lds_order();
-#pragma unroll
-                    for (int t = 0; t < kT; ++t) *reinterpret_cast<F32x4*>(lp + 16 * t + 4 * g) = p[i][t];
-                    lds_order();
-#pragma unroll 1
-                    for (int row = 0; row < kPos; ++row) {
-                        const float w = lp[row];
-                        if ((vis[i] >> row) & 1) {
-#pragma unroll
-                            for (int c = 0; c < 4; ++c)
-#pragma unroll
-                                for (int x = 0; x < 4; ++x)
-                                    acc[i][c][x] += w * element<T::kMayBeInfinite ? DT : KVATTN_KV_F32>(lv, row, 16 * c + 4 * g + x);
-                        }
-                    }
-                    lds_order();
-                } else if constexpr (T::kCoded) {
-#pragma unroll
-                    for (int u = 0; u < kU; ++u)
-#pragma unroll
-                        for (int x = 0; x < 8; ++x) wh[i][u][x] = (_Float16)p[i][2 * u + x / 4][x % 4];
-                } else if constexpr (T::kBf16) {
-#pragma unroll
-                    for (int u = 0; u < kU; ++u) {
-                        U32x4 hi, lo;
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) {          // places 2 j and 2 j + 1
-                            const float p0 = p[i][2 * u + j / 2][2 * (j % 2)], p1 = p[i][2 * u + j / 2][2 * (j % 2) + 1];
-                            const uint32_t b0 = __float_as_uint(p0), b1 = __float_as_uint(p1);
-                            hi[j] = __builtin_amdgcn_perm(b1, b0, 0x07060302u);
-                            const float r0 = p0 - __uint_as_float(b0 & 0xffff0000u), r1 = p1 - __uint_as_float(b1 & 0xffff0000u);
-                            lo[j] = __builtin_amdgcn_perm(__float_as_uint(r1), __float_as_uint(r0), 0x07060302u);
-                        }
-                        wh[i][u] = __builtin_bit_cast(Bf16x8, hi);
-                        wl[i][u] = __builtin_bit_cast(Bf16x8, lo);
-                    }
-                }
-            }
-            if (T::kMayBeInfinite && bad) return;
-            // V's operands, transposed: step u's places of channels 16 c + col.
+        for (int t = 0; t < kT; ++t) {
+            const int row = 16 * t + col;
+            p[t] = F32x4{q_init, q_init, q_init, q_init};
             if constexpr (T::kF32) {
 #pragma unroll
-                for (int t = 0; t < kT; ++t)
+                for (int j = 0; j < 4; ++j) {
+                    const U32x4 kf = *reinterpret_cast<const U32x4*>(lk + row * T::kRow + 16 * T::chunk_at(row, 4 * j + g));
+                    const uint32_t qv[4] = {qw[j].x, qw[j].y, qw[j].z, qw[j].w};
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const int row = 16 * t + 4 * g + e;
-#pragma unroll
-                        for (int c = 0; c < 4; ++c) {
-                            const float v = *reinterpret_cast<const float*>(lv + row * T::kRow + 16 * T::chunk_at(row, 4 * c + (col >> 2)) +
-                                                                            4 * (col & 3));
-#pragma unroll
-                            for (int i = 0; i < kN; ++i) acc[i][c] = __builtin_amdgcn_mfma_f32_16x16x4f32(v, p[i][t][e], acc[i][c], 0, 0, 0);
-                        }
-                    }
+                    for (int e = 0; e < 4; ++e)
+                        p[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kf[e]), __uint_as_float(qv[e]), p[t], 0, 0, 0);
+                }
             } else {
-                if constexpr (T::kInt4) {
+                Bf16x8 ka[2];
+                if constexpr (T::kBf16) {
 #pragma unroll
-                    for (int i = 0; i < kN; ++i)
+                    for (int u = 0; u < 2; ++u)
+                        ka[u] = *reinterpret_cast<const Bf16x8*>(lk + row * T::kRow + 16 * T::chunk_at(row, 4 * u + g));
+                } else if constexpr (T::k8) {
+                    codes_to_bf16<T::kFp8>(*reinterpret_cast<const U32x4*>(lk + row * T::kRow + 16 * T::chunk_at(row, g)), ka);
+                } else {
+                    const uint2 w = *reinterpret_cast<const uint2*>(lk + row * T::kRow + 8 * g);
+                    ka[0] = operand<T::kFp4>(w.x);
+                    ka[1] = operand<T::kFp4>(w.y);
+                }
+                p[t] = mfma(ka[0], qa[0], p[t]);
+                p[t] = mfma(ka[1], qa[1], p[t]);
+            }
+            if constexpr (T::kCoded) p[t] *= *reinterpret_cast<const F32x4*>(ls + 16 * t + 4 * g);
+            else p[t] *= kQScale;
+        }
+        if (tail) {
+            stay_a_branch();
 #pragma unroll
-                        for (int u = 0; u < kU; ++u) acc8[i] = mfma((F16x8)(_Float16)8.0f, wh[i][u], acc8[i]);
+            for (int t = 0; t < kT; ++t)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) p[t][e] = (seen >> (16 * t + e)) & 1 ? p[t][e] : -INFINITY;
+        }
+        float top = p[0][0];
+#pragma unroll
+        for (int t = 0; t < kT; ++t)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) top = fmaxf(top, p[t][e]);
+        // Exponents are taken off a maximum that may lag behind by kSlack: weights up to 2^kSlack lose
+        // nothing, and after a wave's first tile this is rarely entered.
+        if (__any(top > limit)) {
+            top = op_xor32<true>(op_xor16<true>(top));
+            const float mn = fmaxf(m, top), f = weight_of(m, mn);
+            m = mn;
+            off = mn == -INFINITY ? 0.0f : mn;
+            limit = mn + kSlack;
+            l *= f;
+#pragma unroll
+            for (int c = 0; c < 4; ++c) acc[c] *= f;
+            if constexpr (T::kInt4) acc8 *= f;
+        }
+        // Weights, over codes times their rows' scales.
+#pragma unroll
+        for (int t = 0; t < kT; ++t) {
+            F32x4 vs = {1.0f, 1.0f, 1.0f, 1.0f};
+            if constexpr (T::kCoded) vs = *reinterpret_cast<const F32x4*>(ls + kPos + 16 * t + 4 * g);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                // Not fused with the product that made the score: the largest one's difference is exact.
+#pragma clang fp contract(off)
+                const float w = exp2_fast(p[t][e] - off);
+                l += w;
+                p[t][e] = T::kCoded ? w * vs[e] : w;
+            }
+        }
+        if (T::kCoded && tail) {               // a row that is not seen may have any scale
+            stay_a_branch();
+#pragma unroll
+            for (int t = 0; t < kT; ++t)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) p[t][e] = (seen >> (16 * t + e)) & 1 ? p[t][e] : 0.0f;
+        }
+        if (T::kMayBeInfinite && bad) {
+            stay_a_branch();
+            // The weights [query][position] in K's place, then position by position.
+            static_assert(kQ * kPos * 4 <= kTileBytes || !T::kMayBeInfinite, "weights take K's place");
+            float* const lp = reinterpret_cast<float*>(lk) + col * kPos;
+            lds_order();
+#pragma unroll
+            for (int t = 0; t < kT; ++t) *reinterpret_cast<F32x4*>(lp + 16 * t + 4 * g) = p[t];
+            lds_order();
+#pragma unroll 1
+            for (int row = 0; row < kPos; ++row) {
+                const float w = lp[row];
+                if ((vis >> row) & 1) {
+#pragma unroll
+                    for (int c = 0; c < 4; ++c)
+#pragma unroll
+                        for (int x = 0; x < 4; ++x)
+                            acc[c][x] += w * element<T::kMayBeInfinite ? DT : KVATTN_KV_F32>(lv, row, 16 * c + 4 * g + x);
+                }
+            }
+            lds_order();
+            continue;
+        }
+        // Outputs.  V's operands, transposed: step u's places of channels 16 c + col.
+        if constexpr (T::kF32) {
+#pragma unroll
+            for (int t = 0; t < kT; ++t)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int row = 16 * t + 4 * g + e;
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        const float v = *reinterpret_cast<const float*>(lv + row * T::kRow + 16 * T::chunk_at(row, 4 * c + (col >> 2)) +
+                                                                        4 * (col & 3));
+                        acc[c] = __builtin_amdgcn_mfma_f32_16x16x4f32(v, p[t][e], acc[c], 0, 0, 0);
+                    }
+                }
+        } else if constexpr (T::kBf16) {
+            typedef short S16x4 __attribute__((ext_vector_type(4)));
+#pragma unroll
+            for (int u = 0; u < kPos / 32; ++u) {
+                U32x4 hi, lo;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {                  // places 2 j and 2 j + 1
+                    const float p0 = p[2 * u + j / 2][2 * (j % 2)], p1 = p[2 * u + j / 2][2 * (j % 2) + 1];
+                    const uint32_t b0 = __float_as_uint(p0), b1 = __float_as_uint(p1);
+                    hi[j] = __builtin_amdgcn_perm(b1, b0, 0x07060302u);
+                    const float r0 = p0 - __uint_as_float(b0 & 0xffff0000u), r1 = p1 - __uint_as_float(b1 & 0xffff0000u);
+                    lo[j] = __builtin_amdgcn_perm(__float_as_uint(r1), __float_as_uint(r0), 0x07060302u);
                 }
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
-                    Weights va[kU];
-                    if constexpr (T::kBf16) {
-                        typedef short S16x4 __attribute__((ext_vector_type(4)));
+                    S16x4 part[2];
 #pragma unroll
-                        for (int u = 0; u < kU; ++u) {
-                            S16x4 part[2];
-#pragma unroll
-                            for (int e = 0; e < 2; ++e) {
-                                const int row = 32 * u + 16 * e + 4 * g + (col >> 2);
-                                part[e] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                                    (__attribute__((address_space(3))) S16x4*)(lv + row * T::kRow +
-                                        16 * T::chunk_at(row, 2 * c + ((col >> 1) & 1)) + 8 * (col & 1)));
-                            }
-                            va[u] = __builtin_bit_cast(Bf16x8, __builtin_shufflevector(part[0], part[1], 0, 1, 2, 3, 4, 5, 6, 7));
-                        }
-                    } else if constexpr (T::k8) {
-#pragma unroll
-                        for (int u = 0; u < 2; ++u) {
-                            const int e = col >> 1, row = 32 * u + 16 * (e >> 2) + 4 * g + (e & 3);
-                            const I32x2 w = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
-                                (__attribute__((address_space(3))) I32x2*)(lv + row * T::kRow + 16 * T::chunk_at(row, c) + 8 * (col & 1)));
-                            va[u] = codes_to_f16<T::kFp8>((uint32_t)w[0], (uint32_t)w[1]);
-                        }
-                    } else {
-                        const int e = place<T::kFp4>(col & 7), row = 32 * (col >> 3) + 16 * (e >> 2) + 4 * g + (e & 3);
-                        const I32x2 w = __builtin_amdgcn_ds_read_tr4_b64_v2i32(
-                            (__attribute__((address_space(3))) I32x2*)(lv + row * T::kRow + 8 * c));
-                        va[0] = operand16<T::kFp4>((uint32_t)w[0]);
-                        va[1] = operand16<T::kFp4>((uint32_t)w[1]);
+                    for (int e = 0; e < 2; ++e) {
+                        const int row = 32 * u + 16 * e + 4 * g + (col >> 2);
+                        part[e] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                            (__attribute__((address_space(3))) S16x4*)(lv + row * T::kRow +
+                                16 * T::chunk_at(row, 2 * c + ((col >> 1) & 1)) + 8 * (col & 1)));
                     }
-#pragma unroll
-                    for (int i = 0; i < kN; ++i)
-#pragma unroll
-                        for (int u = 0; u < kU; ++u) {
-                            acc[i][c] = mfma(va[u], wh[i][u], acc[i][c]);
-                            if constexpr (T::kBf16) acc[i][c] = mfma(va[u], wl[i][u], acc[i][c]);
-                        }
-                    if constexpr (kN > 1) lds_order();     // (else all of it is read ahead, into registers that are not there)
+                    const Bf16x8 va = __builtin_bit_cast(Bf16x8, __builtin_shufflevector(part[0], part[1], 0, 1, 2, 3, 4, 5, 6, 7));
+                    acc[c] = mfma(va, __builtin_bit_cast(Bf16x8, hi), acc[c]);
+                    acc[c] = mfma(va, __builtin_bit_cast(Bf16x8, lo), acc[c]);
                 }
             }
-        };
-        if (kG == 1 || ng == 1) work(std::integral_constant<int, 1>{});
-        else work(std::integral_constant<int, kG>{});
+        } else {
+            F16x8 w[2];
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+#pragma unroll
+                for (int x = 0; x < 8; ++x) w[u][x] = (_Float16)p[2 * u + x / 4][x % 4];
+                if constexpr (T::kInt4) acc8 = mfma((F16x8)(_Float16)8.0f, w[u], acc8);
+            }
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                F16x8 va[2];
+                if constexpr (T::k8) {
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) {
+                        const int e = col >> 1, row = 32 * u + 16 * (e >> 2) + 4 * g + (e & 3);
+                        const I32x2 v = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
+                            (__attribute__((address_space(3))) I32x2*)(lv + row * T::kRow + 16 * T::chunk_at(row, c) + 8 * (col & 1)));
+                        va[u] = codes_to_f16<T::kFp8>((uint32_t)v[0], (uint32_t)v[1]);
+                    }
+                } else {
+                    const int e = place<T::kFp4>(col & 7), row = 32 * (col >> 3) + 16 * (e >> 2) + 4 * g + (e & 3);
+                    const I32x2 v = __builtin_amdgcn_ds_read_tr4_b64_v2i32(
+                        (__attribute__((address_space(3))) I32x2*)(lv + row * T::kRow + 8 * c));
+                    va[0] = operand16<T::kFp4>((uint32_t)v[0]);
+                    va[1] = operand16<T::kFp4>((uint32_t)v[1]);
+                }
+#pragma unroll
+                for (int u = 0; u < 2; ++u) acc[c] = mfma(va[u], w[u], acc[c]);
+            }
+        }
         lds_order();
     }
 
-    // Join the waves, one group of queries after another.
+    // Join the waves.
     constexpr int kVec = 4, kItems = kHd / kVec;
     const size_t tok0 = (size_t)t0 + q0;
     float* const ro = reinterpret_cast<float*>(lk);
     lds_order();
 #pragma unroll
-    for (int i = 0; i < kG; ++i) {
-        if (i >= ng) break;
-        if (i > 0) __syncthreads();
+    for (int c = 0; c < 4; ++c) {
+        if constexpr (T::kInt4) acc[c] -= acc8;
+        if constexpr (T::kCoded) acc[c] *= unit * 0.03125f;
+        *reinterpret_cast<F32x4*>(ro + col * kOutPad + 16 * c + 4 * g) = acc[c];
+    }
+    const float sum = op_xor32<false>(op_xor16<false>(l));
+    if (g == 0) {
+        red_m[wave][col] = m;
+        red_l[wave][col] = sum;
+    }
+    __syncthreads();
+    for (int e = threadIdx.x; e < nq * kItems; e += kW * kWave) {
+        const int qq = e / kItems, ch = e % kItems * kVec;
+        float M = -INFINITY, L = 0.0f;
+        F32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-            if constexpr (T::kInt4) acc[i][c] -= acc8[i];
-            if constexpr (T::kCoded) acc[i][c] *= unit * 0.03125f;
-            *reinterpret_cast<F32x4*>(ro + col * kOutPad + 16 * c + 4 * g) = acc[i][c];
+        for (int w = 0; w < kW; ++w) M = fmaxf(M, red_m[w][qq]);
+#pragma unroll
+        for (int w = 0; w < kW; ++w) {
+            const float f = weight_of(red_m[w][qq], M);
+            L += f * red_l[w][qq];
+            o += f * *reinterpret_cast<const F32x4*>(lds + w * kWaveLds + (qq * kOutPad + ch) * 4);
         }
-        const float sum = op_xor32<false>(op_xor16<false>(l[i]));
-        if (g == 0) {
-            red_m[wave][col] = m[i];
-            red_l[wave][col] = sum;
-        }
-        __syncthreads();
-        for (int e = threadIdx.x; e < min(kQ, nq - kQ * i) * kItems; e += kW * kWave) {
-            const int qq = e / kItems, ch = e % kItems * kVec;
-            float M = -INFINITY, L = 0.0f;
-            F32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-            for (int w = 0; w < kW; ++w) M = fmaxf(M, red_m[w][qq]);
-#pragma unroll
-            for (int w = 0; w < kW; ++w) {
-                const float f = weight_of(red_m[w][qq], M);
-                L += f * red_l[w][qq];
-                o += f * *reinterpret_cast<const F32x4*>(lds + w * kWaveLds + (qq * kOutPad + ch) * 4);
-            }
-            const size_t head = (tok0 + kQ * i + qq) * a.NH + h;
-            if (segs == 1) {
-                store_out<T::kF32>(a.out, head * kHd + ch, L, o);
-            } else {
-                const size_t slot = head * a.S + s;
-                put4(a.part_out + slot * kHd + ch, o);
-                if (ch == 0) {
-                    put(a.part_max + slot, M);
-                    put(a.part_lse + slot, L);
-                }
+        const size_t head = (tok0 + qq) * a.NH + h;
+        if (segs == 1) {
+            store_out<T::kF32>(a.out, head * kHd + ch, L, o);
+        } else {
+            const size_t slot = head * a.S + s;
+            put4(a.part_out + slot * kHd + ch, o);
+            if (ch == 0) {
+                put(a.part_max + slot, M);
+                put(a.part_lse + slot, L);
             }
         }
     }
@@ -642,9 +579,8 @@ __global__ __launch_bounds__(kW * kWave) __attribute__((amdgpu_waves_per_eu(kG =
 }
 
 template <int DT>
-const void* kernel_for(int queries, int waves) {
-    if (waves == 8) return queries == kQ ? (const void*)&tree_kernel<DT, 1, 8> : (const void*)&tree_kernel<DT, 2, 8>;
-    return queries == kQ ? (const void*)&tree_kernel<DT, 1, 4> : (const void*)&tree_kernel<DT, 2, 4>;
+const void* kernel_for(int waves) {
+    return waves == 8 ? (const void*)&tree_kernel<DT, 8> : (const void*)&tree_kernel<DT, 4>;
 }
 
 // ------------------------------------------------------------------------------------
@@ -710,21 +646,22 @@ namespace kvattn_internal {
 
 int attend_tree(const AttendTree& c) {
     const int most_new = std::min(c.max_new, c.num_tokens);
-    const int queries = most_new <= kQ ? kQ : 2 * kQ;      // of a workgroup
-    const int passes = (most_new + queries - 1) / queries;
+    const int passes = (most_new + kQ - 1) / kQ;
     const long long heads = (long long)c.B * c.NH * passes;
-    // Workgroups of 8 waves where there are few; else 4, in segments of one length (maxT over their number, so that a short
-    // sequence has fewer) that make as many workgroups as run at once, none shorter than 256 positions (8 waves over codes:
-    // 1024, a tile each for two rounds).  us per call, positions of a segment : us:
-    //   BF16  1 x 12 heads of 1000, 26 tokens   8 waves 256: 9.7, 512: 10.8, one 10.6; 4 waves 256: 10.4, one 13.2
-    //   BF16  1 x 12 of 8000, 16                8 waves 512: 11.4, 1024: 10.9, 256: 14.8; 4 waves 512: 11.3
-    //   FP4   1 x 12 of 1000, 7                 8 waves one 6.4, 256: 7.6; 4 waves one 7.0
-    //   FP8   3 x 25 of 1999, 7                 4 waves 256: 9.4, 512: 10.1, one 13.1; 8 waves one 10.4
-    //   BF16  8 x 12 ragged of up to 2048, 16   4 waves 256: 9.3, 512: 10.2, one 14.2; 8 waves 11
-    //   INT8  8 x 12 ragged of up to 4096, 64   4 waves 1024: 20.6, 512: 24.5, 2048: 23.2; 8 waves one 24.7
-    //   INT4 24 x 12 ragged of up to 4096, 32   4 waves 2048: 24.1, one 26.5, 1024: 28.6; 8 waves one 23.0
-    //   BF16 16 x 12 ragged of up to 8192, 64   4 waves 2048: 46.2, 4096: 47.8, one 72; 8 waves one 47.4
-    //   FP8  64 x 12 ragged of up to 1024, 16   4 waves one 16.4, 512: 24
+    // Workgroups of 8 waves where there are few, in segments of at least 1024 positions.  Else 4 waves: up to two workgroups
+    // a CU, as many segments as make the six a CU that run in two rounds, of at least 256 positions; beyond, segments of 32
+    // tiles, so that the longest sequence is not waited for alone.  All segments have one length (a short sequence has
+    // fewer).  us per call, positions of a segment : us:
+    //   BF16  1 x 12 heads of 1000, 26 tokens   8 waves one 7.6, 512: 8.8, 256: 8.0
+    //   BF16  1 x 12 of 8000, 16                8 waves 1024: 10.9, 512: 11.4, 2048: 13.7; 4 waves 512: 11.3
+    //   FP4   1 x 12 of 1000, 7                 8 waves one 6.2, 256: 7.6; 4 waves one 7.0
+    //   FP8   3 x 25 of 1999, 7                 4 waves 256: 9.2, 512: 9.7, one 12.9; 8 waves one 10.4
+    //   BF16  8 x 12 ragged of up to 2048, 16   4 waves 256: 9.2, 512: 10.1, one 13.8; 8 waves 11
+    //   INT8  8 x 12 ragged of up to 4096, 64   4 waves 1024: 20.0, 512: 22.4, 2048: 23.0, one 25.9
+    //   INT4 24 x 12 ragged of up to 4096, 32   4 waves 2048: 23.7, 1024: 26.1, one 27.6
+    //   BF16 16 x 12 ragged of up to 8192, 64   4 waves 1024: 46.6, 512: 50.1, 2048: 50.6, one 53.3
+    //   FP8  64 x 12 ragged of up to 1024, 16   4 waves one 16.4, 512: 23.6
+    //   INT4 64 x 12 ragged of up to 2048, 64   4 waves one 41.0, 1024: 64
     const int waves = heads <= kFewHeads ? 8 : 4;
     const int tiles = (c.maxT + kSeg - 1) / kSeg;
     int S = 1, seg_tiles = 1;
@@ -737,9 +674,10 @@ int attend_tree(const AttendTree& c) {
         S = (tiles + seg_tiles - 1) / seg_tiles;
         if (S > kMaxSegments) return KVATTN_ERR_SPLIT;
     } else {
-        const bool coded = c.kv_dtype != KVATTN_KV_F32 && c.kv_dtype != KVATTN_KV_BF16;
-        const int least = waves == 8 && coded ? 16 : 4;
-        S = (int)std::max<long long>(1, std::min<long long>({3 * kCUs / heads, (tiles + least - 1) / least, 16}));
+        const int tile = c.kv_dtype == KVATTN_KV_F32 ? Kv<KVATTN_KV_F32>::kPos : c.kv_dtype == KVATTN_KV_BF16 ? Kv<KVATTN_KV_BF16>::kPos : 64;
+        const int least = waves == 8 ? 16 : heads <= 2 * kCUs ? 4 : 32 * tile / kSeg;
+        const long long want = heads <= 2 * kCUs ? 6 * kCUs / heads : kMaxSegments;
+        S = (int)std::max<long long>(1, std::min<long long>({want, (tiles + least - 1) / least, 16}));
         seg_tiles = (tiles + S - 1) / S;
     }
     if (c.B > 65535 || heads * S * waves > kMostWaves) return KVATTN_ERR_SHAPE;
@@ -775,12 +713,12 @@ int attend_tree(const AttendTree& c) {
     a.num_tokens = c.num_tokens;
     const void* fn = nullptr;
     switch (c.kv_dtype) {
-        case KVATTN_KV_F32: fn = kernel_for<KVATTN_KV_F32>(queries, waves); break;
-        case KVATTN_KV_BF16: fn = kernel_for<KVATTN_KV_BF16>(queries, waves); break;
-        case KVATTN_KV_INT8: fn = kernel_for<KVATTN_KV_INT8>(queries, waves); break;
-        case KVATTN_KV_FP8_E4M3: fn = kernel_for<KVATTN_KV_FP8_E4M3>(queries, waves); break;
-        case KVATTN_KV_INT4: fn = kernel_for<KVATTN_KV_INT4>(queries, waves); break;
-        default: fn = kernel_for<KVATTN_KV_FP4_E2M1>(queries, waves); break;
+        case KVATTN_KV_F32: fn = kernel_for<KVATTN_KV_F32>(waves); break;
+        case KVATTN_KV_BF16: fn = kernel_for<KVATTN_KV_BF16>(waves); break;
+        case KVATTN_KV_INT8: fn = kernel_for<KVATTN_KV_INT8>(waves); break;
+        case KVATTN_KV_FP8_E4M3: fn = kernel_for<KVATTN_KV_FP8_E4M3>(waves); break;
+        case KVATTN_KV_INT4: fn = kernel_for<KVATTN_KV_INT4>(waves); break;
+        default: fn = kernel_for<KVATTN_KV_FP4_E2M1>(waves); break;
     }
     void* params[] = {&a};
     return hip_status(hipLaunchKernel(fn, dim3(c.NH * passes, c.B, S), dim3(waves * kWave), params, 0, (hipStream_t)c.stream));
