@@ -32,6 +32,7 @@ constexpr int kTogether = 512;                 // workgroups of kSliceThreads th
 constexpr int kMaxVocab = 1 << 18;
 constexpr int kMaxRows = 1 << 21;              // workgroups of a grid: 2^32 threads are too many
 constexpr int kMaxSequences = 1 << 20;
+constexpr int kDenseRuns = 2;                  // of a slice whose table has an entry for every token
 constexpr int kIds = 8, kNamed = 2;             // ids and named tokens of a thread that are asked for ahead
 constexpr int kLdsMost = 156 * 1024;           // a CU's, less what is static here
 constexpr int kLdsTogether = 76 * 1024;        // two workgroups a CU
@@ -109,6 +110,8 @@ __device__ __forceinline__ int sequence_of(const int* start, int B, int row, int
 template <bool kInF32, bool kOutF32, bool kProbs, int kThreads, int kRuns, bool kShare>
 __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(4))) void logits_kernel(LogitArgs a) {
     constexpr int kWaves = kThreads / kWave, kStep = kThreads * kRun;      // tokens from one run of a thread to its next
+    // A small slice's table has an entry for every token, which spares the places, their barriers and gathered logits.
+    constexpr bool kDense = kThreads == kSliceThreads && kRuns > 0 && kRuns <= kDenseRuns;
     static_assert(!kShare || (kProbs && kRuns > 0), "slices in registers");
     extern __shared__ uint32_t lds[];          // map, allowed tokens, named tokens, counts, biases, prefixes (16 bits)
     __shared__ uint32_t wave_words[kWaves];
@@ -129,11 +132,19 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(4))) v
             for (int j = 0; j < kRuns; ++j) load_run<kInF32>(a.x, in0, v0 + tid * kRun + j * kStep, v1, a.vec, x[j]);
         }
     };
+    // Loads come back in order: those that others depend on are asked for before the row.
+    int first = 0, end = 0;
+    if (a.start) {
+        first = a.start[min(lane, a.B - 1)];
+        end = a.start[a.B];
+    }
+    asm volatile("" ::: "memory");
     load();
+    asm volatile("" ::: "memory");
     int b = row, t0 = row;
     if (a.start) {
-        if (row >= a.start[a.B]) return;       // behind the last token
-        b = sequence_of(a.start, a.B, row, lane);
+        if (row >= end) return;                // behind the last token
+        b = a.B <= kWave ? 63 - __clzll((long long)(__ballot(lane < a.B && first <= row) | 1)) : sequence_of(a.start, a.B, row, lane);
         t0 = min(max(a.start[b], 0), row);
     }
 
@@ -146,17 +157,18 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(4))) v
         for (int k = 0; k < kIds; ++k) ids[k] = k * kThreads < a.r.max_history ? history[min(tid + k * kThreads, a.r.max_history - 1)] : -1;
     }
     const float temperature = a.r.temperature ? a.r.temperature[b] : 1.0f;
+    // (Of a dense table counts, biases and allowed tokens alone.)
     uint32_t* const map = lds;
-    uint32_t* const allowed = map + a.words;
-    uint32_t* const names = allowed + (a.r.allowed ? a.words : 0);
-    uint32_t* const count = names + a.entries;
-    uint32_t* const bias_at = count + a.entries;
-    uint16_t* const before = reinterpret_cast<uint16_t*>(bias_at + (a.r.bias_start ? a.entries : 0));
+    uint32_t* const names = map + a.words;
+    uint32_t* const count = kDense ? lds : names + a.entries;
+    uint32_t* const bias_at = count + (kDense && !table ? 0 : a.entries);
+    uint32_t* const allowed = bias_at + (a.r.bias_start ? a.entries : 0);
+    uint16_t* const before = reinterpret_cast<uint16_t*>(allowed + (a.r.allowed ? a.words : 0));
     int line = -1;
     if (a.r.allowed) line = a.r.allowed_of ? a.r.allowed_of[row] : row;
     const bool grammar = a.r.allowed && line >= 0 && line < a.r.num_allowed;
 
-    int held = 0, prompt = 0, branch = -1, bias0 = 0, biases = 0;
+    int held = 0, prompt = 0, branch = -1, bias0 = 0, biases = 0, bias_id = -1;
     float repetition = 1.0f, frequency = 0.0f, presence = 0.0f;
     if (table) {
         held = a.r.history ? min(max(a.r.history_len[b], 0), a.r.max_history) : 0;
@@ -172,16 +184,28 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(4))) v
         if (a.r.bias_start) {
             bias0 = min(max(a.r.bias_start[b], 0), a.r.num_bias);
             biases = min(min(max(a.r.bias_start[b + 1], bias0), a.r.num_bias) - bias0, a.r.max_bias);
+            if (tid < biases) bias_id = a.r.bias_ids[bias0 + tid];
         }
     }
+    auto each_bias = [&](auto&& f) {
+        if (tid < biases) f(bias_id, bias0 + tid);
+        for (int i = tid + kThreads; i < biases; i += kThreads) f(a.r.bias_ids[bias0 + i], bias0 + i);
+    };
+    // A held or biased token's logit.
+    auto adjusted = [&](float z, uint32_t c, uint32_t from) {
+#pragma clang fp contract(off)
+        const float made = (float)((c & 0xffffu) - (c >> 16));
+        if (c) z = z > 0.0f ? z / repetition : z * repetition;
+        z = z - (frequency * made + (made > 0.0f ? presence : 0.0f));
+        if (from) z = z + a.r.bias[from - 1];
+        return z;
+    };
     // Allowed and named tokens of v0 .. v1 - 1.
     auto build = [&] {
         const int first = v0 >> 5, words = (v1 - v0 + 31) >> 5;
         if (grammar)
             for (int w = tid; w < words; w += kThreads) allowed[w] = a.r.allowed[(size_t)line * a.r.allowed_stride + first + w];
         if (!table) return;
-        for (int w = tid; w < words; w += kThreads) map[w] = 0;
-        __syncthreads();
         auto known = [&](int id) { return id >= v0 && id < v1; };
         auto each_held = [&](auto&& f) {
 #pragma unroll
@@ -189,12 +213,28 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(4))) v
                 if (tid + k * kThreads < held) f(ids[k], tid + k * kThreads);
             for (int i = tid + kIds * kThreads; i < held; i += kThreads) f(history[i], i);
         };
+        if constexpr (kDense) {
+            const int all = (a.r.bias_start ? 2 : 1) * a.entries;          // (a multiple of 4)
+            for (int e = 4 * tid; e < all; e += 4 * kThreads) *reinterpret_cast<uint4*>(count + e) = make_uint4(0, 0, 0, 0);
+            __syncthreads();
+            // Times held in the lower half, times of those in the prompt in the upper: at most 2^15 each.
+            each_held([&](int id, int i) {
+                if (known(id)) atomicAdd(count + (id - v0), i < prompt ? 0x10001u : 1u);
+            });
+            if (known(branch)) atomicAdd(count + (branch - v0), 1u);
+            each_bias([&](int id, int i) {     // of an id listed twice the last
+                if (known(id)) atomicMax(bias_at + (id - v0), (uint32_t)(i + 1));
+            });
+            return;
+        }
+        for (int w = tid; w < words; w += kThreads) map[w] = 0;
+        __syncthreads();
         auto mark = [&](int id) {              // (text repeats itself: mostly it is marked)
             if (known(id) && !((map[(id - v0) >> 5] >> (id & 31)) & 1)) atomicOr(map + ((id - v0) >> 5), 1u << (id & 31));
         };
         each_held([&](int id, int) { mark(id); });
         mark(branch);
-        for (int i = tid; i < biases; i += kThreads) mark(a.r.bias_ids[bias0 + i]);
+        each_bias([&](int id, int) { mark(id); });
         __syncthreads();
         // Set bits before every word: a thread's words, then the threads'.
         const int per = (words + kThreads - 1) / kThreads, w0 = min(tid * per, words), w1 = min(w0 + per, words);
@@ -228,28 +268,17 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(4))) v
 #pragma unroll
         for (int k = 0; k < kNamed; ++k) named[k] = tid + k * kThreads < all ? logit<kInF32>(a.x, in0 + names[tid + k * kThreads]) : 0.0f;
         auto entry = [&](int id) { return before[(id - v0) >> 5] + __popc(map[(id - v0) >> 5] & ((1u << (id & 31)) - 1)); };
-        // Times held in the lower half, times of those in the prompt in the upper: at most 2^15 each.
         each_held([&](int id, int i) {
             if (known(id)) atomicAdd(count + entry(id), i < prompt ? 0x10001u : 1u);
         });
         if (known(branch)) atomicAdd(count + entry(branch), 1u);
-        for (int i = tid; i < biases; i += kThreads) {
-            const int id = a.r.bias_ids[bias0 + i];
-            if (known(id)) atomicMax(bias_at + entry(id), (uint32_t)(bias0 + i + 1));   // of an id listed twice the last
-        }
+        each_bias([&](int id, int i) {
+            if (known(id)) atomicMax(bias_at + entry(id), (uint32_t)(i + 1));
+        });
         __syncthreads();
         // A thread for every named token: its logit takes its count's place.
         auto adjust = [&](uint32_t e, float z) {
-#pragma clang fp contract(off)
-            const uint32_t c = count[e];
-            const float made = (float)((c & 0xffffu) - (c >> 16));
-            if (c) z = z > 0.0f ? z / repetition : z * repetition;
-            z = z - (frequency * made + (made > 0.0f ? presence : 0.0f));
-            if (a.r.bias_start) {
-                const uint32_t from = bias_at[e];
-                if (from) z = z + a.r.bias[from - 1];
-            }
-            count[e] = __float_as_uint(z);
+            count[e] = __float_as_uint(adjusted(z, count[e], a.r.bias_start ? bias_at[e] : 0));
         };
 #pragma unroll
         for (int k = 0; k < kNamed; ++k)
@@ -259,7 +288,16 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(4))) v
     auto rules = [&](int v, float (&y)[kRun]) {
         if (v >= v1) return;
         const int w = (v - v0) >> 5;
-        if (table) {
+        if (kDense && table) {
+            const uint4 c = *reinterpret_cast<const uint4*>(count + (v - v0));
+            const uint4 f = a.r.bias_start ? *reinterpret_cast<const uint4*>(bias_at + (v - v0)) : make_uint4(0, 0, 0, 0);
+            if (c.x | c.y | c.z | c.w | f.x | f.y | f.z | f.w) {
+                const uint32_t cs[kRun] = {c.x, c.y, c.z, c.w}, fs[kRun] = {f.x, f.y, f.z, f.w};
+#pragma unroll
+                for (int i = 0; i < kRun; ++i)
+                    if (cs[i] | fs[i]) y[i] = adjusted(y[i], cs[i], fs[i]);
+            }
+        } else if (table) {
             const uint32_t word = map[w], bits = (word >> (v & 31)) & 15u;
             if (bits) {
                 // (Entries of the run are neighbours; those before its first bit and behind its last are read for nothing.)
@@ -451,6 +489,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(4))) v
 struct LogitPlan {
     const void* fn;
     int threads, tokens, slices;               // tokens of a slice
+    bool dense;                                // its table has an entry for every token
 };
 template <bool kInF32, bool kOutF32, bool kProbs, int kRuns>
 LogitPlan slices_plan(int V) {
@@ -459,10 +498,13 @@ LogitPlan slices_plan(int V) {
     if constexpr (kProbs) {
         if (slices > 1) fn = (const void*)&logits_kernel<kInF32, kOutF32, kProbs, kSliceThreads, kRuns, true>;
     }
-    return {fn, kSliceThreads, tokens, slices};
+    return {fn, kSliceThreads, tokens, slices, kRuns <= kDenseRuns};
 }
 template <bool kInF32, bool kOutF32, bool kProbs>
 LogitPlan plan_for(int rows, int V, bool share) {
+    // The smallest slices with which a call's workgroups run at once; of logits alone, which wait for none, up to 8192 tokens.
+    // us per call, 50257 float logits, rows : us (history of 1000): probabilities 1: 6.8, in one workgroup 17.9;
+    // 64: 13.2 / 21.9; 256: 29.9 / 42; logits 512: slices of 8192 43.8, of 16384 48.5.
     constexpr int kToken = kSliceThreads * kRun;
     auto fits = [&](int runs) {
         const long long slices = (V + kToken * runs - 1) / (kToken * runs);
@@ -471,14 +513,14 @@ LogitPlan plan_for(int rows, int V, bool share) {
     };
     if (fits(1)) return slices_plan<kInF32, kOutF32, kProbs, 1>(V);
     if (fits(2)) return slices_plan<kInF32, kOutF32, kProbs, 2>(V);
-    if (fits(4)) return slices_plan<kInF32, kOutF32, kProbs, 4>(V);
-    if (!kProbs || fits(8)) return slices_plan<kInF32, kOutF32, kProbs, 8>(V);
+    if (!kProbs || fits(4)) return slices_plan<kInF32, kOutF32, kProbs, 4>(V);
     if constexpr (kProbs) {
+        if (fits(8)) return slices_plan<kInF32, kOutF32, kProbs, 8>(V);
         if (fits(13)) return slices_plan<kInF32, kOutF32, kProbs, 13>(V);
         constexpr int kRowToken = kRowThreads * kRun;
-        if (V <= 13 * kRowToken) return {(const void*)&logits_kernel<kInF32, kOutF32, true, kRowThreads, 13, false>, kRowThreads, V, 1};
+        if (V <= 13 * kRowToken) return {(const void*)&logits_kernel<kInF32, kOutF32, true, kRowThreads, 13, false>, kRowThreads, V, 1, false};
     }
-    return {(const void*)&logits_kernel<kInF32, kOutF32, true, kRowThreads, 0, false>, kRowThreads, V, 1};
+    return {(const void*)&logits_kernel<kInF32, kOutF32, true, kRowThreads, 0, false>, kRowThreads, V, 1, false};
 }
 template <bool kInF32>
 LogitPlan plan_for(int rows, int V, bool out_f32, bool probs, bool share) {
@@ -534,10 +576,11 @@ extern "C" int kvattn_process_logits(void* out, const void* logits, const kvattn
     a.V = V;
     // Every entry is another token: a workgroup has no more of them than of these.
     const int named = (r.history ? r.max_history : 0) + (branches ? 64 * r.mask_words : 0) + (r.bias_start ? r.max_bias : 0);
-    const auto lds_of = [&](int tokens) {
-        a.words = (std::min(V, tokens) + 31) / 32;
-        a.entries = std::min(std::min(V, tokens), named);
-        return (size_t)a.words * (r.allowed ? 8 : 4) + (size_t)(a.words + 1) / 2 * 4 + (size_t)a.entries * (r.bias_start ? 12 : 8);
+    const auto lds_of = [&](const LogitPlan& p) {
+        a.words = (std::min(V, p.tokens) + 31) / 32;
+        a.entries = named == 0 ? 0 : p.dense ? p.tokens : std::min(std::min(V, p.tokens), named);
+        const size_t masks = r.allowed ? (size_t)a.words * 4 : 0, entry = p.dense ? 4 : 8;
+        return masks + (size_t)a.entries * (entry + (r.bias_start ? 4 : 0)) + (p.dense ? 0 : (size_t)a.words * 4 + (size_t)(a.words + 1) / 2 * 4);
     };
     a.vec = row_stride % kRun == 0 && out_stride % kRun == 0 && ((uintptr_t)logits % (kRun * in)) == 0 &&
             ((uintptr_t)out % (kRun * res)) == 0;
@@ -546,10 +589,10 @@ extern "C" int kvattn_process_logits(void* out, const void* logits, const kvattn
         return dtype == KVATTN_KV_F32 ? plan_for<true>(rows, V, out_f32, probs != 0, share) : plan_for<false>(rows, V, out_f32, probs != 0, share);
     };
     LogitPlan p = plan(r.workspace != nullptr);
-    size_t lds = lds_of(p.tokens);
+    size_t lds = lds_of(p);
     if (probs && p.slices > 1 && lds > kLdsTogether) {     // they would not run at once
         p = plan(false);
-        lds = lds_of(p.tokens);
+        lds = lds_of(p);
     }
     if (lds > kLdsMost) return KVATTN_ERR_LDS;
     a.slices = p.slices;
