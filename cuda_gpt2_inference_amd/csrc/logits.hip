@@ -45,8 +45,9 @@ struct LogitArgs {
     kvattn_logit_rules r;
     size_t in_row, out_row;
     int B, rows, V, words, entries;            // words of the map; entries of the table
+    int row0;                                  // the launch's first row
     int slices, slice;                         // of a row, tokens of one
-    unsigned long long* exchange;              // [rows][slices][2] tagged words
+    unsigned long long* exchange;              // [rows of the launch][slices][2] tagged words
     int polls;
     bool vec;                                  // rows start on boundaries of a run
 };
@@ -120,8 +121,8 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(4))) v
     __shared__ float slice_top[kMostSlices], slice_sum[kMostSlices];       // (sum: of the likeliest token alone, its number)
     __shared__ unsigned long long missing_at;
     const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave;
-    const int row = a.slices > 1 ? blockIdx.x / a.slices : blockIdx.x;
-    const int own = a.slices > 1 ? blockIdx.x - row * a.slices : 0;
+    const int launch_row = a.slices > 1 ? blockIdx.x / a.slices : blockIdx.x, row = a.row0 + launch_row;
+    const int own = a.slices > 1 ? blockIdx.x - launch_row * a.slices : 0;
     constexpr int kHeld = kRuns ? kRuns : 1;
     float x[kHeld][kRun];
     const size_t in0 = (size_t)row * a.in_row, out0 = (size_t)row * a.out_row;
@@ -403,7 +404,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(4))) v
     bool none = top == -INFINITY;
     if constexpr (kShare) {
         // A slice's words: its maximum; its sum, or its likeliest token.
-        unsigned long long* const words = a.exchange + (size_t)row * a.slices * 2;
+        unsigned long long* const words = a.exchange + (size_t)launch_row * a.slices * 2;
         const uint32_t tag = call_tag();
         if (tid == 0) {
             publish_word(words + 2 * own, tagged_word(top, tag), false);
@@ -585,13 +586,24 @@ extern "C" int kvattn_process_logits(void* out, const void* logits, const kvattn
     a.vec = row_stride % kRun == 0 && out_stride % kRun == 0 && ((uintptr_t)logits % (kRun * in)) == 0 &&
             ((uintptr_t)out % (kRun * res)) == 0;
     const bool out_f32 = out_dtype == KVATTN_KV_F32;
-    const auto plan = [&](bool share) {
-        return dtype == KVATTN_KV_F32 ? plan_for<true>(rows, V, out_f32, probs != 0, share) : plan_for<false>(rows, V, out_f32, probs != 0, share);
+    const auto plan = [&](int n, bool share) {
+        return dtype == KVATTN_KV_F32 ? plan_for<true>(n, V, out_f32, probs != 0, share) : plan_for<false>(n, V, out_f32, probs != 0, share);
     };
-    LogitPlan p = plan(r.workspace != nullptr);
+    // Slices may have to read one another's logits again, which must still be there.
+    const uintptr_t x0 = (uintptr_t)logits, y0 = (uintptr_t)out;
+    const uintptr_t x1 = x0 + ((size_t)(rows - 1) * row_stride + V) * in, y1 = y0 + ((size_t)(rows - 1) * out_stride + V) * res;
+    const bool share = r.workspace && (y1 <= x0 || x1 <= y0);
+    LogitPlan p = plan(rows, share);
     size_t lds = lds_of(p);
+    int launch_rows = rows;
     if (probs && p.slices > 1 && lds > kLdsTogether) {     // they would not run at once
-        p = plan(false);
+        p = plan(rows, false);
+        lds = lds_of(p);
+    }
+    if (lds > kLdsMost && probs && share) {                // long histories: some rows at a time, in small slices
+        const int slices = (V + kDenseRuns * kSliceThreads * kRun - 1) / (kDenseRuns * kSliceThreads * kRun);
+        launch_rows = std::max(1, kTogether / slices);
+        p = plan(launch_rows, true);
         lds = lds_of(p);
     }
     if (lds > kLdsMost) return KVATTN_ERR_LDS;
@@ -603,8 +615,12 @@ extern "C" int kvattn_process_logits(void* out, const void* logits, const kvattn
         const int st = hip_status(hipFuncSetAttribute(p.fn, hipFuncAttributeMaxDynamicSharedMemorySize, kLdsMost));
         if (st != KVATTN_OK) return st;
     }
-    const long long grid = (long long)rows * p.slices;
-    if (grid * p.threads >= (1ll << 32)) return KVATTN_ERR_SHAPE;
-    void* params[] = {&a};
-    return hip_status(hipLaunchKernel(p.fn, dim3((unsigned)grid), dim3(p.threads), params, lds, (hipStream_t)stream));
+    for (a.row0 = 0; a.row0 < rows; a.row0 += launch_rows) {
+        const long long grid = (long long)std::min(launch_rows, rows - a.row0) * p.slices;
+        if (grid * p.threads >= (1ll << 32)) return KVATTN_ERR_SHAPE;
+        void* params[] = {&a};
+        const int st = hip_status(hipLaunchKernel(p.fn, dim3((unsigned)grid), dim3(p.threads), params, lds, (hipStream_t)stream));
+        if (st != KVATTN_OK) return st;
+    }
+    return KVATTN_OK;
 }

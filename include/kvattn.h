@@ -588,11 +588,12 @@ typedef struct kvattn_logit_rules {
     size_t workspace_bytes;
 } kvattn_logit_rules;
 
-/* Bytes of a workspace with which up to 256 rows of probabilities are cut into slices, several workgroups a row (without
- * one a row is one workgroup's): 8-byte aligned, zeroed once (kvattn_workspace_init), of no further content between calls.
- * Calls sharing it must be ordered, and only calls of kvattn_process_logits may.  The slices of a row wait for one another's
- * maxima, within the bound of kvattn_set_merge_poll_limit; one that stops waiting works the others' out itself (the
- * result is the same, bit for bit). */
+/* Bytes of a workspace with which rows of probabilities are cut into slices, several workgroups a row, where there are few
+ * rows (without one, and where out overlaps logits, a row is one workgroup's): 8-byte aligned, zeroed once
+ * (kvattn_workspace_init), of no further content between calls.  Calls sharing it must be ordered, and only calls of
+ * kvattn_process_logits may.  The slices of a row wait for one another's maxima, within the bound of
+ * kvattn_set_merge_poll_limit; one that stops waiting works the others' out itself (the result is the same, bit for
+ * bit). */
 size_t kvattn_logits_workspace_bytes(void);
 
 /* The rules on rows of V logits, in the order above, in float: repetition, frequency and presence, bias, allowed.
@@ -604,10 +605,10 @@ size_t kvattn_logits_workspace_bytes(void);
  *            are left as they were.  NULL: row b is sequence b's (rows == B)
  *   dtype, out_dtype  KVATTN_KV_F32 or KVATTN_KV_BF16; out may be logits where the types and strides are the same.
  *            What lies behind a row's V elements is neither read nor written
- * V <= 2^18, rows <= 2^21, B <= 2^20.  KVATTN_ERR_LDS: the table of named tokens does not fit in LDS
- * (V / 8 bytes for the map and V / 16 for its sums, V / 8 with allowed, 8 bytes, with biases 12, for each of
- * min(V, max_history + 64 mask_words + max_bias) entries, in 156 KB; up to V = 8192 it always fits, and so it does where
- * the row is cut into such slices).
+ * V <= 2^18, rows <= 2^21, B <= 2^20.  KVATTN_ERR_LDS: the table of named tokens does not fit in LDS (probabilities of
+ * rows that are one workgroup's: V / 8 bytes for the map and V / 16 for its sums, V / 8 with allowed, 8 bytes, with
+ * biases 12, for each of min(V, max_history + 64 mask_words + max_bias) entries, in 156 KB).  With a workspace, and
+ * outputs that are not the logits' own memory, any table fits: rows are then cut into slices, some rows at a time.
  * No reference counterpart (the reference takes the argmax or samples on the host, without rules). */
 int kvattn_process_logits(void* out, const void* logits, const kvattn_logit_rules* rules, const int* token_start,
                           int B, int rows, int V, long long row_stride, long long out_stride, int dtype, int out_dtype,

@@ -218,3 +218,121 @@ def test_temperature_extremes(dev):
     assert ((out[1].double() - want[1]).abs() <= 1e-5 * want[1]).all()
     assert float((out[0].double() - want[0]).abs().max()) < 1e-2 and out[0].argmax() == x[0].argmax()
     assert out[2].sum() == 1 and out[2].argmax() == x[2].argmax()
+
+
+def _same(c, dev, probs=True, dtype="f32", **extra):
+    """A call's output as bits."""
+    import torch
+    kvattn = _kv()
+    x = torch.zeros((c.N, c.stride), device=dev)
+    x[:] = torch.from_numpy(np.nan_to_num(c.x)).to(dev)
+    out = torch.zeros((c.N, c.stride), device=dev)
+    rules = {k: _dev(v, dev) if isinstance(v, np.ndarray) else v for k, v in c.rules.items()}
+    rules.update(extra)
+    kvattn.process_logits(out, x, kvattn.LogitRules(**rules), _dev(c.start, dev), c.B, c.N, c.V, row_stride=c.stride, out_stride=c.stride,
+                          probs=probs)
+    return out.cpu()
+
+
+@pytest.mark.parametrize("V", [3001, 50257])
+def test_slices_that_wait_in_vain(dev, V):
+    """Every slice works the others out itself: the same bits."""
+    import torch
+    kvattn = _kv()
+    c = Case(20, [2, 1, 3], V, V + 3, "f32", history=300, bias=9, grammar=True, branches=True)
+    want = _same(c, dev)
+    before = kvattn.set_merge_poll_limit(0)
+    try:
+        got = _same(c, dev)
+        torch.cuda.synchronize()
+    finally:
+        kvattn.set_merge_poll_limit(before)
+    assert torch.equal(got, want)
+
+
+def test_without_a_workspace(dev):
+    """A row by one workgroup: the same mathematics in another order."""
+    c = Case(21, [3, 2], 50257, 50304, "f32", history=300, grammar=True, branches=True)
+    c.check(dev)
+    c.rules["workspace"] = None
+    c.check(dev)
+    c.check(dev, "bf16")
+
+
+@pytest.mark.parametrize("rows", [100, 200, 300, 700])
+def test_many_rows(dev, rows):
+    """Every number of slices, and a row a workgroup."""
+    c = Case(22, [rows // 2, 0, rows - rows // 2], 9001, 9004, "f32", history=20, bias=3)
+    c.check(dev)
+    c = Case(22, [rows], 33000, 33000, "bf16", history=20)
+    c.check(dev, "bf16", probs=rows != 200)
+
+
+def test_histories_that_do_not_fit_one_workgroup(dev):
+    """Rows at a time; refused where slices cannot be."""
+    import torch
+    kvattn = _kv()
+    sizes = [1] * 300
+    c = Case(23, sizes, 40000, 40000, "f32", history=20, bias=4)
+    long = np.zeros((300, 32768), dtype=np.int32)
+    long[:, :20] = c.rules["history"]
+    c.rules.update(history=long, max_history=32768)
+    r = np.random.RandomState(1)
+    for b in (0, 150, 299):                              # some are as long as they can be
+        long[b] = r.randint(0, 40000, 32768)
+        c.rules["history_len"][b], c.rules["prompt_len"][b] = 32768, 10000
+    c.check(dev)
+    with pytest.raises(kvattn.KvAttnError) as e:
+        _same(c, dev, workspace=None)
+    assert e.value.status == kvattn.ERR_LDS
+    x = torch.zeros((300, 40000), device=dev)
+    rules = kvattn.LogitRules(**{k: _dev(v, dev) if isinstance(v, np.ndarray) else v for k, v in c.rules.items()})
+    with pytest.raises(kvattn.KvAttnError) as e:
+        kvattn.process_logits(x, x, rules, None, 300, 300, 40000)
+    assert e.value.status == kvattn.ERR_LDS
+
+
+def test_in_place_where_slices_wait_in_vain(dev):
+    """Outputs in the logits' place: no slice reads another's."""
+    import torch
+    kvattn = _kv()
+    x = torch.randn(3, 50257, device=dev)
+    rules = kvattn.LogitRules(temperature=torch.ones(3, device=dev))
+    want = torch.empty_like(x)
+    kvattn.process_logits(want, x, kvattn.LogitRules(temperature=torch.ones(3, device=dev), workspace=None), None, 3, 3, 50257)
+    before = kvattn.set_merge_poll_limit(0)
+    try:
+        kvattn.process_logits(x, x, rules, None, 3, 3, 50257)
+        torch.cuda.synchronize()
+    finally:
+        kvattn.set_merge_poll_limit(before)
+    assert torch.equal(x, want)
+
+
+def test_captured_and_on_another_stream(dev):
+    """One workspace in a graph and in eager calls between its replays, ordered."""
+    import torch
+    c = Case(24, [4, 4], 50257, 50257, "f32", history=100, grammar=True)
+    kvattn = _kv()
+    x = torch.from_numpy(c.x).to(dev)
+    rules = kvattn.LogitRules(**{k: _dev(v, dev) if isinstance(v, np.ndarray) else v for k, v in c.rules.items()})
+    start = _dev(c.start, dev)
+    out, eager = torch.zeros_like(x), torch.zeros_like(x)
+    call = lambda o: kvattn.process_logits(o, x, rules, start, 2, 8, 50257)      # noqa: E731
+    call(eager)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call(out)
+        call(out)
+    side = torch.cuda.Stream()
+    for _ in range(4):
+        out.zero_()
+        graph.replay()
+        assert torch.equal(out, eager)
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            again = torch.zeros_like(x)
+            call(again)
+        torch.cuda.current_stream().wait_stream(side)
+        assert torch.equal(again, eager)
