@@ -4,10 +4,10 @@
 // A sequence's n new tokens are nodes of a tree; their K and V rows are the cache's last n.  Token i attends the
 // prefix before them and the new tokens whose bits its mask has (itself and its ancestors).  A workgroup serves 16 of a
 // tree's tokens, the columns of a product; those of larger trees run side by side, so that what one loads the others
-// find in the caches.  (On one XCD, one behind the other, they share its L2, which reads the cache once, but a long
-// sequence's then wait for one another: BF16 16 x 64 tokens 45.7 us in place of 48.2, INT4 64 x 64 47.6 of 41.1.)  (Two or four groups of 16 in one workgroup take registers that other workgroups hide latency
-// with: BF16, 26 tokens over 1000 positions 9.6 us in place of 7.6, INT4 64 x 64 tokens 43.4 and 41.0, 16 x 64 over
-// 8192 46.0 and 46.6.)
+// find in the caches.  (Two or four groups of 16 in one workgroup take registers that other workgroups hide latency
+// with: BF16, 26 tokens over 1000 positions 9.6 us in place of 7.6, INT4 64 x 64 tokens 43.4 and 41.0, BF16 16 x 64 over
+// 8192 46.0 and 46.6.  One behind the other on one XCD they share its L2, which then reads the cache once, but a long
+// sequence's wait for one another: BF16 16 x 64 45.7 us of 48.2, INT4 64 x 64 47.6 of 41.1.)
 //
 // Both products go to the matrix cores, scores as S^T = K Q^T and outputs as O^T = V^T P^T.  Of S^T lane
 // 16 g + c holds positions 16 t + 4 g .. + 3 of query c.  That makes everything the softmax does (maximum, sum,
@@ -729,7 +729,7 @@ int attend_tree(const AttendTree& c) {
 
 extern "C" int kvattn_tree_masks(unsigned long long* masks, int* positions, const int* parents, const int* token_start,
                                  const int* lens, int B, int num_tokens, int mask_words, void* stream) {
-    if (B < 1 || num_tokens < 0 || num_tokens > (1 << 30) || mask_words < 1 || mask_words > kMaxMaskWords) return KVATTN_ERR_SHAPE;
+    if (B < 1 || B > (1 << 20) || num_tokens < 0 || num_tokens > (1 << 30) || mask_words < 1 || mask_words > kMaxMaskWords) return KVATTN_ERR_SHAPE;
     if (num_tokens == 0) return KVATTN_OK;
     if (!masks || !parents || !token_start || (positions && !lens)) return KVATTN_ERR_NULL_POINTER;
     if (((uintptr_t)masks & 7u) || ((uintptr_t)positions & 3u) || ((uintptr_t)parents & 3u) || ((uintptr_t)token_start & 3u) ||

@@ -429,7 +429,7 @@ int kvattn_paged_decode_tokens(void* out, const void* qkv, const void* pages, co
  *             depth (0 where that is negative); lens [B] as in kvattn_paged_decode_tokens, needed for
  *             positions alone
  * Tokens from 64 * mask_words on get an empty mask, and the position of a root.  Rows behind
- * token_start[B] are left as they were.  B >= 1, num_tokens <= 2^30 (0: nothing is done). */
+ * token_start[B] are left as they were.  B <= 2^20, num_tokens <= 2^30 (0: nothing is done). */
 int kvattn_tree_masks(unsigned long long* masks, int* positions, const int* parents, const int* token_start,
                       const int* lens, int B, int num_tokens, int mask_words, void* stream);
 
@@ -438,7 +438,7 @@ int kvattn_tree_masks(unsigned long long* masks, int* positions, const int* pare
  * position lens[b] - n + j is in [0, lens[b]) and whose bit its mask has, of whatever shape the masks
  * are; one that attends nothing gets zeros.  K and V of positions that a token does not attend never
  * reach its output, also where they are infinite or NaN.  A table entry outside the pool: its positions
- * are skipped.  The cache is read once for 64 tokens of a sequence (32 for F32, INT8, FP8, INT4 and FP4).
+ * are skipped.  16 tokens of a sequence share a pass over the cache.
  *   max_new  the most tokens of one sequence, at most 64 * mask_words (or num_tokens is); a sequence with
  *            more has the first max_new or more of them computed
  * Other arguments, limits and the workspace as in kvattn_paged_decode_tokens; B <= 65535. */

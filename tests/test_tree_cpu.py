@@ -40,7 +40,7 @@ MASKS = dict(masks=A, positions=A, parents=A, start=A, lens=A, B=1, num_tokens=4
 
 
 @pytest.mark.parametrize("kw,status", [
-    (dict(B=0), 4), (dict(num_tokens=-1), 4), (dict(words=0), 4), (dict(words=5), 4), (dict(num_tokens=(1 << 30) + 1), 4),
+    (dict(B=0), 4), (dict(B=(1 << 20) + 1), 4), (dict(num_tokens=-1), 4), (dict(words=0), 4), (dict(words=5), 4), (dict(num_tokens=(1 << 30) + 1), 4),
     (dict(masks=None), 1), (dict(parents=None), 1), (dict(start=None), 1), (dict(lens=None), 1), (dict(masks=A + 4), 2),
     (dict(parents=A + 1), 2), (dict(positions=A + 2), 2), (dict(num_tokens=0, masks=None, parents=None, start=None), 0)])
 def test_tree_masks(kw, status):
