@@ -32,7 +32,8 @@ constexpr int kTogether = 512;                 // workgroups of kSliceThreads th
 constexpr int kMaxVocab = 1 << 18;
 constexpr int kMaxRows = 1 << 21;              // workgroups of a grid: 2^32 threads are too many
 constexpr int kMaxSequences = 1 << 20;
-constexpr int kDenseRuns = 2;                  // of a slice whose table has an entry for every token
+constexpr int kSmallRuns = 2;                  // of a slice whose table always has an entry for every token
+constexpr int kLongHistory = 4096;             // from which larger slices' has
 constexpr int kIds = 8, kNamed = 2;             // ids and named tokens of a thread that are asked for ahead
 constexpr int kLdsMost = 156 * 1024;           // a CU's, less what is static here
 constexpr int kLdsTogether = 76 * 1024;        // two workgroups a CU
@@ -108,11 +109,10 @@ __device__ __forceinline__ int sequence_of(const int* start, int B, int row, int
 
 // kRuns: runs of a thread that are kept in registers; 0: of a longer row none is, and each pass reads it again.
 // kShare: the row's probabilities are those of several workgroups.
-template <bool kInF32, bool kOutF32, bool kProbs, int kThreads, int kRuns, bool kShare>
+// kDense: the table has an entry for every token, which spares the places, their barriers and gathered logits.
+template <bool kInF32, bool kOutF32, bool kProbs, int kThreads, int kRuns, bool kShare, bool kDense>
 __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(4))) void logits_kernel(LogitArgs a) {
     constexpr int kWaves = kThreads / kWave, kStep = kThreads * kRun;      // tokens from one run of a thread to its next
-    // A small slice's table has an entry for every token, which spares the places, their barriers and gathered logits.
-    constexpr bool kDense = kThreads == kSliceThreads && kRuns > 0 && kRuns <= kDenseRuns;
     static_assert(!kShare || (kProbs && kRuns > 0), "slices in registers");
     extern __shared__ uint32_t lds[];          // map, allowed tokens, named tokens, counts, biases, prefixes (16 bits)
     __shared__ uint32_t wave_words[kWaves];
@@ -492,41 +492,46 @@ struct LogitPlan {
     int threads, tokens, slices;               // tokens of a slice
     bool dense;                                // its table has an entry for every token
 };
-template <bool kInF32, bool kOutF32, bool kProbs, int kRuns>
+template <bool kInF32, bool kOutF32, bool kProbs, int kRuns, bool kDense>
 LogitPlan slices_plan(int V) {
     const int tokens = kSliceThreads * kRun * kRuns, slices = (V + tokens - 1) / tokens;
-    const void* fn = (const void*)&logits_kernel<kInF32, kOutF32, kProbs, kSliceThreads, kRuns, false>;
+    const void* fn = (const void*)&logits_kernel<kInF32, kOutF32, kProbs, kSliceThreads, kRuns, false, kDense>;
     if constexpr (kProbs) {
-        if (slices > 1) fn = (const void*)&logits_kernel<kInF32, kOutF32, kProbs, kSliceThreads, kRuns, true>;
+        if (slices > 1) fn = (const void*)&logits_kernel<kInF32, kOutF32, kProbs, kSliceThreads, kRuns, true, kDense>;
     }
-    return {fn, kSliceThreads, tokens, slices, kRuns <= kDenseRuns};
+    return {fn, kSliceThreads, tokens, slices, kDense};
 }
 template <bool kInF32, bool kOutF32, bool kProbs>
-LogitPlan plan_for(int rows, int V, bool share) {
-    // The smallest slices with which a call's workgroups run at once; of logits alone, which wait for none, up to 8192 tokens.
-    // us per call, 50257 float logits, rows : us (history of 1000): probabilities 1: 6.8, in one workgroup 17.9;
-    // 64: 13.2 / 21.9; 256: 29.9 / 42; logits 512: slices of 8192 43.8, of 16384 48.5.
+LogitPlan plan_for(int rows, int V, bool share, const kvattn_logit_rules& r) {
+    // The smallest slices with which a call's workgroups run at once; of logits alone, which wait for none, up to 8192
+    // tokens.  us per call, 50257 logits:
+    //   probabilities of 1 row, history of 1000: slices 6.8, one workgroup 17.9; 64: 13.2 / 21.9; 256: 29.9 / 42
+    //   64 rows, slices of 8192, an entry for every token or for the named: history of 2000 14.4 / 14.0, 100 and biases
+    //     16.2 / 12.0, 8000 and biases 19.3 / 26.8
+    //   logits of about 2000 rows, history of 2000, slices of 8192 tokens, 4096, 16384: 90.9, 113.5, 132; of 250 rows
+    //     26.6, 28.5, 33.4; of 144 rows with biases, history of 4000: 18.2, 15.2, 18.3
     constexpr int kToken = kSliceThreads * kRun;
     auto fits = [&](int runs) {
         const long long slices = (V + kToken * runs - 1) / (kToken * runs);
         if (!kProbs) return rows * slices <= kTogether + kTogether / 4;
         return slices == 1 || (share && slices <= kMostSlices && rows * slices <= kTogether);
     };
-    if (fits(1)) return slices_plan<kInF32, kOutF32, kProbs, 1>(V);
-    if (fits(2)) return slices_plan<kInF32, kOutF32, kProbs, 2>(V);
-    if (!kProbs || fits(4)) return slices_plan<kInF32, kOutF32, kProbs, 4>(V);
+    if (fits(1)) return slices_plan<kInF32, kOutF32, kProbs, 1, true>(V);
+    if (fits(kSmallRuns) || (!kProbs && r.bias_start)) return slices_plan<kInF32, kOutF32, kProbs, kSmallRuns, true>(V);
+    if (!kProbs || (fits(4) && r.history && r.max_history >= kLongHistory)) return slices_plan<kInF32, kOutF32, kProbs, 4, true>(V);
     if constexpr (kProbs) {
-        if (fits(8)) return slices_plan<kInF32, kOutF32, kProbs, 8>(V);
-        if (fits(13)) return slices_plan<kInF32, kOutF32, kProbs, 13>(V);
+        if (fits(4)) return slices_plan<kInF32, kOutF32, kProbs, 4, false>(V);
+        if (fits(8)) return slices_plan<kInF32, kOutF32, kProbs, 8, false>(V);
+        if (fits(13)) return slices_plan<kInF32, kOutF32, kProbs, 13, false>(V);
         constexpr int kRowToken = kRowThreads * kRun;
-        if (V <= 13 * kRowToken) return {(const void*)&logits_kernel<kInF32, kOutF32, true, kRowThreads, 13, false>, kRowThreads, V, 1, false};
+        if (V <= 13 * kRowToken) return {(const void*)&logits_kernel<kInF32, kOutF32, true, kRowThreads, 13, false, false>, kRowThreads, V, 1, false};
     }
-    return {(const void*)&logits_kernel<kInF32, kOutF32, true, kRowThreads, 0, false>, kRowThreads, V, 1, false};
+    return {(const void*)&logits_kernel<kInF32, kOutF32, true, kRowThreads, 0, false, false>, kRowThreads, V, 1, false};
 }
 template <bool kInF32>
-LogitPlan plan_for(int rows, int V, bool out_f32, bool probs, bool share) {
-    if (out_f32) return probs ? plan_for<kInF32, true, true>(rows, V, share) : plan_for<kInF32, true, false>(rows, V, share);
-    return probs ? plan_for<kInF32, false, true>(rows, V, share) : plan_for<kInF32, false, false>(rows, V, share);
+LogitPlan plan_for(int rows, int V, bool out_f32, bool probs, bool share, const kvattn_logit_rules& r) {
+    if (out_f32) return probs ? plan_for<kInF32, true, true>(rows, V, share, r) : plan_for<kInF32, true, false>(rows, V, share, r);
+    return probs ? plan_for<kInF32, false, true>(rows, V, share, r) : plan_for<kInF32, false, false>(rows, V, share, r);
 }
 
 int hip_status(hipError_t e) {
@@ -587,7 +592,8 @@ extern "C" int kvattn_process_logits(void* out, const void* logits, const kvattn
             ((uintptr_t)out % (kRun * res)) == 0;
     const bool out_f32 = out_dtype == KVATTN_KV_F32;
     const auto plan = [&](int n, bool share) {
-        return dtype == KVATTN_KV_F32 ? plan_for<true>(n, V, out_f32, probs != 0, share) : plan_for<false>(n, V, out_f32, probs != 0, share);
+        return dtype == KVATTN_KV_F32 ? plan_for<true>(n, V, out_f32, probs != 0, share, r)
+                                       : plan_for<false>(n, V, out_f32, probs != 0, share, r);
     };
     // Slices may have to read one another's logits again, which must still be there.
     const uintptr_t x0 = (uintptr_t)logits, y0 = (uintptr_t)out;
@@ -601,7 +607,7 @@ extern "C" int kvattn_process_logits(void* out, const void* logits, const kvattn
         lds = lds_of(p);
     }
     if (lds > kLdsMost && probs && share) {                // long histories: some rows at a time, in small slices
-        const int slices = (V + kDenseRuns * kSliceThreads * kRun - 1) / (kDenseRuns * kSliceThreads * kRun);
+        const int slices = (V + kSmallRuns * kSliceThreads * kRun - 1) / (kSmallRuns * kSliceThreads * kRun);
         launch_rows = std::max(1, kTogether / slices);
         p = plan(launch_rows, true);
         lds = lds_of(p);

@@ -336,3 +336,10 @@ def test_captured_and_on_another_stream(dev):
             call(again)
         torch.cuda.current_stream().wait_stream(side)
         assert torch.equal(again, eager)
+
+
+@pytest.mark.parametrize("rows,bias", [(64, 0), (64, 40), (20, 5), (300, 0)])
+def test_histories_of_thousands(dev, rows, bias):
+    c = Case(25, [rows - 3, 3], 33001, 33004, "f32", history=5000, bias=bias, grammar=rows == 64)
+    c.check(dev)
+    c.check(dev, "bf16", probs=False)
