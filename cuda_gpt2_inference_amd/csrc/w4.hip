@@ -500,7 +500,7 @@ int kvattn_gemv_w4(void* out, void* pre_gelu, const void* w4, const void* x, con
     W4Shape s;
     if (!is_4bit(w_dtype) || (out_dtype != KVATTN_KV_F32 && out_dtype != KVATTN_KV_BF16)) return KVATTN_ERR_DTYPE;
     if (!shape_of(M, K, group, s)) return KVATTN_ERR_SHAPE;
-    if (B < 1 || (long long)B * M >= (1ll << 31) || (long long)B * K >= (1ll << 31)) return KVATTN_ERR_SHAPE;
+    if (B < 1 || M >= (1 << 28) || (long long)B * M >= (1ll << 31) || (long long)B * K >= (1ll << 31)) return KVATTN_ERR_SHAPE;
     if (!out || !w4 || !x) return KVATTN_ERR_NULL_POINTER;
     const size_t osz = out_dtype == KVATTN_KV_F32 ? 4 : 2;
     if (((uintptr_t)w4 & 15u) || ((uintptr_t)x & 15u) || ((uintptr_t)out % osz) || ((uintptr_t)pre_gelu % osz) || ((uintptr_t)bias & 1u))
@@ -508,25 +508,37 @@ int kvattn_gemv_w4(void* out, void* pre_gelu, const void* w4, const void* x, con
     W4Args a{out, pre_gelu, (const uint8_t*)w4, (const uint8_t*)w4 + s.scales_at(), (const uint16_t*)x, (const uint16_t*)bias,
              B, M, K, s.steps, gelu ? 1 : 0};
     const bool fp4 = w_dtype == KVATTN_KV_FP4_E2M1, f32 = out_dtype == KVATTN_KV_F32;
-    const int nt = B <= 16 ? 1 : B <= 32 ? 2 : 4;
-    const size_t x_lds = (size_t)s.steps * nt * 16 * (256 + 4 * s.groups);
-    // Two row tiles a workgroup halve the vectors' loads where enough workgroups are left, and 64 vectors the registers for
-    // it are missing; tall matrices keep their vectors in LDS, few vectors from more rows on.  us per call (graph), INT4, groups of 64, one / two row
-    // tiles / vectors in LDS:
-    //   1 vector    8192 x 8192 9.1 / 8.9      12000 x 1024 3.4 / 3.7 / 5.5   20000 x 1024 5.1 / 5.4 / 6.7   50304 x 768 9.6 / 9.2 / 7.5
-    //   16          4096 x 4096 4.6 / 6.4       8192 x 8192 13.5 / 10.4       12000 x 1024 4.8 / 4.1 / 6.8   20000 x 1024 5.9 / 5.6 / 7.6
-    //   26          6400 x 1600 7.2 / 5.5
-    //   32          4096 x 4096 6.1 / 8.4      12000 x 1024 7.6 / 7.1 / 8.0   20000 x 1024 11.7 / 9.9 / 9.0
-    //   64          6400 x 1600 11.9 / 16.6    12000 x 1024 12.5 / 21.4 / 13.7   20000 x 1024 20.4 / 31.6 / 14.8   50304 x 768 49 / 63 / 15.4
-    int row_tiles = nt < 4 && s.tiles >= (nt == 1 ? 512 : 320) ? 2 : 1;
-    if (s.tiles >= (nt == 1 ? 2048 : 1024) && x_lds <= kTallLds) row_tiles = 0;
+    int nt = B <= 16 ? 1 : B <= 32 ? 2 : 4;
+    auto x_lds = [&](int n) { return (size_t)s.steps * n * 16 * (256 + 4 * s.groups); };
+    // us per call (graph), INT4, groups of 64, one / two row tiles a workgroup / vectors in LDS for their whole length:
+    //   vectors       6400 x 1600         12000 x 768        20000 x 1600         32000 x 1600         50304 x 768         50304 x 1600
+    //    1         3.7 / 3.8 / 7.5    3.6 / 3.7 / 5.0     5.8 / 6.0 / 9.2     8.2 / 7.2 / 9.5    7.8 / 8.1 / 7.1    11.9 / 11.3 / 12.1
+    //   16         4.2 / 4.1 / 8.1    4.8 / 4.1 / 6.1     8.2 / 7.0 / 9.8    12.6 / 9.5 / 10.2  11.5 / 9.4 / 8.1    19.1 / 15.0 / 13.1
+    //   32         5.7 / 5.4 / 10.5   5.8 / 7.0 / 7.2    11.9 / 12.9 / 12.3  19.1 / 17.9 / 12.9 19.1 / 21.1 / 10.1  29.5 / 29.9 / 16.4
+    //   64        12.0 / 8.8          12.1 / 11.2 / 10.7  30.1 / 24.1         49.6 / 32.7        50.7 / 36.4 / 14.0  81.0 / 56.0
+    // Two row tiles halve the vectors' loads, where workgroups for the GPU are left.  Of 32 vectors 512 row tiles run at once
+    // either way, and a last round that is less than half full is shorter with one; of 64 vectors 256 and 512 run at once.
+    // Vectors in LDS pay where a matrix is tall, the more the vectors (their filling: one vector over long rows never);
+    // 64 that do not fit go in two halves (64 x 32000 x 1600 25.8 us).
+    const long long work = (long long)s.tiles * ((B + 16 * nt - 1) / (16 * nt)), last = work % 512;
+    int row_tiles = 1;
+    if (nt == 1) row_tiles = work >= (B <= 4 ? 512 : 320) ? 2 : 1;
+    else if (nt == 2) row_tiles = work >= 320 && (last == 0 || last >= 320) ? 2 : 1;
+    else row_tiles = work > 256 ? 2 : 1;
+    const int tall = nt == 1 ? (B <= 4 && K > 1024 ? kRowMask : 2400) : nt == 2 ? 1250 : B <= 64 ? 513 : 1024;
+    if (s.tiles >= tall && x_lds(nt) <= kTallLds) {
+        row_tiles = 0;
+    } else if (nt == 4 && s.tiles >= 1536 && x_lds(2) <= kTallLds) {
+        nt = 2;
+        row_tiles = 0;
+    }
     const void* fn = nt == 1 ? kernel_for<1>(fp4, s.groups, row_tiles, B, f32)
                              : nt == 2 ? kernel_for<2>(fp4, s.groups, row_tiles, B, f32) : kernel_for<4>(fp4, s.groups, row_tiles, B, f32);
     const long long cols = (B + 16 * nt - 1) / (16 * nt);
     if (cols > 65535) return KVATTN_ERR_SHAPE;
     int groups = kTallGroups;
     const int grid = row_tiles ? (s.tiles + row_tiles - 1) / row_tiles : groups, waves = row_tiles ? kW4Waves : kTallW4Waves;
-    const size_t lds = row_tiles ? (size_t)kW4Waves * nt * 16 * std::max(256, (row_tiles * kRows + 4) * 4) : x_lds;
+    const size_t lds = row_tiles ? (size_t)kW4Waves * nt * 16 * std::max(256, (row_tiles * kRows + 4) * 4) : x_lds(nt);
     if (lds > 64 * 1024) {
         const int st = hip_status(hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024));
         if (st != KVATTN_OK) return st;

@@ -67,6 +67,15 @@ def test_rows_that_end_inside_a_block(dev, kind, B, M, K, group):
     Layer(dev, kind, B, M, K, group).check("f32")
 
 
+@pytest.mark.parametrize("kind,group", [("int4", 64), ("fp4", 32), ("int4", 128)])
+@pytest.mark.parametrize("B,M,K", [(4, 9001, 1280), (1, 40007, 640), (7, 5200, 256), (16, 39000, 256), (26, 6400, 512), (20, 12000, 256),
+                                   (30, 20011, 384), (64, 4115, 256), (64, 9000, 256), (40, 24601, 1408), (130, 4100, 256),
+                                   (100, 16400, 256)])
+def test_tall(dev, kind, group, B, M, K):
+    """Each way of tiling, rows that end inside a tile."""
+    Layer(dev, kind, B, M, K, group).check("f32")
+
+
 @pytest.mark.parametrize("kind", ["int4", "fp4"])
 @pytest.mark.parametrize("B", [1, 26, 70])
 @pytest.mark.parametrize("kw", [dict(), dict(gelu=True), dict(gelu=True, pre=True), dict(bias=False), dict(pre=True),

@@ -110,7 +110,7 @@ GEMV = dict(out=A, pre=None, w4=A, x=A, bias=None, B=1, M=10, K=256, group=64, w
 
 
 @pytest.mark.parametrize("kw,status", [
-    (dict(w=1), 5), (dict(w=6), 5), (dict(out_dtype=2), 5), (dict(group=16), 4), (dict(group=256), 4), (dict(K=250), 4),
+    (dict(M=1 << 28, K=1024), 4), (dict(w=1), 5), (dict(w=6), 5), (dict(out_dtype=2), 5), (dict(group=16), 4), (dict(group=256), 4), (dict(K=250), 4),
     (dict(K=32, group=64), 4), (dict(M=0), 4), (dict(B=0), 4), (dict(K=(1 << 20) + 64), 4), (dict(B=1 << 20, M=1 << 12), 4),
     (dict(out=None), 1), (dict(w4=None), 1), (dict(x=None), 1), (dict(w4=A + 8), 2), (dict(x=A + 2), 2), (dict(out=A + 1), 2),
     (dict(bias=A + 1), 2), (dict(pre=A + 2, out_dtype=0), 2)])
