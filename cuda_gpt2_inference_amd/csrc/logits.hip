@@ -19,6 +19,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <cfloat>
 
 #include "lanes.hpp"
 #include "tree.hpp"
@@ -346,7 +347,8 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(4))) v
         return;
     }
     const bool likeliest = !(temperature > 0.0f);
-    const float scale = kLog2e / temperature;
+    // (A factor of zero or infinity would make NaN of forbidden tokens, and of the likeliest.)
+    const float scale = fminf(fmaxf(kLog2e / temperature, FLT_MIN), FLT_MAX);
     float top = -INFINITY, sum = 0.0f;         // of this workgroup's tokens
     int token = -1;                            // its likeliest, the lowest of several
     auto weigh = [&](float (&y)[kRun]) {

@@ -343,3 +343,26 @@ def test_histories_of_thousands(dev, rows, bias):
     c = Case(25, [rows - 3, 3], 33001, 33004, "f32", history=5000, bias=bias, grammar=rows == 64)
     c.check(dev)
     c.check(dev, "bf16", probs=False)
+
+
+@pytest.mark.parametrize("V", [900, 50257])
+def test_temperatures_whose_quotients_end(dev, V):
+    """Temperatures so small or large that 1 / T is infinite or zero: the largest share, all share."""
+    import torch
+    kvattn = _kv()
+    T = [1e-44, 1e-39, 3e38, float("inf")]
+    x = torch.randn(4, V, device=dev)
+    x[:, 7] = x[:, 80] = 9.0
+    x[:, 3] = 20.0                                       # is forbidden
+    allowed = torch.full((1, (V + 31) // 32), -1, dtype=torch.int32, device=dev)
+    allowed[0, 0] = ~(1 << 3)
+    rules = kvattn.LogitRules(temperature=torch.tensor(T, device=dev), allowed=allowed, num_allowed=1, allowed_stride=allowed.shape[1],
+                              allowed_of=torch.zeros(4, dtype=torch.int32, device=dev))
+    out = torch.full_like(x, -1.0)
+    kvattn.process_logits(out, x, rules, None, 4, 4, V)
+    want = torch.zeros_like(x)
+    want[:2, 7] = want[:2, 80] = 0.5
+    want[2:] = 1.0 / (V - 1)
+    want[2:, 3] = 0.0
+    # (Weights of one and their sums are whole: a quotient and a product round.)
+    assert ((out - want).abs() <= 2.0 ** -20 * want).all()
