@@ -180,8 +180,9 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(4))) v
         if (a.r.presence) presence = a.r.presence[b];
         // This thread's token of the row's branch, and the sequence's biases.
         if (a.r.tokens && tid < 64 * a.r.mask_words) {
-            const int its = a.r.tokens[min(t0 + tid, a.rows - 1)];
-            if (t0 + tid < a.rows && (a.r.masks[(size_t)row * a.r.mask_words + (tid >> 6)] >> (tid & 63)) & 1) branch = its;
+            // (Bits behind the sequence's last row are no tokens of it.)
+            const int its = a.r.tokens[min(t0 + tid, a.rows - 1)], last = min(a.start ? a.start[b + 1] : row + 1, a.rows);
+            if (t0 + tid < last && (a.r.masks[(size_t)row * a.r.mask_words + (tid >> 6)] >> (tid & 63)) & 1) branch = its;
         }
         if (a.r.bias_start) {
             bias0 = min(max(a.r.bias_start[b], 0), a.r.num_bias);

@@ -366,3 +366,21 @@ def test_temperatures_whose_quotients_end(dev, V):
     want[2:, 3] = 0.0
     # (Weights of one and their sums are whole: a quotient and a product round.)
     assert ((out - want).abs() <= 2.0 ** -20 * want).all()
+
+
+@pytest.mark.parametrize("starts", [True, False])
+def test_bits_behind_the_last_row(dev, starts):
+    """Masks with bits of tokens that the sequence does not have."""
+    import torch
+    kvattn = _kv()
+    start = np.array([0, 3, 3, 5, 8] if starts else range(9), dtype=np.int32)
+    x = torch.full((8, 1000), 4.0, device=dev)
+    rules = kvattn.LogitRules(tokens=torch.arange(100, 108, dtype=torch.int32, device=dev), mask_words=2,
+                              masks=torch.full((8, 2), -1, dtype=torch.int64, device=dev),
+                              presence=torch.full((len(start) - 1,), 1.0, device=dev))
+    out = torch.zeros_like(x)
+    kvattn.process_logits(out, x, rules, _dev(start, dev) if starts else None, len(start) - 1, 8, 1000, probs=False)
+    want = torch.full_like(x, 4.0)
+    for lo, hi in zip(start[:-1].tolist(), start[1:].tolist()):
+        want[lo:hi, 100 + lo:100 + hi] = 3.0
+    assert torch.equal(out, want)
