@@ -303,3 +303,76 @@ def test_keep(dev, kv, NH):
     assert torch.equal(pages.cpu().view(torch.uint8), want.view(torch.uint8))
     if scale is not None:
         assert torch.equal(scales.cpu(), want_s)
+
+
+@pytest.mark.parametrize("kv", ["f32", "int4"])
+def test_pools_beyond_32_bits(dev, kv):
+    """Pages whose bytes lie past 2^32: the same rows as in a small pool, read and moved."""
+    import torch
+    kvattn = _kv()
+    NH, R, n = 12, 256, 5
+    c = Case(dev, kv, [n], [700], NH, R, seed=60)
+    near = c.stored.to(dev)
+    page_bytes = near[0].numel() * near.element_size()
+    extra = (1 << 32) // page_bytes + 1
+    far = torch.zeros((extra + c.P,) + tuple(near.shape[1:]), dtype=near.dtype, device=dev)
+    far[extra:] = near
+    scales = far_scales = None
+    if c.scale is not None:
+        scales = c.scale.to(dev)
+        far_scales = torch.zeros((extra + c.P,) + tuple(scales.shape[1:]), device=dev)
+        far_scales[extra:] = scales
+    start, lens, masks = _dev(c.start, dev), _dev(np.array([700], dtype=np.int32), dev), _dev(c.masks, dev)
+    qkv = torch.from_numpy(c.q).to(c.act).to(dev)
+    ws = kvattn.Workspace(c.N, NH, c.max_pages * R)
+    path = torch.tensor([0, 2, 4, -1, -1], dtype=torch.int32, device=dev)
+    outs = []
+    for pages, sc, first in ((near, scales, 0), (far, far_scales, extra)):
+        cache = kvattn.PagedCache(pages, _dev(c.table + first, dev).int(), c.max_pages, R, first + c.P, sc)
+        out = torch.zeros((c.N, NH, HS), dtype=c.act, device=dev)
+        kvattn.paged_decode_tree(out, qkv, cache, start, lens, masks, 1, c.N, NH, HS, kv_dtype=kv, max_new=n, **ws.kwargs())
+        outs.append(out)
+        slots = torch.tensor([(int(c.table[0, t // R]) + first) * R + t % R for t in range(695, 700)], device=dev)
+        kvattn.paged_keep(cache, slots, path, start, 1, c.N, NH, HS, kv_dtype=kv)
+    assert torch.equal(outs[0], outs[1])
+    assert torch.equal(far[extra:].view(torch.uint8), near.view(torch.uint8)) and not far[:extra].any()
+    assert not torch.equal(near.cpu().view(torch.uint8), c.stored.view(torch.uint8))
+
+
+@pytest.mark.parametrize("kv", ["bf16", "fp8"])
+def test_captured_calls_and_other_streams(dev, kv):
+    """Two graphs and eager calls on one workspace, ordered, with lengths that change between replays."""
+    import torch
+    kvattn = _kv()
+    NH, R = 5, 64
+    c = Case(dev, kv, [20, 3, 33], [1500, 40, 900], NH, R, seed=61)
+    cache = kvattn.PagedCache(c.stored.to(dev), _dev(c.table, dev), c.max_pages, R, c.P, None if c.scale is None else c.scale.to(dev))
+    start, masks = _dev(c.start, dev), _dev(c.masks, dev)
+    lens = _dev(np.array(c.lens, dtype=np.int32), dev)
+    qkv = torch.from_numpy(c.q).to(c.act).to(dev)
+    ws = kvattn.Workspace(c.N, NH, c.max_pages * R, S=6)
+    outs = [torch.zeros((c.N, NH, HS), dtype=c.act, device=dev) for _ in range(3)]
+
+    def call(out):
+        kvattn.paged_decode_tree(out, qkv, cache, start, lens, masks, 3, c.N, NH, HS, kv_dtype=kv, max_new=33, S=6, **ws.kwargs())
+
+    call(outs[0])
+    torch.cuda.synchronize()
+    graphs = []
+    for out in outs[:2]:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            call(out)
+    side = torch.cuda.Stream()
+    for step in range(4):
+        lens.copy_(_dev(np.array(c.lens, dtype=np.int32) - 7 * step, dev))
+        for out in outs:
+            out.fill_(9.0)
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            call(outs[2])
+        torch.cuda.current_stream().wait_stream(side)
+        for g in graphs:
+            g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(outs[0], outs[2]) and torch.equal(outs[1], outs[2]) and not (outs[2] == 9.0).any()
