@@ -384,3 +384,24 @@ def test_bits_behind_the_last_row(dev, starts):
     for lo, hi in zip(start[:-1].tolist(), start[1:].tolist()):
         want[lo:hi, 100 + lo:100 + hi] = 3.0
     assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("rows,history,bias", [(120, 20000, 0), (120, 20000, 30), (90, 9000, 0), (100, 3, 17000), (250, 12000, 0)])
+def test_tables_of_many_ids(dev, rows, history, bias):
+    c = Case(26, [1] * rows, 33001, 33004, "f32", history=20, bias=4)
+    r = np.random.RandomState(2)
+    long = np.zeros((rows, history), dtype=np.int32)
+    for b in (0, rows // 2, rows - 1):
+        long[b] = r.randint(0, 33001, history)
+        c.rules["history_len"][b], c.rules["prompt_len"][b] = history, history // 3
+    for b in range(rows):
+        c.rules["history_len"][b] = min(c.rules["history_len"][b], history)
+        if b not in (0, rows // 2, rows - 1):
+            long[b, :min(20, history)] = c.rules["history"][b, :min(20, history)]
+    c.rules.update(history=long, max_history=history)
+    if bias:                                             # one sequence has nearly all of them
+        n = int(c.rules["bias_start"][-1])
+        ids = np.concatenate([c.rules["bias_ids"][:n], r.permutation(33001)[:bias - 5]]).astype(np.int32)
+        c.rules["bias_start"][-1] = len(ids)
+        c.rules.update(bias_ids=ids, bias=r.standard_normal(len(ids)).astype(np.float32), num_bias=len(ids), max_bias=bias)
+    c.check(dev)
