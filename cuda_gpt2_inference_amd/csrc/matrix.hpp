@@ -68,51 +68,6 @@ __device__ __forceinline__ Bf16x8 operand(uint32_t w) {
     return __builtin_bit_cast(Bf16x8, d);
 }
 
-typedef _Float16 F16x8 __attribute__((ext_vector_type(8)));
-typedef _Float16 F16x2 __attribute__((ext_vector_type(2)));
-
-__device__ __forceinline__ F32x4 mfma(F16x8 a, F16x8 b, F32x4 c) {
-    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
-}
-
-// The same operands in float16, in which every code is exact too: operand()'s eight, and eight 8-bit codes in order.
-template <bool kFp4>
-__device__ __forceinline__ F16x8 operand16(uint32_t w) {
-    U32x4 d;
-    if constexpr (kFp4) {
-        d[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, 1.0f, 0));
-        d[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, 1.0f, 1));
-        d[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, 1.0f, 2));
-        d[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, 1.0f, 3));
-    } else {
-        const uint32_t even = w & 0x0F0F0F0Fu, odd = (w >> 4) & 0x0F0F0F0Fu;
-        d[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(even, 512.0f, false));
-        d[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(even, 512.0f, true));
-        d[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(odd, 512.0f, false));
-        d[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(odd, 512.0f, true));
-    }
-    return __builtin_bit_cast(F16x8, d);
-}
-template <bool kFp8>
-__device__ __forceinline__ F16x8 codes_to_f16(uint32_t w0, uint32_t w1) {
-    U32x4 d;
-    const uint32_t w[2] = {w0, w1};
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        if constexpr (kFp8) {
-            d[2 * i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w[i], 1.0f, false));
-            d[2 * i + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w[i], 1.0f, true));
-        } else {
-            // code + 128 below the 64 of 1024.0 is 1024 + 128 + code.
-            const uint32_t u = w[i] ^ 0x80808080u;
-            const F16x2 off = {(_Float16)1152.0f, (_Float16)1152.0f};
-            d[2 * i] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(F16x2, __builtin_amdgcn_perm(0x64646464u, u, 0x04010400u)) - off);
-            d[2 * i + 1] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(F16x2, __builtin_amdgcn_perm(0x64646464u, u, 0x04030402u)) - off);
-        }
-    }
-    return __builtin_bit_cast(F16x8, d);
-}
-
 // The place of code r of eight in operand().
 template <bool kFp4>
 __device__ __forceinline__ int place(int r) { return kFp4 ? r : ((r & 1) << 2) + (r >> 1); }

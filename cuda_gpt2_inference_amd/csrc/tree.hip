@@ -16,13 +16,11 @@
 // in a sum is free, so a lane's eight places of step s are positions 32 s + 4 g .. + 3 and 32 s + 16 + 4 g .. + 3,
 // and V, which is needed channel-major, is read from LDS by the transposing reads (ds_read_b64_tr_b16, b8, b4)
 // in that order.
-//   Types.  BF16 rows are operands as they are; 8-bit and 4-bit codes are exact in bf16 and in float16, and their
-//   scales go to the scores and the weights in float.  FP32 rows take 16x16x4 float products.  Weights are rounded
-//   finer than the outputs (2^-8), since one bf16 would round a sharp head's output twice: over BF16 rows a weight is two
-//   bf16 halves, upper and rest (2^-14); over codes one float16 (2^-11) of the weight times its row's scale, in a unit
-//   that the wave's largest scale so far sets (a power of two; float16 then holds weights down to 2^-29 of the largest
-//   possible, and a smaller one's error is 2^-18 of it times the largest scale at most).  With two halves over codes
-//   too: INT4, 24 sequences of up to 4096, 32 tokens each, 26.5 us.
+//   Types.  BF16 rows are operands as they are; 8-bit and 4-bit codes are exact in bf16, and their scales go to
+//   the scores and the weights in float.  FP32 rows take 16x16x4 float products.  Weights (over codes times their rows'
+//   scales) are two bf16 halves, upper and rest, 2^-14 of each, whatever the others are: one half alone would round a sharp
+//   head's output (2^-8) twice.  (One float16 is less work, but scales need all of a float's exponents: it takes a unit
+//   that the rows share, and rows whose scales lie far below another's, which may not even be attended, were lost in it.)
 //   Masks.  Only tiles that reach the new tokens look at any.  There a value that one query must not see may be
 //   infinite or NaN, which a weight of zero does not take out of a product: such a tile, found by looking at its V
 //   rows, has its outputs summed on the vector units, position by position.
@@ -250,7 +248,6 @@ __global__ __launch_bounds__(kW * kWave) __attribute__((amdgpu_waves_per_eu(3)))
     float* const ls = reinterpret_cast<float*>(lv + kTileBytes);
     F32x4 acc[4] = {};                     // channels 16 c + 4 g + i of query col
     F32x4 acc8 = {};                       // INT4: 8 sum of the weights, taken off at the end
-    float unit = 0.0f, per_unit = 0.0f;    // codes: of the weights
     // off: what the exponents are taken off (zero before the first score); limit: the score from which m follows.
     float m = -INFINITY, limit = -INFINITY, off = 0.0f, l = 0.0f;
 
@@ -277,20 +274,8 @@ __global__ __launch_bounds__(kW * kWave) __attribute__((amdgpu_waves_per_eu(3)))
             *reinterpret_cast<uint4*>(lv + at) = rv[j];
         }
         if constexpr (T::kCoded) {
-            // The weights' unit: a power of two not below the largest scale, followed where that has grown fourfold.
-            const float size = fabsf(rvs);
-            const float most = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(wave_max(size < INFINITY ? size : 0.0f))));
-            if (most > 4.0f * unit) {
-                const int e = min(max((int)(__float_as_uint(most) >> 23) + 1, 27), 254);
-                const float grown = __uint_as_float((uint32_t)e << 23), f = unit / grown;
-                unit = grown;
-                per_unit = __uint_as_float((uint32_t)(259 - e) << 23);      // 32 / unit
-#pragma unroll
-                for (int c = 0; c < 4; ++c) acc[c] *= f;
-                if constexpr (T::kInt4) acc8 *= f;
-            }
             ls[lane] = rks * kQScale;
-            ls[kPos + lane] = rvs * per_unit;
+            ls[kPos + lane] = rvs;
         }
         lds_order();
         if (k + 1 < mine) request(k + 1);
@@ -426,62 +411,63 @@ __global__ __launch_bounds__(kW * kWave) __attribute__((amdgpu_waves_per_eu(3)))
                         acc[c] = __builtin_amdgcn_mfma_f32_16x16x4f32(v, p[t][e], acc[c], 0, 0, 0);
                     }
                 }
-        } else if constexpr (T::kBf16) {
-            typedef short S16x4 __attribute__((ext_vector_type(4)));
+        } else {
+            // Step u's weights in two halves.
+            constexpr int kU = kPos / 32;
+            Bf16x8 hi[kU], lo[kU];
 #pragma unroll
-            for (int u = 0; u < kPos / 32; ++u) {
-                U32x4 hi, lo;
+            for (int u = 0; u < kU; ++u) {
+                U32x4 h, l;
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {                  // places 2 j and 2 j + 1
                     const float p0 = p[2 * u + j / 2][2 * (j % 2)], p1 = p[2 * u + j / 2][2 * (j % 2) + 1];
                     const uint32_t b0 = __float_as_uint(p0), b1 = __float_as_uint(p1);
-                    hi[j] = __builtin_amdgcn_perm(b1, b0, 0x07060302u);
+                    h[j] = __builtin_amdgcn_perm(b1, b0, 0x07060302u);
                     const float r0 = p0 - __uint_as_float(b0 & 0xffff0000u), r1 = p1 - __uint_as_float(b1 & 0xffff0000u);
-                    lo[j] = __builtin_amdgcn_perm(__float_as_uint(r1), __float_as_uint(r0), 0x07060302u);
+                    l[j] = __builtin_amdgcn_perm(__float_as_uint(r1), __float_as_uint(r0), 0x07060302u);
                 }
+                hi[u] = __builtin_bit_cast(Bf16x8, h);
+                lo[u] = __builtin_bit_cast(Bf16x8, l);
+                if constexpr (T::kInt4) {
+                    acc8 = mfma((Bf16x8)(__bf16)8.0f, hi[u], acc8);
+                    acc8 = mfma((Bf16x8)(__bf16)8.0f, lo[u], acc8);
+                }
+            }
 #pragma unroll
-                for (int c = 0; c < 4; ++c) {
+            for (int c = 0; c < 4; ++c) {
+                Bf16x8 va[2];
+                if constexpr (T::kBf16) {
+                    typedef short S16x4 __attribute__((ext_vector_type(4)));
                     S16x4 part[2];
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
-                        const int row = 32 * u + 16 * e + 4 * g + (col >> 2);
+                        const int row = 16 * e + 4 * g + (col >> 2);
                         part[e] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
                             (__attribute__((address_space(3))) S16x4*)(lv + row * T::kRow +
                                 16 * T::chunk_at(row, 2 * c + ((col >> 1) & 1)) + 8 * (col & 1)));
                     }
-                    const Bf16x8 va = __builtin_bit_cast(Bf16x8, __builtin_shufflevector(part[0], part[1], 0, 1, 2, 3, 4, 5, 6, 7));
-                    acc[c] = mfma(va, __builtin_bit_cast(Bf16x8, hi), acc[c]);
-                    acc[c] = mfma(va, __builtin_bit_cast(Bf16x8, lo), acc[c]);
-                }
-            }
-        } else {
-            F16x8 w[2];
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-#pragma unroll
-                for (int x = 0; x < 8; ++x) w[u][x] = (_Float16)p[2 * u + x / 4][x % 4];
-                if constexpr (T::kInt4) acc8 = mfma((F16x8)(_Float16)8.0f, w[u], acc8);
-            }
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                F16x8 va[2];
-                if constexpr (T::k8) {
+                    va[0] = __builtin_bit_cast(Bf16x8, __builtin_shufflevector(part[0], part[1], 0, 1, 2, 3, 4, 5, 6, 7));
+                } else if constexpr (T::k8) {
+                    I32x2 part[2];
 #pragma unroll
                     for (int u = 0; u < 2; ++u) {
                         const int e = col >> 1, row = 32 * u + 16 * (e >> 2) + 4 * g + (e & 3);
-                        const I32x2 v = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
+                        part[u] = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
                             (__attribute__((address_space(3))) I32x2*)(lv + row * T::kRow + 16 * T::chunk_at(row, c) + 8 * (col & 1)));
-                        va[u] = codes_to_f16<T::kFp8>((uint32_t)v[0], (uint32_t)v[1]);
                     }
+                    codes_to_bf16<T::kFp8>(U32x4{(uint32_t)part[0][0], (uint32_t)part[0][1], (uint32_t)part[1][0], (uint32_t)part[1][1]}, va);
                 } else {
                     const int e = place<T::kFp4>(col & 7), row = 32 * (col >> 3) + 16 * (e >> 2) + 4 * g + (e & 3);
                     const I32x2 v = __builtin_amdgcn_ds_read_tr4_b64_v2i32(
                         (__attribute__((address_space(3))) I32x2*)(lv + row * T::kRow + 8 * c));
-                    va[0] = operand16<T::kFp4>((uint32_t)v[0]);
-                    va[1] = operand16<T::kFp4>((uint32_t)v[1]);
+                    va[0] = operand<T::kFp4>((uint32_t)v[0]);
+                    va[1] = operand<T::kFp4>((uint32_t)v[1]);
                 }
 #pragma unroll
-                for (int u = 0; u < 2; ++u) acc[c] = mfma(va[u], w[u], acc[c]);
+                for (int u = 0; u < kU; ++u) {
+                    acc[c] = mfma(va[u], hi[u], acc[c]);
+                    acc[c] = mfma(va[u], lo[u], acc[c]);
+                }
             }
         }
         lds_order();
@@ -495,7 +481,6 @@ __global__ __launch_bounds__(kW * kWave) __attribute__((amdgpu_waves_per_eu(3)))
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
         if constexpr (T::kInt4) acc[c] -= acc8;
-        if constexpr (T::kCoded) acc[c] *= unit * 0.03125f;
         *reinterpret_cast<F32x4*>(ro + col * kOutPad + 16 * c + 4 * g) = acc[c];
     }
     const float sum = op_xor32<false>(op_xor16<false>(l));

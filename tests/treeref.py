@@ -92,10 +92,8 @@ def attend(q, k, v, seen, kscale, vscale, kv):
     roundings of 2^-24 of the sum of magnitudes, in which an INT4 code counts 15 + 8 (the operand adds 8, and -8 times
     the sum of q starts the sum); two roundings of the scale's product; the exponent's difference rounds once more.  A
     weight is exp2 of that (2^-22 for the instruction); over BF16 rows it is cut to two bf16 halves (2^-14), over codes its
-    product with the row's scale is rounded to float16: half a step, 2^-11 of it (float16 keeps 10 bits behind the first),
-    or, below 2^-14 in the wave's unit, 2^-25: the unit is the largest scale over 32 to 128, so 2^-18 of w times that
-    scale over the codes.  Sums: a rounding for each 32 rows of a product, the joins of waves and segments, the total's
-    division; then half a step of the output."""
+    product with the row's scale, with room for a float16 of it (2^-11).  Sums: a rounding for each 32 rows of a product,
+    the joins of waves and segments, the total's division; then half a step of the output."""
     n = len(seen)
     if n == 0:
         return np.zeros(HS), np.full(HS, 2.0 ** -126)
