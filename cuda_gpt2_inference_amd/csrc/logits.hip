@@ -359,7 +359,8 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(4))) v
 #pragma unroll
         for (int i = 0; i < kRun; ++i) y[i] = exp2_fast((y[i] - top) * scale);
     };
-    // The tokens' maximum, and the sum of their weights against it (in their places), or which one is the largest.
+    // The tokens' maximum, and the sum of their weights against it (in their places), or which one is the largest.  (Maxima
+    // pass NaN over.  Beside a number its weight makes the sum NaN; where there is none but -inf it is looked for.)
     auto reduce = [&] {
         top = -INFINITY;
         each([&](int, float (&y)[kRun]) {
@@ -376,8 +377,8 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(4))) v
             each([&](int v, float (&y)[kRun]) {
 #pragma unroll
                 for (int i = 0; i < kRun; ++i) {
-                    const unsigned long long key = 0xffffffffu - (uint32_t)(v + i);
-                    if (y[i] == top && v + i < v1 && key > best) best = key;
+                    const unsigned long long key = y[i] != y[i] ? 1ull << 32 : 0xffffffffu - (uint32_t)(v + i);
+                    if ((y[i] == top || (y[i] != y[i] && top == -INFINITY)) && v + i < v1 && key > best) best = key;
                 }
             });
 #pragma unroll
@@ -390,7 +391,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(4))) v
 #pragma unroll
             for (int w = 0; w < kWaves; ++w) best = wave_keys[w] > best ? wave_keys[w] : best;
             token = top == -INFINITY ? -1 : (int)(0xffffffffu - (uint32_t)best);
-            sum = 0.0f;
+            sum = !likeliest && best >> 32 ? NAN : 0.0f;
         } else {
             sum = 0.0f;
             each([&](int, float (&y)[kRun]) {
@@ -407,7 +408,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(4))) v
     };
     reduce();
     float one = 1.0f / sum;                    // what a weight is multiplied with
-    bool none = top == -INFINITY;
+    bool none = top == -INFINITY && sum == 0.0f;
     if constexpr (kShare) {
         // A slice's words: its maximum; its sum, or its likeliest token.
         unsigned long long* const words = a.exchange + (size_t)launch_row * a.slices * 2;
@@ -461,16 +462,19 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(4))) v
             }
         }
         // A lane for every slice.
-        const float its_top = lane < a.slices ? slice_top[lane] : -INFINITY, its_sum = slice_sum[lane];
+        const float its_top = lane < a.slices ? slice_top[lane] : -INFINITY, its_sum = lane < a.slices ? slice_sum[lane] : 0.0f;
         const float all = wave_max(its_top);
         none = all == -INFINITY;
         if (likeliest) {
             const unsigned long long at = __ballot(its_top == all);
             token = __builtin_amdgcn_readlane(__float_as_int(its_sum), __ffsll((long long)(at | 1ull << 63)) - 1);
         } else {
-            // (A slice that allows nothing has a sum of zero, and its maximum may not be taken a difference of.)
-            const float total = wave_sum(its_top == -INFINITY ? 0.0f : exp2_fast((its_top - all) * scale) * its_sum);
-            one = (top == -INFINITY ? 0.0f : exp2_fast((top - all) * scale)) / total;
+            // (A slice without a number has a sum of zero, or NaN, and its maximum may not be taken a difference of.)
+            const float total = wave_sum(its_top == -INFINITY ? its_sum : exp2_fast((its_top - all) * scale) * its_sum);
+            none = none && total == 0.0f;
+            // (Beside an infinity in another slice nothing weighs anything.)
+            const float part = top == -INFINITY ? 0.0f : exp2_fast((top - all) * scale);
+            one = part == 0.0f ? 0.0f : part / total;
         }
     }
     if (likeliest || none) {
@@ -484,10 +488,13 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(4))) v
     }
     const bool empty = top == -INFINITY;       // (of a slice: its logits were left as they are)
     each([&](int v, float (&y)[kRun]) {
-        if constexpr (kRuns == 0) weigh(y);
+        if (kRuns == 0 && !empty) weigh(y);
         // (A forbidden token has none, also where the others' is NaN.)
 #pragma unroll
-        for (int i = 0; i < kRun; ++i) y[i] = empty || y[i] == 0.0f ? 0.0f : y[i] * one;
+        for (int i = 0; i < kRun; ++i) {
+            if (empty) y[i] = y[i] != y[i] ? y[i] : 0.0f;
+            else y[i] = y[i] == 0.0f ? 0.0f : y[i] * one;
+        }
         store_run<kOutF32>(a.out, out0, v, v1, a.vec, y);
     });
 }

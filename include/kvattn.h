@@ -599,7 +599,8 @@ size_t kvattn_logits_workspace_bytes(void);
 /* The rules on rows of V logits, in the order above, in float: repetition, frequency and presence, bias, allowed.
  *   probs 0: the logits (-inf where not allowed); 1: softmax(x / temperature), as kvattn_verify_drafts and
  *            kvattn_verify_tree take it; a row that allows nothing becomes zeros, one with a NaN or +inf that is
- *            allowed NaN where it is not zero
+ *            allowed NaN where it is not zero (the likeliest token is looked for among numbers; zeros where there
+ *            are none)
  *   rules    host struct, read by the call (the arrays it names are read when the kernel runs); NULL: none
  *   token_start [B+1] device: rows token_start[b] .. token_start[b+1]-1 are sequence b's; rows behind token_start[B]
  *            are left as they were.  NULL: row b is sequence b's (rows == B)
