@@ -477,24 +477,24 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(4))) v
             one = part == 0.0f ? 0.0f : part / total;
         }
     }
-    if (likeliest || none) {
-        // The likeliest token alone; nothing where no token is left.
+    if (likeliest || none || top == -INFINITY) {
+        // The likeliest token alone; nothing where no token is left; of tokens without a number among them, whose logits were
+        // left as they are, NaN alone.
         each([&](int v, float (&y)[kRun]) {
 #pragma unroll
-            for (int i = 0; i < kRun; ++i) y[i] = !none && v + i == token ? 1.0f : 0.0f;
+            for (int i = 0; i < kRun; ++i) {
+                const float other = likeliest || none || y[i] == y[i] ? 0.0f : y[i];
+                y[i] = likeliest && !none && v + i == token ? 1.0f : other;
+            }
             store_run<kOutF32>(a.out, out0, v, v1, a.vec, y);
         });
         return;
     }
-    const bool empty = top == -INFINITY;       // (of a slice: its logits were left as they are)
     each([&](int v, float (&y)[kRun]) {
-        if (kRuns == 0 && !empty) weigh(y);
+        if constexpr (kRuns == 0) weigh(y);
         // (A forbidden token has none, also where the others' is NaN.)
 #pragma unroll
-        for (int i = 0; i < kRun; ++i) {
-            if (empty) y[i] = y[i] != y[i] ? y[i] : 0.0f;
-            else y[i] = y[i] == 0.0f ? 0.0f : y[i] * one;
-        }
+        for (int i = 0; i < kRun; ++i) y[i] = y[i] == 0.0f ? 0.0f : y[i] * one;
         store_run<kOutF32>(a.out, out0, v, v1, a.vec, y);
     });
 }
