@@ -95,7 +95,7 @@ __global__ __launch_bounds__(kGemmWaves * kWave) void gemm_kernel(
     constexpr int kXP = F::kXBytes / 16;    // 16-byte pieces of x per weight chunk
     constexpr int kIts = (kR * kCols + kGemmWaves * kWave - 1) / (kGemmWaves * kWave);
     static_assert(kR % 16 == 0, "whole operands");
-    extern __shared__ float red[];          // [waves][kCols][kPitch]
+    extern __shared__ __align__(16) float red[];       // [waves][kCols][kPitch]
     a.B = pk_B;
     a.M = pk_M & kRowMask;
     const int K = pk_K;

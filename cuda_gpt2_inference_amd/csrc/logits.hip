@@ -118,7 +118,7 @@ template <bool kInF32, bool kOutF32, bool kProbs, int kThreads, int kRuns, bool 
 __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(4))) void logits_kernel(LogitArgs a) {
     constexpr int kWaves = kThreads / kWave, kStep = kThreads * kRun;      // tokens from one run of a thread to its next
     static_assert(!kShare || (kProbs && kRuns > 0), "slices in registers");
-    extern __shared__ uint32_t lds[];          // map, allowed tokens, named tokens, counts, biases, prefixes (16 bits)
+    extern __shared__ __align__(16) uint32_t lds[];    // map, allowed tokens, named tokens, counts, biases, prefixes (16 bits)
     __shared__ uint32_t wave_words[kWaves];
     __shared__ float wave_floats[2][kWaves];
     __shared__ unsigned long long wave_keys[kWaves];
