@@ -34,7 +34,7 @@ constexpr int kSliceThreads = 512, kRowThreads = 1024;     // of a slice's workg
 constexpr int kMostSlices = 64;                // of a row whose slices exchange words: a lane each
 constexpr int kTogether = 512;                 // workgroups of kSliceThreads that run at once: two a CU
 constexpr int kMaxVocab = 1 << 18;
-constexpr int kMaxRows = 1 << 21;              // workgroups of a grid: 2^32 threads are too many
+constexpr int kMaxRows = 1 << 21;              // whole rows of a grid: 2^32 threads are too many
 constexpr int kMaxSequences = 1 << 20;
 constexpr int kSmallRuns = 2;                  // of a slice whose table always has an entry for every token
 constexpr int kManyIds = 4096;                 // of a history and its biases, from which slices of 4 runs have such a table
@@ -626,6 +626,8 @@ extern "C" int kvattn_process_logits(void* out, const void* logits, const kvattn
         lds = lds_of(p);
     }
     if (lds > kLdsMost) return KVATTN_ERR_LDS;
+    // (Nor may a grid of slices have 2^32 threads.)
+    launch_rows = (int)std::min<long long>(launch_rows, ((1ll << 32) - 1) / ((long long)p.slices * p.threads));
     a.slices = p.slices;
     a.slice = p.tokens;
     a.exchange = (unsigned long long*)r.workspace;
@@ -636,7 +638,6 @@ extern "C" int kvattn_process_logits(void* out, const void* logits, const kvattn
     }
     for (a.row0 = 0; a.row0 < rows; a.row0 += launch_rows) {
         const long long grid = (long long)std::min(launch_rows, rows - a.row0) * p.slices;
-        if (grid * p.threads >= (1ll << 32)) return KVATTN_ERR_SHAPE;
         void* params[] = {&a};
         const int st = hip_status(hipLaunchKernel(p.fn, dim3((unsigned)grid), dim3(p.threads), params, lds, (hipStream_t)stream));
         if (st != KVATTN_OK) return st;
