@@ -285,6 +285,10 @@ using kvattn_layout::guess_slot_live;
 using kvattn_layout::xcd_slot;
 using kvattn_layout::xcd_slot_rotated;
 
+// The wave's LDS operations run in order, so what its lanes hand one another there needs no barrier;
+// this keeps the compiler from moving one lane's reads over another's writes.
+__device__ __forceinline__ void lds_order() { asm volatile("" ::: "memory"); }
+
 // s_waitcnt vmcnt(0) (GFX9 encoding: expcnt and lgkmcnt fields left at their maximum),
 // fenced against compiler reordering on both sides.
 __device__ __forceinline__ void wait_vm_stores() {

@@ -101,10 +101,6 @@ __device__ __forceinline__ void put4(float* p, const F32x4& v) {
 // exp2(m - M) with an empty side (m = -inf) weighing nothing.
 __device__ __forceinline__ float weight_of(float m, float M) { return m == -INFINITY ? 0.0f : exp2_fast(m - M); }
 
-// The wave's LDS operations run in order, so what its lanes hand one another there needs no barrier;
-// this keeps the compiler from moving one lane's reads over another's writes.
-__device__ __forceinline__ void lds_order() { asm volatile("" ::: "memory"); }
-
 // Keeps a wave's rare branch from becoming selects that every tile runs.
 __device__ __forceinline__ void stay_a_branch() { asm volatile(""); }
 

@@ -214,11 +214,13 @@ __device__ __forceinline__ Walk walk_tree(const VerifyArgs& a, int t0, int n, in
                 }
             }
         }
-        if (next < 0) return w;
+        if (next < 0) break;
         at = next;
         ++w.depth;
         if (lane == 0) path[w.depth] = at;
     }
+    lds_order();                           // every lane reads what the first one wrote
+    return w;
 }
 
 template <bool kF32, bool kVec, bool kTree>
