@@ -31,6 +31,7 @@ constexpr int kBlockBytes = kRows * kCols / 2;
 constexpr int kW4Waves = 8;
 constexpr int kTallGroups = 256;               // workgroups: one a CU
 constexpr size_t kTallLds = 152 * 1024;
+constexpr int kMostCols = 65535;               // the grid's second side
 // Where a matrix's blocks and scales lie.
 struct W4Shape {
     int M, K, group, tiles, steps, groups;     // row tiles, blocks of a row tile, groups of a block
@@ -534,8 +535,6 @@ int kvattn_gemv_w4(void* out, void* pre_gelu, const void* w4, const void* x, con
     }
     const void* fn = nt == 1 ? kernel_for<1>(fp4, s.groups, row_tiles, B, f32)
                              : nt == 2 ? kernel_for<2>(fp4, s.groups, row_tiles, B, f32) : kernel_for<4>(fp4, s.groups, row_tiles, B, f32);
-    const long long cols = (B + 16 * nt - 1) / (16 * nt);
-    if (cols > 65535) return KVATTN_ERR_SHAPE;
     int groups = kTallGroups;
     const int grid = row_tiles ? (s.tiles + row_tiles - 1) / row_tiles : groups, waves = row_tiles ? kW4Waves : kTallW4Waves;
     const size_t lds = row_tiles ? (size_t)kW4Waves * nt * 16 * std::max(256, (row_tiles * kRows + 4) * 4) : x_lds(nt);
@@ -544,7 +543,17 @@ int kvattn_gemv_w4(void* out, void* pre_gelu, const void* w4, const void* x, con
         if (st != KVATTN_OK) return st;
     }
     void* params[] = {&a, &groups};
-    return hip_status(hipLaunchKernel(fn, dim3((unsigned)grid, (unsigned)cols), dim3(waves * kWave), params, lds, (hipStream_t)stream));
+    // More vectors than a grid has columns for go in several launches.
+    for (int b0 = 0; b0 < B; b0 += kMostCols * 16 * nt) {
+        a.B = std::min(B - b0, kMostCols * 16 * nt);
+        a.x = (const uint16_t*)x + (size_t)b0 * K;
+        a.out = (uint8_t*)out + (size_t)b0 * M * osz;
+        if (pre_gelu) a.pre_gelu = (uint8_t*)pre_gelu + (size_t)b0 * M * osz;
+        const int cols = (a.B + 16 * nt - 1) / (16 * nt);
+        const int st = hip_status(hipLaunchKernel(fn, dim3((unsigned)grid, (unsigned)cols), dim3(waves * kWave), params, lds, (hipStream_t)stream));
+        if (st != KVATTN_OK) return st;
+    }
+    return KVATTN_OK;
 }
 
 }  // extern "C"
