@@ -31,6 +31,7 @@ constexpr int kBlockBytes = kRows * kCols / 2;
 constexpr int kW4Waves = 8;
 constexpr int kTallGroups = 256;               // workgroups: one a CU
 constexpr size_t kTallLds = 152 * 1024;
+constexpr int kMostRows = (1 << 28) - 32;      // workgroups of two row tiles: 2^32 threads are too many
 constexpr int kMostCols = 65535;               // the grid's second side
 // Where a matrix's blocks and scales lie.
 struct W4Shape {
@@ -501,7 +502,7 @@ int kvattn_gemv_w4(void* out, void* pre_gelu, const void* w4, const void* x, con
     W4Shape s;
     if (!is_4bit(w_dtype) || (out_dtype != KVATTN_KV_F32 && out_dtype != KVATTN_KV_BF16)) return KVATTN_ERR_DTYPE;
     if (!shape_of(M, K, group, s)) return KVATTN_ERR_SHAPE;
-    if (B < 1 || M >= (1 << 28) || (long long)B * M >= (1ll << 31) || (long long)B * K >= (1ll << 31)) return KVATTN_ERR_SHAPE;
+    if (B < 1 || M > kMostRows || (long long)B * M >= (1ll << 31) || (long long)B * K >= (1ll << 31)) return KVATTN_ERR_SHAPE;
     if (!out || !w4 || !x) return KVATTN_ERR_NULL_POINTER;
     const size_t osz = out_dtype == KVATTN_KV_F32 ? 4 : 2;
     if (((uintptr_t)w4 & 15u) || ((uintptr_t)x & 15u) || ((uintptr_t)out % osz) || ((uintptr_t)pre_gelu % osz) || ((uintptr_t)bias & 1u))

@@ -691,8 +691,8 @@ int kvattn_w4_pack(void* w4, const void* codes, const void* scales, int M, int K
 int kvattn_w4_quantize(void* w4, const void* W, int M, int K, int group, int src_dtype, int w_dtype, void* stream);
 
 /* out[b][m] = act(sum_k weight[m][k] x[b][k] + bias[m]) with FP32 sums; x, bias (may be NULL) bf16, out and pre_gelu
- * (may be NULL) float or bf16 by out_dtype; gelu as in kvattn_gemv.  Any B, on the matrix cores; M < 2^28, B M and B K
- * < 2^31.  A vector that is not finite spoils its own outputs alone (of INT4 codes an infinity gives NaN). */
+ * (may be NULL) float or bf16 by out_dtype; gelu as in kvattn_gemv.  Any B, on the matrix cores; M <= 2^28 - 32, B M and
+ * B K < 2^31.  A vector that is not finite spoils its own outputs alone (of INT4 codes an infinity gives NaN). */
 int kvattn_gemv_w4(void* out, void* pre_gelu, const void* w4, const void* x, const void* bias, int B, int M, int K,
                    int group, int w_dtype, int out_dtype, int gelu, void* stream);
 
