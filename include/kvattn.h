@@ -593,7 +593,8 @@ typedef struct kvattn_logit_rules {
  * (kvattn_workspace_init), of no further content between calls.  Calls sharing it must be ordered, and only calls of
  * kvattn_process_logits may.  The slices of a row wait for one another's maxima, within the bound of
  * kvattn_set_merge_poll_limit; one that stops waiting works the others' out itself (the result is the same, bit for
- * bit). */
+ * bit).  So where another stream's work keeps some of them off the GPU for long, the others wait for the whole bound and
+ * then do up to as many slices' work as their row has: without a workspace a call has no such wait. */
 size_t kvattn_logits_workspace_bytes(void);
 
 /* The rules on rows of V logits, in the order above, in float: repetition, frequency and presence, bias, allowed.
