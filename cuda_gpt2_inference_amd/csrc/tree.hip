@@ -663,7 +663,7 @@ int attend_tree(const AttendTree& c) {
         const int tile = c.kv_dtype == KVATTN_KV_F32 ? Kv<KVATTN_KV_F32>::kPos : c.kv_dtype == KVATTN_KV_BF16 ? Kv<KVATTN_KV_BF16>::kPos : 64;
         const int least = waves == 8 ? 16 : heads <= 2 * kCUs ? 4 : 32 * tile / kSeg;
         const long long want = heads <= 2 * kCUs ? 6 * kCUs / heads : kMaxSegments;
-        S = (int)std::max<long long>(1, std::min<long long>({want, (tiles + least - 1) / least, 16}));
+        S = (int)std::max<long long>(1, std::min<long long>({want, (tiles + least - 1) / least, 16, kMostWaves / waves / heads}));
         seg_tiles = (tiles + S - 1) / S;
     }
     if (c.B > 65535 || heads * S * waves > kMostWaves) return KVATTN_ERR_SHAPE;

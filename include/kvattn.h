@@ -441,7 +441,8 @@ int kvattn_tree_masks(unsigned long long* masks, int* positions, const int* pare
  * are skipped.  16 tokens of a sequence share a pass over the cache.
  *   max_new  the most tokens of one sequence, at most 64 * mask_words (or num_tokens is); a sequence with
  *            more has the first max_new or more of them computed
- * Other arguments, limits and the workspace as in kvattn_paged_decode_tokens; B <= 65535. */
+ * B <= 65535; B * NH, num_tokens * NH and B * NH * (max_new or num_tokens, the smaller, / 16 rounded up) below 2^24.
+ * Other arguments, limits and the workspace as in kvattn_paged_decode_tokens. */
 int kvattn_paged_decode_tree(void* out, const void* qkv, const void* pages, const float* page_scales,
                              const int* block_table, int max_pages, int page_rows, int num_pages,
                              const int* token_start, const int* lens, const unsigned long long* masks, int mask_words,
