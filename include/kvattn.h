@@ -679,7 +679,7 @@ int kvattn_gemv_qkv_append(void* qkv, const void* W, const float* w_scale, const
 /* ---- 4-bit weights with a scale for every group --------------------------------------------
  * kvattn_gemv_ex on INT4 or FP4_E2M1 codes whose scales are bf16, one for every `group` (32, 64 or 128)
  * neighbours of a row: weight [m][k] = code * scale[m][k / group], codes as in the 4-bit caches (INT4: half byte - 8,
- * here -8 too; FP4: sign and one of 0 .5 1 1.5 2 3 4 6).  K is a multiple of group, K <= 2^20, M any.
+ * here -8 too; FP4: sign and one of 0 .5 1 1.5 2 3 4 6).  K is a multiple of group, K <= 2^20, M < 2^29, M K < 2^40.
  * No reference counterpart (its weights end at 8 bits, with one scale a row).
  * Weights are laid out once for the kernels: w4, 16-byte aligned, of kvattn_w4_bytes(M, K, group) bytes (0: such a
  * matrix is refused); what is in it depends on M, K and group. */
