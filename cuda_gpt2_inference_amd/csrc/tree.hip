@@ -7,7 +7,8 @@
 // find in the caches.  (Two or four groups of 16 in one workgroup take registers that other workgroups hide latency
 // with: BF16, 26 tokens over 1000 positions 9.6 us in place of 7.6, INT4 64 x 64 tokens 43.4 and 41.0, BF16 16 x 64 over
 // 8192 46.0 and 46.6.  One behind the other on one XCD they share its L2, which then reads the cache once, but a long
-// sequence's wait for one another: BF16 16 x 64 45.7 us of 48.2, INT4 64 x 64 47.6 of 41.1.)
+// sequence's wait for one another: BF16 16 x 64 45.7 us of 48.2, INT4 64 x 64 47.6 of 41.1.  All on one state, whose cache
+// rows the Infinity Cache holds, INT4's in weights of one float16; in turn with others BF16 16 x 64 takes 60.)
 //
 // Both products go to the matrix cores, scores as S^T = K Q^T and outputs as O^T = V^T P^T.  Of S^T lane
 // 16 g + c holds positions 16 t + 4 g .. + 3 of query c.  That makes everything the softmax does (maximum, sum,
@@ -637,17 +638,19 @@ int attend_tree(const AttendTree& c) {
     // Workgroups of 8 waves where there are few, in segments of at least 1024 positions.  Else 4 waves: up to two workgroups
     // a CU, as many segments as make the six a CU that run in two rounds, of at least 256 positions; beyond, segments of 32
     // tiles, so that the longest sequence is not waited for alone.  All segments have one length (a short sequence has
-    // fewer).  us per call, positions of a segment : us:
+    // fewer).  us per call in a graph on one state, positions of a segment : us:
     //   BF16  1 x 12 heads of 1000, 26 tokens   8 waves one 7.6, 512: 8.8, 256: 8.0
     //   BF16  1 x 12 of 8000, 16                8 waves 1024: 10.9, 512: 11.4, 2048: 13.7; 4 waves 512: 11.3
-    //   FP4   1 x 12 of 1000, 7                 8 waves one 6.2, 256: 7.6; 4 waves one 7.0
-    //   FP8   3 x 25 of 1999, 7                 4 waves 256: 9.2, 512: 9.7, one 12.9; 8 waves one 10.4
+    //   FP4   1 x 12 of 1000, 7                 8 waves one 6.2, 256: 7.6; 4 waves one 6.8
+    //   FP8   3 x 25 of 1999, 7                 4 waves 256: 9.2, 512: 10.1, one 13.2; 8 waves one 10.9
     //   BF16  8 x 12 ragged of up to 2048, 16   4 waves 256: 9.2, 512: 10.1, one 13.8; 8 waves 11
-    //   INT8  8 x 12 ragged of up to 4096, 64   4 waves 1024: 20.0, 512: 22.4, 2048: 23.0, one 25.9
-    //   INT4 24 x 12 ragged of up to 4096, 32   4 waves 2048: 23.7, 1024: 26.1, one 27.6
+    //   INT8  8 x 12 ragged of up to 4096, 64   4 waves 1024: 20.5, 512: 22.5, 2048: 24.0, one 28.1; 8 waves one 19.3
+    //   INT4 24 x 12 ragged of up to 4096, 32   4 waves 2048: 26.0, 1024: 25.3, one 28.9; 8 waves one 23.0
     //   BF16 16 x 12 ragged of up to 8192, 64   4 waves 1024: 46.6, 512: 50.1, 2048: 50.6, one 53.3
-    //   FP8  64 x 12 ragged of up to 1024, 16   4 waves one 16.4, 512: 23.6
-    //   INT4 64 x 12 ragged of up to 2048, 64   4 waves one 41.0, 1024: 64
+    //   FP8  64 x 12 ragged of up to 1024, 16   4 waves one 16.4, 512: 23.4; 8 waves one 21.0
+    //   INT4 64 x 12 ragged of up to 2048, 64   4 waves one 39.4, 1024: 61; 8 waves one 44.6
+    // Behind other work (256 MB written before every call), by segments of 512, 1024, 2048, one: BF16 16 x 12 71.8, 72.8,
+    // 79.0, 88.6; INT4 24 x 12 34.9, 33.3, 31.8, 35.6; INT8 8 x 12 25.5, 23.8, 26.3, 30.4.
     const int waves = heads <= kFewHeads ? 8 : 4;
     const int tiles = (c.maxT + kSeg - 1) / kSeg;
     int S = 1, seg_tiles = 1;

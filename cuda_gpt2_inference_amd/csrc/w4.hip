@@ -521,7 +521,9 @@ int kvattn_gemv_w4(void* out, void* pre_gelu, const void* w4, const void* x, con
     // Two row tiles halve the vectors' loads, where workgroups for the GPU are left.  Of 32 vectors 512 row tiles run at once
     // either way, and a last round that is less than half full is shorter with one; of 64 vectors 256 and 512 run at once.
     // Vectors in LDS pay where a matrix is tall, the more the vectors (their filling: one vector over long rows never);
-    // 64 that do not fit go in two halves (64 x 32000 x 1600 25.8 us).
+    // 64 that do not fit go in two halves (64 x 32000 x 1600 23.7 us).  FP4 and groups of 32 go by the same borders: at these
+    // sizes within 5 % of the fastest of the three, but for INT4 in groups of 32 at 1 x 50304 x 768 (7.7, two row tiles 6.8) and
+    // 32 x 20000 x 1600 (13.8, one row tile 12.2).
     const long long work = (long long)s.tiles * ((B + 16 * nt - 1) / (16 * nt)), last = work % 512;
     int row_tiles = 1;
     if (nt == 1) row_tiles = work >= (B <= 4 ? 512 : 320) ? 2 : 1;
