@@ -359,8 +359,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(4))) v
 #pragma unroll
         for (int i = 0; i < kRun; ++i) y[i] = exp2_fast((y[i] - top) * scale);
     };
-    // The tokens' maximum, and the sum of their weights against it (in their places), or which one is the largest.  (Maxima
-    // pass NaN over.  Beside a number its weight makes the sum NaN; where there is none but -inf it is looked for.)
+    // The tokens' maximum, and the sum of their weights against it (in their places), or which one is the largest.
     auto reduce = [&] {
         top = -INFINITY;
         each([&](int, float (&y)[kRun]) {
@@ -377,8 +376,8 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(4))) v
             each([&](int v, float (&y)[kRun]) {
 #pragma unroll
                 for (int i = 0; i < kRun; ++i) {
-                    const unsigned long long key = y[i] != y[i] ? 1ull << 32 : 0xffffffffu - (uint32_t)(v + i);
-                    if ((y[i] == top || (y[i] != y[i] && top == -INFINITY)) && v + i < v1 && key > best) best = key;
+                    const unsigned long long key = 0xffffffffu - (uint32_t)(v + i);
+                    if (y[i] == top && v + i < v1 && key > best) best = key;
                 }
             });
 #pragma unroll
@@ -391,7 +390,21 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(4))) v
 #pragma unroll
             for (int w = 0; w < kWaves; ++w) best = wave_keys[w] > best ? wave_keys[w] : best;
             token = top == -INFINITY ? -1 : (int)(0xffffffffu - (uint32_t)best);
-            sum = !likeliest && best >> 32 ? NAN : 0.0f;
+            sum = 0.0f;
+            // NaN, which maxima pass over, makes the sum NaN beside a number; without one it is found here, as every sum of
+            // -inf alone is -inf.  (Weights taken against zero would show it too, but beside that branch alone the compiler
+            // spills a hundred registers of 13 runs: 256 rows 43 us in place of 31.)
+            if (!likeliest) {
+                sum = 0.0f;
+                each([&](int, float (&y)[kRun]) { sum += (y[0] + y[1]) + (y[2] + y[3]); });
+                sum = wave_sum(sum);
+                if (lane == 0) wave_floats[1][wave] = sum;
+                __syncthreads();
+                sum = 0.0f;
+#pragma unroll
+                for (int w = 0; w < kWaves; ++w) sum += wave_floats[1][w];
+                sum = sum == sum ? 0.0f : sum;
+            }
         } else {
             sum = 0.0f;
             each([&](int, float (&y)[kRun]) {
