@@ -9,13 +9,13 @@
 // sequence holds is a list of ids, so the tokens that any rule names are few against the vocabulary: they are set bits of
 // a map in LDS (a bit a token), and a token's place among the set bits, from a prefix sum over the map's words, is its
 // entry in a table: a thread for every entry works its logit out.  A row's four neighbouring tokens look at four
-// bits, and only where one is set at the table.  In small slices of a row, and in larger ones of long lists, the table has
-// an entry for every token (counts, that each thread works its own logits out from), which takes no map, no places and fewer
-// barriers.  The row of a token of a tree holds its branch too (the bits of its mask), so every row builds its own table.
+// bits, and only where one is set at the table.  In slices of a row whose counts fit beside another workgroup's, the table
+// has an entry for every token (counts, that each thread works its own logits out from), which takes no map, no places and
+// fewer barriers.  The row of a token of a tree holds its branch too (the bits of its mask), so every row builds its own table.
 // (Eight rows of a sequence in one workgroup with one table: 32 trees of up to 8 rows 24 us in place of 19, since fewer
 // workgroups hide the same chain of loads and barriers.)
 //
-// A row on one CU takes the CU's time for its arithmetic (a dozen instructions a token and the table: 18 us for one row of
+// A row on one CU takes the CU's time for its arithmetic (a dozen instructions a token and the table: 19 us for one row of
 // 50257), so few rows are cut into slices, a workgroup each (7 us).  Of probabilities the slices of a row exchange their
 // maxima and sums as tagged words in the workspace, while all of them are on the GPU; a slice that waits in vain works the
 // missing ones out itself.
@@ -36,8 +36,7 @@ constexpr int kTogether = 512;                 // workgroups of kSliceThreads th
 constexpr int kMaxVocab = 1 << 18;
 constexpr int kMaxRows = 1 << 21;              // whole rows of a grid: 2^32 threads are too many
 constexpr int kMaxSequences = 1 << 20;
-constexpr int kSmallRuns = 2;                  // of a slice whose table always has an entry for every token
-constexpr int kManyIds = 4096;                 // of a history and its biases, from which slices of 4 runs have such a table
+constexpr int kSmallRuns = 2;                  // of a slice of logits whose table has biases too
 constexpr int kIds = 8, kNamed = 2;             // ids and named tokens of a thread that are asked for ahead
 constexpr int kLdsMost = 156 * 1024;           // a CU's, less what is static here
 constexpr int kLdsTogether = 76 * 1024;        // two workgroups a CU
@@ -395,7 +394,6 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(4))) v
             // -inf alone is -inf.  (Weights taken against zero would show it too, but beside that branch alone the compiler
             // spills a hundred registers of 13 runs: 256 rows 43 us in place of 31.)
             if (!likeliest) {
-                sum = 0.0f;
                 each([&](int, float (&y)[kRun]) { sum += (y[0] + y[1]) + (y[2] + y[3]); });
                 sum = wave_sum(sum);
                 if (lane == 0) wave_floats[1][wave] = sum;
@@ -531,11 +529,12 @@ template <bool kInF32, bool kOutF32, bool kProbs>
 LogitPlan plan_for(int rows, int V, bool share, const kvattn_logit_rules& r) {
     // The smallest slices with which a call's workgroups run at once; of logits alone, which wait for none, up to 8192
     // tokens.  us per call, 50257 logits:
-    //   probabilities of 1 row, history of 1000: slices 6.8, one workgroup 17.9; 64: 13.2 / 21.9; 256: 29.9 / 42
-    //   64 rows, slices of 8192, an entry for every token or for the named: history of 2000 14.4 / 14.0, 100 and biases
-    //     16.2 / 12.0, 8000 and biases 19.3 / 26.8; 120 rows, of 16384, history of 20000 35 / 84, 5000 24.9 / 23.1
-    //   logits of about 2000 rows, history of 2000, slices of 8192 tokens, 4096, 16384: 90.9, 113.5, 132; of 250 rows
-    //     26.6, 28.5, 33.4; of 144 rows with biases, history of 4000: 18.2, 15.2, 18.3
+    //   probabilities of 1 row, history of 1000: slices 6.9, one workgroup 19.4; 64: 12.1 / 21.4; 256: 30.7 / 31.0
+    //   64 rows, slices of 8192, an entry for every token or for the named: history of 10 10.5 / 11.7, 2000 12.6 / 13.9, 100 and
+    //     biases 11.7 / 12.4, 8000 and biases 16.2 / 32.4; 120 rows, of 16384, history of 10 17.6 / 18.3, 5000 24.0 / 24.8, 20000
+    //     32.6 / 79.4 (with biases the entries do not fit beside another workgroup's)
+    //   logits of 2000 rows, history of 2000, slices of 8192 tokens, 4096, 16384: 184, 225, 258; of 250 rows 24.2, 28.0, 31.6;
+    //     of 144 rows with biases, history of 4000: 23.9, 21.3, 42.4
     constexpr int kToken = kSliceThreads * kRun;
     auto fits = [&](int runs) {
         const long long slices = (V + kToken * runs - 1) / (kToken * runs);
@@ -544,11 +543,9 @@ LogitPlan plan_for(int rows, int V, bool share, const kvattn_logit_rules& r) {
     };
     if (fits(1)) return slices_plan<kInF32, kOutF32, kProbs, 1, true>(V);
     if (fits(kSmallRuns) || (!kProbs && r.bias_start)) return slices_plan<kInF32, kOutF32, kProbs, kSmallRuns, true>(V);
-    const int ids = (r.history ? r.max_history : 0) + (r.bias_start ? r.max_bias : 0);
-    if (!kProbs || (fits(4) && ids >= kManyIds)) return slices_plan<kInF32, kOutF32, kProbs, 4, true>(V);
+    if (!kProbs || fits(4)) return slices_plan<kInF32, kOutF32, kProbs, 4, true>(V);
     if constexpr (kProbs) {
-        if (fits(4)) return slices_plan<kInF32, kOutF32, kProbs, 4, false>(V);
-        if (fits(8) && !r.bias_start && ids >= 2 * kManyIds) return slices_plan<kInF32, kOutF32, kProbs, 8, true>(V);
+        if (fits(8) && !r.bias_start) return slices_plan<kInF32, kOutF32, kProbs, 8, true>(V);
         if (fits(8)) return slices_plan<kInF32, kOutF32, kProbs, 8, false>(V);
         if (fits(13)) return slices_plan<kInF32, kOutF32, kProbs, 13, false>(V);
         constexpr int kRowToken = kRowThreads * kRun;
